@@ -5,7 +5,7 @@
 Produces, inside ``kernel-lab_b200/kernel_lab/``:
 
 * ``libkernel_lab_b200.so`` -- the kernels and the C ABI declared in
-  ``include/kernel_lab_b200.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
+  ``include/kernel_lab_b200.h`` and ``include/kernel_lab_b200_block8.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
   CUDA runtime linked statically, no PyTorch);
 * ``_C<ext-suffix>.so`` -- the ``torch.ops.kernel_lab`` registrations, a thin C++
   layer over the C ABI, linked against the library above (rpath ``$ORIGIN``).
@@ -34,7 +34,17 @@ OBJ_DIR = PKG_ROOT / "_build"
 LIB = OUT_DIR / "libkernel_lab_b200.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-CU_SOURCES = ["rmsnorm.cu", "paged_decode.cu", "kv_append.cu"]
+BLOCK8_HEADERS = [CSRC / "block8.cuh", INCLUDE / "kernel_lab_b200_block8.h"]
+# Source -> the headers it includes beyond HEADERS.
+CU_SOURCES = {
+    "rmsnorm.cu": [],
+    "paged_decode.cu": [],
+    "kv_append.cu": [],
+    "rmsnorm_fp8.cu": BLOCK8_HEADERS,
+    "block8_append.cu": BLOCK8_HEADERS,
+    "block8_decode.cu": BLOCK8_HEADERS,
+    "block8_select.cu": BLOCK8_HEADERS,
+}
 HEADERS = [CSRC / "common.cuh", INCLUDE / "kernel_lab_b200.h"]
 
 
@@ -106,10 +116,10 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     rel_include, rel_csrc = INCLUDE.relative_to(REPO), CSRC.relative_to(REPO)
     base = [*ARCH, "-O3", "-std=c++17", "-Xcompiler", "-fPIC", f"-I{rel_include}", f"-I{rel_csrc}", "-Xptxas", "-v"]
     objs = []
-    for src in CU_SOURCES:
+    for src, more in CU_SOURCES.items():
         obj = OBJ_DIR / (Path(src).stem + ".o")
         objs.append(obj)
-        if not (force or stale(obj, [CSRC / src, *HEADERS])):
+        if not (force or stale(obj, [CSRC / src, *HEADERS, *more])):
             continue
         rel_src = str(rel_csrc / src)
         if src != "paged_decode.cu":
@@ -141,7 +151,7 @@ def build_torch_ext(force: bool = False, verbose: bool = False) -> Path:
 
     target = ext_module_path()
     src = CSRC / "torch_bindings.cpp"
-    if not (force or stale(target, [src, LIB, INCLUDE / "kernel_lab_b200.h"])):
+    if not (force or stale(target, [src, LIB, INCLUDE / "kernel_lab_b200.h", INCLUDE / "kernel_lab_b200_block8.h"])):
         return target
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = [

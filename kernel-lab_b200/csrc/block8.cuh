@@ -1,0 +1,81 @@
+// What the kernels of the block-scaled 8-bit cache share: the two code types.
+#pragma once
+
+#include <atomic>
+
+#include "common.cuh"
+
+namespace klb {
+
+// Scales below this have no finite reciprocal worth using: codes of 0.
+constexpr float kLeastScale = 0x1p-126f;
+constexpr float kPer127 = 1.0f / 127.0f;  // int8 scales are products with this, one rounding, no division
+
+struct E4m3Code {
+  static constexpr float kMax = 448.0f;
+  static constexpr int kBoundUnit = 4;  // 448 / 4 = 112 fits int8
+  // The least power of two 2^k, k >= -126, with a <= 448 * 2^k: powers of two lose nothing (a code's
+  // relative precision does not depend on the scale) and make a later growth exact. From the bits
+  // of a = f * 2^e, f in [1, 2): 448 = 1.75 * 2^8, so k = e - 8, one more when f > 1.75.
+  static __device__ __forceinline__ float scale_for(float amax) {
+    if (!(amax > 0.0f)) return 0.0f;
+    const uint32_t bits = __float_as_uint(amax);
+    const int k = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return __uint_as_float(static_cast<uint32_t>(max(k, -126) + 127) << 23);
+  }
+  static __device__ __forceinline__ float value(uint32_t code) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(e4m3x2_lo_to_f16x2(code & 0xffu) & 0xffffu)));
+  }
+  static __device__ __forceinline__ uint32_t code(float v) {
+    return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+  }
+  static __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+    return lo | (hi << 16);
+  }
+};
+
+struct Int8Code {
+  static constexpr float kMax = 127.0f;
+  static constexpr int kBoundUnit = 1;
+  static __device__ __forceinline__ float scale_for(float amax) {
+    return amax > 0.0f ? fmaxf(amax * kPer127, kLeastScale) : 0.0f;
+  }
+  static __device__ __forceinline__ float value(uint32_t code) {
+    return static_cast<float>(static_cast<int8_t>(code & 0xffu));
+  }
+  // Rounds to nearest even; NaN converts to 0.
+  static __device__ __forceinline__ uint32_t code(float v) {
+    return static_cast<uint32_t>(max(-127, min(127, __float2int_rn(v)))) & 0xffu;
+  }
+  static __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
+    return code(a) | (code(b) << 8) | (code(c) << 16) | (code(d) << 24);
+  }
+};
+
+__device__ __forceinline__ float reciprocal_scale(float scale) { return scale >= kLeastScale ? 1.0f / scale : 0.0f; }
+
+// Host side: lets `kernel` use up to `bytes` of dynamic shared memory on the current device, asked
+// of the runtime once for each kernel and device.
+template <typename... Params>
+inline cudaError_t allow_shared_memory(void (*kernel)(Params...), int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
+// SMs of the current device.
+inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  return n;
+}
+
+}  // namespace klb

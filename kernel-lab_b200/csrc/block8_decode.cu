@@ -1,0 +1,922 @@
+// Single-token decode attention over a paged cache held in 8 bits (e4m3 or int8) with a scale for
+// each page and KV head, for sm_100a: over all pages of a sequence, or over a list of pages for each
+// sequence and KV head (block-sparse decode).
+//
+//   s_t = scale * k_scale[page(t), h] * sum_d q_d ck_{t,d}
+//   out = (sum_t 2^(s_t - m) * v_scale[page(t), h] * cv_t) / sum_t 2^(s_t - m)     (s in base 2)
+//
+// HBM-bound: every code is read once and used for the group's query heads (4 to 16 operations a byte).
+// One CTA of eight warps an SM. A "tile" is 16 tokens of one KV head, 2 * 16 * head_dim bytes; each
+// warp (or team of warps, below) streams its own tiles through its own ring of shared-memory stages
+// with 16-byte cp.async, so no warp waits for another while it streams and page and token strides
+// may be any. Rows past the sequence's end are zero-filled by the copy: code 0 is 0 in both formats, so
+// whatever the page holds there (NaN codes included) never reaches a product.
+//
+// Warps of a CTA. Up to 8 * NT query heads of one KV head share a warp's products (NT = 1 for groups
+// of at most 8). Larger groups take HG warps, which form a team: they share one ring, each copies 1/HG
+// of a tile and meets the others at a named barrier once a tile. The CTA's teams are HB KV heads times
+// TS parts of the token range; the TS parts' states are joined through shared memory at the end of a
+// range. Many parallel KV heads and one part where there is work for every warp (fewest joins, and
+// a page's heads are read together), more parts of fewer heads where the whole call is small.
+//
+// Balance. Rows (sequence, block of HB heads) are laid end to end, each as long as its tiles plus a
+// fixed charge for starting it, and CTA c takes the c-th equal piece, found by every CTA alone from
+// seq_lens (no host synchronisation). A row that a boundary cuts has chunks: each chunk publishes
+// its unnormalised state (fp32) and counts itself; the one that completes the count joins all of
+// them in chunk order, so the result does not depend on which came last, and sets the counter back to
+// zero. Nobody waits for another CTA.
+//
+// Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
+// to f16 exactly, q is divided by a power of two so that f16 holds it, k_scale and that power enter
+// with the softmax scale. P is at most 2^8 (the running maximum is only raised when a score passes it
+// by 8) and rounded to f16; v_scale enters P relative to the largest one met so far, so that P stays
+// in f16's range whatever the scales' magnitude.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "block8.cuh"
+#include "kernel_lab_b200_block8.h"
+
+namespace klb {
+namespace {
+
+constexpr int kB8Warps = 8;
+constexpr int kB8Threads = 32 * kB8Warps;
+constexpr int kB8Tile = 16;
+constexpr int kB8Meta = 32;        // bytes of a stage after its codes: 2 k scales, 2 v scales, 2 valid counts
+constexpr float kRaiseBy = 8.0f;   // the running maximum is raised when a score passes it by this (base 2)
+constexpr int kMaxShared = 227 * 1024 - 128;  // dynamic, beside the plan's static part
+constexpr int kTeamBarrier = 1, kGroupBarrier = 8;  // named barriers: 1.. teams, 8.. groups
+
+struct Block8Args {
+  void* out;
+  const void* q;
+  const uint8_t* k_cache;
+  const uint8_t* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* selected;  // null: every page
+  int64_t page_stride, token_stride, head_stride;
+  int64_t bt_stride;
+  int64_t num_pages;
+  int batch, num_q_heads, num_kv_heads, group, head_dim, page_size, max_pages;
+  int num_selected;
+  int q_bf16;
+  float scale_log2;
+  int hb, ts, units;   // KV heads and token parts of a CTA; units = ceil(num_kv_heads / hb)
+  int min_tiles;       // least length of a CTA's piece
+  int row_charge;      // tiles' worth of time charged for starting a row
+  uint32_t* sync;      // [0] status, [1 + (b * num_kv_heads + h) * HG + hg] arrival counters
+  float* part_o;       // [slot][8 / ts][8 * NT][DP]
+  float2* part_ml;     // [slot][8 / ts][8 * NT]: (maximum, sum)
+};
+
+// Stages of a team's ring: what 227 KB hold beside the boxes of the joins (4 warps' states).
+__host__ __device__ constexpr int ring_stages(int dp, int nt, int hg) {
+  const int per_warp = dp == 64 ? 12 : dp == 256 ? 3 : nt == 1 ? 6 : 5;
+  return hg * per_warp < 12 ? hg * per_warp : 12;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
+               "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// Four codes of a word -> two f16 pairs, exactly.
+template <typename Code>
+__device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi);
+template <>
+__device__ __forceinline__ void widen<E4m3Code>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  lo = e4m3x2_lo_to_f16x2(w);
+  hi = e4m3x2_hi_to_f16x2(w);
+}
+// The byte c + 128 below the exponent of 1024 is the f16 1024 + 128 + c.
+template <>
+__device__ __forceinline__ void widen<Int8Code>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  const uint32_t u = w ^ 0x80808080u;
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+  const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+  const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&l), bias);
+  const __half2 b = __hsub2(*reinterpret_cast<const __half2*>(&h), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+
+// Byte offset of 16-byte unit `u` of token row `r` of a tile: rows DP bytes apart, the units of each
+// 128 bytes permuted so that the score product's reads (8 lanes: 2 rows x 4 units) and the value
+// product's (8 lanes: rows 0, 2, 4, 6 or 1, 3, 5, 7 x 2 units) each meet 8 different units.
+template <int DP>
+__device__ __forceinline__ uint32_t unit_offset(int r, int u) {
+  if constexpr (DP == 64) {
+    const int line = r >> 1;
+    return line * 128 + ((((r & 1) * 4 + u) ^ ((line & 3) << 1)) << 4);
+  } else {
+    const int f = (((r ^ (r >> 2)) & 1) << 2) | (r & 2);
+    return r * DP + ((u ^ f) << 4);
+  }
+}
+
+struct Segment {
+  int b, u;         // row: sequence, block of heads
+  int x0, x1;       // tiles
+  int tiles;        // of the whole row
+  int len;
+  int64_t start;    // position of the row's first tile
+};
+
+// Walks the rows of a CTA's piece [p, p1).
+struct RowWalk {
+  int64_t p, p1, start;  // start: position of row (b, u)
+  int b, u, len, tiles;
+
+  __device__ __forceinline__ void read_row(const Block8Args& a) {
+    const int cap = a.max_pages * a.page_size;
+    len = b < a.batch ? max(0, min(a.seq_lens[b], cap)) : 0;
+    tiles = row_tiles(a, len);
+  }
+  static __device__ __forceinline__ int row_tiles(const Block8Args& a, int len) {
+    const int n = a.selected ? a.num_selected * a.page_size : len;
+    return len > 0 && n > 0 ? (n - 1) / kB8Tile + 1 : 1;  // an empty row has one tile, all masked
+  }
+  __device__ __forceinline__ bool next(const Block8Args& a, Segment& s) {
+    while (p < p1) {
+      const int cost = tiles + a.row_charge;
+      const int x0 = static_cast<int>(p - start);
+      const bool some = x0 < tiles;
+      s = Segment{b, u, x0, static_cast<int>(min(static_cast<int64_t>(tiles), p1 - start)), tiles, len, start};
+      start += cost;
+      p = start;
+      if (++u == a.units) {
+        u = 0;
+        ++b;
+        read_row(a);
+      }
+      if (some) return true;
+    }
+    return false;
+  }
+};
+
+struct PlanShared {
+  long long warp_sum[kB8Warps + 1];
+  long long before;  // positions of the sequences before the first one, divided by units
+  int b;
+};
+
+// All threads: this CTA's piece and the row it starts in; returns false for an empty piece.
+__device__ __forceinline__ bool plan_piece(const Block8Args& a, PlanShared* ps, RowWalk& w, int64_t& piece) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.batch + kB8Threads - 1) / kB8Threads;
+  const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
+  const int cap = a.max_pages * a.page_size;
+  long long local = 0;
+  bool over = false;
+  for (int b = lo; b < hi; ++b) {
+    const int len = a.seq_lens[b];
+    over |= len > cap;
+    local += RowWalk::row_tiles(a, max(0, min(len, cap))) + a.row_charge;
+  }
+  if (over && blockIdx.x == 0) atomicOr(a.sync, kStatusLenClamped);
+  long long inc = local;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) ps->warp_sum[warp] = inc;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kB8Warps; ++i) {
+    const long long v = ps->warp_sum[i];
+    if (i < warp) before += v;
+    total += v;
+  }
+  before += inc - local;
+  total *= a.units;
+  piece = max(static_cast<long long>(a.min_tiles), (total + gridDim.x - 1) / gridDim.x);
+  const int64_t p0 = piece * blockIdx.x;
+  if (p0 >= total) return false;
+  if (p0 >= before * a.units && p0 < (before + local) * a.units) {  // one thread's
+    int b = lo;
+    for (; b < hi - 1; ++b) {
+      const int cost = RowWalk::row_tiles(a, max(0, min(a.seq_lens[b], cap))) + a.row_charge;
+      if (p0 < (before + cost) * a.units) break;
+      before += cost;
+    }
+    ps->b = b;
+    ps->before = before;
+  }
+  __syncthreads();
+  w.b = ps->b;
+  w.read_row(a);
+  const int cost = w.tiles + a.row_charge;
+  const int64_t first = ps->before * a.units;
+  w.u = static_cast<int>((p0 - first) / cost);
+  w.start = first + static_cast<int64_t>(w.u) * cost;
+  w.p = p0;
+  w.p1 = min(p0 + piece, static_cast<int64_t>(total));
+  return true;
+}
+
+// DP: head_dim rounded up to 64, 128 or 256 (the copies zero-fill the rest). NT: groups of 8 query
+// heads a warp. HG: warps a team.
+template <typename Code, int DP, int NT, int HG>
+__global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Block8Args a) {
+  constexpr int kStages = ring_stages(DP, NT, HG);
+  constexpr int kTileBytes = kB8Tile * DP;
+  constexpr int kStageBytes = 2 * kTileBytes + kB8Meta;
+  constexpr int kUnits = DP / 16;             // 16-byte units of a row
+  constexpr int kRows = 32 / kUnits;          // rows one copy instruction of a warp covers
+  constexpr int kBlocks = kB8Tile / kRows;    // copy instructions of one tensor's tile
+  constexpr int kHalves = DP == 256 ? 2 : 1;  // 128-byte parts of a row
+  constexpr int kM = DP == 64 ? 4 : 8;        // value products (16 output channels) of a part
+  constexpr int kSteps = DP / 16;             // score products (16 channels)
+  constexpr int NH = 8 * NT;
+
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ PlanShared s_plan;
+  __shared__ int s_last[kB8Warps];
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, c = lane & 3;
+  const int team = warp / HG, hg = warp % HG;
+  const int hb = team / a.ts, ts = team % a.ts;
+  const int groups = kB8Warps / a.ts;      // (hb, hg) pairs of the CTA
+  const int grp = hb * HG + hg;
+
+  wait_prior_grid();
+  allow_next_grid();
+  RowWalk cons;
+  int64_t piece;
+  if (!plan_piece(a, &s_plan, cons, piece)) return;
+  // No block-wide barrier from here on: teams without a head leave.
+
+  const uint32_t ring = smem_u32(smem) + team * (kStages * kStageBytes);
+  float* const joint = reinterpret_cast<float*>(smem + (kB8Warps / HG) * kStages * kStageBytes);
+  const uint64_t policy = l2_policy_evict_first();
+
+  // ---- loading side: the team's next tile
+  RowWalk ahead = cons;
+  int l_t = 0, l_t1 = 0;          // tiles left of the segment's part
+  int l_entry = 0, l_sub = 0;     // page entry of the next tile and the tile's place in that page
+  int l_win = 0;                  // first entry of the window
+  int w_page = -1, w_col = 0, n_page = -1, n_col = 0;  // this lane's entry of the window, of the next one
+  int l_b = 0, l_h = 0, l_len = 0;
+  const int page_tiles = max(1, a.page_size / kB8Tile);
+
+  const auto read_entry = [&](int e, int& page, int& col) {
+    page = -1;
+    col = e;
+    const int used = (l_len + a.page_size - 1) / a.page_size;
+    if (a.selected) {
+      col = -1;
+      if (e < a.num_selected) {
+        col = a.selected[(static_cast<int64_t>(l_b) * a.num_kv_heads + l_h) * a.num_selected + e];
+      }
+    }
+    if (col < 0 || col >= used) return;
+    page = a.block_table[l_b * a.bt_stride + col];
+    if (page < 0 || page >= a.num_pages) {
+      atomicOr(a.sync, kStatusBadPage);
+      page = -1;
+    }
+  };
+
+  const auto issue = [&](int slot) {
+    while (l_t >= l_t1) {
+      Segment s;
+      if (!ahead.next(a, s)) {
+        cp_async_commit();
+        return;
+      }
+      l_b = s.b;
+      l_h = s.u * a.hb + hb;
+      l_len = s.len;
+      if (l_h >= a.num_kv_heads) continue;
+      const int part = (s.x1 - s.x0 + a.ts - 1) / a.ts;
+      l_t = s.x0 + ts * part;
+      l_t1 = min(s.x1, l_t + part);
+      if (l_t >= l_t1) continue;
+      if (a.page_size == 8) {
+        l_entry = 2 * l_t;
+      } else {
+        l_entry = l_t / page_tiles;
+        l_sub = l_t - l_entry * page_tiles;
+      }
+      l_win = l_entry;
+      read_entry(l_win + lane, w_page, w_col);
+      read_entry(l_win + 32 + lane, n_page, n_col);
+    }
+    if (l_entry - l_win >= 32) {
+      l_win += 32;
+      w_page = n_page;
+      w_col = n_col;
+      read_entry(l_win + 32 + lane, n_page, n_col);
+    }
+    int page[2], valid[2];
+    int64_t base[2];
+#pragma unroll
+    for (int o = 0; o < 2; ++o) {  // the tile's two octets of tokens
+      const int e = a.page_size == 8 ? l_entry + o : l_entry;
+      const int off = a.page_size == 8 ? 0 : l_sub * kB8Tile + o * 8;
+      page[o] = __shfl_sync(0xffffffffu, w_page, e - l_win);
+      const int col = __shfl_sync(0xffffffffu, w_col, e - l_win);
+      valid[o] = page[o] < 0 ? 0 : max(0, min(8, l_len - (col * a.page_size + off)));
+      base[o] = max(page[o], 0) * a.page_stride + off * a.token_stride + l_h * a.head_stride;
+    }
+    const uint32_t stage = ring + slot * kStageBytes;
+    const int unit = lane % kUnits, sub = lane / kUnits;
+#pragma unroll
+    for (int i = 0; i < (2 * kBlocks + HG - 1) / HG; ++i) {
+      const int blk = i * HG + hg;
+      if (2 * kBlocks % HG == 0 || blk < 2 * kBlocks) {
+        const int tensor = blk / kBlocks, row = (blk % kBlocks) * kRows + sub;
+        const bool second = ((blk % kBlocks) * kRows) >> 3;
+        const bool there = (row & 7) < (second ? valid[1] : valid[0]) && unit * 16 < a.head_dim;
+        const uint8_t* src = (tensor ? a.v_cache : a.k_cache) +
+                             (there ? (second ? base[1] : base[0]) + (row & 7) * a.token_stride + unit * 16 : 0);
+        cp_async16(stage + tensor * kTileBytes + unit_offset<DP>(row, unit), src, there ? 16u : 0u, policy);
+      }
+    }
+    if (hg == 0 && lane < 4) {
+      const bool there = (lane & 1 ? valid[1] : valid[0]) > 0;
+      const float* src = (lane >> 1 ? a.v_scale : a.k_scale) +
+                         (there ? static_cast<int64_t>(lane & 1 ? page[1] : page[0]) * a.num_kv_heads + l_h : 0);
+      cp_async4(stage + 2 * kTileBytes + lane * 4, src, there ? 4u : 0u);
+      if (lane == 0) {
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + 2 * kTileBytes + 16), "r"(valid[0]),
+                     "r"(valid[1])
+                     : "memory");
+      }
+    }
+    cp_async_commit();
+    ++l_t;
+    if (a.page_size == 8) {
+      l_entry += 2;
+    } else if (++l_sub == page_tiles) {
+      l_sub = 0;
+      ++l_entry;
+    }
+  };
+  const auto team_barrier = [&]() {
+    if constexpr (HG == 1) {
+      __syncwarp();
+    } else {
+      named_barrier(kTeamBarrier + team, 32 * HG);
+    }
+  };
+  const auto group_barrier = [&]() {
+    if (a.ts == 1) {
+      __syncwarp();
+    } else {
+      named_barrier(kGroupBarrier + grp, 32 * a.ts);
+    }
+  };
+
+#pragma unroll 1
+  for (int i = 0; i < kStages - 1; ++i) issue(i);
+  int slot = 0;
+
+  Segment s;
+  while (cons.next(a, s)) {
+    const int h = s.u * a.hb + hb;
+    if (h >= a.num_kv_heads) continue;
+    const int heads = max(0, min(NH, a.group - hg * NH));  // query heads of this warp
+    const int64_t q_row = static_cast<int64_t>(s.b) * a.num_q_heads + h * a.group + hg * NH;
+
+    // Q as the score product's B operand: lane (g, c) holds query head g of each group of 8. The
+    // contraction runs over a row's codes in the order in which a lane's 16-byte reads deliver them.
+    uint32_t qf[NT][kSteps][2];
+    float q_mul[NT][2];  // scale of the scores of this lane's two heads (2c, 2c + 1)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float v[kSteps][4];
+      float top = 0.0f;
+      const bool mine = n * 8 + g < heads;
+#pragma unroll
+      for (int j = 0; j < kSteps / 4; ++j) {
+        const int d = (j * 4 + c) * 16;
+        uint4 raw[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (mine && d < a.head_dim) {
+          const uint4* p = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                                          (q_row + n * 8 + g) * a.head_dim + d);
+          raw[0] = __ldg(p);
+          raw[1] = __ldg(p + 1);
+        }
+        const uint32_t w[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 f = a.q_bf16 ? Storage<__nv_bfloat16>::unpack2(w[i]) : Storage<__half>::unpack2(w[i]);
+          v[j * 4 + i / 2][(i & 1) * 2] = f.x;
+          v[j * 4 + i / 2][(i & 1) * 2 + 1] = f.y;
+          top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e just below the largest element; kept to where 2^-e is a normal number too.
+      const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        qf[n][i][0] = Storage<__half>::pack2(v[i][0] * down, v[i][1] * down);
+        qf[n][i][1] = Storage<__half>::pack2(v[i][2] * down, v[i][3] * down);
+      }
+      q_mul[n][0] = __shfl_sync(0xffffffffu, up, 8 * c);
+      q_mul[n][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
+    }
+
+    float acc[NT][kHalves][kM][4];
+    float m[NT][2], l[NT][2];
+    float v_ref = 0.0f, v_inv = 0.0f;  // the largest value scale so far, its reciprocal
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.0f;
+#pragma unroll
+      for (int f = 0; f < kHalves; ++f)
+#pragma unroll
+        for (int i = 0; i < kM; ++i) acc[n][f][i][0] = acc[n][f][i][1] = acc[n][f][i][2] = acc[n][f][i][3] = 0.0f;
+    }
+
+    const int part = (s.x1 - s.x0 + a.ts - 1) / a.ts;
+    const int t0 = s.x0 + ts * part, t1 = min(s.x1, t0 + part);
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      cp_async_wait<kStages - 2>();
+      team_barrier();
+      issue(slot == 0 ? kStages - 1 : slot - 1);
+      const uint32_t kt = ring + slot * kStageBytes, vt = kt + kTileBytes, meta = vt + kTileBytes;
+      slot = slot + 1 == kStages ? 0 : slot + 1;
+
+      // S = K.Q^T: rows (tokens) g and g + 8, columns (heads) 2c and 2c + 1.
+      float sc[NT][2][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kSteps / 4; ++j) {
+        const uint4 k0 = lds128(kt + unit_offset<DP>(g, j * 4 + c));
+        const uint4 k1 = lds128(kt + unit_offset<DP>(g + 8, j * 4 + c));
+        const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w}, r1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t a0, a1, a2, a3;
+          widen<Code>(r0[i], a0, a2);
+          widen<Code>(r1[i], a1, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            Mma<__half>::run(sc[n][i & 1], a0, a1, a2, a3, qf[n][j * 4 + i][0], qf[n][j * 4 + i][1]);
+          }
+        }
+      }
+
+      const float2 ks = lds_f2(meta), vs = lds_f2(meta + 8);
+      const uint2 valid = lds64(meta + 16);
+      const bool there0 = g < static_cast<int>(valid.x), there1 = g < static_cast<int>(valid.y);
+      const float v_top = fmaxf(fabsf(vs.x), fabsf(vs.y));
+      if (v_top > v_ref && v_top >= kLeastScale) {  // the same for the whole warp
+        const float f = v_ref / v_top;
+        v_ref = v_top;
+        v_inv = 1.0f / v_top;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int x = 0; x < kHalves; ++x)
+#pragma unroll
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[n][x][i][e] *= f;
+      }
+      const float vr0 = vs.x * v_inv, vr1 = vs.y * v_inv;
+
+      float x[NT][4];
+      bool raise = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[n][e] = there0 ? (sc[n][0][e] + sc[n][1][e]) * (q_mul[n][e] * ks.x) : -INFINITY;
+          x[n][2 + e] = there1 ? (sc[n][0][2 + e] + sc[n][1][2 + e]) * (q_mul[n][e] * ks.y) : -INFINITY;
+          raise |= fmaxf(x[n][e], x[n][2 + e]) > m[n][e] + kRaiseBy;
+        }
+      }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(x[n][e], x[n][2 + e]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float next = fmaxf(m[n][e], top);
+            const float f = next == -INFINITY ? 1.0f : exp2_fast(m[n][e] - next);
+            m[n][e] = next;
+            l[n][e] *= f;
+#pragma unroll
+            for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+              for (int i = 0; i < kM; ++i) {
+                acc[n][y][i][e] *= f;
+                acc[n][y][i][2 + e] *= f;
+              }
+          }
+        }
+      }
+
+      // P^T as the value product's B operand.
+      uint32_t p0[NT], p1[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base = m[n][e] == -INFINITY ? 0.0f : m[n][e];
+          p[e] = exp2_fast(x[n][e] - base);
+          p[2 + e] = exp2_fast(x[n][2 + e] - base);
+          l[n][e] += p[e] + p[2 + e];
+        }
+        p0[n] = movmatrix_trans(Storage<__half>::pack2(p[0] * vr0, p[1] * vr0));
+        p1[n] = movmatrix_trans(Storage<__half>::pack2(p[2] * vr1, p[3] * vr1));
+      }
+
+      // O^T += V^T.P^T: a lane reads the same channels of tokens 2c, 2c + 1, 2c + 8, 2c + 9 and pairs
+      // tokens bytewise before widening; rows g and g + 8 of product i are channels 2i and 2i + 1 of
+      // the lane's unit.
+#pragma unroll
+      for (int y = 0; y < kHalves; ++y) {
+        constexpr int kWords = DP == 64 ? 2 : 4;
+        uint32_t w[4][kWords];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 2 * c + (k & 1) + (k >> 1) * 8;
+          if constexpr (DP == 64) {
+            const uint2 u = lds64(vt + unit_offset<DP>(row, g >> 1) + (g & 1) * 8);
+            w[k][0] = u.x, w[k][1] = u.y;
+          } else {
+            const uint4 u = lds128(vt + unit_offset<DP>(row, y * 8 + g));
+            w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kM; ++i) {
+          const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+          uint32_t a0, a1, a2, a3;
+          widen<Code>(__byte_perm(w[0][i / 2], w[1][i / 2], sel), a0, a1);
+          widen<Code>(__byte_perm(w[2][i / 2], w[3][i / 2], sel), a2, a3);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) Mma<__half>::run(acc[n][y][i], a0, a1, a2, a3, p0[n], p1[n]);
+        }
+      }
+    }
+
+    // ---- end of the segment: this warp's state, values in units of 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 4);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 8);
+        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], 16);
+      }
+#pragma unroll
+      for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+        for (int i = 0; i < kM; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= v_ref;
+    }
+    // Join the TS parts: the upper half hands its state to the lower half, fragment by fragment.
+    for (int half = a.ts >> 1; half > 0; half >>= 1) {
+      constexpr int kFloats = NT * (4 + kHalves * kM * 4);
+      float* box = joint + ((grp * (a.ts >> 1) + (ts % half)) * kFloats) * 32 + lane;
+      if (ts >= half && ts < 2 * half) {
+        int k = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            box[32 * k++] = m[n][e];
+            box[32 * k++] = l[n][e];
+          }
+#pragma unroll
+          for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) box[32 * k++] = acc[n][y][i][e];
+        }
+      }
+      group_barrier();
+      if (ts < half) {
+        int k = 0;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float mine[2], other[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float om = box[32 * k++], ol = box[32 * k++];
+            const float next = fmaxf(m[n][e], om);
+            mine[e] = next == -INFINITY ? 0.0f : exp2_fast(m[n][e] - next);
+            other[e] = next == -INFINITY ? 0.0f : exp2_fast(om - next);
+            m[n][e] = next;
+            l[n][e] = l[n][e] * mine[e] + ol * other[e];
+          }
+#pragma unroll
+          for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+            for (int i = 0; i < kM; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                acc[n][y][i][e] = acc[n][y][i][e] * mine[e & 1] + box[32 * k++] * other[e & 1];
+              }
+        }
+      }
+      group_barrier();  // the boxes are free again
+    }
+
+    const int64_t c_first = s.start / piece;
+    const int chunks = static_cast<int>((s.start + s.tiles - 1) / piece - c_first) + 1;
+    const auto store_out = [&](int64_t row, int d, float v0, float v1, float v2, float v3) {
+      uint2 w;
+      if (a.q_bf16) {
+        w = make_uint2(Storage<__nv_bfloat16>::pack2(v0, v1), Storage<__nv_bfloat16>::pack2(v2, v3));
+      } else {
+        w = make_uint2(Storage<__half>::pack2(v0, v1), Storage<__half>::pack2(v2, v3));
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * a.head_dim + d) = w;
+    };
+    const auto slot_rows = [&](int64_t chunk) {  // first row of a chunk's partial state
+      const int64_t sl = (c_first + chunk) * 2 + (chunk == 0 ? 1 : 0);
+      return (sl * groups + grp) * NH;
+    };
+    if (ts == 0) {
+      // f(head of this warp, channel, 4 values) over the lane's values, four channels at a time.
+      const auto for_values = [&](auto&& f) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = n * 8 + 2 * c + e;
+            if (r >= heads) continue;
+#pragma unroll
+            for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+              for (int i = 0; i < kM; i += 2) {
+                const int d = y * 128 + g * (2 * kM) + 2 * i;
+                if (d < a.head_dim) f(r, n, e, d, acc[n][y][i][e], acc[n][y][i][2 + e], acc[n][y][i + 1][e], acc[n][y][i + 1][2 + e]);
+              }
+          }
+      };
+      if (chunks == 1) {
+        for_values([&](int r, int n, int e, int d, float v0, float v1, float v2, float v3) {
+          const float f = l[n][e] != 0.0f ? 1.0f / l[n][e] : 0.0f;
+          store_out(q_row + r, d, v0 * f, v1 * f, v2 * f, v3 * f);
+        });
+      } else {
+        const int64_t row = slot_rows(static_cast<int64_t>(blockIdx.x) - c_first);
+        for_values([&](int r, int, int, int d, float v0, float v1, float v2, float v3) {
+          *reinterpret_cast<float4*>(a.part_o + (row + r) * DP + d) = make_float4(v0, v1, v2, v3);
+        });
+        if (g == 0) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = n * 8 + 2 * c + e;
+              if (r < heads) a.part_ml[row + r] = make_float2(m[n][e], l[n][e]);
+            }
+        }
+        __syncwarp();
+        if (lane == 0) {
+          uint32_t* counter = a.sync + 1 + (static_cast<int64_t>(s.b) * a.num_kv_heads + h) * HG + hg;
+          const uint32_t old = atom_add_acq_rel_gpu(counter, 1);
+          const bool last = old == static_cast<uint32_t>(chunks - 1);
+          if (last) *counter = 0;
+          s_last[grp] = last;
+        }
+      }
+    }
+    if (chunks > 1) {
+      group_barrier();
+      if (s_last[grp]) {
+        // The group's threads share out (head, 4 channels); chunks in order.
+        const int quads = a.head_dim / 4;
+        for (int i = ts * 32 + lane; i < heads * quads; i += 32 * a.ts) {
+          const int r = i / quads, d = (i - r * quads) * 4;
+          float top = -INFINITY;
+          for (int k = 0; k < chunks; ++k) top = fmaxf(top, __ldcg(&a.part_ml[slot_rows(k) + r]).x);
+          float sum = 0.0f;
+          float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+          for (int k = 0; k < chunks; ++k) {
+            const int64_t row = slot_rows(k) + r;
+            const float2 ml = __ldcg(&a.part_ml[row]);
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row * DP + d));
+            const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
+            sum += w * ml.y;
+            o.x += w * v.x;
+            o.y += w * v.y;
+            o.z += w * v.z;
+            o.w += w * v.w;
+          }
+          const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
+          store_out(q_row + r, d, o.x * f, o.y * f, o.z * f, o.w * f);
+        }
+      }
+      group_barrier();  // s_last may be written again
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// ------------------------------------------------------------------------- host side
+
+struct Block8Plan {
+  int dp, nt, hg, hb, ts, units, min_tiles, grid;
+  size_t smem, partial_bytes, sync_bytes;
+};
+
+// False: the shape is not supported.
+bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages, int selected, Block8Plan& p) {
+  if (batch < 0 || hkv <= 0 || hq <= 0 || hq % hkv != 0 || d <= 0 || d % 16 != 0 || d > 256 || page <= 0 ||
+      (page != 8 && page % 16 != 0) || max_pages < 0 || selected < 0 ||
+      static_cast<int64_t>(max_pages) * page > INT32_MAX - 64 || static_cast<int64_t>(selected) * page > INT32_MAX - 64) {
+    return false;
+  }
+  const int group = hq / hkv;
+  p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  p.nt = group > 8 && p.dp < 256 ? 2 : 1;
+  p.hg = 1;
+  while (p.hg * 8 * p.nt < group) p.hg *= 2;
+  if (p.hg > kB8Warps) return false;
+  const int teams = kB8Warps / p.hg;
+  const int sms = sm_count();
+  const int64_t tokens = selected > 0 ? static_cast<int64_t>(selected) * page : static_cast<int64_t>(max_pages) * page;
+  const int64_t tiles = std::max<int64_t>(1, (tokens + kB8Tile - 1) / kB8Tile);
+  // As many heads side by side as fill the CTA, halved while a CTA would get fewer than 4 tiles.
+  p.hb = 1;
+  while (2 * p.hb <= teams && 2 * p.hb <= hkv) p.hb *= 2;
+  while (p.hb > 1 && batch * tiles * ((hkv + p.hb - 1) / p.hb) < 4 * static_cast<int64_t>(sms)) p.hb /= 2;
+  p.ts = teams / p.hb;
+  p.units = (hkv + p.hb - 1) / p.hb;
+  p.min_tiles = std::max(4, p.ts);
+  const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + 4);
+  p.grid = static_cast<int>(std::min<int64_t>(sms, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
+  const int stages = ring_stages(p.dp, p.nt, p.hg);
+  const int frag = p.nt * (4 + (p.dp == 256 ? 64 : p.dp == 128 ? 32 : 16));
+  p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * (2 * kB8Tile * p.dp + kB8Meta);
+  if (p.ts > 1) p.smem += static_cast<size_t>(kB8Warps / p.ts) * (p.ts / 2) * frag * 32 * sizeof(float);
+  const size_t rows = static_cast<size_t>(p.grid) * 2 * (kB8Warps / p.ts) * 8 * p.nt;
+  p.partial_bytes = rows * (p.dp * sizeof(float) + sizeof(float2));
+  p.sync_bytes = (1 + static_cast<size_t>(batch) * hkv * p.hg) * sizeof(uint32_t);
+  return true;
+}
+
+bool decode_pdl() {  // the same switch as the other decode kernels'
+  static const bool on = env_switch_on("KL_DECODE_PDL");
+  return on;
+}
+
+template <typename Code, int DP, int NT, int HG>
+cudaError_t launch_block8(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
+  const auto kernel = decode_block8_kernel<Code, DP, NT, HG>;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_shared_memory(kernel, kMaxShared, done);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(decode_pdl(), kernel, dim3(static_cast<unsigned>(p.grid)), dim3(kB8Threads), p.smem, st, a);
+}
+
+template <typename Code, int DP, int NT>
+cudaError_t launch_heads(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
+  switch (p.hg) {
+    case 1: return launch_block8<Code, DP, NT, 1>(a, p, st);
+    case 2: return launch_block8<Code, DP, NT, 2>(a, p, st);
+    case 4: return launch_block8<Code, DP, NT, 4>(a, p, st);
+    default: return launch_block8<Code, DP, NT, 8>(a, p, st);
+  }
+}
+
+template <typename Code>
+cudaError_t launch_code(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
+  if (p.dp == 256) return launch_heads<Code, 256, 1>(a, p, st);
+  if (p.nt == 1) return p.dp == 64 ? launch_block8<Code, 64, 1, 1>(a, p, st) : launch_block8<Code, 128, 1, 1>(a, p, st);
+  return p.dp == 64 ? launch_heads<Code, 64, 2>(a, p, st) : launch_heads<Code, 128, 2>(a, p, st);
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+}  // namespace klb
+
+extern "C" int kl_paged_decode_block8_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim,
+                                                     int page_size, int max_pages_per_seq, int num_selected,
+                                                     size_t* partial_bytes, size_t* sync_bytes) {
+  if (!partial_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  *partial_bytes = 0;
+  *sync_bytes = sizeof(uint32_t);
+  if (batch == 0) return 0;
+  klb::Block8Plan p;
+  if (!klb::make_block8_plan(batch, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, num_selected, p)) {
+    return static_cast<int>(cudaErrorInvalidValue);
+  }
+  *partial_bytes = p.partial_bytes;
+  *sync_bytes = p.sync_bytes;
+  return 0;
+}
+
+extern "C" int kl_paged_decode_block8(int dtype, int code_type, void* out, const void* q, const void* k_cache,
+                                      const void* v_cache, const float* k_scale, const float* v_scale,
+                                      const int32_t* block_table, const int32_t* seq_lens, const int32_t* selected,
+                                      int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                      int64_t page_stride, int64_t token_stride, int64_t head_stride,
+                                      int64_t block_table_stride, int max_pages_per_seq, int64_t num_pages,
+                                      int num_selected, float scale, void* partials, size_t partial_bytes, void* sync,
+                                      size_t sync_bytes, void* stream) {
+  using namespace klb;
+  constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
+  if (batch == 0) return 0;
+  if ((dtype != KL_FLOAT16 && dtype != KL_BFLOAT16) || (code_type != KL_CODE_E4M3 && code_type != KL_CODE_INT8) ||
+      !out || !q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !seq_lens || !sync ||
+      num_pages < 0 || num_pages > INT32_MAX || block_table_stride < max_pages_per_seq ||
+      (selected == nullptr) != (num_selected == 0) || page_stride < 0 || token_stride < 0 || head_stride < 0 ||
+      page_stride % 16 != 0 || token_stride % 16 != 0 || head_stride % 16 != 0 || !aligned16(k_cache) ||
+      !aligned16(v_cache) || !aligned16(q) || !aligned16(out)) {
+    return kInvalid;
+  }
+  Block8Plan p;
+  if (!make_block8_plan(batch, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, num_selected, p)) {
+    return kInvalid;
+  }
+  if (partial_bytes < p.partial_bytes || sync_bytes < p.sync_bytes || !partials || !aligned16(partials)) return kInvalid;
+  Block8Args a{};
+  a.out = out;
+  a.q = q;
+  a.k_cache = static_cast<const uint8_t*>(k_cache);
+  a.v_cache = static_cast<const uint8_t*>(v_cache);
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.block_table = block_table;
+  a.seq_lens = seq_lens;
+  a.selected = selected;
+  a.page_stride = page_stride;
+  a.token_stride = token_stride;
+  a.head_stride = head_stride;
+  a.bt_stride = block_table_stride;
+  a.num_pages = num_pages;
+  a.batch = batch;
+  a.num_q_heads = num_q_heads;
+  a.num_kv_heads = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.head_dim = head_dim;
+  a.page_size = page_size;
+  a.max_pages = max_pages_per_seq;
+  a.num_selected = num_selected;
+  a.q_bf16 = dtype == KL_BFLOAT16;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.hb = p.hb;
+  a.ts = p.ts;
+  a.units = p.units;
+  a.min_tiles = p.min_tiles;
+  a.row_charge = 4;
+  a.sync = static_cast<uint32_t*>(sync);
+  a.part_o = static_cast<float*>(partials);
+  const size_t rows = static_cast<size_t>(p.grid) * 2 * (kB8Warps / p.ts) * 8 * p.nt;
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * p.dp);
+  const auto st = static_cast<cudaStream_t>(stream);
+  return static_cast<int>(code_type == KL_CODE_E4M3 ? launch_code<E4m3Code>(a, p, st) : launch_code<Int8Code>(a, p, st));
+}

@@ -12,6 +12,9 @@
 // the C ABI becomes "kernel_lab: <op> failed: <reason>". Meta kernels (no-ops: the ops
 // only mutate their outputs) let torch.compile(fullgraph=True) trace the ops.
 //
+// The 8-bit serving step (kernel_lab_b200_block8.h): rms_norm_fp8, fused_add_rms_norm_fp8,
+// paged_kv_append_block8, paged_decode_attention_block8 and paged_block_select.
+//
 // Decode scratch (split partials and arrival counters) is owned here, one pair of
 // buffers per (device, stream), allocated through PyTorch's caching allocator and grown
 // on demand. The counters are zeroed once at allocation; every call leaves them zero.
@@ -26,6 +29,7 @@
 #include <utility>
 
 #include "kernel_lab_b200.h"
+#include "kernel_lab_b200_block8.h"
 
 namespace {
 
@@ -387,6 +391,242 @@ void paged_decode_attention_cascade(at::Tensor& out, const at::Tensor& q, const 
       "paged_decode_attention_cascade");
 }
 
+// RMSNorm with an e4m3 output and a scale a row (group_size 0) or a group of columns
+// (kl_rms_norm_fp8); with a residual, residual_out receives x + residual (it may be `residual`).
+void rms_norm_fp8_impl(at::Tensor& codes, at::Tensor& scales, at::Tensor* residual_out, const at::Tensor& x,
+                       const at::Tensor* residual, const at::Tensor& weight, double eps, int64_t group_size,
+                       const char* what) {
+  TORCH_CHECK(x.is_cuda() && weight.is_cuda() && codes.is_cuda() && scales.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK(x.dim() >= 1 && x.stride(-1) == 1, "x must have a contiguous last dimension");
+  TORCH_CHECK(codes.is_contiguous() && scales.is_contiguous() && weight.is_contiguous(),
+              "codes, scales and weight must be contiguous");
+  const int64_t hidden = x.size(-1);
+  TORCH_CHECK(hidden > 0 && hidden <= INT32_MAX, "x must have columns");
+  TORCH_CHECK(weight.numel() == hidden, "weight size ", weight.numel(), " != hidden ", hidden);
+  TORCH_CHECK(x.scalar_type() == weight.scalar_type(), "x and weight must share a dtype");
+  TORCH_CHECK(is_e4m3(codes) && codes.sizes() == x.sizes(), "codes must be float8_e4m3fn (or uint8) and match x");
+  TORCH_CHECK(group_size >= 0 && group_size <= INT32_MAX, "group_size must be >= 0");
+  const int64_t groups = group_size == 0 ? 1 : (hidden + group_size - 1) / group_size;
+  TORCH_CHECK(scales.scalar_type() == at::kFloat && scales.numel() == x.numel() / hidden * groups,
+              "scales must be float32 with ", groups, " per row");
+  TORCH_CHECK(weight.device() == x.device() && codes.device() == x.device() && scales.device() == x.device(),
+              "tensors must be on one device");
+  const at::Tensor x2 = x.dim() == 2 ? x : x.reshape({-1, hidden});
+  TORCH_CHECK(x2.stride(-1) == 1, "x cannot be viewed as rows with a contiguous last dim");
+  TORCH_CHECK(x2.size(0) <= INT32_MAX, "too many rows");
+  for (const at::Tensor* t : {residual, static_cast<const at::Tensor*>(residual_out)}) {
+    TORCH_CHECK(t == nullptr || (t->is_contiguous() && t->sizes() == x.sizes() && t->scalar_type() == x.scalar_type() &&
+                                 t->device() == x.device()),
+                "residual must be contiguous, same shape and dtype as x");
+  }
+  const c10::cuda::CUDAGuard guard(x.device());
+  check_status(kl_rms_norm_fp8(to_dtype(x.scalar_type()), codes.data_ptr(), scales.data_ptr<float>(),
+                               residual_out ? residual_out->data_ptr() : nullptr, x2.data_ptr(),
+                               residual ? residual->data_ptr() : nullptr, weight.data_ptr(),
+                               static_cast<int>(x2.size(0)), static_cast<int>(hidden), x2.stride(0),
+                               static_cast<int>(group_size), static_cast<float>(eps),
+                               at::cuda::getCurrentCUDAStream().stream()),
+               what);
+}
+
+void rms_norm_fp8(at::Tensor& codes, at::Tensor& scales, const at::Tensor& x, const at::Tensor& weight, double eps,
+                  int64_t group_size) {
+  rms_norm_fp8_impl(codes, scales, nullptr, x, nullptr, weight, eps, group_size, "rms_norm_fp8");
+}
+
+void fused_add_rms_norm_fp8(at::Tensor& codes, at::Tensor& scales, at::Tensor& residual_out, const at::Tensor& x,
+                            const at::Tensor& residual, const at::Tensor& weight, double eps, int64_t group_size) {
+  rms_norm_fp8_impl(codes, scales, &residual_out, x, &residual, weight, eps, group_size, "fused_add_rms_norm_fp8");
+}
+
+int code_type_of(const at::Tensor& cache) {
+  TORCH_CHECK(cache.scalar_type() == at::kFloat8_e4m3fn || cache.scalar_type() == at::kChar,
+              "block-scaled caches are float8_e4m3fn or int8");
+  return cache.scalar_type() == at::kChar ? KL_CODE_INT8 : KL_CODE_E4M3;
+}
+
+// [num_pages, page_size, num_kv_heads, head_dim] caches of one layout (pages, tokens and heads in any
+// order, head_dim contiguous) with [num_pages, num_kv_heads] scales.
+void check_block8_cache(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+                        const at::Tensor& v_scale) {
+  TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda() && k_scale.is_cuda() && v_scale.is_cuda(),
+              "tensors must be on CUDA");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes() && k_cache.strides() == v_cache.strides() &&
+                  k_cache.scalar_type() == v_cache.scalar_type(),
+              "caches are [num_pages, page_size, num_kv_heads, head_dim] of one shape, layout and dtype");
+  TORCH_CHECK(k_cache.size(3) > 0 && k_cache.stride(3) == 1, "caches need a contiguous head_dim");
+  for (const at::Tensor* t : {&k_scale, &v_scale}) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 2 &&
+                    t->size(0) == k_cache.size(0) && t->size(1) == k_cache.size(2),
+                "k_scale and v_scale are contiguous float32 [num_pages, num_kv_heads]");
+  }
+  TORCH_CHECK(v_cache.device() == k_cache.device() && k_scale.device() == k_cache.device() &&
+                  v_scale.device() == k_cache.device(),
+              "tensors must be on one device");
+  for (int64_t d : k_cache.sizes()) TORCH_CHECK(d <= INT32_MAX, "cache dimensions must fit 32 bits");
+}
+
+// A dimension's stride; 0 where it has one entry (its stride means nothing there).
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) == 1 ? 0 : t.stride(dim); }
+
+void check_bounds(const at::Tensor& k_bounds, const at::Tensor& k_cache) {
+  TORCH_CHECK(k_bounds.scalar_type() == at::kChar && k_bounds.is_contiguous() && k_bounds.dim() == 4 &&
+                  k_bounds.size(0) == k_cache.size(0) && k_bounds.size(1) == k_cache.size(2) &&
+                  k_bounds.size(2) == 2 && k_bounds.size(3) == k_cache.size(3) &&
+                  k_bounds.device() == k_cache.device(),
+              "k_bounds is contiguous int8 [num_pages, num_kv_heads, 2, head_dim] on the caches' device");
+}
+
+void check_tables(const at::Tensor& block_table, const at::Tensor& per_sequence, int64_t batch, const at::Device& dev,
+                  const char* name) {
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && per_sequence.scalar_type() == at::kInt &&
+                  block_table.dim() == 2 && block_table.stride(-1) == 1 && per_sequence.is_contiguous(),
+              "block_table rows and ", name, " must be contiguous int32");
+  TORCH_CHECK(per_sequence.numel() == batch && block_table.size(0) == batch, "block_table and ", name,
+              " need one row / entry per sequence");
+  TORCH_CHECK(block_table.device() == dev && per_sequence.device() == dev, "tensors must be on one device");
+}
+
+// Append into a block-scaled 8-bit cache (kl_paged_kv_append_block8): one token a sequence, or with
+// indptr [batch + 1] the rows indptr[b] .. indptr[b + 1] - 1 at positions[b], positions[b] + 1, ...
+void paged_kv_append_block8(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& k_scale, at::Tensor& v_scale,
+                            const std::optional<at::Tensor>& k_bounds, const at::Tensor& k_new,
+                            const at::Tensor& v_new, const at::Tensor& block_table, const at::Tensor& positions,
+                            const std::optional<at::Tensor>& indptr) {
+  check_block8_cache(k_cache, v_cache, k_scale, v_scale);
+  const int code_type = code_type_of(k_cache);
+  const int64_t num_kv_heads = k_cache.size(2), head_dim = k_cache.size(3);
+  TORCH_CHECK(k_new.sizes() == v_new.sizes() && k_new.strides() == v_new.strides() &&
+                  k_new.scalar_type() == v_new.scalar_type(),
+              "k_new and v_new must have one shape, layout and dtype");
+  TORCH_CHECK((k_new.dim() == 3 && k_new.size(1) == num_kv_heads && k_new.size(2) == head_dim &&
+               k_new.stride(2) == 1 && (k_new.stride(1) == head_dim || num_kv_heads == 1)) ||
+                  (k_new.dim() == 2 && k_new.size(1) == num_kv_heads * head_dim && k_new.stride(1) == 1),
+              "k_new is [tokens, num_kv_heads, head_dim] (or [tokens, num_kv_heads*head_dim]) with contiguous rows");
+  const int64_t tokens = k_new.size(0), batch = positions.numel();
+  check_tables(block_table, positions, batch, k_cache.device(), "positions");
+  TORCH_CHECK(k_new.device() == k_cache.device() && v_new.device() == k_cache.device(),
+              "tensors must be on one device");
+  if (indptr) {
+    TORCH_CHECK(indptr->scalar_type() == at::kInt && indptr->is_contiguous() && indptr->numel() == batch + 1 &&
+                    indptr->device() == k_cache.device(),
+                "indptr is contiguous int32 [batch + 1] on the caches' device");
+  } else {
+    TORCH_CHECK(tokens == batch, "without indptr there is one new row per sequence");
+  }
+  if (k_bounds) check_bounds(*k_bounds, k_cache);
+  if (batch == 0 || tokens == 0) return;
+  // A row stride is arbitrary where there is one row.
+  const int64_t row_stride = tokens == 1 ? num_kv_heads * head_dim : k_new.stride(0);
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  Scratch& s = scratch_for(k_cache.device(), stream, 0, 4);
+  check_status(
+      kl_paged_kv_append_block8(to_dtype(k_new.scalar_type()), code_type, k_cache.data_ptr(), v_cache.data_ptr(),
+                                k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                                k_bounds ? k_bounds->data_ptr() : nullptr, k_new.data_ptr(), v_new.data_ptr(),
+                                block_table.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
+                                indptr ? indptr->data_ptr<int32_t>() : nullptr, static_cast<int>(batch), tokens,
+                                static_cast<int>(num_kv_heads), static_cast<int>(head_dim),
+                                static_cast<int>(k_cache.size(1)), stride_of(k_cache, 0), stride_of(k_cache, 1),
+                                stride_of(k_cache, 2), block_table.stride(0), static_cast<int>(block_table.size(1)),
+                                k_cache.size(0), row_stride, static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+      "paged_kv_append_block8");
+}
+
+// Decode over a block-scaled 8-bit cache (kl_paged_decode_block8), over every page or over the
+// block-table columns in `selected` [batch, num_kv_heads, n].
+void paged_decode_attention_block8(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache,
+                                   const at::Tensor& v_cache, const at::Tensor& k_scale, const at::Tensor& v_scale,
+                                   const at::Tensor& block_table, const at::Tensor& seq_lens, double scale,
+                                   const std::optional<at::Tensor>& selected) {
+  check_block8_cache(k_cache, v_cache, k_scale, v_scale);
+  const int code_type = code_type_of(k_cache);
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && out.is_contiguous() && out.sizes() == q.sizes() &&
+                  out.scalar_type() == q.scalar_type(),
+              "q is a contiguous [batch, heads, dim] and out matches it");
+  TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "q and out are fp16 or bf16");
+  TORCH_CHECK(q.device() == k_cache.device() && out.device() == k_cache.device(), "tensors must be on one device");
+  const int64_t batch = q.size(0), num_q_heads = q.size(1), num_kv_heads = k_cache.size(2);
+  TORCH_CHECK(k_cache.size(3) == q.size(2), "cache head_dim differs from q");
+  TORCH_CHECK(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+              "num_q_heads must be a multiple of num_kv_heads");
+  check_tables(block_table, seq_lens, batch, q.device(), "seq_lens");
+  int num_selected = 0;
+  if (selected) {
+    TORCH_CHECK(selected->scalar_type() == at::kInt && selected->is_contiguous() && selected->dim() == 3 &&
+                    selected->size(0) == batch && selected->size(1) == num_kv_heads && selected->size(2) > 0 &&
+                    selected->size(2) <= INT32_MAX && selected->device() == q.device(),
+                "selected is contiguous int32 [batch, num_kv_heads, n] on q's device");
+    num_selected = static_cast<int>(selected->size(2));
+  }
+  if (batch == 0) return;
+  const int d = static_cast<int>(q.size(2)), page = static_cast<int>(k_cache.size(1));
+  const int max_pages = static_cast<int>(block_table.size(1));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  size_t partial_bytes = 0, sync_bytes = 0;
+  check_status(kl_paged_decode_block8_workspace_size(static_cast<int>(batch), static_cast<int>(num_q_heads),
+                                                     static_cast<int>(num_kv_heads), d, page, max_pages, num_selected,
+                                                     &partial_bytes, &sync_bytes),
+               "paged_decode_attention_block8 (workspace)");
+  Scratch& s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  check_status(
+      kl_paged_decode_block8(to_dtype(q.scalar_type()), code_type, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+                             v_cache.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
+                             block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
+                             selected ? selected->data_ptr<int32_t>() : nullptr, static_cast<int>(batch),
+                             static_cast<int>(num_q_heads), static_cast<int>(num_kv_heads), d, page,
+                             stride_of(k_cache, 0), stride_of(k_cache, 1), stride_of(k_cache, 2), block_table.stride(0), max_pages,
+                             k_cache.size(0), num_selected, static_cast<float>(scale), s.partials.data_ptr(),
+                             static_cast<size_t>(s.partials.numel()), s.sync.data_ptr(),
+                             static_cast<size_t>(s.sync.numel()), stream),
+      "paged_decode_attention_block8");
+}
+
+// The pages a decode step should read, by their key bounds (kl_paged_block_select).
+void paged_block_select(at::Tensor& selected, const at::Tensor& q, const at::Tensor& k_cache,
+                        const at::Tensor& k_scale, const at::Tensor& k_bounds, const at::Tensor& block_table,
+                        const at::Tensor& seq_lens, int64_t sink_pages, int64_t recent_pages) {
+  check_block8_cache(k_cache, k_cache, k_scale, k_scale);
+  const int code_type = code_type_of(k_cache);
+  check_bounds(k_bounds, k_cache);
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.is_contiguous() && q.device() == k_cache.device(),
+              "q is a contiguous [batch, heads, dim] on the cache's device");
+  const int64_t batch = q.size(0), num_q_heads = q.size(1), num_kv_heads = k_cache.size(2);
+  TORCH_CHECK(k_cache.size(3) == q.size(2), "cache head_dim differs from q");
+  TORCH_CHECK(num_kv_heads > 0 && num_q_heads > 0 && num_q_heads % num_kv_heads == 0,
+              "num_q_heads must be a multiple of num_kv_heads");
+  check_tables(block_table, seq_lens, batch, q.device(), "seq_lens");
+  TORCH_CHECK(selected.scalar_type() == at::kInt && selected.is_contiguous() && selected.dim() == 3 &&
+                  selected.size(0) == batch && selected.size(1) == num_kv_heads && selected.size(2) > 0 &&
+                  selected.size(2) <= INT32_MAX && selected.device() == q.device(),
+              "selected is contiguous int32 [batch, num_kv_heads, n] on q's device");
+  TORCH_CHECK(sink_pages >= 0 && recent_pages >= 0 && sink_pages <= selected.size(2) &&
+                  recent_pages <= selected.size(2) - sink_pages,
+              "sink_pages and recent_pages must fit in the selection");
+  if (batch == 0) return;
+  const int max_pages = static_cast<int>(block_table.size(1));
+  const c10::cuda::CUDAGuard guard(q.device());
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  size_t scratch_bytes = 0, sync_bytes = 0;
+  check_status(kl_paged_block_select_workspace_size(static_cast<int>(batch), static_cast<int>(num_kv_heads), max_pages,
+                                                    &scratch_bytes, &sync_bytes),
+               "paged_block_select (workspace)");
+  Scratch& s = scratch_for(q.device(), stream, scratch_bytes, sync_bytes);
+  check_status(
+      kl_paged_block_select(to_dtype(q.scalar_type()), code_type, selected.data_ptr<int32_t>(), q.data_ptr(),
+                            k_bounds.data_ptr(), k_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
+                            seq_lens.data_ptr<int32_t>(), static_cast<int>(batch), static_cast<int>(num_q_heads),
+                            static_cast<int>(num_kv_heads), static_cast<int>(q.size(2)),
+                            static_cast<int>(k_cache.size(1)), block_table.stride(0), max_pages, k_cache.size(0),
+                            static_cast<int>(selected.size(2)), static_cast<int>(sink_pages),
+                            static_cast<int>(recent_pages), s.partials.data_ptr(),
+                            static_cast<size_t>(s.partials.numel()), s.sync.data_ptr(),
+                            static_cast<size_t>(s.sync.numel()), stream),
+      "paged_block_select");
+}
+
 // Status bits (KL_STATUS_*) left by decode calls on the current device and stream.
 int64_t decode_status(bool clear) {
   const at::Device dev(at::kCUDA, c10::cuda::current_device());
@@ -401,6 +641,58 @@ int64_t decode_status(bool clear) {
   uint32_t status = 0;
   check_status(kl_paged_decode_read_status(sync.data_ptr(), &status, clear ? 1 : 0, stream), "decode_status");
   return status;
+}
+
+// Functional forms of the 8-bit ops for eager callers (kernel_lab.cuda_ops): outputs allocated here and
+// the implementation called directly, which costs a host 4-8 us less a call than allocating in Python
+// and going through the dispatcher. Traced code takes the torch.ops, which have Meta kernels.
+std::pair<at::Tensor, at::Tensor> fp8_outputs(const at::Tensor& x, int64_t group_size) {
+  TORCH_CHECK(group_size >= 0, "group_size must be >= 0");
+  TORCH_CHECK(x.dim() >= 1 && x.is_cuda(), "x must be rows on CUDA");
+  at::DimVector shape(x.sizes().begin(), x.sizes().end());
+  at::Tensor codes = at::empty(shape, x.options().dtype(at::kFloat8_e4m3fn));
+  shape.back() = group_size == 0 ? 1 : (x.size(-1) + group_size - 1) / group_size;
+  return {codes, at::empty(shape, x.options().dtype(at::kFloat))};
+}
+
+std::tuple<at::Tensor, at::Tensor> rms_norm_fp8_new(const at::Tensor& x, const at::Tensor& weight, double eps,
+                                                    int64_t group_size) {
+  auto [codes, scales] = fp8_outputs(x, group_size);
+  rms_norm_fp8(codes, scales, x, weight, eps, group_size);
+  return {codes, scales};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> fused_add_rms_norm_fp8_new(const at::Tensor& x,
+                                                                          const at::Tensor& residual,
+                                                                          const at::Tensor& weight, double eps,
+                                                                          int64_t group_size) {
+  auto [codes, scales] = fp8_outputs(x, group_size);
+  at::Tensor residual_out = at::empty(x.sizes(), x.options());
+  fused_add_rms_norm_fp8(codes, scales, residual_out, x, residual.contiguous(), weight, eps, group_size);
+  return {codes, scales, residual_out};
+}
+
+at::Tensor paged_decode_attention_block8_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                             const at::Tensor& k_scale, const at::Tensor& v_scale,
+                                             const at::Tensor& block_table, const at::Tensor& seq_lens, double scale,
+                                             const std::optional<at::Tensor>& selected) {
+  at::Tensor rows = q.contiguous();
+  if (reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 != 0) rows = rows.clone();  // a view may start anywhere
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  paged_decode_attention_block8(out, rows, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected);
+  return out;
+}
+
+at::Tensor paged_block_select_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& k_scale,
+                                  const at::Tensor& k_bounds, const at::Tensor& block_table,
+                                  const at::Tensor& seq_lens, int64_t num_selected, int64_t sink_pages,
+                                  int64_t recent_pages) {
+  TORCH_CHECK(q.dim() == 3 && k_cache.dim() == 4 && num_selected > 0,
+              "q is [batch, heads, dim], the cache is 4-D and num_selected is positive");
+  at::Tensor selected = at::empty({q.size(0), k_cache.size(2), num_selected}, q.options().dtype(at::kInt));
+  paged_block_select(selected, q.contiguous(), k_cache, k_scale, k_bounds, block_table, seq_lens, sink_pages,
+                     recent_pages);
+  return selected;
 }
 
 void noop_rms_norm(at::Tensor&, const at::Tensor&, const at::Tensor&, double) {}
@@ -418,6 +710,18 @@ void noop_append_fp8(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tens
 void noop_cascade(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                   const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, double,
                   const std::optional<at::Tensor>&, const std::optional<at::Tensor>&) {}
+
+void noop_norm_fp8(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&, double, int64_t) {}
+void noop_fused_fp8(at::Tensor&, at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                    double, int64_t) {}
+void noop_append_block8(at::Tensor&, at::Tensor&, at::Tensor&, at::Tensor&, const std::optional<at::Tensor>&,
+                        const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                        const std::optional<at::Tensor>&) {}
+void noop_decode_block8(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                        const at::Tensor&, const at::Tensor&, const at::Tensor&, double,
+                        const std::optional<at::Tensor>&) {}
+void noop_select(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                 const at::Tensor&, const at::Tensor&, int64_t, int64_t) {}
 
 }  // namespace
 
@@ -443,6 +747,20 @@ TORCH_LIBRARY(kernel_lab, m) {
       "paged_decode_attention_cascade(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, "
       "Tensor prefix_block_table, Tensor prefix_lens, Tensor prefix_indptr, Tensor block_table, "
       "Tensor seq_lens, float scale, Tensor? k_scale=None, Tensor? v_scale=None) -> ()");
+  m.def("rms_norm_fp8(Tensor! codes, Tensor! scales, Tensor x, Tensor weight, float eps, int group_size) -> ()");
+  m.def(
+      "fused_add_rms_norm_fp8(Tensor! codes, Tensor! scales, Tensor! residual_out, Tensor x, Tensor residual, "
+      "Tensor weight, float eps, int group_size) -> ()");
+  m.def(
+      "paged_kv_append_block8(Tensor! k_cache, Tensor! v_cache, Tensor! k_scale, Tensor! v_scale, "
+      "Tensor(a!)? k_bounds, Tensor k_new, Tensor v_new, Tensor block_table, Tensor positions, "
+      "Tensor? indptr=None) -> ()");
+  m.def(
+      "paged_decode_attention_block8(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, "
+      "Tensor v_scale, Tensor block_table, Tensor seq_lens, float scale, Tensor? selected=None) -> ()");
+  m.def(
+      "paged_block_select(Tensor! selected, Tensor q, Tensor k_cache, Tensor k_scale, Tensor k_bounds, "
+      "Tensor block_table, Tensor seq_lens, int sink_pages, int recent_pages) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
@@ -454,6 +772,11 @@ TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
   m.impl("paged_decode_attention_fp8", &paged_decode_attention_fp8);
   m.impl("paged_kv_append_fp8", &paged_kv_append_fp8);
   m.impl("paged_decode_attention_cascade", &paged_decode_attention_cascade);
+  m.impl("rms_norm_fp8", &rms_norm_fp8);
+  m.impl("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8);
+  m.impl("paged_kv_append_block8", &paged_kv_append_block8);
+  m.impl("paged_decode_attention_block8", &paged_decode_attention_block8);
+  m.impl("paged_block_select", &paged_block_select);
 }
 
 TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
@@ -465,11 +788,21 @@ TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
   m.impl("paged_decode_attention_fp8", &noop_decode_fp8);
   m.impl("paged_kv_append_fp8", &noop_append_fp8);
   m.impl("paged_decode_attention_cascade", &noop_cascade);
+  m.impl("rms_norm_fp8", &noop_norm_fp8);
+  m.impl("fused_add_rms_norm_fp8", &noop_fused_fp8);
+  m.impl("paged_kv_append_block8", &noop_append_block8);
+  m.impl("paged_decode_attention_block8", &noop_decode_block8);
+  m.impl("paged_block_select", &noop_select);
 }
 
 // Importing kernel_lab._C runs the registrations above.
 PYBIND11_MODULE(_C, m) {
   m.def("decode_status", &decode_status, pybind11::arg("clear") = false,
         "Status bits left by paged_decode_attention on the current device and stream.");
+  m.def("rms_norm_fp8", &rms_norm_fp8_new);
+  m.def("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8_new);
+  m.def("paged_kv_append_block8", &paged_kv_append_block8);
+  m.def("paged_decode_attention_block8", &paged_decode_attention_block8_new);
+  m.def("paged_block_select", &paged_block_select_new);
   m.attr("version") = kl_version();
 }

@@ -85,6 +85,29 @@ SIGNATURES = {
     "kl_ipc_free": (_c_int, [_c_vp]),
 }
 
+# The same for include/kernel_lab_b200_block8.h.
+BLOCK8_SIGNATURES = {
+    "kl_rms_norm_fp8": (_c_int, [_c_int] + [_c_vp] * 6 + [_c_int, _c_int, _c_i64, _c_int, _c_float, _c_vp]),
+    "kl_paged_kv_append_block8": (
+        _c_int,
+        [_c_int, _c_int] + [_c_vp] * 10 + [_c_int, _c_i64, _c_int, _c_int, _c_int] + [_c_i64] * 4
+        + [_c_int, _c_i64, _c_i64, _c_vp, _c_vp],
+    ),
+    "kl_paged_decode_block8_workspace_size": (_c_int, [_c_int] * 7 + [_c_szp, _c_szp]),
+    "kl_paged_decode_block8": (
+        _c_int,
+        [_c_int, _c_int] + [_c_vp] * 9 + [_c_int] * 5 + [_c_i64] * 4
+        + [_c_int, _c_i64, _c_int, _c_float, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
+    ),
+    "kl_paged_block_select_workspace_size": (_c_int, [_c_int] * 3 + [_c_szp, _c_szp]),
+    "kl_paged_block_select": (
+        _c_int,
+        [_c_int, _c_int] + [_c_vp] * 6 + [_c_int] * 5 + [_c_i64, _c_int, _c_i64, _c_int, _c_int, _c_int]
+        + [_c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
+    ),
+}
+
+KL_CODE_E4M3, KL_CODE_INT8 = 0, 1
 KL_STATUS_PEER_TIMEOUT = 16
 KL_GATHER_MAX_RANKS = 8
 KL_IPC_HANDLE_BYTES = 64
@@ -119,7 +142,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH.name} is not built; run `python kernel-lab_b200/build.py`")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in (SIGNATURES | BLOCK8_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

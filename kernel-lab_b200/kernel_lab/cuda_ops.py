@@ -2,7 +2,8 @@
 
 Same API as kernel-lab's ``kernel_lab/cuda_ops.py:11-61`` (``available``,
 ``why_unavailable``, ``rms_norm``, ``fused_add_rms_norm``, ``paged_decode_attention``),
-plus ``num_splits`` on ``paged_decode_attention`` and ``decode_status``. There is no
+plus ``num_splits`` on ``paged_decode_attention``, ``decode_status`` and the serving step around decode
+(append, e4m3 and block-scaled 8-bit caches, page selection, e4m3 norms). There is no
 fallback: if the extension is not built these functions raise RuntimeError.
 """
 
@@ -154,6 +155,126 @@ def paged_decode_attention_cascade(
         q.shape[-1] ** -0.5 if scale is None else scale, k_scale, v_scale,
     )
     return out
+
+
+def rms_norm_fp8(
+    x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group_size: int = 0
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm with an e4m3 output: (codes, scales), y = codes * scales. ``group_size`` columns share
+    a scale (0: a whole row); codes are torch.float8_e4m3fn in x's shape, scales float32
+    [..., ceil(hidden / group_size)]. A scale is its group's largest magnitude / 448."""
+    _require()
+    if not torch.compiler.is_compiling():
+        return _C.rms_norm_fp8(x, weight, eps, group_size)
+    codes, scales = _fp8_outputs(x, group_size)
+    torch.ops.kernel_lab.rms_norm_fp8(codes, scales, x, weight, eps, group_size)
+    return codes, scales
+
+
+def fused_add_rms_norm_fp8(
+    x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group_size: int = 0
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Functional form: (codes, scales, new_residual) of x + residual, ``residual`` left untouched.
+    Call torch.ops.kernel_lab.fused_add_rms_norm_fp8 with residual_out = residual to update in place."""
+    _require()
+    if not torch.compiler.is_compiling():
+        return _C.fused_add_rms_norm_fp8(x, residual, weight, eps, group_size)
+    codes, scales = _fp8_outputs(x, group_size)
+    new_residual = torch.empty_like(x, memory_format=torch.contiguous_format)
+    torch.ops.kernel_lab.fused_add_rms_norm_fp8(
+        codes, scales, new_residual, x, residual.contiguous(), weight, eps, group_size
+    )
+    return codes, scales, new_residual
+
+
+def _fp8_outputs(x: torch.Tensor, group_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+    groups = 1 if group_size == 0 else -(-x.shape[-1] // group_size)
+    codes = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    return codes, torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device)
+
+
+def paged_kv_append_block8(
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    k_new: torch.Tensor,
+    v_new: torch.Tensor,
+    block_table: torch.Tensor,
+    positions: torch.Tensor,
+    indptr: torch.Tensor | None = None,
+    k_bounds: torch.Tensor | None = None,
+) -> None:
+    """Append to an 8-bit cache (float8_e4m3fn or int8, [num_pages, page_size, num_kv_heads, head_dim],
+    any order of pages, tokens and heads in memory) with a float32 scale for each page and KV head
+    (in place). Sequence b's new rows ``indptr[b]`` .. ``indptr[b + 1] - 1`` (one row per sequence
+    without ``indptr``) take the positions from ``positions[b]`` on (negative skips the sequence). A page's
+    scale covers its largest element: it starts with the page's first token and grows when a later
+    one needs it, the page's earlier codes being rounded again. ``k_bounds`` (int8 [num_pages,
+    num_kv_heads, 2, head_dim]) keeps each touched page's per-channel key extremes for
+    :func:`paged_block_select`. Two sequences must not append to one page. Page ids outside the pool
+    are skipped and reported by :func:`decode_status`."""
+    _require()
+    append = torch.ops.kernel_lab.paged_kv_append_block8 if torch.compiler.is_compiling() else _C.paged_kv_append_block8
+    append(
+        k_cache, v_cache, k_scale, v_scale, k_bounds, k_new, v_new, block_table, positions, indptr
+    )
+
+
+def paged_decode_attention_block8(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    scale: float | None = None,
+    selected: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Decode attention over an 8-bit cache with a scale for each page and KV head: K = code *
+    k_scale[page, h], V = code * v_scale[page, h]. q is fp16 or bf16. With ``selected`` (int32 [batch,
+    num_kv_heads, n], :func:`paged_block_select`) KV head h of sequence b reads only the pages in those
+    columns of its block-table row (each at most once; -1 selects nothing)."""
+    _require()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if not torch.compiler.is_compiling():
+        return _C.paged_decode_attention_block8(
+            q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected
+        )
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    torch.ops.kernel_lab.paged_decode_attention_block8(
+        out, q.contiguous(), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected
+    )
+    return out
+
+
+def paged_block_select(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    k_bounds: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    num_selected: int,
+    sink_pages: int = 1,
+    recent_pages: int = 1,
+) -> torch.Tensor:
+    """The pages a decode step should read: for each sequence and KV head the ``num_selected``
+    block-table columns (int32 [batch, num_kv_heads, num_selected], ascending, then -1) whose key
+    bounds allow the largest scores, the first ``sink_pages`` and the last ``recent_pages`` always among
+    them. Scores are sums of whole numbers (q rounded to int8 per head), ties go to the lower column:
+    the choice is the same on every run and rank."""
+    _require()
+    if not torch.compiler.is_compiling():
+        return _C.paged_block_select(
+            q, k_cache, k_scale, k_bounds, block_table, seq_lens, num_selected, sink_pages, recent_pages
+        )
+    selected = torch.empty((q.shape[0], k_cache.shape[2], num_selected), dtype=torch.int32, device=q.device)
+    torch.ops.kernel_lab.paged_block_select(
+        selected, q.contiguous(), k_cache, k_scale, k_bounds, block_table, seq_lens, sink_pages, recent_pages
+    )
+    return selected
 
 
 def decode_status(clear: bool = False) -> int:
