@@ -56,6 +56,12 @@ struct Int8Code {
 
 __device__ __forceinline__ float reciprocal_scale(float scale) { return scale >= kLeastScale ? 1.0f / scale : 0.0f; }
 
+// 16 bytes from global to shared memory, asynchronously (both 16-byte aligned).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Host side: lets `kernel` use up to `bytes` of dynamic shared memory on the current device, asked
 // of the runtime once for each kernel and device.
 template <typename... Params>

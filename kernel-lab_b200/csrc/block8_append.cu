@@ -3,9 +3,9 @@
 //
 // The work falls into units of one page, KV head and tensor: the largest magnitude of the page's
 // new elements gives the scale, so a unit is a reduction and then an elementwise pass over the same
-// elements. A team of one warp (pages of up to 2048 elements a head) or of four warps takes a unit,
-// keeps its new elements in registers between the two and so reads them once; larger pages re-read
-// theirs from L2. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
+// elements. A team of one warp (pages of up to 2048 elements a head) or of four warps takes a unit
+// and copies its new elements to shared memory, all in flight at once and without registers, so that
+// it reads them once; larger pages re-read theirs from L2. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
 // latency-bound for single tokens, where the chain is indptr / position, block-table entry, new row.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
@@ -15,9 +15,13 @@
 // Bounds: rounding is monotone, so the least and largest code of a channel are the codes of the
 // least and largest scaled element, and only those two are rounded; they are combined over the
 // team's tokens through shared memory.
+//
+// 16-bit elements are compared two at a time as they are (packed maximum of magnitudes, packed
+// extremes), which is exact; only a unit that holds a NaN or an infinity takes the element-wise path.
 #include <algorithm>
 #include <cfloat>
 #include <cstdint>
+#include <type_traits>
 
 #include <cuda_runtime.h>
 
@@ -73,9 +77,106 @@ struct NewPack {
     if constexpr (VEC == 8) {
       constexpr int kWords = sizeof(E) * 8 / 16;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(v)[i] = reinterpret_cast<const uint4*>(p)[i];
     } else {
       v[0] = *p;
+    }
+  }
+  __device__ __forceinline__ void unpack(float (&f)[VEC]) const {
+    if constexpr (VEC == 8 && sizeof(E) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 p = Storage<E>::unpack2(reinterpret_cast<const uint32_t*>(v)[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) f[j] = Storage<E>::load(v[j]);
+    }
+  }
+};
+
+// Extremes of packs element by element and the largest magnitude, in the element type (exact). NaN
+// and infinities show in the magnitude (not finite), after which the extremes are not used.
+template <typename E, int VEC>
+struct PackExtremes {
+  static constexpr bool kPairs = VEC == 8 && sizeof(E) == 2;
+  using Pair = std::conditional_t<std::is_same_v<E, __half>, __half2, __nv_bfloat162>;
+  static constexpr int kN = kPairs ? 4 : VEC;
+  using Unit = std::conditional_t<kPairs, Pair, float>;
+  Unit lo[kN], hi[kN];
+  __device__ __forceinline__ void reset() {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if constexpr (std::is_same_v<Unit, __half2>) {
+        lo[i] = __half2half2(__ushort_as_half(0x7c00)), hi[i] = __half2half2(__ushort_as_half(0xfc00));
+      } else if constexpr (std::is_same_v<Unit, __nv_bfloat162>) {
+        lo[i] = __bfloat162bfloat162(__ushort_as_bfloat16(0x7f80));
+        hi[i] = __bfloat162bfloat162(__ushort_as_bfloat16(0xff80));
+      } else {
+        lo[i] = INFINITY, hi[i] = -INFINITY;
+      }
+    }
+  }
+  __device__ __forceinline__ void add(const NewPack<E, VEC>& p) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if constexpr (kPairs) {
+        const Unit u = reinterpret_cast<const Unit*>(p.v)[i];
+        lo[i] = __hmin2(lo[i], u);
+        hi[i] = __hmax2(hi[i], u);
+      } else {
+        const float u = Storage<E>::load(p.v[i]);
+        lo[i] = fminf(lo[i], u);
+        hi[i] = fmaxf(hi[i], u);
+      }
+    }
+  }
+  __device__ __forceinline__ void get(float (&l)[VEC], float (&h)[VEC]) const {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      if constexpr (kPairs) {
+        const float2 a = Storage<E>::unpack2(reinterpret_cast<const uint32_t*>(lo)[i]);
+        const float2 b = Storage<E>::unpack2(reinterpret_cast<const uint32_t*>(hi)[i]);
+        l[2 * i] = a.x, l[2 * i + 1] = a.y;
+        h[2 * i] = b.x, h[2 * i + 1] = b.y;
+      } else {
+        l[i] = lo[i], h[i] = hi[i];
+      }
+    }
+  }
+};
+
+template <typename E, int VEC>
+struct Magnitude {
+  using X = PackExtremes<E, VEC>;
+  typename X::Unit top;
+  __device__ __forceinline__ void reset() {
+    if constexpr (X::kPairs) {
+      const uint32_t zero = 0;
+      top = *reinterpret_cast<const typename X::Unit*>(&zero);
+    } else {
+      top = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void add(const NewPack<E, VEC>& p) {
+#pragma unroll
+    for (int i = 0; i < X::kN; ++i) {
+      if constexpr (X::kPairs) {
+        top = __hmax2_nan(top, __habs2(reinterpret_cast<const typename X::Unit*>(p.v)[i]));
+      } else {
+        const float f = fabsf(Storage<E>::load(p.v[i]));
+        top = f > top || f != f ? f : top;  // NaN stays
+      }
+    }
+  }
+  __device__ __forceinline__ float get() const {  // NaN or infinity if an element was
+    if constexpr (X::kPairs) {
+      const float2 p = Storage<E>::unpack2(*reinterpret_cast<const uint32_t*>(&top));
+      return p.x != p.x ? p.x : p.y != p.y ? p.y : fmaxf(p.x, p.y);
+    } else {
+      return top;
     }
   }
 };
@@ -104,6 +205,7 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, float (&y)[VEC]) {
   }
 }
 
+// Extremes of scaled elements; NaN counts as 0.
 template <int VEC>
 struct Extremes {
   float lo[VEC], hi[VEC];
@@ -129,6 +231,12 @@ __device__ __forceinline__ void team_sync() {
 }
 
 template <int TEAM>
+__device__ __forceinline__ bool team_all(bool v) {
+  if constexpr (TEAM == 32) return __all_sync(0xffffffffu, v);
+  else return __syncthreads_and(v);
+}
+
+template <int TEAM>
 __device__ __forceinline__ float team_max(float v, float* red) {
   v = warp_allreduce_max(v);
   if constexpr (TEAM > 32) {
@@ -144,8 +252,10 @@ __device__ __forceinline__ float team_max(float v, float* red) {
 template <typename E, typename Code, int VEC, int TEAM>
 __global__ void __launch_bounds__(kBlock8AppendThreads) kv_append_block8(const Block8AppendArgs a) {
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
-  constexpr int kKeep = VEC == 8 ? 8 : 1;  // packs a thread keeps in registers
-  __shared__ float s_ext[kTeams][2][TEAM * VEC];
+  using Pack = NewPack<E, VEC>;
+  constexpr int kKeep = VEC == 8 ? 8 : 1;  // packs a thread keeps in shared memory
+  __shared__ __align__(16) Pack s_new[kTeams][kKeep][TEAM];
+  __shared__ __align__(16) float s_ext[kTeams][2][TEAM * VEC];
   __shared__ float s_red[kBlock8AppendThreads / 32];
   const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
   const int h = blockIdx.y * kTeams + team;
@@ -153,9 +263,6 @@ __global__ void __launch_bounds__(kBlock8AppendThreads) kv_append_block8(const B
   allow_next_grid();
   if (h >= a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
   const bool keys = blockIdx.z == 0;
-  const E* rows = static_cast<const E*>(keys ? a.k_new : a.v_new) + static_cast<int64_t>(h) * a.head_dim;
-  uint8_t* cache = (keys ? a.k_cache : a.v_cache) + h * a.head_stride;
-  float* scales = (keys ? a.k_scale : a.v_scale) + h;
   const bool bounds = keys && a.k_bounds != nullptr;
 
   const int units = a.head_dim / VEC;
@@ -188,49 +295,64 @@ __global__ void __launch_bounds__(kBlock8AppendThreads) kv_append_block8(const B
     const int64_t first = t;
     t += n;
     if (first != begin && s0 != 0) continue;  // not the sequence's first token in this page
+
+    // The new packs first (they need no page), then the page and its present scale.
+    const E* src = static_cast<const E*>(keys ? a.k_new : a.v_new) + first * a.new_stride +
+                   static_cast<int64_t>(h) * a.head_dim + my_unit * VEC;
+    const bool kept = VEC == 8 && units <= across && n <= kKeep * down;  // they fit in shared memory
+    if constexpr (VEC == 8) {
+      if (kept && active) {
+        for (int i = 0, tok = my_tok; tok < n; ++i, tok += down) {
+#pragma unroll
+          for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) {
+            cp_async16(smem_u32(&s_new[team][i][tid]) + k, reinterpret_cast<const uint8_t*>(src + tok * a.new_stride) + k);
+          }
+        }
+      }
+    }
     int64_t page = -1;
     if (col < a.max_pages) page = a.block_table[b * a.bt_stride + col];
     if (page < 0 || page >= a.num_pages) {
       if (tid == 0 && a.status) atomicOr(a.status, kStatusBadPage);
+      cp_async_wait_all();  // the next unit's copies may take the same places
       continue;
     }
-
-    float* scale_at = scales + page * a.num_kv_heads;
+    float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
     const float old = s0 > 0 ? *scale_at : 0.0f;
-    const E* src = rows + first * a.new_stride;
-    uint8_t* dst = cache + page * a.page_stride;
-    const auto for_new = [&](int c0, auto&& f) {  // f(pack, token) over this thread's new packs
+    uint8_t* dst = (keys ? a.k_cache : a.v_cache) + page * a.page_stride + h * a.head_stride + my_unit * VEC;
+
+    cp_async_wait_all();  // each thread reads back what it copied itself
+
+    // f(pack, token) over this thread's new packs of channel units c0, c0 + 1, ...
+    const auto for_new = [&](int c0, auto&& f) {
       if (!active || c0 + my_unit >= units) return;
-      for (int tok = my_tok; tok < n; tok += down) {
-        NewPack<E, VEC> p;
-        p.load(src + tok * a.new_stride + (c0 + my_unit) * VEC);
+      const E* at = kept ? s_new[team][0][tid].v : src + my_tok * a.new_stride + c0 * VEC;
+      const int64_t step = kept ? static_cast<int64_t>(TEAM) * VEC : down * a.new_stride;
+#pragma unroll 2
+      for (int tok = my_tok; tok < n; tok += down, at += step) {
+        Pack p;
+        p.load(at);
         f(p, tok);
       }
     };
 
-    // The largest finite magnitude, keeping the packs when they fit in registers.
-    const bool kept = units <= across && n <= kKeep * down;
-    NewPack<E, VEC> keep[kKeep];
-    float amax = 0.0f;
-    const auto magnitude = [&](const NewPack<E, VEC>& p) {
+    Magnitude<E, VEC> mag;
+    mag.reset();
+    for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p, int) { mag.add(p); });
+    float amax = mag.get();
+    const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
+    if (!plain) {
+      amax = 0.0f;
+      for (int c0 = 0; c0 < units; c0 += across) {
+        for_new(c0, [&](const Pack& p, int) {
+          float f[VEC];
+          p.unpack(f);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float f = fabsf(Storage<E>::load(p.v[j]));
-        if (f <= FLT_MAX) amax = fmaxf(amax, f);
+          for (int j = 0; j < VEC; ++j) {
+            if (fabsf(f[j]) <= FLT_MAX) amax = fmaxf(amax, fabsf(f[j]));
+          }
+        });
       }
-    };
-    if (kept) {
-#pragma unroll
-      for (int i = 0; i < kKeep; ++i) {
-        const int tok = my_tok + i * down;
-        if (active && tok < n) keep[i].load(src + tok * a.new_stride + my_unit * VEC);
-      }
-#pragma unroll
-      for (int i = 0; i < kKeep; ++i) {
-        if (active && my_tok + i * down < n) magnitude(keep[i]);
-      }
-    } else {
-      for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const NewPack<E, VEC>& p, int) { magnitude(p); });
     }
     amax = team_max<TEAM>(amax, s_red);
     const float scale = fmaxf(old, Code::scale_for(amax));
@@ -242,55 +364,68 @@ __global__ void __launch_bounds__(kBlock8AppendThreads) kv_append_block8(const B
 
     for (int c0 = 0; c0 < units; c0 += across) {
       Extremes<VEC> ext;
-      ext.reset();
-      const int unit = c0 + my_unit;
-      const auto put = [&](const NewPack<E, VEC>& p, int tok) {
-        float y[VEC];
+      {
+        PackExtremes<E, VEC> raw;
+        raw.reset();
+        for_new(c0, [&](const Pack& p, int tok) {
+          float y[VEC];
+          p.unpack(y);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) y[j] = Storage<E>::load(p.v[j]) * inv;
-        store_codes<Code, VEC>(dst + (s0 + tok) * a.token_stride + unit * VEC, y);
-        if (bounds) ext.add(y);
-      };
-      if (kept) {
-#pragma unroll
-        for (int i = 0; i < kKeep; ++i) {
-          const int tok = my_tok + i * down;
-          if (active && tok < n) put(keep[i], tok);
-        }
-      } else {
-        for_new(c0, put);
+          for (int j = 0; j < VEC; ++j) y[j] *= inv;
+          store_codes<Code, VEC>(dst + c0 * VEC + (s0 + tok) * a.token_stride, y);
+          if (bounds) raw.add(p);
+        });
+        raw.get(ext.lo, ext.hi);
       }
-      if ((grew || bounds) && active && unit < units) {
-#pragma unroll 4
-        for (int tok = my_tok; tok < s0; tok += down) {
-          uint8_t* at = dst + tok * a.token_stride + unit * VEC;
+      const bool had = plain && active && my_tok < n;  // this thread's own extremes, to be scaled
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        ext.lo[j] = had ? ext.lo[j] * inv : FLT_MAX;
+        ext.hi[j] = had ? ext.hi[j] * inv : -FLT_MAX;
+      }
+      // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
+      const auto for_codes = [&](int from, int to, float by, bool write) {
+        if (!active || c0 + my_unit >= units) return;
+#pragma unroll 2
+        for (int tok = from + my_tok; tok < to; tok += down) {
+          uint8_t* at = dst + c0 * VEC + tok * a.token_stride;
           float y[VEC];
           load_codes<Code, VEC>(at, y);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] *= ratio;
-          if (grew) store_codes<Code, VEC>(at, y);
+          for (int j = 0; j < VEC; ++j) y[j] *= by;
+          if (write) store_codes<Code, VEC>(at, y);
           if (bounds) ext.add(y);
         }
+      };
+      if (grew || bounds) for_codes(0, s0, ratio, grew);
+      if (bounds && !plain) {
+        team_sync<TEAM>();
+        for_codes(s0, s0 + n, 1.0f, false);
       }
       if (bounds) {
         float* lo = s_ext[team][0];
         float* hi = s_ext[team][1];
+        const int width = across * VEC;
         team_sync<TEAM>();
+        if (active) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) lo[j * TEAM + tid] = ext.lo[j], hi[j * TEAM + tid] = ext.hi[j];
+          for (int j = 0; j < VEC; ++j) {
+            lo[my_tok * width + my_unit * VEC + j] = ext.lo[j];
+            hi[my_tok * width + my_unit * VEC + j] = ext.hi[j];
+          }
+        }
         team_sync<TEAM>();
-        int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim;
-        const int here = min(across, units - c0);
-        for (int i = tid; i < here * VEC; i += TEAM) {
-          const int u = i / VEC, j = i % VEC;
+        int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim + c0 * VEC;
+        const int here = min(width, a.head_dim - c0 * VEC);
+        for (int i = tid; i < here; i += TEAM) {
           float l = FLT_MAX, m = -FLT_MAX;
           for (int k = 0; k < down; ++k) {
-            l = fminf(l, lo[j * TEAM + k * across + u]);
-            m = fmaxf(m, hi[j * TEAM + k * across + u]);
+            l = fminf(l, lo[k * width + i]);
+            m = fmaxf(m, hi[k * width + i]);
           }
-          const float unit_size = static_cast<float>(Code::kBoundUnit);
-          out[c0 * VEC + i] = static_cast<int8_t>(floorf(Code::value(Code::code(l)) / unit_size));
-          out[a.head_dim + c0 * VEC + i] = static_cast<int8_t>(ceilf(Code::value(Code::code(m)) / unit_size));
+          constexpr float kPerUnit = 1.0f / Code::kBoundUnit;  // a power of two
+          out[i] = static_cast<int8_t>(floorf(Code::value(Code::code(l)) * kPerUnit));
+          out[a.head_dim + i] = static_cast<int8_t>(ceilf(Code::value(Code::code(m)) * kPerUnit));
         }
       }
     }

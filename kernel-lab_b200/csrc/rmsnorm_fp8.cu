@@ -5,8 +5,8 @@
 //   a  = max |y| over a group of columns (NaN ignored): a whole row, or group_size columns
 //   scale = a / 448,  code = e4m3(y * 448 / a), nearest-even, saturating
 // rstd is common to y and a, so the codes need none of it: with t = r' * w (exact in fp32 for 16-bit
-// types) and b = max |t|, code = e4m3(t * (448 / b)) and a = b * rstd. That is two roundings an
-// element, and one product. A group whose a or b is below 2^-100 (448 / b would overflow) gets scale
+// types) and b = max |t|, code = e4m3(t * (448 / b)) and a = b * rstd: one product and few roundings
+// an element. A group whose a or b is below 2^-100 (448 / b would overflow) gets scale
 // 0 and codes 0; a row whose rstd is NaN or infinite gets NaN codes, as its y are.
 //
 // HBM-bound: x, residual in; residual out, one byte an element and the scales out. As in the 16-bit
@@ -30,15 +30,35 @@ namespace klb {
 namespace {
 
 constexpr float kE4m3Max = 448.0f;
+constexpr float kPerE4m3Max = 1.0f / 448.0f;
 constexpr float kLeastAmax = 0x1p-100f;  // below it a group's scale is 0
 
+// 16 bytes of a row as floats, and back with one rounding (16-bit types two at a time).
 template <typename T>
 struct RowPack {
   static constexpr int N = 16 / sizeof(T);
-  union {
-    uint4 raw;
-    T v[N];
-  };
+  uint4 raw;
+  __device__ __forceinline__ void unpack(float (&f)[N]) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 8) {
+        const float2 p = Storage<T>::unpack2(w[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+      } else {
+        f[i] = __uint_as_float(w[i]);
+      }
+    }
+  }
+  __device__ __forceinline__ void pack(const float (&f)[N]) {
+    if constexpr (N == 8) {
+      raw = make_uint4(Storage<T>::pack2(f[0], f[1]), Storage<T>::pack2(f[2], f[3]), Storage<T>::pack2(f[4], f[5]),
+                       Storage<T>::pack2(f[6], f[7]));
+    } else {
+      raw = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    }
+  }
 };
 
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
@@ -53,8 +73,8 @@ struct GroupScale {
   __device__ __forceinline__ GroupScale(float b, float rstd) {
     const float a = b * rstd;
     const bool some = a >= kLeastAmax && b >= kLeastAmax;  // false for NaN too
-    inv = some ? kE4m3Max / b : 0.0f * rstd;
-    scale = some ? a / kE4m3Max : 0.0f;
+    inv = some ? kE4m3Max * __frcp_rn(b) : 0.0f * rstd;
+    scale = some ? a * kPerE4m3Max : 0.0f;
   }
 };
 
@@ -119,22 +139,26 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_row_regs(const NormFp8Args g,
     }
   }
 
+  // a[] becomes the row, w[] is read again for the codes (t is not kept: it would double the registers).
   float ss = 0.0f, top = 0.0f;
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int pk = threadIdx.x + i * blockDim.x;
+    float f[P::N], v[P::N];
+    a[i].unpack(f);
     if constexpr (RES) {
+      r[i].unpack(v);
 #pragma unroll
-      for (int j = 0; j < P::N; ++j) {
-        a[i].v[j] = Storage<T>::store(Storage<T>::load(a[i].v[j]) + Storage<T>::load(r[i].v[j]));
-      }
+      for (int j = 0; j < P::N; ++j) f[j] += v[j];
+      a[i].pack(f);
+      a[i].unpack(f);
       if (pk < packs) ro[pk] = a[i].raw;
     }
+    w[i].unpack(v);
 #pragma unroll
     for (int j = 0; j < P::N; ++j) {
-      const float f = Storage<T>::load(a[i].v[j]);
-      ss = fmaf(f, f, ss);
-      top = fmaxf(top, fabsf(f * Storage<T>::load(w[i].v[j])));
+      ss = fmaf(f[j], f[j], ss);
+      if (lanes == 0) top = fmaxf(top, fabsf(f[j] * v[j]));
     }
   }
 
@@ -147,11 +171,13 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_row_regs(const NormFp8Args g,
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int pk = threadIdx.x + i * blockDim.x;
-    float t[P::N];
+    float t[P::N], v[P::N];
+    a[i].unpack(t);
+    w[i].unpack(v);
     float b = 0.0f;
 #pragma unroll
     for (int j = 0; j < P::N; ++j) {
-      t[j] = Storage<T>::load(a[i].v[j]) * Storage<T>::load(w[i].v[j]);
+      t[j] *= v[j];
       b = fmaxf(b, fabsf(t[j]));
     }
     float inv = whole.inv;
