@@ -41,7 +41,7 @@ enum {
  * group of group_size columns (0: the whole row; the last group may be short)
  *   a = max |y|, scale = a / 448, code = e4m3(y * 448 / a) (nearest-even, saturating; NaN stays NaN),
  * or scale = 0 and codes of 0 where a or max |r * weight| is below 2^-100. The codes are formed from
- * r * weight, which has to fit fp32.
+ * r * weight, whose magnitude has to stay below 2^126.
  *   codes   [rows, hidden] bytes            scales   [rows, ceil(hidden / group_size)] fp32
  * x rows are x_row_stride elements apart; the other tensors are contiguous. rows == 0 is a no-op.
  */

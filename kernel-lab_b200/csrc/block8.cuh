@@ -29,10 +29,15 @@ struct E4m3Code {
   static __device__ __forceinline__ uint32_t code(float v) {
     return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
   }
+  // code() of four at once.
   static __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
     return lo | (hi << 16);
+  }
+  // code4() for numbers within the codes' range.
+  static __device__ __forceinline__ uint32_t code4_in_range(float a, float b, float c, float d) {
+    return code4(a, b, c, d);
   }
 };
 
@@ -52,6 +57,14 @@ struct Int8Code {
   static __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
     return code(a) | (code(b) << 8) | (code(c) << 16) | (code(d) << 24);
   }
+  // Adding 1.5 * 2^23 rounds to a whole number (nearest even) and leaves it in the low bits; never
+  // fused with the product that made the number, which would round once instead of twice.
+  static __device__ __forceinline__ uint32_t code4_in_range(float a, float b, float c, float d) {
+    constexpr float kRound = 12582912.0f;
+    const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(a, kRound)), __float_as_uint(__fadd_rn(b, kRound)), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(c, kRound)), __float_as_uint(__fadd_rn(d, kRound)), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
+  }
 };
 
 __device__ __forceinline__ float reciprocal_scale(float scale) { return scale >= kLeastScale ? 1.0f / scale : 0.0f; }
@@ -59,6 +72,9 @@ __device__ __forceinline__ float reciprocal_scale(float scale) { return scale >=
 // 16 bytes from global to shared memory, asynchronously (both 16-byte aligned).
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 

@@ -3,9 +3,10 @@
 //
 // The work falls into units of one page, KV head and tensor: the largest magnitude of the page's
 // new elements gives the scale, so a unit is a reduction and then an elementwise pass over the same
-// elements. A team of one warp (pages of up to 2048 elements a head) or of four warps takes a unit
+// elements. A team of one warp (pages of up to 4096 elements a head) or of four warps takes a unit
 // and copies its new elements to shared memory, all in flight at once and without registers, so that
-// it reads them once; larger pages re-read theirs from L2. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
+// it reads them once; larger pages re-read theirs from L2. A team takes several heads of a page in turn
+// where the call is large: finding the page costs about as many instructions as a unit's elements. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
 // latency-bound for single tokens, where the chain is indptr / position, block-table entry, new row.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
@@ -52,6 +53,9 @@ struct Block8AppendArgs {
   int64_t tokens;
   int batch, num_kv_heads, head_dim, page_size, max_pages;
   int window;              // new tokens a team looks at
+  int across, down;        // channel units (of VEC) side by side in a team, tokens beside them
+  uint32_t per_across;     // 65536 / across + 1: thread / across without a division
+  int keep;                // packs a thread can keep in shared memory
 };
 
 // Last b with indptr[b] <= t, by all lanes of a warp (32 samples a step).
@@ -68,6 +72,52 @@ __device__ __forceinline__ int sequence_of(const int32_t* indptr, int batch, int
   }
   return lo;
 }
+
+// Which sequence a new row belongs to, its rows and its first position. For up to 127 sequences each
+// warp reads the whole of indptr and positions at once (one latency, not one for each step of a search).
+struct Sequences {
+  static constexpr int kWords = 4;
+  int ptr[kWords], pos[kWords];
+  bool whole;
+  __device__ __forceinline__ void read(const Block8AppendArgs& a) {
+    whole = a.indptr != nullptr && a.batch < 32 * kWords;
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      const int i = 32 * k + lane;
+      ptr[k] = whole && i <= a.batch ? a.indptr[i] : INT32_MAX;
+      pos[k] = whole && i < a.batch ? a.positions[i] : -1;
+    }
+  }
+  __device__ __forceinline__ int pick(const int (&v)[kWords], int i) const {
+    const int w = i >> 5;
+    const int got = w == 0 ? v[0] : w == 1 ? v[1] : w == 2 ? v[2] : v[3];
+    return __shfl_sync(0xffffffffu, got, i & 31);
+  }
+  __device__ __forceinline__ void find(const Block8AppendArgs& a, int64_t t, int& b, int64_t& begin, int64_t& end,
+                                       int& start) const {
+    if (whole) {
+      int count = 0;
+#pragma unroll
+      for (int k = 0; k < kWords; ++k) count += __popc(__ballot_sync(0xffffffffu, ptr[k] <= t));
+      b = max(0, min(count, a.batch) - 1);
+      begin = pick(ptr, b);
+      end = pick(ptr, b + 1);
+      start = pick(pos, b);
+    } else if (a.indptr) {
+      b = sequence_of(a.indptr, a.batch, t);
+      begin = a.indptr[b];
+      end = a.indptr[b + 1];
+      start = a.positions[b];
+    } else {
+      b = static_cast<int>(t);
+      begin = t;
+      end = t + 1;
+      start = a.positions[b];
+    }
+    end = min(end, a.tokens);
+  }
+};
 
 // VEC consecutive elements of a new row (VEC 8: 16-byte aligned), as loaded.
 template <typename E, int VEC>
@@ -182,10 +232,17 @@ struct Magnitude {
 };
 
 template <typename Code, int VEC>
-__device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[VEC]) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&y)[VEC], bool in_range) {
   if constexpr (VEC == 8) {
-    *reinterpret_cast<uint2*>(p) =
-        make_uint2(Code::code4(y[0], y[1], y[2], y[3]), Code::code4(y[4], y[5], y[6], y[7]));
+    uint2 w;
+    if (in_range) {
+      w.x = Code::code4_in_range(y[0], y[1], y[2], y[3]);
+      w.y = Code::code4_in_range(y[4], y[5], y[6], y[7]);
+    } else {
+      w.x = Code::code4(y[0], y[1], y[2], y[3]);
+      w.y = Code::code4(y[4], y[5], y[6], y[7]);
+    }
+    *reinterpret_cast<uint2*>(p) = w;
   } else {
     *p = static_cast<uint8_t>(Code::code(y[0]));
   }
@@ -230,6 +287,12 @@ __device__ __forceinline__ void team_sync() {
   if constexpr (TEAM == 32) __syncwarp(); else __syncthreads();
 }
 
+template <typename E, int VEC, int TEAM>
+__host__ __device__ constexpr int team_bytes(int keep) {
+  const int codes = keep * VEC, extremes = 2 * VEC * static_cast<int>(sizeof(float));
+  return TEAM * (keep * static_cast<int>(sizeof(E)) * VEC + (codes > extremes ? codes : extremes));
+}
+
 template <int TEAM>
 __device__ __forceinline__ bool team_all(bool v) {
   if constexpr (TEAM == 32) return __all_sync(0xffffffffu, v);
@@ -250,184 +313,223 @@ __device__ __forceinline__ float team_max(float v, float* red) {
 }
 
 template <typename E, typename Code, int VEC, int TEAM>
-__global__ void __launch_bounds__(kBlock8AppendThreads) kv_append_block8(const Block8AppendArgs a) {
+__global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(const Block8AppendArgs a) {
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
   using Pack = NewPack<E, VEC>;
-  constexpr int kKeep = VEC == 8 ? 8 : 1;  // packs a thread keeps in shared memory
-  __shared__ __align__(16) Pack s_new[kTeams][kKeep][TEAM];
-  __shared__ __align__(16) float s_ext[kTeams][2][TEAM * VEC];
+  // Per team: the kept packs [keep][TEAM]; then a page's present codes (VEC bytes a thread and row)
+  // and, after those are used, the threads' extremes [2][TEAM * VEC].
+  extern __shared__ __align__(16) uint8_t s_dyn[];
   __shared__ float s_red[kBlock8AppendThreads / 32];
   const int team = threadIdx.x / TEAM, tid = threadIdx.x % TEAM;
-  const int h = blockIdx.y * kTeams + team;
+  Pack* const s_new = reinterpret_cast<Pack*>(s_dyn + team * team_bytes<E, VEC, TEAM>(a.keep));
+  uint8_t* const s_codes = reinterpret_cast<uint8_t*>(s_new + a.keep * TEAM);
+  float* const s_lo = reinterpret_cast<float*>(s_codes);
+  float* const s_hi = s_lo + TEAM * VEC;
   wait_prior_grid();
   allow_next_grid();
-  if (h >= a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
+  const int first_head = blockIdx.y * kTeams + team;
+  if (first_head >= a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
   const bool keys = blockIdx.z == 0;
   const bool bounds = keys && a.k_bounds != nullptr;
 
   const int units = a.head_dim / VEC;
-  const int across = min(units, TEAM), down = TEAM / across;
-  const int my_tok = tid / across, my_unit = tid % across;
+  const int across = a.across, down = a.down;
+  const int my_tok = static_cast<int>((static_cast<uint32_t>(tid) * a.per_across) >> 16);
+  const int my_unit = tid - my_tok * across;
   const bool active = my_tok < down;
+  const int64_t src_step = down * a.new_stride, dst_step = down * a.token_stride;
+  const auto barrier = [] { team_sync<TEAM>(); };
 
+  Sequences seqs;
+  seqs.read(a);
   const int64_t w1 = min(a.tokens, (static_cast<int64_t>(blockIdx.x) + 1) * a.window);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * a.window; t < w1;) {
-    int64_t begin = t, end = t + 1;
-    int b = static_cast<int>(t);
-    if (a.indptr) {
-      b = sequence_of(a.indptr, a.batch, t);
-      begin = a.indptr[b];
-      end = min(static_cast<int64_t>(a.indptr[b + 1]), a.tokens);
-    }
+    int64_t begin, end;
+    int b, start;
+    seqs.find(a, t, b, begin, end, start);
     if (t < begin || t >= end) {  // a row of no sequence
       ++t;
       continue;
     }
-    const int start = a.positions[b];
     if (start < 0) {
       t = end;
       continue;
     }
-    const int64_t pos = start + (t - begin);
-    const int64_t col = pos / a.page_size;
-    const int s0 = static_cast<int>(pos - col * a.page_size);
+    const uint32_t pos = static_cast<uint32_t>(start) + static_cast<uint32_t>(t - begin);  // below 2^32
+    const uint32_t col = pos / static_cast<uint32_t>(a.page_size);
+    const int s0 = static_cast<int>(pos - col * static_cast<uint32_t>(a.page_size));
     const int n = static_cast<int>(min(static_cast<int64_t>(a.page_size - s0), end - t));
     const int64_t first = t;
     t += n;
     if (first != begin && s0 != 0) continue;  // not the sequence's first token in this page
 
-    // The new packs first (they need no page), then the page and its present scale.
-    const E* src = static_cast<const E*>(keys ? a.k_new : a.v_new) + first * a.new_stride +
-                   static_cast<int64_t>(h) * a.head_dim + my_unit * VEC;
-    const bool kept = VEC == 8 && units <= across && n <= kKeep * down;  // they fit in shared memory
-    if constexpr (VEC == 8) {
-      if (kept && active) {
-        for (int i = 0, tok = my_tok; tok < n; ++i, tok += down) {
+    int64_t page = -1;
+    if (col < static_cast<uint32_t>(a.max_pages)) page = a.block_table[b * a.bt_stride + col];
+    const bool kept = VEC == 8 && units <= across && n <= a.keep * down;  // they fit in shared memory
+    const bool staged = VEC == 8 && units <= across && s0 <= a.keep * down;
+    const E* const row = static_cast<const E*>(keys ? a.k_new : a.v_new) + (first + my_tok) * a.new_stride + my_unit * VEC;
+
+    for (int h = first_head; h < a.num_kv_heads; h += gridDim.y * kTeams) {
+      const E* const src = row + h * a.head_dim;
+      // The new packs first (they need no page), then the page, its present scale and its codes.
+      if constexpr (VEC == 8) {
+        if (kept && active) {
+          const uint8_t* from = reinterpret_cast<const uint8_t*>(src);
+          uint32_t to = smem_u32(s_new + tid);
+#pragma unroll 4
+          for (int i = my_tok; i < n; i += down) {
 #pragma unroll
-          for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) {
-            cp_async16(smem_u32(&s_new[team][i][tid]) + k, reinterpret_cast<const uint8_t*>(src + tok * a.new_stride) + k);
+            for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) cp_async16(to + k, from + k);
+            from += src_step * static_cast<int64_t>(sizeof(E));
+            to += TEAM * sizeof(Pack);
           }
         }
       }
-    }
-    int64_t page = -1;
-    if (col < a.max_pages) page = a.block_table[b * a.bt_stride + col];
-    if (page < 0 || page >= a.num_pages) {
-      if (tid == 0 && a.status) atomicOr(a.status, kStatusBadPage);
-      cp_async_wait_all();  // the next unit's copies may take the same places
-      continue;
-    }
-    float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
-    const float old = s0 > 0 ? *scale_at : 0.0f;
-    uint8_t* dst = (keys ? a.k_cache : a.v_cache) + page * a.page_stride + h * a.head_stride + my_unit * VEC;
-
-    cp_async_wait_all();  // each thread reads back what it copied itself
-
-    // f(pack, token) over this thread's new packs of channel units c0, c0 + 1, ...
-    const auto for_new = [&](int c0, auto&& f) {
-      if (!active || c0 + my_unit >= units) return;
-      const E* at = kept ? s_new[team][0][tid].v : src + my_tok * a.new_stride + c0 * VEC;
-      const int64_t step = kept ? static_cast<int64_t>(TEAM) * VEC : down * a.new_stride;
-#pragma unroll 2
-      for (int tok = my_tok; tok < n; tok += down, at += step) {
-        Pack p;
-        p.load(at);
-        f(p, tok);
+      if (page < 0 || page >= a.num_pages) {
+        if (tid == 0 && a.status) atomicOr(a.status, kStatusBadPage);
+        cp_async_wait_all();  // the next unit's copies may take the same places
+        break;
       }
-    };
+      float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
+      const float old = s0 > 0 ? *scale_at : 0.0f;
+      // This thread's first slot; slot s0 + my_tok is its first new one.
+      uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + page * a.page_stride + h * a.head_stride +
+                           my_tok * a.token_stride + my_unit * VEC;
+      if (staged && active) {
+        const uint32_t to = smem_u32(s_codes) + tid * VEC;
+        const uint8_t* from = dst;
+        for (int i = 0; my_tok + i * down < s0; ++i, from += dst_step) cp_async8(to + i * (TEAM * VEC), from);
+      }
+      cp_async_wait_all();  // each thread reads back what it copied itself
 
-    Magnitude<E, VEC> mag;
-    mag.reset();
-    for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p, int) { mag.add(p); });
-    float amax = mag.get();
-    const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
-    if (!plain) {
-      amax = 0.0f;
-      for (int c0 = 0; c0 < units; c0 += across) {
-        for_new(c0, [&](const Pack& p, int) {
-          float f[VEC];
-          p.unpack(f);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            if (fabsf(f[j]) <= FLT_MAX) amax = fmaxf(amax, fabsf(f[j]));
-          }
-        });
-      }
-    }
-    amax = team_max<TEAM>(amax, s_red);
-    const float scale = fmaxf(old, Code::scale_for(amax));
-    const float inv = reciprocal_scale(scale);
-    const bool grew = s0 > 0 && scale > old;
-    const float ratio = grew ? old / scale : 1.0f;
-    team_sync<TEAM>();  // every thread has read the old scale
-    if (tid == 0) *scale_at = scale;
-
-    for (int c0 = 0; c0 < units; c0 += across) {
-      Extremes<VEC> ext;
-      {
-        PackExtremes<E, VEC> raw;
-        raw.reset();
-        for_new(c0, [&](const Pack& p, int tok) {
-          float y[VEC];
-          p.unpack(y);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] *= inv;
-          store_codes<Code, VEC>(dst + c0 * VEC + (s0 + tok) * a.token_stride, y);
-          if (bounds) raw.add(p);
-        });
-        raw.get(ext.lo, ext.hi);
-      }
-      const bool had = plain && active && my_tok < n;  // this thread's own extremes, to be scaled
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        ext.lo[j] = had ? ext.lo[j] * inv : FLT_MAX;
-        ext.hi[j] = had ? ext.hi[j] * inv : -FLT_MAX;
-      }
-      // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
-      const auto for_codes = [&](int from, int to, float by, bool write) {
+      // f(pack, index) over this thread's new packs of channel units c0, c0 + 1, ...
+      const auto for_new = [&](int c0, auto&& f) {
         if (!active || c0 + my_unit >= units) return;
+        if (kept) {
 #pragma unroll 2
-        for (int tok = from + my_tok; tok < to; tok += down) {
-          uint8_t* at = dst + c0 * VEC + tok * a.token_stride;
-          float y[VEC];
-          load_codes<Code, VEC>(at, y);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] *= by;
-          if (write) store_codes<Code, VEC>(at, y);
-          if (bounds) ext.add(y);
+          for (int i = 0; my_tok + i * down < n; ++i) f(s_new[i * TEAM + tid], i);
+          return;
+        }
+        const E* at = src + c0 * VEC;
+#pragma unroll 1
+        for (int i = 0; my_tok + i * down < n; ++i, at += src_step) {
+          Pack p;
+          p.load(at);
+          f(p, i);
         }
       };
-      if (grew || bounds) for_codes(0, s0, ratio, grew);
-      if (bounds && !plain) {
-        team_sync<TEAM>();
-        for_codes(s0, s0 + n, 1.0f, false);
-      }
-      if (bounds) {
-        float* lo = s_ext[team][0];
-        float* hi = s_ext[team][1];
-        const int width = across * VEC;
-        team_sync<TEAM>();
-        if (active) {
+
+      Magnitude<E, VEC> mag;
+      mag.reset();
+      for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p, int) { mag.add(p); });
+      float amax = mag.get();
+      const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
+      if (!plain) {
+        amax = 0.0f;
+        for (int c0 = 0; c0 < units; c0 += across) {
+          for_new(c0, [&](const Pack& p, int) {
+            float f[VEC];
+            p.unpack(f);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            lo[my_tok * width + my_unit * VEC + j] = ext.lo[j];
-            hi[my_tok * width + my_unit * VEC + j] = ext.hi[j];
-          }
-        }
-        team_sync<TEAM>();
-        int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim + c0 * VEC;
-        const int here = min(width, a.head_dim - c0 * VEC);
-        for (int i = tid; i < here; i += TEAM) {
-          float l = FLT_MAX, m = -FLT_MAX;
-          for (int k = 0; k < down; ++k) {
-            l = fminf(l, lo[k * width + i]);
-            m = fmaxf(m, hi[k * width + i]);
-          }
-          constexpr float kPerUnit = 1.0f / Code::kBoundUnit;  // a power of two
-          out[i] = static_cast<int8_t>(floorf(Code::value(Code::code(l)) * kPerUnit));
-          out[a.head_dim + i] = static_cast<int8_t>(ceilf(Code::value(Code::code(m)) * kPerUnit));
+            for (int j = 0; j < VEC; ++j) {
+              if (fabsf(f[j]) <= FLT_MAX) amax = fmaxf(amax, fabsf(f[j]));
+            }
+          });
         }
       }
+      amax = team_max<TEAM>(amax, s_red);
+      const float scale = fmaxf(old, Code::scale_for(amax));
+      const float inv = reciprocal_scale(scale);
+      const bool grew = s0 > 0 && scale > old;
+      const float ratio = grew ? old / scale : 1.0f;
+      barrier();  // every thread has read the old scale
+      if (tid == 0) *scale_at = scale;
+
+      for (int c0 = 0; c0 < units; c0 += across) {
+        Extremes<VEC> ext;
+        {
+          PackExtremes<E, VEC> raw;
+          raw.reset();
+          uint8_t* const put = dst + c0 * VEC + s0 * a.token_stride;
+          for_new(c0, [&](const Pack& p, int i) {
+            float y[VEC];
+            p.unpack(y);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] *= inv;
+            store_codes<Code, VEC>(put + i * dst_step, y, plain);  // plain: |y| is at most a rounding above kMax
+            if (bounds) raw.add(p);
+          });
+          raw.get(ext.lo, ext.hi);
+        }
+        const bool had = plain && active && my_tok < n;  // this thread's own extremes, to be scaled
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          ext.lo[j] = had ? ext.lo[j] * inv : FLT_MAX;
+          ext.hi[j] = had ? ext.hi[j] * inv : -FLT_MAX;
+        }
+        // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
+        const auto for_codes = [&](int count, uint8_t* at, float by, bool write, bool in_shared) {
+          if (!active || c0 + my_unit >= units) return;
+          const uint8_t* in = in_shared ? s_codes + tid * VEC : at;
+          const int64_t in_step = in_shared ? TEAM * VEC : dst_step;
+#pragma unroll 2
+          for (int tok = my_tok; tok < count; tok += down, at += dst_step, in += in_step) {
+            float y[VEC];
+            load_codes<Code, VEC>(in, y);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) y[j] *= by;
+            if (write) store_codes<Code, VEC>(at, y, false);
+            if (bounds) ext.add(y);
+          }
+        };
+        if (grew || bounds) for_codes(s0, dst + c0 * VEC, ratio, grew, staged);
+        if (bounds && !plain) {
+          barrier();
+          for_codes(n, dst + c0 * VEC + s0 * a.token_stride, 1.0f, false, false);
+        }
+        if (bounds) {
+          const int width = across * VEC;
+          barrier();
+          if (active) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              s_lo[my_tok * width + my_unit * VEC + j] = ext.lo[j];
+              s_hi[my_tok * width + my_unit * VEC + j] = ext.hi[j];
+            }
+          }
+          barrier();
+          int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim + c0 * VEC;
+          const int here = min(width, a.head_dim - c0 * VEC);
+          constexpr int kAtOnce = VEC == 8 ? 4 : 1;  // channels a thread writes
+          for (int i = tid * kAtOnce; i < here; i += TEAM * kAtOnce) {
+            float l[kAtOnce], m[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) l[j] = FLT_MAX, m[j] = -FLT_MAX;
+            for (int k = 0; k < down; ++k) {
+#pragma unroll
+              for (int j = 0; j < kAtOnce; ++j) {
+                l[j] = fminf(l[j], s_lo[k * width + i + j]);
+                m[j] = fmaxf(m[j], s_hi[k * width + i + j]);
+              }
+            }
+            constexpr float kPerUnit = 1.0f / Code::kBoundUnit;  // a power of two
+            int8_t low[kAtOnce], high[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; ++j) {
+              low[j] = static_cast<int8_t>(__float2int_rd(Code::value(Code::code(l[j])) * kPerUnit));
+              high[j] = static_cast<int8_t>(__float2int_ru(Code::value(Code::code(m[j])) * kPerUnit));
+            }
+            if constexpr (VEC == 8) {
+              *reinterpret_cast<char4*>(out + i) = make_char4(low[0], low[1], low[2], low[3]);
+              *reinterpret_cast<char4*>(out + a.head_dim + i) = make_char4(high[0], high[1], high[2], high[3]);
+            } else {
+              out[i] = low[0];
+              out[a.head_dim + i] = high[0];
+            }
+          }
+        }
+      }
+      barrier();  // another unit may follow: the extremes' place is free again
     }
   }
 }
@@ -438,18 +540,35 @@ bool append_pdl() {  // the same switch as the 16-bit append's
 }
 
 template <typename E, typename Code, int VEC, int TEAM>
-cudaError_t launch_team(const Block8AppendArgs& a, cudaStream_t st) {
+cudaError_t launch_team(Block8AppendArgs a, cudaStream_t st) {
+  a.across = std::min(a.head_dim / VEC, TEAM);
+  a.down = TEAM / a.across;
+  a.per_across = 65536u / static_cast<uint32_t>(a.across) + 1u;
+  // A page's packs a thread, up to 16 (of a larger page all are read again).
+  const int64_t packs = (static_cast<int64_t>(a.page_size) + a.down - 1) / a.down;
+  a.keep = VEC == 8 ? static_cast<int>(std::min<int64_t>(packs, 16)) : 0;
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
   const int64_t windows = (a.tokens + a.window - 1) / a.window;
-  const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>((a.num_kv_heads + kTeams - 1) / kTeams), 2);
-  return launch_kernel(append_pdl(), kv_append_block8<E, Code, VEC, TEAM>, grid, dim3(kBlock8AppendThreads), 0, st, a);
+  // Heads a team takes in turn: as many as leave about four waves of blocks.
+  const int blocks = (a.num_kv_heads + kTeams - 1) / kTeams;
+  const int64_t waves = 2 * windows * blocks / (static_cast<int64_t>(sm_count()) * 7);
+  const int turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(waves / 4, 4)));
+  const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>((blocks + turns - 1) / turns), 2);
+  const int bytes = kTeams * team_bytes<E, VEC, TEAM>(a.keep);
+  const auto kernel = kv_append_block8<E, Code, VEC, TEAM>;
+  if (bytes > 48 * 1024 - 64) {
+    static std::atomic<uint64_t> done{0};
+    const cudaError_t e = allow_shared_memory(kernel, kTeams * team_bytes<E, VEC, TEAM>(16), done);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_kernel(append_pdl(), kernel, grid, dim3(kBlock8AppendThreads), static_cast<size_t>(bytes), st, a);
 }
 
 template <typename E, typename Code>
 cudaError_t launch_codes(const Block8AppendArgs& a, bool vec, cudaStream_t st) {
   if (!vec) return launch_team<E, Code, 1, kBlock8AppendThreads>(a, st);
-  // A warp keeps 8 packs of 8 elements a lane.
-  const bool small = static_cast<int64_t>(a.page_size) * a.head_dim <= 2048 && a.head_dim <= 256;
+  // A warp keeps up to 16 packs of 8 elements a lane.
+  const bool small = static_cast<int64_t>(a.page_size) * a.head_dim <= 4096 && a.head_dim <= 256;
   return small ? launch_team<E, Code, 8, 32>(a, st) : launch_team<E, Code, 8, kBlock8AppendThreads>(a, st);
 }
 
@@ -511,7 +630,7 @@ extern "C" int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache
   const int elem = dtype == KL_FLOAT32 ? 4 : 2;
   const bool vec = head_dim % 8 == 0 && (new_row_stride * elem) % 16 == 0 && multiple_of(16, k_new) &&
                    multiple_of(16, v_new) && multiple_of(8, k_cache) && multiple_of(8, v_cache) &&
-                   page_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0;
+                   page_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0 && multiple_of(4, k_bounds);
   const auto st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case KL_FLOAT32: return static_cast<int>(launch_elements<float>(a, code_type, vec, st));

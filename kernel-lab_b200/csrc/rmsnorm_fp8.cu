@@ -33,33 +33,93 @@ constexpr float kE4m3Max = 448.0f;
 constexpr float kPerE4m3Max = 1.0f / 448.0f;
 constexpr float kLeastAmax = 0x1p-100f;  // below it a group's scale is 0
 
-// 16 bytes of a row as floats, and back with one rounding (16-bit types two at a time).
+// lo += a.low * b.low, hi += a.high * b.high for packed 16-bit pairs, by mixed-precision multiply-adds
+// (no unpacking into floats first).
+template <typename T>
+__device__ __forceinline__ void fma_pair_to(uint32_t a, uint32_t b, float& lo, float& hi);
+template <>
+__device__ __forceinline__ void fma_pair_to<__nv_bfloat16>(uint32_t a, uint32_t b, float& lo, float& hi) {
+  asm("{\n.reg .b16 al, ah, bl, bh;\nmov.b32 {al, ah}, %2;\nmov.b32 {bl, bh}, %3;\n"
+      "fma.rn.f32.bf16 %0, al, bl, %0;\nfma.rn.f32.bf16 %1, ah, bh, %1;\n}"
+      : "+f"(lo), "+f"(hi)
+      : "r"(a), "r"(b));
+}
+template <>
+__device__ __forceinline__ void fma_pair_to<__half>(uint32_t a, uint32_t b, float& lo, float& hi) {
+  asm("{\n.reg .b16 al, ah, bl, bh;\nmov.b32 {al, ah}, %2;\nmov.b32 {bl, bh}, %3;\n"
+      "fma.rn.f32.f16 %0, al, bl, %0;\nfma.rn.f32.f16 %1, ah, bh, %1;\n}"
+      : "+f"(lo), "+f"(hi)
+      : "r"(a), "r"(b));
+}
+
+// lo = a.low * b.low, hi = a.high * b.high (exact).
+template <typename T>
+__device__ __forceinline__ void mul_pair(uint32_t a, uint32_t b, float& lo, float& hi);
+template <>
+__device__ __forceinline__ void mul_pair<__nv_bfloat16>(uint32_t a, uint32_t b, float& lo, float& hi) {
+  asm("{\n.reg .b16 al, ah, bl, bh;\nmov.b32 {al, ah}, %2;\nmov.b32 {bl, bh}, %3;\n"
+      "fma.rn.f32.bf16 %0, al, bl, %4;\nfma.rn.f32.bf16 %1, ah, bh, %4;\n}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(a), "r"(b), "f"(0.0f));
+}
+template <>
+__device__ __forceinline__ void mul_pair<__half>(uint32_t a, uint32_t b, float& lo, float& hi) {
+  asm("{\n.reg .b16 al, ah, bl, bh;\nmov.b32 {al, ah}, %2;\nmov.b32 {bl, bh}, %3;\n"
+      "fma.rn.f32.f16 %0, al, bl, %4;\nfma.rn.f32.f16 %1, ah, bh, %4;\n}"
+      : "=f"(lo), "=f"(hi)
+      : "r"(a), "r"(b), "f"(0.0f));
+}
+
+// 16 bytes of a row.
 template <typename T>
 struct RowPack {
   static constexpr int N = 16 / sizeof(T);
-  uint4 raw;
-  __device__ __forceinline__ void unpack(float (&f)[N]) const {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t w[4];
+  __device__ __forceinline__ void load(uint4 v) { w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w; }
+  __device__ __forceinline__ uint4 raw() const { return make_uint4(w[0], w[1], w[2], w[3]); }
+  // this = T(float(this) + float(r))
+  __device__ __forceinline__ void add(const RowPack& r) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (N == 8) {
-        const float2 p = Storage<T>::unpack2(w[i]);
-        f[2 * i] = p.x;
-        f[2 * i + 1] = p.y;
+        float2 f = Storage<T>::unpack2(r.w[i]);
+        add_pair_to<T>(w[i], f.x, f.y);
+        w[i] = Storage<T>::pack2(f.x, f.y);
       } else {
-        f[i] = __uint_as_float(w[i]);
+        w[i] = __float_as_uint(__uint_as_float(w[i]) + __uint_as_float(r.w[i]));
       }
     }
   }
-  __device__ __forceinline__ void pack(const float (&f)[N]) {
-    if constexpr (N == 8) {
-      raw = make_uint4(Storage<T>::pack2(f[0], f[1]), Storage<T>::pack2(f[2], f[3]), Storage<T>::pack2(f[4], f[5]),
-                       Storage<T>::pack2(f[6], f[7]));
-    } else {
-      raw = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  __device__ __forceinline__ void add_squares(float& s0, float& s1) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 8) {
+        fma_pair_to<T>(w[i], w[i], s0, s1);
+      } else {
+        float& s = i & 1 ? s1 : s0;
+        s = fmaf(__uint_as_float(w[i]), __uint_as_float(w[i]), s);
+      }
+    }
+  }
+  // t = this * weights
+  __device__ __forceinline__ void times(const RowPack& k, float (&t)[N]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (N == 8) {
+        mul_pair<T>(w[i], k.w[i], t[2 * i], t[2 * i + 1]);
+      } else {
+        t[i] = __uint_as_float(w[i]) * __uint_as_float(k.w[i]);
+      }
     }
   }
 };
+
+template <int N>
+__device__ __forceinline__ float largest(const float (&t)[N], float top) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(t[j]));
+  return top;
+}
 
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -72,8 +132,8 @@ struct GroupScale {
   float inv, scale;
   __device__ __forceinline__ GroupScale(float b, float rstd) {
     const float a = b * rstd;
-    const bool some = a >= kLeastAmax && b >= kLeastAmax;  // false for NaN too
-    inv = some ? kE4m3Max * __frcp_rn(b) : 0.0f * rstd;
+    const bool some = a >= kLeastAmax && b >= kLeastAmax;  // false for NaN too; b is at most 2^126
+    inv = some ? __fdividef(kE4m3Max, b) : 0.0f * rstd;  // within 2 units in the last place
     scale = some ? a * kPerE4m3Max : 0.0f;
   }
 };
@@ -111,10 +171,10 @@ struct NormFp8Args {
   float eps;
 };
 
-// One CTA per row; each thread owns NPT 16-byte packs of the row, strided by blockDim. `lanes`:
-// packs (adjacent lanes) of a group, 0 for one scale a row.
-template <typename T, int NPT, bool RES>
-__global__ void __launch_bounds__(512) rmsnorm_fp8_row_regs(const NormFp8Args g, int lanes) {
+// One CTA per row; each thread owns NPT 16-byte packs of the row, strided by blockDim. GROUPS: a
+// scale for each `lanes` packs (adjacent lanes), else one for the row.
+template <typename T, int NPT, bool RES, bool GROUPS>
+__global__ void __launch_bounds__(512, 2) rmsnorm_fp8_row_regs(const NormFp8Args g, int lanes) {
   using P = RowPack<T>;
   __shared__ SumMax red[32];
   const int packs = g.hidden / P::N;
@@ -131,61 +191,52 @@ __global__ void __launch_bounds__(512) rmsnorm_fp8_row_regs(const NormFp8Args g,
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int pk = threadIdx.x + i * blockDim.x;
-    a[i].raw = r[i].raw = w[i].raw = make_uint4(0, 0, 0, 0);  // packs past the row add nothing
-    if (pk < packs) {
-      a[i].raw = __ldcs(xr + pk);
-      if constexpr (RES) r[i].raw = __ldcs(rr + pk);
-      w[i].raw = __ldg(wr + pk);
-    }
+    const uint4 none = make_uint4(0, 0, 0, 0);  // packs past the row add nothing
+    a[i].load(pk < packs ? __ldcs(xr + pk) : none);
+    if constexpr (RES) r[i].load(pk < packs ? __ldcs(rr + pk) : none);
+    w[i].load(pk < packs ? __ldg(wr + pk) : none);
   }
 
-  // a[] becomes the row, w[] is read again for the codes (t is not kept: it would double the registers).
-  float ss = 0.0f, top = 0.0f;
+  float s0 = 0.0f, s1 = 0.0f, top = 0.0f;
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int pk = threadIdx.x + i * blockDim.x;
-    float f[P::N], v[P::N];
-    a[i].unpack(f);
     if constexpr (RES) {
-      r[i].unpack(v);
-#pragma unroll
-      for (int j = 0; j < P::N; ++j) f[j] += v[j];
-      a[i].pack(f);
-      a[i].unpack(f);
-      if (pk < packs) ro[pk] = a[i].raw;
+      a[i].add(r[i]);
+      if (pk < packs) ro[pk] = a[i].raw();
     }
-    w[i].unpack(v);
-#pragma unroll
-    for (int j = 0; j < P::N; ++j) {
-      ss = fmaf(f[j], f[j], ss);
-      if (lanes == 0) top = fmaxf(top, fabsf(f[j] * v[j]));
+    a[i].add_squares(s0, s1);
+    if constexpr (!GROUPS) {
+      float t[P::N];
+      a[i].times(w[i], t);
+      top = largest(t, top);
     }
   }
 
-  const SumMax all = block_allreduce(ss, top, red);
+  const SumMax all = block_allreduce(s0 + s1, top, red);
   const float rstd = 1.0f / sqrtf(all.sum / static_cast<float>(g.hidden) + g.eps);
   allow_next_grid();
-  const GroupScale whole(all.max, rstd);
-  if (lanes == 0 && threadIdx.x == 0) scales[0] = whole.scale;
+  float inv = 0.0f;
+  if constexpr (!GROUPS) {
+    const GroupScale whole(all.max, rstd);
+    inv = whole.inv;
+    if (threadIdx.x == 0) scales[0] = whole.scale;
+  }
 
 #pragma unroll
   for (int i = 0; i < NPT; ++i) {
     const int pk = threadIdx.x + i * blockDim.x;
-    float t[P::N], v[P::N];
-    a[i].unpack(t);
-    w[i].unpack(v);
-    float b = 0.0f;
+    float t[P::N];
+    a[i].times(w[i], t);
+    if constexpr (GROUPS) {
+      float b = largest(t, 0.0f);
 #pragma unroll
-    for (int j = 0; j < P::N; ++j) {
-      t[j] *= v[j];
-      b = fmaxf(b, fabsf(t[j]));
-    }
-    float inv = whole.inv;
-    if (lanes != 0) {
-      for (int m = lanes >> 1; m > 0; m >>= 1) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, m));
+      for (int m = 16; m > 0; m >>= 1) {
+        if (m < lanes) b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, m));
+      }
       const GroupScale s(b, rstd);
       inv = s.inv;
-      if (pk < packs && (pk & (lanes - 1)) == 0) scales[pk / lanes] = s.scale;
+      if (pk < packs && (pk & (lanes - 1)) == 0) scales[pk >> (31 - __clz(lanes))] = s.scale;
     }
     if (pk < packs) {
       uint32_t c[P::N / 4];
@@ -270,8 +321,12 @@ cudaError_t launch_rows(void (*kernel)(Params...), int rows, int threads, cudaSt
 
 template <typename T, int NPT>
 cudaError_t launch_regs(const NormFp8Args& g, int rows, int threads, int lanes, cudaStream_t st) {
-  return g.residual ? launch_rows(rmsnorm_fp8_row_regs<T, NPT, true>, rows, threads, st, g, lanes)
-                    : launch_rows(rmsnorm_fp8_row_regs<T, NPT, false>, rows, threads, st, g, lanes);
+  if (g.groups > 1) {
+    return g.residual ? launch_rows(rmsnorm_fp8_row_regs<T, NPT, true, true>, rows, threads, st, g, lanes)
+                      : launch_rows(rmsnorm_fp8_row_regs<T, NPT, false, true>, rows, threads, st, g, lanes);
+  }
+  return g.residual ? launch_rows(rmsnorm_fp8_row_regs<T, NPT, true, false>, rows, threads, st, g, lanes)
+                    : launch_rows(rmsnorm_fp8_row_regs<T, NPT, false, false>, rows, threads, st, g, lanes);
 }
 
 template <typename T>
