@@ -55,6 +55,7 @@ struct Block8AppendArgs {
   int window;              // new tokens a team looks at
   int across, down;        // channel units (of VEC) side by side in a team, tokens beside them
   uint32_t per_across;     // 65536 / across + 1: thread / across without a division
+  uint32_t per_down;       // 2^32 / down + 1 (0 where down is 1): tokens / down likewise
   int keep;                // packs a thread can keep in shared memory
 };
 
@@ -363,6 +364,13 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
     t += n;
     if (first != begin && s0 != 0) continue;  // not the sequence's first token in this page
 
+    // Tokens of [0, m) that are this thread's: my_tok, my_tok + down, ...
+    const auto mine = [&](int m) {
+      if (!active || m <= my_tok) return 0;
+      const uint32_t x = static_cast<uint32_t>(m - my_tok + down - 1);
+      return static_cast<int>(a.per_down ? __umulhi(x, a.per_down) : x);
+    };
+    const int my_new = mine(n), my_old = mine(s0);
     int64_t page = -1;
     if (col < static_cast<uint32_t>(a.max_pages)) page = a.block_table[b * a.bt_stride + col];
     const bool kept = VEC == 8 && units <= across && n <= a.keep * down;  // they fit in shared memory
@@ -373,11 +381,11 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
       const E* const src = row + h * a.head_dim;
       // The new packs first (they need no page), then the page, its present scale and its codes.
       if constexpr (VEC == 8) {
-        if (kept && active) {
+        if (kept) {
           const uint8_t* from = reinterpret_cast<const uint8_t*>(src);
           uint32_t to = smem_u32(s_new + tid);
 #pragma unroll 4
-          for (int i = my_tok; i < n; i += down) {
+          for (int i = 0; i < my_new; ++i) {
 #pragma unroll
             for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) cp_async16(to + k, from + k);
             from += src_step * static_cast<int64_t>(sizeof(E));
@@ -395,39 +403,44 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
       // This thread's first slot; slot s0 + my_tok is its first new one.
       uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + page * a.page_stride + h * a.head_stride +
                            my_tok * a.token_stride + my_unit * VEC;
-      if (staged && active) {
-        const uint32_t to = smem_u32(s_codes) + tid * VEC;
+      if (staged) {
+        uint32_t to = smem_u32(s_codes) + tid * VEC;
         const uint8_t* from = dst;
-        for (int i = 0; my_tok + i * down < s0; ++i, from += dst_step) cp_async8(to + i * (TEAM * VEC), from);
+#pragma unroll 4
+        for (int i = 0; i < my_old; ++i, from += dst_step, to += TEAM * VEC) cp_async8(to, from);
       }
       cp_async_wait_all();  // each thread reads back what it copied itself
 
-      // f(pack, index) over this thread's new packs of channel units c0, c0 + 1, ...
+      // f(pack) over this thread's new packs of channel units c0, c0 + 1, ..., in token order.
       const auto for_new = [&](int c0, auto&& f) {
-        if (!active || c0 + my_unit >= units) return;
         if (kept) {
-#pragma unroll 2
-          for (int i = 0; my_tok + i * down < n; ++i) f(s_new[i * TEAM + tid], i);
-          return;
-        }
-        const E* at = src + c0 * VEC;
+          const Pack* at = s_new + tid;
+#pragma unroll 4
+          for (int i = 0; i < my_new; ++i, at += TEAM) {
+            Pack p;
+            p.load(at->v);
+            f(p);
+          }
+        } else if (c0 + my_unit < units) {
+          const E* at = src + c0 * VEC;
 #pragma unroll 1
-        for (int i = 0; my_tok + i * down < n; ++i, at += src_step) {
-          Pack p;
-          p.load(at);
-          f(p, i);
+          for (int i = 0; i < my_new; ++i, at += src_step) {
+            Pack p;
+            p.load(at);
+            f(p);
+          }
         }
       };
 
       Magnitude<E, VEC> mag;
       mag.reset();
-      for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p, int) { mag.add(p); });
+      for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p) { mag.add(p); });
       float amax = mag.get();
       const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
       if (!plain) {
         amax = 0.0f;
         for (int c0 = 0; c0 < units; c0 += across) {
-          for_new(c0, [&](const Pack& p, int) {
+          for_new(c0, [&](const Pack& p) {
             float f[VEC];
             p.unpack(f);
 #pragma unroll
@@ -447,33 +460,38 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
 
       for (int c0 = 0; c0 < units; c0 += across) {
         Extremes<VEC> ext;
-        {
+        ext.reset();
+        uint8_t* put = dst + c0 * VEC + s0 * a.token_stride;
+        const auto quantise = [&](const Pack& p) {
+          float y[VEC];
+          p.unpack(y);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) y[j] *= inv;
+          store_codes<Code, VEC>(put, y, plain);  // plain: |y| is at most a rounding above kMax
+          put += dst_step;
+        };
+        if (bounds) {
           PackExtremes<E, VEC> raw;
           raw.reset();
-          uint8_t* const put = dst + c0 * VEC + s0 * a.token_stride;
-          for_new(c0, [&](const Pack& p, int i) {
-            float y[VEC];
-            p.unpack(y);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) y[j] *= inv;
-            store_codes<Code, VEC>(put + i * dst_step, y, plain);  // plain: |y| is at most a rounding above kMax
-            if (bounds) raw.add(p);
+          for_new(c0, [&](const Pack& p) {
+            quantise(p);
+            raw.add(p);
           });
-          raw.get(ext.lo, ext.hi);
-        }
-        const bool had = plain && active && my_tok < n;  // this thread's own extremes, to be scaled
+          if (plain && my_new > 0) {  // this thread's own extremes, scaled
+            raw.get(ext.lo, ext.hi);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          ext.lo[j] = had ? ext.lo[j] * inv : FLT_MAX;
-          ext.hi[j] = had ? ext.hi[j] * inv : -FLT_MAX;
+            for (int j = 0; j < VEC; ++j) ext.lo[j] *= inv, ext.hi[j] *= inv;
+          }
+        } else {
+          for_new(c0, quantise);
         }
         // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
         const auto for_codes = [&](int count, uint8_t* at, float by, bool write, bool in_shared) {
-          if (!active || c0 + my_unit >= units) return;
+          if (c0 + my_unit >= units) return;
           const uint8_t* in = in_shared ? s_codes + tid * VEC : at;
           const int64_t in_step = in_shared ? TEAM * VEC : dst_step;
 #pragma unroll 2
-          for (int tok = my_tok; tok < count; tok += down, at += dst_step, in += in_step) {
+          for (int i = 0; i < count; ++i, at += dst_step, in += in_step) {
             float y[VEC];
             load_codes<Code, VEC>(in, y);
 #pragma unroll
@@ -482,10 +500,10 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
             if (bounds) ext.add(y);
           }
         };
-        if (grew || bounds) for_codes(s0, dst + c0 * VEC, ratio, grew, staged);
+        if (grew || bounds) for_codes(my_old, dst + c0 * VEC, ratio, grew, staged);
         if (bounds && !plain) {
           barrier();
-          for_codes(n, dst + c0 * VEC + s0 * a.token_stride, 1.0f, false, false);
+          for_codes(my_new, dst + c0 * VEC + s0 * a.token_stride, 1.0f, false, false);
         }
         if (bounds) {
           const int width = across * VEC;
@@ -544,6 +562,7 @@ cudaError_t launch_team(Block8AppendArgs a, cudaStream_t st) {
   a.across = std::min(a.head_dim / VEC, TEAM);
   a.down = TEAM / a.across;
   a.per_across = 65536u / static_cast<uint32_t>(a.across) + 1u;
+  a.per_down = a.down == 1 ? 0u : 0xffffffffu / static_cast<uint32_t>(a.down) + 1u;
   // A page's packs a thread, up to 16 (of a larger page all are read again).
   const int64_t packs = (static_cast<int64_t>(a.page_size) + a.down - 1) / a.down;
   a.keep = VEC == 8 ? static_cast<int>(std::min<int64_t>(packs, 16)) : 0;
