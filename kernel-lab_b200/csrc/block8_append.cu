@@ -5,8 +5,8 @@
 // new elements gives the scale, so a unit is a reduction and then an elementwise pass over the same
 // elements. A team of one warp (pages of up to 4096 elements a head) or of four warps takes a unit
 // and copies its new elements to shared memory, all in flight at once and without registers, so that
-// it reads them once; larger pages re-read theirs from L2. A team takes several heads of a page in turn
-// where the call is large: finding the page costs about as many instructions as a unit's elements. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
+// it reads them once; larger pages re-read theirs from L2. A team takes several parts of a page (keys
+// or values of a head) in turn where the call is large: finding the page costs about as many instructions as a unit's elements. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
 // latency-bound for single tokens, where the chain is indptr / position, block-table entry, new row.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
@@ -33,6 +33,7 @@ namespace klb {
 namespace {
 
 constexpr int kBlock8AppendThreads = 128;
+constexpr int kAppendBlocks = 6;  // resident an SM that the registers are held to (5: 51.8 us for 35k prompt tokens, 6: 50.0, 7: 62.3 with spills)
 
 struct Block8AppendArgs {
   uint8_t* k_cache;
@@ -184,6 +185,17 @@ struct PackExtremes {
       }
     }
   }
+  // With the extremes of the lane `o` away.
+  __device__ __forceinline__ void combine_lanes(int o) {
+    static_assert(kPairs);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const uint32_t l = __shfl_xor_sync(0xffffffffu, reinterpret_cast<const uint32_t&>(lo[i]), o);
+      const uint32_t h = __shfl_xor_sync(0xffffffffu, reinterpret_cast<const uint32_t&>(hi[i]), o);
+      lo[i] = __hmin2(lo[i], reinterpret_cast<const Unit&>(l));
+      hi[i] = __hmax2(hi[i], reinterpret_cast<const Unit&>(h));
+    }
+  }
   __device__ __forceinline__ void get(float (&l)[VEC], float (&h)[VEC]) const {
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -263,6 +275,20 @@ __device__ __forceinline__ void load_codes(const uint8_t* p, float (&y)[VEC]) {
   }
 }
 
+// N channels' bounds (UP: the upper ones) of extremes times `by`, as bytes: the code's value in units, outward.
+template <typename Code, bool UP, int N>
+__device__ __forceinline__ uint32_t bound_codes(const float* x, float by) {
+  constexpr float kPerUnit = 1.0f / Code::kBoundUnit;  // a power of two
+  uint32_t w = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float v = Code::value(Code::code(x[j] * by)) * kPerUnit;
+    const int r = UP ? __float2int_ru(v) : __float2int_rd(v);
+    w |= static_cast<uint32_t>(r & 0xff) << (8 * j);
+  }
+  return w;
+}
+
 // Extremes of scaled elements; NaN counts as 0.
 template <int VEC>
 struct Extremes {
@@ -313,8 +339,60 @@ __device__ __forceinline__ float team_max(float v, float* red) {
   return v;
 }
 
+// Eight packs a lane of a page that is filled whole by one call (the bulk of a prompt): straight-line,
+// from registers. Returns false, with nothing written, when the page holds a NaN or an infinity.
+constexpr int kWhole = 8;
+template <typename E, typename Code>
+__device__ __forceinline__ bool append_whole_page(const E* src, int64_t src_step, uint8_t* dst, int64_t dst_step,
+                                                  float* scale_at, int8_t* bounds, int head_dim, int across) {
+  using Pack = NewPack<E, 8>;
+  Pack p[kWhole];
+#pragma unroll
+  for (int i = 0; i < kWhole; ++i, src += src_step) p[i].load(src);
+  Magnitude<E, 8> mag;
+  mag.reset();
+#pragma unroll
+  for (int i = 0; i < kWhole; ++i) mag.add(p[i]);
+  float amax = mag.get();
+  if (!__all_sync(0xffffffffu, amax <= FLT_MAX)) return false;
+  amax = warp_allreduce_max(amax);
+  const float scale = Code::scale_for(amax);
+  const float inv = reciprocal_scale(scale);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) *scale_at = scale;
+#pragma unroll
+  for (int i = 0; i < kWhole; ++i, dst += dst_step) {
+    float y[8];
+    p[i].unpack(y);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] *= inv;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(Code::code4_in_range(y[0], y[1], y[2], y[3]),
+                                                Code::code4_in_range(y[4], y[5], y[6], y[7]));
+  }
+  if (bounds) {
+    PackExtremes<E, 8> x;
+    x.reset();
+#pragma unroll
+    for (int i = 0; i < kWhole; ++i) x.add(p[i]);
+    for (int o = across; o < 32; o <<= 1) x.combine_lanes(o);
+    if (lane < across) {
+      float lo[8], hi[8];
+      x.get(lo, hi);
+      uint32_t low[2], high[2];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        low[w] = bound_codes<Code, false, 4>(lo + 4 * w, inv);
+        high[w] = bound_codes<Code, true, 4>(hi + 4 * w, inv);
+      }
+      *reinterpret_cast<uint2*>(bounds + lane * 8) = make_uint2(low[0], low[1]);
+      *reinterpret_cast<uint2*>(bounds + head_dim + lane * 8) = make_uint2(high[0], high[1]);
+    }
+  }
+  return true;
+}
+
 template <typename E, typename Code, int VEC, int TEAM>
-__global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(const Block8AppendArgs a) {
+__global__ void __launch_bounds__(kBlock8AppendThreads, kAppendBlocks) kv_append_block8(const Block8AppendArgs a) {
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
   using Pack = NewPack<E, VEC>;
   // Per team: the kept packs [keep][TEAM]; then a page's present codes (VEC bytes a thread and row)
@@ -328,10 +406,8 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
   float* const s_hi = s_lo + TEAM * VEC;
   wait_prior_grid();
   allow_next_grid();
-  const int first_head = blockIdx.y * kTeams + team;
-  if (first_head >= a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
-  const bool keys = blockIdx.z == 0;
-  const bool bounds = keys && a.k_bounds != nullptr;
+  const int first_part = blockIdx.y * kTeams + team;  // part 2 * head + (0: keys, 1: values) of a page
+  if (first_part >= 2 * a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
 
   const int units = a.head_dim / VEC;
   const int across = a.across, down = a.down;
@@ -375,10 +451,24 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
     if (col < static_cast<uint32_t>(a.max_pages)) page = a.block_table[b * a.bt_stride + col];
     const bool kept = VEC == 8 && units <= across && n <= a.keep * down;  // they fit in shared memory
     const bool staged = VEC == 8 && units <= across && s0 <= a.keep * down;
-    const E* const row = static_cast<const E*>(keys ? a.k_new : a.v_new) + (first + my_tok) * a.new_stride + my_unit * VEC;
+    // The whole page at once, eight packs a lane, channel units a power of two.
+    const bool whole = VEC == 8 && n == a.page_size && n == kWhole * down && across * down == 32 && units == across;
+    const int64_t row = (first + my_tok) * a.new_stride + my_unit * VEC;
+    const int64_t place = page * a.page_stride + my_tok * a.token_stride + my_unit * VEC;
 
-    for (int h = first_head; h < a.num_kv_heads; h += gridDim.y * kTeams) {
-      const E* const src = row + h * a.head_dim;
+    for (int part = first_part; part < 2 * a.num_kv_heads; part += gridDim.y * kTeams) {
+      const int h = part >> 1;
+      const bool keys = (part & 1) == 0;
+      const bool bounds = keys && a.k_bounds != nullptr;
+      const E* const src = static_cast<const E*>(keys ? a.k_new : a.v_new) + row + h * a.head_dim;
+      if constexpr (TEAM == 32 && PackExtremes<E, VEC>::kPairs) {
+        if (whole && page >= 0 && page < a.num_pages) {
+          uint8_t* const to = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
+          float* const scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
+          int8_t* const out = bounds ? a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim : nullptr;
+          if (append_whole_page<E, Code>(src, src_step, to, dst_step, scale_at, out, a.head_dim, across)) continue;
+        }
+      }
       // The new packs first (they need no page), then the page, its present scale and its codes.
       if constexpr (VEC == 8) {
         if (kept) {
@@ -401,8 +491,7 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
       float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
       const float old = s0 > 0 ? *scale_at : 0.0f;
       // This thread's first slot; slot s0 + my_tok is its first new one.
-      uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + page * a.page_stride + h * a.head_stride +
-                           my_tok * a.token_stride + my_unit * VEC;
+      uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
       if (staged) {
         uint32_t to = smem_u32(s_codes) + tid * VEC;
         const uint8_t* from = dst;
@@ -530,19 +619,12 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, 7) kv_append_block8(cons
                 m[j] = fmaxf(m[j], s_hi[k * width + i + j]);
               }
             }
-            constexpr float kPerUnit = 1.0f / Code::kBoundUnit;  // a power of two
-            int8_t low[kAtOnce], high[kAtOnce];
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) {
-              low[j] = static_cast<int8_t>(__float2int_rd(Code::value(Code::code(l[j])) * kPerUnit));
-              high[j] = static_cast<int8_t>(__float2int_ru(Code::value(Code::code(m[j])) * kPerUnit));
-            }
             if constexpr (VEC == 8) {
-              *reinterpret_cast<char4*>(out + i) = make_char4(low[0], low[1], low[2], low[3]);
-              *reinterpret_cast<char4*>(out + a.head_dim + i) = make_char4(high[0], high[1], high[2], high[3]);
+              *reinterpret_cast<uint32_t*>(out + i) = bound_codes<Code, false, 4>(l, 1.0f);
+              *reinterpret_cast<uint32_t*>(out + a.head_dim + i) = bound_codes<Code, true, 4>(m, 1.0f);
             } else {
-              out[i] = low[0];
-              out[a.head_dim + i] = high[0];
+              out[i] = static_cast<int8_t>(bound_codes<Code, false, 1>(l, 1.0f));
+              out[a.head_dim + i] = static_cast<int8_t>(bound_codes<Code, true, 1>(m, 1.0f));
             }
           }
         }
@@ -568,11 +650,11 @@ cudaError_t launch_team(Block8AppendArgs a, cudaStream_t st) {
   a.keep = VEC == 8 ? static_cast<int>(std::min<int64_t>(packs, 16)) : 0;
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
   const int64_t windows = (a.tokens + a.window - 1) / a.window;
-  // Heads a team takes in turn: as many as leave about four waves of blocks.
-  const int blocks = (a.num_kv_heads + kTeams - 1) / kTeams;
-  const int64_t waves = 2 * windows * blocks / (static_cast<int64_t>(sm_count()) * 7);
+  // Parts of a page that a team takes in turn: up to four, as many as leave about four waves of blocks.
+  const int blocks = (2 * a.num_kv_heads + kTeams - 1) / kTeams;
+  const int64_t waves = windows * blocks / (static_cast<int64_t>(sm_count()) * kAppendBlocks);
   const int turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(waves / 4, 4)));
-  const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>((blocks + turns - 1) / turns), 2);
+  const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>((blocks + turns - 1) / turns));
   const int bytes = kTeams * team_bytes<E, VEC, TEAM>(a.keep);
   const auto kernel = kv_append_block8<E, Code, VEC, TEAM>;
   if (bytes > 48 * 1024 - 64) {
@@ -611,7 +693,7 @@ extern "C" int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache
   using namespace klb;
   constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
   if (batch == 0 || tokens == 0) return 0;
-  if (batch < 0 || tokens < 0 || tokens > INT32_MAX || num_kv_heads <= 0 || num_kv_heads > 65535 || head_dim <= 0 ||
+  if (batch < 0 || tokens < 0 || tokens > INT32_MAX || num_kv_heads <= 0 || num_kv_heads > 32767 || head_dim <= 0 ||
       head_dim > 1024 || page_size <= 0 || max_pages_per_seq < 0 || block_table_stride < max_pages_per_seq ||
       num_pages < 0 || page_stride < 0 || token_stride < 0 || head_stride < 0 ||
       new_row_stride < static_cast<int64_t>(num_kv_heads) * head_dim || (!indptr && tokens != batch) || !k_cache ||
@@ -649,7 +731,7 @@ extern "C" int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache
   const int elem = dtype == KL_FLOAT32 ? 4 : 2;
   const bool vec = head_dim % 8 == 0 && (new_row_stride * elem) % 16 == 0 && multiple_of(16, k_new) &&
                    multiple_of(16, v_new) && multiple_of(8, k_cache) && multiple_of(8, v_cache) &&
-                   page_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0 && multiple_of(4, k_bounds);
+                   page_stride % 8 == 0 && token_stride % 8 == 0 && head_stride % 8 == 0 && multiple_of(8, k_bounds);
   const auto st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case KL_FLOAT32: return static_cast<int>(launch_elements<float>(a, code_type, vec, st));
