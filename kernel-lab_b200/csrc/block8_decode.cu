@@ -6,18 +6,21 @@
 //   out = (sum_t 2^(s_t - m) * v_scale[page(t), h] * cv_t) / sum_t 2^(s_t - m)     (s in base 2)
 //
 // HBM-bound: every code is read once and used for the group's query heads (4 to 16 operations a byte).
-// One CTA of eight warps an SM. A "tile" is 16 tokens of one KV head, 2 * 16 * head_dim bytes; each
+// CTAs of eight warps. A "tile" is 16 tokens of one KV head, 2 * 16 * head_dim bytes; each
 // warp (or team of warps, below) streams its own tiles through its own ring of shared-memory stages
 // with 16-byte cp.async, so no warp waits for another while it streams and page and token strides
 // may be any. Rows past the sequence's end are zero-filled by the copy: code 0 is 0 in both formats, so
 // whatever the page holds there (NaN codes included) never reaches a product.
 //
-// Warps of a CTA. Up to 8 * NT query heads of one KV head share a warp's products (NT = 1 for groups
-// of at most 8). Larger groups take HG warps, which form a team: they share one ring, each copies 1/HG
-// of a tile and meets the others at a named barrier once a tile. The CTA's teams are HB KV heads times
-// TS parts of the token range; the TS parts' states are joined through shared memory at the end of a
+// Warps of a CTA. Up to 8 * NT query heads of one KV head share a warp's products, so that codes are
+// widened once for them (NT = 1 for groups of at most 8, else 2 where the registers allow). Larger groups
+// take HG warps, which form a team: they share one ring, each copies 1/HG of a tile and meets the others
+// at a named barrier once a step. The CTA's teams are HB KV heads times TS parts of the token range; the
+// TS parts' states are joined through shared memory at the end of a
 // range. Many parallel KV heads and one part where there is work for every warp (fewest joins, and
-// a page's heads are read together), more parts of fewer heads where the whole call is small.
+// a page's heads are read together), more parts of fewer heads where the whole call is small. A warp
+// takes two tiles a step (one for head_dim above 128, whose ring has no room for more): a tile is a
+// chain of dependent steps, and two of them fill each other's gaps.
 //
 // Balance. Rows (sequence, block of HB heads) are laid end to end, each as long as its tiles plus a
 // fixed charge for starting it, and CTA c takes the c-th equal piece, found by every CTA alone from
@@ -45,8 +48,9 @@ namespace {
 constexpr int kB8Warps = 8;
 constexpr int kB8Threads = 32 * kB8Warps;
 constexpr int kB8Tile = 16;
-constexpr int kB8Meta = 32;        // bytes of a stage after its codes: 2 k scales, 2 v scales, 2 valid counts
+constexpr int kB8Meta = 32;        // bytes of a stage after its codes: scales (k, v) of its octets, valid counts
 constexpr float kRaiseBy = 8.0f;   // the running maximum is raised when a score passes it by this (base 2)
+constexpr float kNoMax = -1e30f;   // running maximum before the first score
 constexpr int kMaxShared = 227 * 1024 - 128;  // dynamic, beside the plan's static part
 constexpr int kTeamBarrier = 1, kGroupBarrier = 8;  // named barriers: 1.. teams, 8.. groups
 
@@ -60,7 +64,7 @@ struct Block8Args {
   const int32_t* block_table;
   const int32_t* seq_lens;
   const int32_t* selected;  // null: every page
-  int64_t page_stride, token_stride, head_stride;
+  int32_t page_stride, token_stride, head_stride;
   int64_t bt_stride;
   int64_t num_pages;
   int batch, num_q_heads, num_kv_heads, group, head_dim, page_size, max_pages;
@@ -75,11 +79,16 @@ struct Block8Args {
   float2* part_ml;     // [slot][8 / ts][8 * NT]: (maximum, sum)
 };
 
-// Stages of a team's ring: what 227 KB hold beside the boxes of the joins (4 warps' states).
-__host__ __device__ constexpr int ring_stages(int dp, int nt, int hg) {
-  const int per_warp = dp == 64 ? 12 : dp == 256 ? 3 : nt == 1 ? 6 : 5;
+// Tiles of a step, and stages (of a step's tiles) of a team's ring: what 227 KB hold beside the boxes of
+// the joins.
+__host__ __device__ constexpr int step_tiles(int dp) { return dp == 256 ? 1 : 2; }
+__host__ __device__ constexpr int ring_stages(int dp, int hg) {
+  const int per_warp = dp == 64 ? 6 : 3;
   return hg * per_warp < 12 ? hg * per_warp : 12;
 }
+// Floats a lane hands over at a time in a join: the maxima and sums of 8 query heads and half of their
+// outputs.
+__host__ __device__ constexpr int box_floats(int dp) { return 4 + dp / 8; }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -106,9 +115,9 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float2 lds_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
 
@@ -134,16 +143,19 @@ __device__ __forceinline__ void widen<Int8Code>(uint32_t w, uint32_t& lo, uint32
 
 // Byte offset of 16-byte unit `u` of token row `r` of a tile: rows DP bytes apart, the units of each
 // 128 bytes permuted so that the score product's reads (8 lanes: 2 rows x 4 units) and the value
-// product's (8 lanes: rows 0, 2, 4, 6 or 1, 3, 5, 7 x 2 units) each meet 8 different units.
+// product's (8 lanes: rows 0, 2, 4, 6 or 1, 3, 5, 7 x 2 units) each meet 8 different units. Rows 8
+// apart are permuted alike; the permutation is an exclusive or that is linear in the row's bits.
 template <int DP>
-__device__ __forceinline__ uint32_t unit_offset(int r, int u) {
-  if constexpr (DP == 64) {
-    const int line = r >> 1;
-    return line * 128 + ((((r & 1) * 4 + u) ^ ((line & 3) << 1)) << 4);
-  } else {
-    const int f = (((r ^ (r >> 2)) & 1) << 2) | (r & 2);
-    return r * DP + ((u ^ f) << 4);
-  }
+__host__ __device__ constexpr uint32_t unit_offset(int r, int u) {
+  if (DP == 64) return (r >> 1) * 128 + ((((r & 1) * 4 + u) ^ (((r >> 1) & 3) << 1)) << 4);
+  const int f = (((r ^ (r >> 2)) & 1) << 2) | (r & 2);
+  return r * DP + ((u ^ f) << 4);
+}
+// unit_offset(r + sub, u) from unit_offset(sub, u), for rows r that are a multiple of a copy's rows.
+template <int DP>
+__device__ __forceinline__ uint32_t row_block(uint32_t offset, int r) {
+  const uint32_t flips = DP == 64 ? 0u : unit_offset<DP>(r, 0) & 127u;
+  return (offset ^ flips) + r * DP;
 }
 
 struct Segment {
@@ -151,12 +163,12 @@ struct Segment {
   int x0, x1;       // tiles
   int tiles;        // of the whole row
   int len;
-  int64_t start;    // position of the row's first tile
+  int start;        // position of the row's first tile, relative to the CTA's piece
 };
 
-// Walks the rows of a CTA's piece [p, p1).
+// Walks the rows of a CTA's piece; positions are relative to its begin.
 struct RowWalk {
-  int64_t p, p1, start;  // start: position of row (b, u)
+  int p, p1, start;  // start: position of row (b, u)
   int b, u, len, tiles;
 
   __device__ __forceinline__ void read_row(const Block8Args& a) {
@@ -170,11 +182,10 @@ struct RowWalk {
   }
   __device__ __forceinline__ bool next(const Block8Args& a, Segment& s) {
     while (p < p1) {
-      const int cost = tiles + a.row_charge;
-      const int x0 = static_cast<int>(p - start);
+      const int x0 = p - start;
       const bool some = x0 < tiles;
-      s = Segment{b, u, x0, static_cast<int>(min(static_cast<int64_t>(tiles), p1 - start)), tiles, len, start};
-      start += cost;
+      s = Segment{b, u, x0, min(tiles, p1 - start), tiles, len, start};
+      start += tiles + a.row_charge;
       p = start;
       if (++u == a.units) {
         u = 0;
@@ -243,9 +254,9 @@ __device__ __forceinline__ bool plan_piece(const Block8Args& a, PlanShared* ps, 
   const int cost = w.tiles + a.row_charge;
   const int64_t first = ps->before * a.units;
   w.u = static_cast<int>((p0 - first) / cost);
-  w.start = first + static_cast<int64_t>(w.u) * cost;
-  w.p = p0;
-  w.p1 = min(p0 + piece, static_cast<int64_t>(total));
+  w.start = static_cast<int>(first + static_cast<int64_t>(w.u) * cost - p0);
+  w.p = 0;
+  w.p1 = static_cast<int>(min(piece, static_cast<int64_t>(total) - p0));
   return true;
 }
 
@@ -253,9 +264,11 @@ __device__ __forceinline__ bool plan_piece(const Block8Args& a, PlanShared* ps, 
 // heads a warp. HG: warps a team.
 template <typename Code, int DP, int NT, int HG>
 __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Block8Args a) {
-  constexpr int kStages = ring_stages(DP, NT, HG);
+  constexpr int kTiles = step_tiles(DP);
+  constexpr int kStages = ring_stages(DP, HG);
   constexpr int kTileBytes = kB8Tile * DP;
-  constexpr int kStageBytes = 2 * kTileBytes + kB8Meta;
+  constexpr int kPlace = 2 * kTileBytes + kB8Meta;  // a tile's codes (keys, values) and what goes with them
+  constexpr int kStageBytes = kTiles * kPlace;
   constexpr int kUnits = DP / 16;             // 16-byte units of a row
   constexpr int kRows = 32 / kUnits;          // rows one copy instruction of a warp covers
   constexpr int kBlocks = kB8Tile / kRows;    // copy instructions of one tensor's tile
@@ -293,7 +306,10 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
   int l_win = 0;                  // first entry of the window
   int w_page = -1, w_col = 0, n_page = -1, n_col = 0;  // this lane's entry of the window, of the next one
   int l_b = 0, l_h = 0, l_len = 0;
-  const int page_tiles = max(1, a.page_size / kB8Tile);
+  const int page_tiles = a.page_size / kB8Tile;  // 0: pages of 8 tokens
+  const int unit = lane % kUnits, sub = lane / kUnits;
+  const uint32_t unit_bytes = unit * 16 < a.head_dim ? 16u : 0u;  // channels past head_dim are zero-filled
+  const uint32_t dst0 = unit_offset<DP>(sub, unit);
 
   const auto read_entry = [&](int e, int& page, int& col) {
     page = -1;
@@ -313,6 +329,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
     }
   };
 
+  // Copies the team's next step to a stage; a segment's last step may end in tiles of nothing.
   const auto issue = [&](int slot) {
     while (l_t >= l_t1) {
       Segment s;
@@ -328,7 +345,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       l_t = s.x0 + ts * part;
       l_t1 = min(s.x1, l_t + part);
       if (l_t >= l_t1) continue;
-      if (a.page_size == 8) {
+      if (page_tiles == 0) {
         l_entry = 2 * l_t;
       } else {
         l_entry = l_t / page_tiles;
@@ -338,56 +355,77 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       read_entry(l_win + lane, w_page, w_col);
       read_entry(l_win + 32 + lane, n_page, n_col);
     }
-    if (l_entry - l_win >= 32) {
-      l_win += 32;
-      w_page = n_page;
-      w_col = n_col;
-      read_entry(l_win + 32 + lane, n_page, n_col);
-    }
-    int page[2], valid[2];
-    int64_t base[2];
+    const uint8_t* const base = a.k_cache + static_cast<int64_t>(l_h) * a.head_stride +
+                                static_cast<int64_t>(sub) * a.token_stride + unit * 16;
+    const int64_t to_values = a.v_cache - a.k_cache;
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {  // the tile's two octets of tokens
-      const int e = a.page_size == 8 ? l_entry + o : l_entry;
-      const int off = a.page_size == 8 ? 0 : l_sub * kB8Tile + o * 8;
-      page[o] = __shfl_sync(0xffffffffu, w_page, e - l_win);
-      const int col = __shfl_sync(0xffffffffu, w_col, e - l_win);
-      valid[o] = page[o] < 0 ? 0 : max(0, min(8, l_len - (col * a.page_size + off)));
-      base[o] = max(page[o], 0) * a.page_stride + off * a.token_stride + l_h * a.head_stride;
-    }
-    const uint32_t stage = ring + slot * kStageBytes;
-    const int unit = lane % kUnits, sub = lane / kUnits;
-#pragma unroll
-    for (int i = 0; i < (2 * kBlocks + HG - 1) / HG; ++i) {
-      const int blk = i * HG + hg;
-      if (2 * kBlocks % HG == 0 || blk < 2 * kBlocks) {
-        const int tensor = blk / kBlocks, row = (blk % kBlocks) * kRows + sub;
-        const bool second = ((blk % kBlocks) * kRows) >> 3;
-        const bool there = (row & 7) < (second ? valid[1] : valid[0]) && unit * 16 < a.head_dim;
-        const uint8_t* src = (tensor ? a.v_cache : a.k_cache) +
-                             (there ? (second ? base[1] : base[0]) + (row & 7) * a.token_stride + unit * 16 : 0);
-        cp_async16(stage + tensor * kTileBytes + unit_offset<DP>(row, unit), src, there ? 16u : 0u, policy);
+    for (int q = 0; q < kTiles; ++q, ++l_t) {
+      const uint32_t stage = ring + slot * kStageBytes + q * kPlace;
+      if (l_entry - l_win >= 32) {
+        l_win += 32;
+        w_page = n_page;
+        w_col = n_col;
+        read_entry(l_win + 32 + lane, n_page, n_col);
       }
-    }
-    if (hg == 0 && lane < 4) {
-      const bool there = (lane & 1 ? valid[1] : valid[0]) > 0;
-      const float* src = (lane >> 1 ? a.v_scale : a.k_scale) +
-                         (there ? static_cast<int64_t>(lane & 1 ? page[1] : page[0]) * a.num_kv_heads + l_h : 0);
-      cp_async4(stage + 2 * kTileBytes + lane * 4, src, there ? 4u : 0u);
-      if (lane == 0) {
-        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(stage + 2 * kTileBytes + 16), "r"(valid[0]),
-                     "r"(valid[1])
-                     : "memory");
+      int page0 = __shfl_sync(0xffffffffu, w_page, l_entry - l_win), page1 = page0;
+      const int col = a.selected ? __shfl_sync(0xffffffffu, w_col, l_entry - l_win) : l_entry;
+      int valid0, valid1;  // tokens of the tile's two octets
+      const bool some = l_t < l_t1;
+      // A row past the valid ones is still a row of its page (or of page 0): only its size is 0.
+      if (page_tiles != 0) {
+        const int left = some && page0 >= 0 ? l_len - col * a.page_size - l_sub * kB8Tile : 0;
+        const uint8_t* const src = base + static_cast<int64_t>(max(page0, 0)) * a.page_stride +
+                                   static_cast<int64_t>(l_sub * kB8Tile) * a.token_stride;
+        valid0 = max(0, min(8, left));
+        valid1 = max(0, min(8, left - 8));
+        const int64_t step = static_cast<int64_t>(kRows) * a.token_stride;
+#pragma unroll
+        for (int i = 0; i < (2 * kBlocks + HG - 1) / HG; ++i) {
+          const int blk = i * HG + hg;
+          if (2 * kBlocks % HG == 0 || blk < 2 * kBlocks) {
+            const int tensor = blk / kBlocks, j = blk % kBlocks;
+            cp_async16(stage + tensor * kTileBytes + row_block<DP>(dst0, j * kRows),
+                       src + j * step + (tensor ? to_values : 0), j * kRows + sub < left ? unit_bytes : 0u, policy);
+          }
+        }
+        if (++l_sub == page_tiles) {
+          l_sub = 0;
+          ++l_entry;
+        }
+      } else {  // two pages of 8 tokens
+        page1 = __shfl_sync(0xffffffffu, w_page, l_entry + 1 - l_win);
+        const int col1 = a.selected ? __shfl_sync(0xffffffffu, w_col, l_entry + 1 - l_win) : l_entry + 1;
+        valid0 = some && page0 >= 0 ? max(0, min(8, l_len - col * 8)) : 0;
+        valid1 = some && page1 >= 0 ? max(0, min(8, l_len - col1 * 8)) : 0;
+#pragma unroll
+        for (int i = 0; i < (2 * kBlocks + HG - 1) / HG; ++i) {
+          const int blk = i * HG + hg;
+          if (2 * kBlocks % HG == 0 || blk < 2 * kBlocks) {
+            const int tensor = blk / kBlocks, j = blk % kBlocks;
+            const bool second = j * kRows >= 8;
+            const int in_page = j * kRows & 7;
+            const uint8_t* src = base + static_cast<int64_t>(max(second ? page1 : page0, 0)) * a.page_stride +
+                                 static_cast<int64_t>(in_page) * a.token_stride + (tensor ? to_values : 0);
+            cp_async16(stage + tensor * kTileBytes + row_block<DP>(dst0, j * kRows), src,
+                       in_page + sub < (second ? valid1 : valid0) ? unit_bytes : 0u, policy);
+          }
+        }
+        l_entry += 2;
+      }
+      if (hg == 0 && lane < 5) {  // (k, v) scale of either octet; the valid counts
+        const uint32_t meta = stage + 2 * kTileBytes + lane * 4;
+        if (lane < 4) {
+          const int page = lane < 2 ? page0 : page1;
+          const bool there = (lane < 2 ? valid0 : valid1) > 0;
+          const float* src = (lane & 1 ? a.v_scale : a.k_scale) +
+                             (there ? static_cast<int64_t>(page) * a.num_kv_heads + l_h : 0);
+          cp_async4(meta, src, there ? 4u : 0u);
+        } else {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(meta), "r"(valid0 | valid1 << 16) : "memory");
+        }
       }
     }
     cp_async_commit();
-    ++l_t;
-    if (a.page_size == 8) {
-      l_entry += 2;
-    } else if (++l_sub == page_tiles) {
-      l_sub = 0;
-      ++l_entry;
-    }
   };
   const auto team_barrier = [&]() {
     if constexpr (HG == 1) {
@@ -407,6 +445,9 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 #pragma unroll 1
   for (int i = 0; i < kStages - 1; ++i) issue(i);
   int slot = 0;
+  // Where this lane reads: rows g and g + 8 of the keys; rows 2c, 2c + 1, 2c + 8, 2c + 9 of the values.
+  const uint32_t k_at = unit_offset<DP>(g, c);
+  const uint32_t v_at = DP == 64 ? unit_offset<DP>(2 * c, g >> 1) + (g & 1) * 8 : unit_offset<DP>(2 * c, g);
 
   Segment s;
   while (cons.next(a, s)) {
@@ -463,7 +504,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
     float v_ref = 0.0f, v_inv = 0.0f;  // the largest value scale so far, its reciprocal
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      m[n][0] = m[n][1] = -INFINITY;
+      m[n][0] = m[n][1] = kNoMax;
       l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
       for (int f = 0; f < kHalves; ++f)
@@ -474,7 +515,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
     const int part = (s.x1 - s.x0 + a.ts - 1) / a.ts;
     const int t0 = s.x0 + ts * part, t1 = min(s.x1, t0 + part);
 #pragma unroll 1
-    for (int t = t0; t < t1; ++t) {
+    for (int t = t0; t < t1; t += kTiles) {
       cp_async_wait<kStages - 2>();
       team_barrier();
       issue(slot == 0 ? kStages - 1 : slot - 1);
@@ -482,32 +523,50 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       slot = slot + 1 == kStages ? 0 : slot + 1;
 
       // S = K.Q^T: rows (tokens) g and g + 8, columns (heads) 2c and 2c + 1.
-      float sc[NT][2][4];
+      float sc[kTiles][NT][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int q = 0; q < kTiles; ++q)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][0][i] = sc[n][1][i] = 0.0f;
+        for (int n = 0; n < NT; ++n) sc[q][n][0] = sc[q][n][1] = sc[q][n][2] = sc[q][n][3] = 0.0f;
 #pragma unroll
       for (int j = 0; j < kSteps / 4; ++j) {
-        const uint4 k0 = lds128(kt + unit_offset<DP>(g, j * 4 + c));
-        const uint4 k1 = lds128(kt + unit_offset<DP>(g + 8, j * 4 + c));
-        const uint32_t r0[4] = {k0.x, k0.y, k0.z, k0.w}, r1[4] = {k1.x, k1.y, k1.z, k1.w};
+        uint4 k0[kTiles], k1[kTiles];
+#pragma unroll
+        for (int q = 0; q < kTiles; ++q) {
+          const uint32_t at = kt + q * kPlace + (k_at ^ ((j & 1) * 64)) + (j >> 1) * 128;
+          k0[q] = lds128(at);
+          k1[q] = lds128(at + 8 * DP);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          uint32_t a0, a1, a2, a3;
-          widen<Code>(r0[i], a0, a2);
-          widen<Code>(r1[i], a1, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            Mma<__half>::run(sc[n][i & 1], a0, a1, a2, a3, qf[n][j * 4 + i][0], qf[n][j * 4 + i][1]);
+          for (int q = 0; q < kTiles; ++q) {
+            const uint32_t w0 = i == 0 ? k0[q].x : i == 1 ? k0[q].y : i == 2 ? k0[q].z : k0[q].w;
+            const uint32_t w1 = i == 0 ? k1[q].x : i == 1 ? k1[q].y : i == 2 ? k1[q].z : k1[q].w;
+            uint32_t a0, a1, a2, a3;
+            widen<Code>(w0, a0, a2);
+            widen<Code>(w1, a1, a3);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              Mma<__half>::run(sc[q][n], a0, a1, a2, a3, qf[n][j * 4 + i][0], qf[n][j * 4 + i][1]);
+            }
           }
         }
       }
 
-      const float2 ks = lds_f2(meta), vs = lds_f2(meta + 8);
-      const uint2 valid = lds64(meta + 16);
-      const bool there0 = g < static_cast<int>(valid.x), there1 = g < static_cast<int>(valid.y);
-      const float v_top = fmaxf(fabsf(vs.x), fabsf(vs.y));
+      float ks[kTiles][2], vs[kTiles][2];  // scales of the octets
+      bool there[kTiles][2];               // rows g and g + 8 within the length
+      float v_top = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kTiles; ++q) {
+        const uint4 v = lds128(meta + q * kPlace);
+        ks[q][0] = __uint_as_float(v.x), vs[q][0] = __uint_as_float(v.y);
+        ks[q][1] = __uint_as_float(v.z), vs[q][1] = __uint_as_float(v.w);
+        v_top = fmaxf(v_top, fmaxf(fabsf(vs[q][0]), fabsf(vs[q][1])));
+        const uint32_t valid = lds32(meta + q * kPlace + 16);
+        there[q][0] = g < static_cast<int>(valid & 0xffffu);
+        there[q][1] = g < static_cast<int>(valid >> 16);
+      }
       if (v_top > v_ref && v_top >= kLeastScale) {  // the same for the whole warp
         const float f = v_ref / v_top;
         v_ref = v_top;
@@ -521,31 +580,44 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[n][x][i][e] *= f;
       }
-      const float vr0 = vs.x * v_inv, vr1 = vs.y * v_inv;
 
-      float x[NT][4];
-      bool raise = false;
+      // Scores less the running maximum, in base 2; rows past the end at -infinity.
+      float x[kTiles][NT][4];
+      float most = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
+      for (int q = 0; q < kTiles; ++q)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[n][e] = there0 ? (sc[n][0][e] + sc[n][1][e]) * (q_mul[n][e] * ks.x) : -INFINITY;
-          x[n][2 + e] = there1 ? (sc[n][0][2 + e] + sc[n][1][2 + e]) * (q_mul[n][e] * ks.y) : -INFINITY;
-          raise |= fmaxf(x[n][e], x[n][2 + e]) > m[n][e] + kRaiseBy;
-        }
-      }
-      if (__any_sync(0xffffffffu, raise)) {
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = fmaf(sc[q][n][e], q_mul[n][e & 1] * ks[q][e >> 1], -m[n][e & 1]);
+            x[q][n][e] = there[q][e >> 1] ? v : -INFINITY;
+            most = fmaxf(most, x[q][n][e]);
+          }
+      if (__any_sync(0xffffffffu, most > kRaiseBy)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(x[n][e], x[n][2 + e]);
+            float top = -INFINITY;
+#pragma unroll
+            for (int q = 0; q < kTiles; ++q)
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                x[q][n][2 * o + e] = there[q][o] ? sc[q][n][2 * o + e] * (q_mul[n][e] * ks[q][o]) : -INFINITY;
+                top = fmaxf(top, x[q][n][2 * o + e]);
+              }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
             const float next = fmaxf(m[n][e], top);
-            const float f = next == -INFINITY ? 1.0f : exp2_fast(m[n][e] - next);
+            const float f = exp2_fast(m[n][e] - next);
             m[n][e] = next;
+#pragma unroll
+            for (int q = 0; q < kTiles; ++q) {
+              x[q][n][e] -= next;
+              x[q][n][2 + e] -= next;
+            }
             l[n][e] *= f;
 #pragma unroll
             for (int y = 0; y < kHalves; ++y)
@@ -559,19 +631,21 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       }
 
       // P^T as the value product's B operand.
-      uint32_t p0[NT], p1[NT];
+      uint32_t p0[kTiles][NT], p1[kTiles][NT];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float p[4];
+      for (int q = 0; q < kTiles; ++q) {
+        const float r0 = vs[q][0] * v_inv, r1 = vs[q][1] * v_inv;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float base = m[n][e] == -INFINITY ? 0.0f : m[n][e];
-          p[e] = exp2_fast(x[n][e] - base);
-          p[2 + e] = exp2_fast(x[n][2 + e] - base);
-          l[n][e] += p[e] + p[2 + e];
+        for (int n = 0; n < NT; ++n) {
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = exp2_fast(x[q][n][e]);
+            l[n][e & 1] += p[e];
+          }
+          p0[q][n] = movmatrix_trans(Storage<__half>::pack2(p[0] * r0, p[1] * r0));
+          p1[q][n] = movmatrix_trans(Storage<__half>::pack2(p[2] * r1, p[3] * r1));
         }
-        p0[n] = movmatrix_trans(Storage<__half>::pack2(p[0] * vr0, p[1] * vr0));
-        p1[n] = movmatrix_trans(Storage<__half>::pack2(p[2] * vr1, p[3] * vr1));
       }
 
       // O^T += V^T.P^T: a lane reads the same channels of tokens 2c, 2c + 1, 2c + 8, 2c + 9 and pairs
@@ -579,27 +653,32 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       // the lane's unit.
 #pragma unroll
       for (int y = 0; y < kHalves; ++y) {
-        constexpr int kWords = DP == 64 ? 2 : 4;
-        uint32_t w[4][kWords];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = 2 * c + (k & 1) + (k >> 1) * 8;
-          if constexpr (DP == 64) {
-            const uint2 u = lds64(vt + unit_offset<DP>(row, g >> 1) + (g & 1) * 8);
-            w[k][0] = u.x, w[k][1] = u.y;
-          } else {
-            const uint4 u = lds128(vt + unit_offset<DP>(row, y * 8 + g));
-            w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+        for (int q = 0; q < kTiles; ++q) {
+          constexpr int kWords = DP == 64 ? 2 : 4;
+          constexpr uint32_t kNext = unit_offset<DP>(1, 0) & 127;  // the permutation's change from row 2c to 2c + 1
+          uint32_t w[4][kWords];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = vt + q * kPlace + (k & 1 ? (v_at ^ kNext) + (DP == 64 ? 0 : DP) : v_at) +
+                                (k >> 1) * 8 * DP + y * 128;
+            if constexpr (DP == 64) {
+              const uint2 u = lds64(at);
+              w[k][0] = u.x, w[k][1] = u.y;
+            } else {
+              const uint4 u = lds128(at);
+              w[k][0] = u.x, w[k][1] = u.y, w[k][2] = u.z, w[k][3] = u.w;
+            }
           }
-        }
 #pragma unroll
-        for (int i = 0; i < kM; ++i) {
-          const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
-          uint32_t a0, a1, a2, a3;
-          widen<Code>(__byte_perm(w[0][i / 2], w[1][i / 2], sel), a0, a1);
-          widen<Code>(__byte_perm(w[2][i / 2], w[3][i / 2], sel), a2, a3);
+          for (int i = 0; i < kM; ++i) {
+            const uint32_t sel = i & 1 ? 0x7362u : 0x5140u;
+            uint32_t a0, a1, a2, a3;
+            widen<Code>(__byte_perm(w[0][i / 2], w[1][i / 2], sel), a0, a1);
+            widen<Code>(__byte_perm(w[2][i / 2], w[3][i / 2], sel), a2, a3);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) Mma<__half>::run(acc[n][y][i], a0, a1, a2, a3, p0[n], p1[n]);
+            for (int n = 0; n < NT; ++n) Mma<__half>::run(acc[n][y][i], a0, a1, a2, a3, p0[q][n], p1[q][n]);
+          }
         }
       }
     }
@@ -620,57 +699,61 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= v_ref;
     }
-    // Join the TS parts: the upper half hands its state to the lower half, fragment by fragment.
+    // Join the TS parts: the upper half hands its state to the lower half, fragment by fragment, half
+    // of the outputs of 8 query heads at a time.
     for (int half = a.ts >> 1; half > 0; half >>= 1) {
-      constexpr int kFloats = NT * (4 + kHalves * kM * 4);
-      float* box = joint + ((grp * (a.ts >> 1) + (ts % half)) * kFloats) * 32 + lane;
-      if (ts >= half && ts < 2 * half) {
-        int k = 0;
+      float* const box = joint + ((grp * (a.ts >> 1) + (ts % half)) * box_floats(DP)) * 32 + lane;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+      for (int n = 0; n < NT; ++n) {
+        float mine[2], other[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            box[32 * k++] = m[n][e];
-            box[32 * k++] = l[n][e];
+        for (int hf = 0; hf < 2; ++hf) {
+          if (ts >= half && ts < 2 * half) {
+            int k = 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              box[32 * k++] = m[n][e];
+              box[32 * k++] = l[n][e];
+            }
+#pragma unroll
+            for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+              for (int i = 0; i < kM / 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) box[32 * k++] = acc[n][y][hf * (kM / 2) + i][e];
           }
+          group_barrier();
+          if (ts < half) {
+            int k = 0;
 #pragma unroll
-          for (int y = 0; y < kHalves; ++y)
-#pragma unroll
-            for (int i = 0; i < kM; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) box[32 * k++] = acc[n][y][i][e];
-        }
-      }
-      group_barrier();
-      if (ts < half) {
-        int k = 0;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          float mine[2], other[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float om = box[32 * k++], ol = box[32 * k++];
-            const float next = fmaxf(m[n][e], om);
-            mine[e] = next == -INFINITY ? 0.0f : exp2_fast(m[n][e] - next);
-            other[e] = next == -INFINITY ? 0.0f : exp2_fast(om - next);
-            m[n][e] = next;
-            l[n][e] = l[n][e] * mine[e] + ol * other[e];
-          }
-#pragma unroll
-          for (int y = 0; y < kHalves; ++y)
-#pragma unroll
-            for (int i = 0; i < kM; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                acc[n][y][i][e] = acc[n][y][i][e] * mine[e & 1] + box[32 * k++] * other[e & 1];
+            for (int e = 0; e < 2; ++e) {
+              const float om = box[32 * k++], ol = box[32 * k++];
+              if (hf == 0) {
+                const float next = fmaxf(m[n][e], om);
+                mine[e] = exp2_fast(m[n][e] - next);
+                other[e] = exp2_fast(om - next);
+                m[n][e] = next;
+                l[n][e] = l[n][e] * mine[e] + ol * other[e];
               }
+            }
+#pragma unroll
+            for (int y = 0; y < kHalves; ++y)
+#pragma unroll
+              for (int i = 0; i < kM / 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  float& v = acc[n][y][hf * (kM / 2) + i][e];
+                  v = v * mine[e & 1] + box[32 * k++] * other[e & 1];
+                }
+          }
+          group_barrier();  // the boxes are free again
         }
       }
-      group_barrier();  // the boxes are free again
     }
 
-    const int64_t c_first = s.start / piece;
-    const int chunks = static_cast<int>((s.start + s.tiles - 1) / piece - c_first) + 1;
+    const int64_t row_start = piece * blockIdx.x + s.start;
+    const int64_t c_first = row_start / piece;
+    const int chunks = static_cast<int>((row_start + s.tiles - 1) / piece - c_first) + 1;
     const auto store_out = [&](int64_t row, int d, float v0, float v1, float v2, float v3) {
       uint2 w;
       if (a.q_bf16) {
@@ -738,7 +821,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
         const int quads = a.head_dim / 4;
         for (int i = ts * 32 + lane; i < heads * quads; i += 32 * a.ts) {
           const int r = i / quads, d = (i - r * quads) * 4;
-          float top = -INFINITY;
+          float top = kNoMax;
           for (int k = 0; k < chunks; ++k) top = fmaxf(top, __ldcg(&a.part_ml[slot_rows(k) + r]).x);
           float sum = 0.0f;
           float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -747,7 +830,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             const int64_t row = slot_rows(k) + r;
             const float2 ml = __ldcg(&a.part_ml[row]);
             const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row * DP + d));
-            const float w = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
+            const float w = exp2_fast(ml.x - top);
             sum += w * ml.y;
             o.x += w * v.x;
             o.y += w * v.y;
@@ -780,27 +863,26 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   }
   const int group = hq / hkv;
   p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
-  p.nt = group > 8 && p.dp < 256 ? 2 : 1;
+  if (group > (p.dp == 256 ? 64 : 128)) return false;
+  p.nt = group <= 8 || p.dp == 256 ? 1 : 2;
   p.hg = 1;
   while (p.hg * 8 * p.nt < group) p.hg *= 2;
-  if (p.hg > kB8Warps) return false;
   const int teams = kB8Warps / p.hg;
-  const int sms = sm_count();
+  const int ctas = sm_count();
   const int64_t tokens = selected > 0 ? static_cast<int64_t>(selected) * page : static_cast<int64_t>(max_pages) * page;
   const int64_t tiles = std::max<int64_t>(1, (tokens + kB8Tile - 1) / kB8Tile);
   // As many heads side by side as fill the CTA, halved while a CTA would get fewer than 4 tiles.
   p.hb = 1;
   while (2 * p.hb <= teams && 2 * p.hb <= hkv) p.hb *= 2;
-  while (p.hb > 1 && batch * tiles * ((hkv + p.hb - 1) / p.hb) < 4 * static_cast<int64_t>(sms)) p.hb /= 2;
+  while (p.hb > 1 && batch * tiles * ((hkv + p.hb - 1) / p.hb) < 4 * static_cast<int64_t>(ctas)) p.hb /= 2;
   p.ts = teams / p.hb;
   p.units = (hkv + p.hb - 1) / p.hb;
   p.min_tiles = std::max(4, p.ts);
   const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + 4);
-  p.grid = static_cast<int>(std::min<int64_t>(sms, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
-  const int stages = ring_stages(p.dp, p.nt, p.hg);
-  const int frag = p.nt * (4 + (p.dp == 256 ? 64 : p.dp == 128 ? 32 : 16));
-  p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * (2 * kB8Tile * p.dp + kB8Meta);
-  if (p.ts > 1) p.smem += static_cast<size_t>(kB8Warps / p.ts) * (p.ts / 2) * frag * 32 * sizeof(float);
+  p.grid = static_cast<int>(std::min<int64_t>(ctas, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
+  const int stages = ring_stages(p.dp, p.hg);
+  p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * step_tiles(p.dp) * (2 * kB8Tile * p.dp + kB8Meta);
+  if (p.ts > 1) p.smem += static_cast<size_t>(kB8Warps / 2) * box_floats(p.dp) * 32 * sizeof(float);
   const size_t rows = static_cast<size_t>(p.grid) * 2 * (kB8Warps / p.ts) * 8 * p.nt;
   p.partial_bytes = rows * (p.dp * sizeof(float) + sizeof(float2));
   p.sync_bytes = (1 + static_cast<size_t>(batch) * hkv * p.hg) * sizeof(uint32_t);
@@ -831,11 +913,18 @@ cudaError_t launch_heads(const Block8Args& a, const Block8Plan& p, cudaStream_t 
   }
 }
 
+// Groups of up to 8 query heads are one warp's.
+template <typename Code, int DP>
+cudaError_t launch_narrow(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
+  if (p.nt == 1) return launch_block8<Code, DP, 1, 1>(a, p, st);
+  return launch_heads<Code, DP, 2>(a, p, st);
+}
+
 template <typename Code>
 cudaError_t launch_code(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
-  if (p.dp == 256) return launch_heads<Code, 256, 1>(a, p, st);
-  if (p.nt == 1) return p.dp == 64 ? launch_block8<Code, 64, 1, 1>(a, p, st) : launch_block8<Code, 128, 1, 1>(a, p, st);
-  return p.dp == 64 ? launch_heads<Code, 64, 2>(a, p, st) : launch_heads<Code, 128, 2>(a, p, st);
+  if (p.dp == 64) return launch_narrow<Code, 64>(a, p, st);
+  if (p.dp == 128) return launch_narrow<Code, 128>(a, p, st);
+  return launch_heads<Code, 256, 1>(a, p, st);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -873,8 +962,8 @@ extern "C" int kl_paged_decode_block8(int dtype, int code_type, void* out, const
   if ((dtype != KL_FLOAT16 && dtype != KL_BFLOAT16) || (code_type != KL_CODE_E4M3 && code_type != KL_CODE_INT8) ||
       !out || !q || !k_cache || !v_cache || !k_scale || !v_scale || !block_table || !seq_lens || !sync ||
       num_pages < 0 || num_pages > INT32_MAX || block_table_stride < max_pages_per_seq ||
-      (selected == nullptr) != (num_selected == 0) || page_stride < 0 || token_stride < 0 || head_stride < 0 ||
-      page_stride % 16 != 0 || token_stride % 16 != 0 || head_stride % 16 != 0 || !aligned16(k_cache) ||
+      (selected == nullptr) != (num_selected == 0) || page_stride < 0 || token_stride < 0 || head_stride < 0 || page_stride > INT32_MAX ||
+      token_stride > INT32_MAX || head_stride > INT32_MAX || page_stride % 16 != 0 || token_stride % 16 != 0 || head_stride % 16 != 0 || !aligned16(k_cache) ||
       !aligned16(v_cache) || !aligned16(q) || !aligned16(out)) {
     return kInvalid;
   }
@@ -893,9 +982,9 @@ extern "C" int kl_paged_decode_block8(int dtype, int code_type, void* out, const
   a.block_table = block_table;
   a.seq_lens = seq_lens;
   a.selected = selected;
-  a.page_stride = page_stride;
-  a.token_stride = token_stride;
-  a.head_stride = head_stride;
+  a.page_stride = static_cast<int32_t>(page_stride);
+  a.token_stride = static_cast<int32_t>(token_stride);
+  a.head_stride = static_cast<int32_t>(head_stride);
   a.bt_stride = block_table_stride;
   a.num_pages = num_pages;
   a.batch = batch;
