@@ -817,25 +817,42 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
     if (chunks > 1) {
       group_barrier();
       if (s_last[grp]) {
-        // The group's threads share out (head, 4 channels); chunks in order.
+        // The group's threads share out (head, 4 channels). Chunks in order, eight loads in flight.
+        constexpr int kAhead = 8;
         const int quads = a.head_dim / 4;
         for (int i = ts * 32 + lane; i < heads * quads; i += 32 * a.ts) {
           const int r = i / quads, d = (i - r * quads) * 4;
-          float top = kNoMax;
-          for (int k = 0; k < chunks; ++k) top = fmaxf(top, __ldcg(&a.part_ml[slot_rows(k) + r]).x);
-          float sum = 0.0f;
+          float top = kNoMax, sum = 0.0f;
           float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-          for (int k = 0; k < chunks; ++k) {
-            const int64_t row = slot_rows(k) + r;
-            const float2 ml = __ldcg(&a.part_ml[row]);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(a.part_o + row * DP + d));
-            const float w = exp2_fast(ml.x - top);
-            sum += w * ml.y;
-            o.x += w * v.x;
-            o.y += w * v.y;
-            o.z += w * v.z;
-            o.w += w * v.w;
+          for (int k0 = 0; k0 < chunks; k0 += kAhead) {
+            float2 ml[kAhead];
+            float4 v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              ml[k] = make_float2(kNoMax, 0.0f);
+              v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+              if (k0 + k < chunks) {
+                const int64_t row = slot_rows(k0 + k) + r;
+                ml[k] = __ldcg(&a.part_ml[row]);
+                v[k] = __ldcg(reinterpret_cast<const float4*>(a.part_o + row * DP + d));
+              }
+            }
+            float next = top;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) next = fmaxf(next, ml[k].x);
+            const float f = exp2_fast(top - next);
+            top = next;
+            sum *= f;
+            o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+              const float w = exp2_fast(ml[k].x - top);
+              sum = fmaf(w, ml[k].y, sum);
+              o.x = fmaf(w, v[k].x, o.x);
+              o.y = fmaf(w, v[k].y, o.y);
+              o.z = fmaf(w, v[k].z, o.z);
+              o.w = fmaf(w, v[k].w, o.w);
+            }
           }
           const float f = sum != 0.0f ? 1.0f / sum : 0.0f;
           store_out(q_row + r, d, o.x * f, o.y * f, o.z * f, o.w * f);
@@ -850,7 +867,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 // ------------------------------------------------------------------------- host side
 
 struct Block8Plan {
-  int dp, nt, hg, hb, ts, units, min_tiles, grid;
+  int dp, nt, hg, hb, ts, units, min_tiles, row_charge, grid;
   size_t smem, partial_bytes, sync_bytes;
 };
 
@@ -871,14 +888,20 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   const int ctas = sm_count();
   const int64_t tokens = selected > 0 ? static_cast<int64_t>(selected) * page : static_cast<int64_t>(max_pages) * page;
   const int64_t tiles = std::max<int64_t>(1, (tokens + kB8Tile - 1) / kB8Tile);
-  // As many heads side by side as fill the CTA, halved while a CTA would get fewer than 4 tiles.
+  // As many heads side by side as fill the CTA, halved while the rows are under a fifth of the CTAs: a
+  // row that many CTAs share is joined from as many states. Measured (us, 32/8 heads of 128; HB 8, 4,
+  // 2, 1): batch 1 x 32768 tokens 76, 35, 25.5, 23.5; 8 x 4096 30.0, 24.0, 23.3, 24.8; 16 x 2048 27.1,
+  // 22.5, 24.3, 27.4; 64 x 4096 94.7, 96.0, 100, 108.
   p.hb = 1;
   while (2 * p.hb <= teams && 2 * p.hb <= hkv) p.hb *= 2;
-  while (p.hb > 1 && batch * tiles * ((hkv + p.hb - 1) / p.hb) < 4 * static_cast<int64_t>(ctas)) p.hb /= 2;
+  while (p.hb > 1 && batch * static_cast<int64_t>((hkv + p.hb - 1) / p.hb) * 5 < ctas) p.hb /= 2;
   p.ts = teams / p.hb;
   p.units = (hkv + p.hb - 1) / p.hb;
+  // Starting a row costs a CTA a few microseconds whatever its heads, 8 tiles of every one of its TS
+  // parts; a short row, split or not, is not worth charging more than half of itself.
+  p.row_charge = static_cast<int>(std::min<int64_t>(8 * p.ts, std::max<int64_t>(4, tiles / 2)));
   p.min_tiles = std::max(4, p.ts);
-  const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + 4);
+  const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + p.row_charge);
   p.grid = static_cast<int>(std::min<int64_t>(ctas, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
   const int stages = ring_stages(p.dp, p.hg);
   p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * step_tiles(p.dp) * (2 * kB8Tile * p.dp + kB8Meta);
@@ -1001,7 +1024,7 @@ extern "C" int kl_paged_decode_block8(int dtype, int code_type, void* out, const
   a.ts = p.ts;
   a.units = p.units;
   a.min_tiles = p.min_tiles;
-  a.row_charge = 4;
+  a.row_charge = p.row_charge;
   a.sync = static_cast<uint32_t*>(sync);
   a.part_o = static_cast<float*>(partials);
   const size_t rows = static_cast<size_t>(p.grid) * 2 * (kB8Warps / p.ts) * 8 * p.nt;
