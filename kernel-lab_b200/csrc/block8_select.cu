@@ -32,6 +32,7 @@ namespace {
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelPages = 4;          // pages in flight a lane
+constexpr int kSelPasses = 2;         // passes of a block where the call has many
 constexpr int kSelKeys = 8192;        // keys a block holds in shared memory; longer rows stay in L2
 
 struct SelectArgs {
@@ -123,7 +124,7 @@ __device__ __forceinline__ WarpCounts count_before(int gt, int eq, int2* part) {
 
 // LANES: lanes side by side on a page (head_dim / 16 rounded up to a power of two).
 template <typename E, int LANES>
-__global__ void __launch_bounds__(kSelThreads) block_select_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const SelectArgs a) {
   constexpr int kRow = LANES * 4;           // words of one head's q part
   constexpr int kAtOnce = kSelThreads / LANES;
   extern __shared__ __align__(16) uint32_t s_dyn[];  // q words and scales; then the keys
@@ -148,38 +149,47 @@ __global__ void __launch_bounds__(kSelThreads) block_select_kernel(const SelectA
   if (lo >= n) return;
   uint32_t* const keys = a.keys + row * a.max_pages;
 
-  // ---- scores of pages [lo, hi)
+  // ---- scores of pages [lo, hi): page ids first, then their bounds, q's rounding under those loads
   uint32_t* const q_words = s_dyn;
   float* const sq = reinterpret_cast<float*>(s_dyn + a.group * 2 * kRow);
-  quantise_q<E>(a, row * a.group, kRow, q_words, sq);
-  __syncthreads();
   const int hi = min(n, lo + a.slice);
   const int sub = tid % LANES, col = tid / LANES;
   const bool wide = sub * 16 < a.head_dim;
+  const int32_t* const table = a.block_table + b * a.bt_stride;
+  int page[kSelPages];
+#pragma unroll
+  for (int k = 0; k < kSelPages; ++k) {
+    const int p = lo + k * kAtOnce + col;
+    page[k] = p < hi ? table[p] : -1;
+  }
   for (int p0 = lo; p0 < hi; p0 += kAtOnce * kSelPages) {
     uint4 bl[kSelPages], bh[kSelPages];
     float scale[kSelPages];
-    int64_t page[kSelPages];
+    uint32_t bad = 0;  // pages outside the pool
 #pragma unroll
     for (int k = 0; k < kSelPages; ++k) {
-      const int p = p0 + k * kAtOnce + col;
-      page[k] = p < hi ? a.block_table[b * a.bt_stride + p] : 0;
-    }
-#pragma unroll
-    for (int k = 0; k < kSelPages; ++k) {
-      const int p = p0 + k * kAtOnce + col;
       const bool ok = page[k] >= 0 && page[k] < a.num_pages;
-      if (p < hi && !ok && sub == 0) atomicOr(a.sync, kStatusBadPage);
+      bad |= ok ? 0u : 1u << k;
+      const int64_t at = static_cast<int64_t>(ok ? page[k] : 0) * a.num_kv_heads + h;
       bl[k] = bh[k] = make_uint4(0, 0, 0, 0);
       scale[k] = 0.0f;
-      if (p < hi && ok) {
-        const int8_t* at = a.bounds + ((page[k] * a.num_kv_heads + h) * 2) * a.head_dim + sub * 16;
+      if (ok) {
+        const int8_t* from = a.bounds + at * 2 * a.head_dim + sub * 16;
         if (wide) {
-          bl[k] = __ldg(reinterpret_cast<const uint4*>(at));
-          bh[k] = __ldg(reinterpret_cast<const uint4*>(at + a.head_dim));
+          bl[k] = __ldg(reinterpret_cast<const uint4*>(from));
+          bh[k] = __ldg(reinterpret_cast<const uint4*>(from + a.head_dim));
         }
-        scale[k] = __ldg(a.k_scale + page[k] * a.num_kv_heads + h) * a.unit;
+        scale[k] = __ldg(a.k_scale + at) * a.unit;
       }
+    }
+#pragma unroll
+    for (int k = 0; k < kSelPages; ++k) {  // the next pass's pages
+      const int p = p0 + (kSelPages + k) * kAtOnce + col;
+      page[k] = p < hi ? table[p] : -1;
+    }
+    if (p0 == lo) {
+      quantise_q<E>(a, row * a.group, kRow, q_words, sq);
+      __syncthreads();
     }
     float best = -INFINITY;  // of the page this lane ends up with
 #pragma unroll 2
@@ -214,8 +224,8 @@ __global__ void __launch_bounds__(kSelThreads) block_select_kernel(const SelectA
     const int p = p0 + k * kAtOnce + col;
     if (sub % (LANES / 4) == 0 && p < hi) {
       const float f = k == 0 ? scale[0] : k == 1 ? scale[1] : k == 2 ? scale[2] : scale[3];
-      const int64_t id = k == 0 ? page[0] : k == 1 ? page[1] : k == 2 ? page[2] : page[3];
-      const bool ok = id >= 0 && id < a.num_pages;
+      const bool ok = (bad >> k & 1u) == 0;
+      if (!ok) atomicOr(a.sync, kStatusBadPage);
       keys[p] = ok ? key_of(best * f) : key_of(-INFINITY);
     }
   }
@@ -427,15 +437,14 @@ extern "C" int kl_paged_block_select(int dtype, int code_type, int32_t* selected
   a.sink = sink_pages;
   a.recent = recent_pages;
   a.unit = static_cast<float>(code_type == KL_CODE_E4M3 ? E4m3Code::kBoundUnit : Int8Code::kBoundUnit);
-  // Slices of whole passes of a block (its threads' four pages each), so many that the grid holds
-  // about four blocks an SM where the rows allow.
+  // A block scores kSelPasses passes (its threads' four pages each): the second pass's loads hide behind
+  // the first, and short rows leave no block idle for long.
   const int units = head_dim / 16;
   const int lanes = units <= 4 ? 4 : units <= 8 ? 8 : 16;
   const int pass = kSelThreads / lanes * kSelPages;
-  const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
   const int64_t passes = std::max<int64_t>(1, (static_cast<int64_t>(max_pages_per_seq) + pass - 1) / pass);
-  const int64_t cut = std::max<int64_t>(1, std::min<int64_t>(passes, 4 * static_cast<int64_t>(sm_count()) / rows));
-  const int64_t per = (passes + cut - 1) / cut;
+  const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
+  const int64_t per = rows * passes <= 4 * static_cast<int64_t>(sm_count()) ? 1 : kSelPasses;
   a.slice = static_cast<int>(std::min<int64_t>(per * pass, INT32_MAX));
   const dim3 grid(static_cast<unsigned>((passes + per - 1) / per), static_cast<unsigned>(num_kv_heads),
                   static_cast<unsigned>(batch));
