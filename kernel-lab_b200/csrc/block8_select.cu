@@ -14,7 +14,7 @@
 // flight a lane; the group's q sits in shared memory and is read once for the four pages. The four
 // sums are reduced over the lanes by halving (each step exchanges half of the sums), then the score
 // goes to scratch as an order-preserving integer. The block that completes the row's count selects:
-// a radix selection over the keys in shared memory (a digit of 8 bits a pass, from the first bit in
+// a radix selection over the keys in its registers (a digit of 8 bits a pass, from the first bit in
 // which they differ, ending when a digit's keys are all wanted), then a compaction in page order.
 // Blocks wait for no other.
 #include <cuda_runtime.h>
@@ -33,7 +33,7 @@ constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kSelPages = 4;          // pages in flight a lane
 constexpr int kSelPasses = 2;         // passes of a block where the call has many
-constexpr int kSelKeys = 8192;        // keys a block holds in shared memory; longer rows stay in L2
+constexpr int kSelFew = 8, kSelMany = 16;  // keys a thread holds: rows of up to 2048 pages, chunks of 4096
 
 struct SelectArgs {
   int32_t* selected;
@@ -63,63 +63,197 @@ __device__ __forceinline__ int pages_in_use(const SelectArgs& a, int b) {
   return len > 0 ? static_cast<int>((len - 1) / a.page_size + 1) : 0;
 }
 
-// q of the group's query heads as int8: the positive parts, then the negative parts, `row` words each.
+// This lane's 8 elements of a query head: channels 4 * lane .. + 3 and 128 more.
 template <typename E>
-__device__ __forceinline__ void quantise_q(const SelectArgs& a, int64_t first_head, int row, uint32_t* words,
-                                           float* sq) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int n = warp; n < a.group; n += kSelWarps) {
-    const E* q = static_cast<const E*>(a.q) + (first_head + n) * a.head_dim;
-    float v[8];
-    float top = 0.0f;
+__device__ __forceinline__ void load_q(const SelectArgs& a, int64_t head, float (&v)[8]) {
+  const E* q = static_cast<const E*>(a.q) + head * a.head_dim;
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+  for (int i = 0; i < 8; ++i) {
+    const int d = (i >> 2) * 128 + lane * 4 + (i & 3);
+    v[i] = d < a.head_dim ? Storage<E>::load(q[d]) : 0.0f;
+  }
+}
+
+// A query head as int8: the positive parts, then the negative parts, `row` words each. By one warp.
+__device__ __forceinline__ void quantise_q(const float (&v)[8], int row, uint32_t* words, float* sq) {
+  const int lane = threadIdx.x & 31;
+  float top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = (k * 32 + lane) * 4 + j;
-        v[k * 4 + j] = d < a.head_dim ? Storage<E>::load(q[d]) : 0.0f;
-        const float f = fabsf(v[k * 4 + j]);
-        if (f <= FLT_MAX) top = fmaxf(top, f);
-      }
+  for (int i = 0; i < 8; ++i) {
+    if (fabsf(v[i]) <= FLT_MAX) top = fmaxf(top, fabsf(v[i]));
+  }
+  const float scale = warp_allreduce_max(top) * kPer127;
+  const float inv = reciprocal_scale(scale);
+  if (lane == 0) *sq = scale;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    uint32_t up = 0, down = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int qi = max(-127, min(127, __float2int_rn(v[k * 4 + j] * inv)));  // NaN: 0
+      up |= static_cast<uint32_t>(max(qi, 0) & 0xff) << (8 * j);
+      down |= static_cast<uint32_t>(min(qi, 0) & 0xff) << (8 * j);
     }
-    const float scale = warp_allreduce_max(top) * kPer127;
-    const float inv = reciprocal_scale(scale);
-    if (lane == 0) sq[n] = scale;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t up = 0, down = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int qi = max(-127, min(127, __float2int_rn(v[k * 4 + j] * inv)));  // NaN: 0
-        up |= static_cast<uint32_t>(max(qi, 0) & 0xff) << (8 * j);
-        down |= static_cast<uint32_t>(min(qi, 0) & 0xff) << (8 * j);
-      }
-      const int w = k * 32 + lane;
-      if (w < row) {
-        words[n * 2 * row + w] = up;
-        words[n * 2 * row + row + w] = down;
-      }
+    const int w = k * 32 + lane;
+    if (w < row) {
+      words[w] = up;
+      words[row + w] = down;
     }
   }
 }
 
-// Sum over the block of two counts and the exclusive sums before this warp.
-struct WarpCounts {
-  int gt_before, eq_before, gt, eq;
+struct SelectShared {
+  uint32_t hist[2][kSelThreads];  // a digit of 8 bits, two passes in turn
+  uint32_t red[2][kSelWarps];
+  int2 before[kSelMany * kSelWarps];  // keys above / at the threshold before each 32 of a chunk
+  int2 total;
+  int digit, rest, exact;
 };
-__device__ __forceinline__ WarpCounts count_before(int gt, int eq, int2* part) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  __syncthreads();
-  if (lane == 0) part[warp] = make_int2(gt, eq);
-  __syncthreads();
-  WarpCounts c{0, 0, 0, 0};
+
+// All threads: writes to `out` the indices of the `want` largest of keys[0, count) in ascending order,
+// `first` added, ties to the lower index. A thread holds PER keys, index j * 256 + its own; rows longer
+// than that are read again from L2 for each pass.
+template <int PER>
+__device__ __forceinline__ void select_largest(const uint32_t* keys, int count, int want, int first, int32_t* out,
+                                               SelectShared& sh) {
+  constexpr int kChunk = PER * kSelThreads;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t k[PER];
+  const auto read = [&](int c0) {
 #pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) {
-    if (w < warp) c.gt_before += part[w].x, c.eq_before += part[w].y;
-    c.gt += part[w].x;
-    c.eq += part[w].y;
+    for (int j = 0; j < PER; ++j) {
+      const int i = c0 + j * kSelThreads + tid;
+      k[j] = i < count ? __ldcg(keys + i) : 0u;
+    }
+  };
+  // f(key) over the chunk's keys of this thread; a chunk that is the only one stays in registers.
+  const bool once = count <= kChunk;
+  read(0);
+  const auto for_keys = [&](auto&& f) {
+    for (int c0 = 0; c0 < count; c0 += kChunk) {
+      if (!once) read(c0);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        if (c0 + j * kSelThreads + tid < count) f(k[j]);
+      }
+    }
+  };
+
+  // The bits in which the keys differ: from the highest of (and ^ or) down.
+  uint32_t all_and = 0xffffffffu, all_or = 0;
+  for_keys([&](uint32_t key) { all_and &= key, all_or |= key; });
+  all_and = __reduce_and_sync(0xffffffffu, all_and);
+  all_or = __reduce_or_sync(0xffffffffu, all_or);
+  if (lane == 0) sh.red[0][warp] = all_and, sh.red[1][warp] = all_or;
+  sh.hist[0][tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kSelWarps; ++w) all_and &= sh.red[0][w], all_or |= sh.red[1][w];
+  const uint32_t differ = all_and ^ all_or;
+  int low = differ ? 32 - __clz(differ) : 0;  // bits from `low` up are decided
+  // The threshold's decided bits. Keys above it are in; of the keys equal to it in those bits the first
+  // `rest` are.
+  uint32_t prefix = low < 32 ? all_or >> low << low : 0u;
+  int rest = want;
+  for (int pass = 0; low > 0; ++pass) {
+    uint32_t* const hist = sh.hist[pass & 1];
+    const int shift = max(0, low - 8);
+    const uint32_t decided = low < 32 ? 0xffffffffu << low : 0u, digits = 0xffu >> (8 - (low - shift));
+    for_keys([&](uint32_t key) {
+      if ((key & decided) == prefix) atomicAdd(&hist[(key >> shift) & digits], 1u);
+    });
+    __syncthreads();
+    sh.hist[(pass + 1) & 1][tid] = 0;
+    if (warp == 0) {  // lane l: digits 255 - 8l down; the digit at which the count reaches `rest`
+      const uint4 hi = *reinterpret_cast<const uint4*>(&hist[252 - lane * 8]);
+      const uint4 lo = *reinterpret_cast<const uint4*>(&hist[248 - lane * 8]);
+      const uint32_t c[8] = {hi.w, hi.z, hi.y, hi.x, lo.w, lo.z, lo.y, lo.x};
+      const uint32_t sum = c[0] + c[1] + c[2] + c[3] + c[4] + c[5] + c[6] + c[7];
+      uint32_t inc = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      uint32_t above = inc - sum;
+      const uint32_t target = static_cast<uint32_t>(rest);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (above < target && above + c[j] >= target) {
+          sh.digit = 255 - (lane * 8 + j);
+          sh.rest = static_cast<int>(target - above);
+          sh.exact = above + c[j] == target;  // every key of this digit is wanted
+        }
+        above += c[j];
+      }
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(sh.digit) << shift;
+    rest = sh.rest;
+    low = shift;
+    if (sh.exact) break;
   }
-  return c;
+  const uint32_t mask = 0xffffffffu << low;  // low < 32: the first digit decides eight bits
+
+  // Compaction: counts of each 32 keys, their sums before each, then the indices.
+  int gt_at = 0, eq_at = 0;
+  for (int c0 = 0; c0 < count; c0 += kChunk) {
+    if (!once) read(c0);
+    const auto votes = [&](int j, uint32_t& gt, uint32_t& eq) {
+      const bool in = c0 + j * kSelThreads + tid < count;
+      const uint32_t key = k[j] & mask;
+      gt = __ballot_sync(0xffffffffu, in && key > prefix);
+      eq = __ballot_sync(0xffffffffu, in && key == prefix);
+    };
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      uint32_t gt, eq;
+      votes(j, gt, eq);
+      if (lane == 0) sh.before[j * kSelWarps + warp] = make_int2(__popc(gt), __popc(eq));
+    }
+    __syncthreads();
+    if (warp == 0) {
+      constexpr int kEach = PER * kSelWarps / 32;
+      int2 c[kEach];
+      int g = 0, e = 0;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        c[i] = sh.before[lane * kEach + i];
+        g += c[i].x;
+        e += c[i].y;
+      }
+      int gi = g, ei = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, gi, o), y = __shfl_up_sync(0xffffffffu, ei, o);
+        if (lane >= o) gi += x, ei += y;
+      }
+      if (lane == 31) sh.total = make_int2(gi, ei);
+      g = gi - g;
+      e = ei - e;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        sh.before[lane * kEach + i] = make_int2(g, e);
+        g += c[i].x;
+        e += c[i].y;
+      }
+    }
+    __syncthreads();
+    const uint32_t below = (1u << lane) - 1u;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      uint32_t gt, eq;
+      votes(j, gt, eq);
+      const int2 b = sh.before[j * kSelWarps + warp];
+      const int g = gt_at + b.x + __popc(gt & below), e = eq_at + b.y + __popc(eq & below);
+      const bool tie = (eq >> lane) & 1u;
+      if (((gt >> lane) & 1u) || (tie && e < rest)) out[g + min(e, rest)] = first + c0 + j * kSelThreads + tid;
+    }
+    gt_at += sh.total.x;
+    eq_at += sh.total.y;
+    __syncthreads();
+  }
 }
 
 // LANES: lanes side by side on a page (head_dim / 16 rounded up to a power of two).
@@ -127,18 +261,28 @@ template <typename E, int LANES>
 __global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const SelectArgs a) {
   constexpr int kRow = LANES * 4;           // words of one head's q part
   constexpr int kAtOnce = kSelThreads / LANES;
-  extern __shared__ __align__(16) uint32_t s_dyn[];  // q words and scales; then the keys
-  __shared__ uint32_t s_hist[kSelThreads];  // a digit of 8 bits
-  __shared__ uint32_t s_red[2][kSelWarps];
-  __shared__ int2 s_part[kSelWarps];
-  __shared__ int s_last, s_digit, s_rest;
+  extern __shared__ __align__(16) uint32_t s_dyn[];  // q words and scales
+  __shared__ __align__(16) SelectShared s_sel;
+  __shared__ int s_last;
 
   wait_prior_grid();
   allow_next_grid();
-  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int n = pages_in_use(a, b);
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5;
+  // What needs no length is asked for together with it: this warp's first query head and the first
+  // pass's pages (entries past the length lie in the table and are not used).
+  const int sub = tid % LANES, col = tid / LANES;
+  const int32_t* const table = a.block_table + b * a.bt_stride;
   const int lo = blockIdx.x * a.slice;
   const int64_t row = static_cast<int64_t>(b) * a.num_kv_heads + h;
+  int page[kSelPages];
+#pragma unroll
+  for (int k = 0; k < kSelPages; ++k) {
+    const int p = lo + k * kAtOnce + col;
+    page[k] = p < a.max_pages ? table[p] : -1;
+  }
+  float q_first[8];
+  if (warp < a.group) load_q<E>(a, row * a.group + warp, q_first);
+  const int n = pages_in_use(a, b);
   int32_t* out = a.selected + row * a.num_selected;
   if (n <= a.num_selected) {  // every page
     if (blockIdx.x == 0) {
@@ -149,26 +293,18 @@ __global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const Sele
   if (lo >= n) return;
   uint32_t* const keys = a.keys + row * a.max_pages;
 
-  // ---- scores of pages [lo, hi): page ids first, then their bounds, q's rounding under those loads
+  // ---- scores of pages [lo, hi), q's rounding under the first bounds' loads
   uint32_t* const q_words = s_dyn;
   float* const sq = reinterpret_cast<float*>(s_dyn + a.group * 2 * kRow);
   const int hi = min(n, lo + a.slice);
-  const int sub = tid % LANES, col = tid / LANES;
   const bool wide = sub * 16 < a.head_dim;
-  const int32_t* const table = a.block_table + b * a.bt_stride;
-  int page[kSelPages];
-#pragma unroll
-  for (int k = 0; k < kSelPages; ++k) {
-    const int p = lo + k * kAtOnce + col;
-    page[k] = p < hi ? table[p] : -1;
-  }
   for (int p0 = lo; p0 < hi; p0 += kAtOnce * kSelPages) {
     uint4 bl[kSelPages], bh[kSelPages];
     float scale[kSelPages];
     uint32_t bad = 0;  // pages outside the pool
 #pragma unroll
     for (int k = 0; k < kSelPages; ++k) {
-      const bool ok = page[k] >= 0 && page[k] < a.num_pages;
+      const bool ok = p0 + k * kAtOnce + col < hi && page[k] >= 0 && page[k] < a.num_pages;
       bad |= ok ? 0u : 1u << k;
       const int64_t at = static_cast<int64_t>(ok ? page[k] : 0) * a.num_kv_heads + h;
       bl[k] = bh[k] = make_uint4(0, 0, 0, 0);
@@ -188,7 +324,10 @@ __global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const Sele
       page[k] = p < hi ? table[p] : -1;
     }
     if (p0 == lo) {
-      quantise_q<E>(a, row * a.group, kRow, q_words, sq);
+      for (int m = warp; m < a.group; m += kSelWarps) {
+        if (m != warp) load_q<E>(a, row * a.group + m, q_first);
+        quantise_q(q_first, kRow, q_words + m * 2 * kRow, sq + m);
+      }
       __syncthreads();
     }
     float best = -INFINITY;  // of the page this lane ends up with
@@ -247,114 +386,16 @@ __global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const Sele
 
   // Pages [first, end) compete for `want` places; the sinks and the recent ones are in.
   const int first = min(a.sink, n), end = max(first, n - a.recent);
-  int want = a.num_selected - (n - (end - first));
-  const int count = end - first;
-  const uint32_t* row_keys = keys + first;
-  if (count <= kSelKeys) {
-    for (int i = tid; i < count; i += kSelThreads) s_dyn[i] = __ldcg(keys + first + i);
-    row_keys = s_dyn;
-    __syncthreads();
-  }
-  const auto key_at = [&](int i) { return row_keys == s_dyn ? s_dyn[i] : __ldcg(keys + first + i); };
-
-  // The bits in which the keys differ: from the highest of (and ^ or) down.
-  uint32_t all_and = 0xffffffffu, all_or = 0;
-  for (int i = tid; i < count; i += kSelThreads) {
-    const uint32_t k = key_at(i);
-    all_and &= k;
-    all_or |= k;
-  }
-  all_and = __reduce_and_sync(0xffffffffu, all_and);
-  all_or = __reduce_or_sync(0xffffffffu, all_or);
-  if (lane == 0) s_red[0][warp] = all_and, s_red[1][warp] = all_or;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kSelWarps; ++w) all_and &= s_red[0][w], all_or |= s_red[1][w];
-  const uint32_t differ = all_and ^ all_or;
-  int low = differ ? 32 - __clz(differ) : 0;  // bits from `low` up are decided
-  // The threshold's decided bits. Keys above it are in; of the keys equal to it in those bits the first
-  // `want` are.
-  uint32_t prefix = low < 32 ? all_or >> low << low : 0u;
-  if (want == 0) {
-    prefix = 0xffffffffu;
-    low = 0;
-  }
-  const int wanted = want;
-  while (low > 0) {
-    const int shift = max(0, low - 8);
-    s_hist[tid] = 0;
-    __syncthreads();
-    const uint32_t decided = low < 32 ? 0xffffffffu << low : 0u;
-    for (int i = tid; i < count; i += kSelThreads) {
-      const uint32_t k = key_at(i);
-      if ((k & decided) == prefix) atomicAdd(&s_hist[(k >> shift) & (0xffu >> (8 - (low - shift)))], 1u);
-    }
-    __syncthreads();
-    if (warp == 0) {  // lane l: digits 255 - 8l down; the digit at which the count reaches `want`
-      uint32_t c[8], sum = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        c[j] = s_hist[255 - (lane * 8 + j)];
-        sum += c[j];
-      }
-      uint32_t inc = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      uint32_t above = inc - sum;
-      const uint32_t target = static_cast<uint32_t>(want);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (above < target && above + c[j] >= target) {
-          s_digit = 255 - (lane * 8 + j);
-          s_rest = static_cast<int>(target - above);
-          s_last = above + c[j] == target;  // every key of this digit is wanted
-        }
-        above += c[j];
-      }
-    }
-    __syncthreads();
-    prefix |= static_cast<uint32_t>(s_digit) << shift;
-    want = s_rest;
-    low = shift;
-    if (s_last) break;
-  }
-  const uint32_t mask = 0xffffffffu << low;  // low < 32: the first digit decides eight bits
-
-  // Compaction in page order: each warp takes a run of keys, counts, then writes.
-  const int run = ((count + kSelWarps - 1) / kSelWarps + 31) & ~31;
-  const int r0 = min(count, warp * run), r1 = min(count, r0 + run);
-  int gt = 0, eq = 0;
-  for (int i = r0; i < r1; i += 32) {
-    const bool in = i + lane < r1;
-    const uint32_t k = in ? key_at(i + lane) & mask : 0u;
-    gt += __popc(__ballot_sync(0xffffffffu, in && k > prefix));
-    eq += __popc(__ballot_sync(0xffffffffu, in && k == prefix));
-  }
-  const WarpCounts c = count_before(gt, eq, s_part);
-  int gt_at = c.gt_before, eq_at = c.eq_before;
+  const int count = end - first, want = a.num_selected - (n - count);
   for (int i = tid; i < first; i += kSelThreads) out[i] = i;
-  for (int i = tid; i < n - end; i += kSelThreads) out[first + wanted + i] = end + i;
-  for (int i = r0; i < r1; i += 32) {
-    const bool in = i + lane < r1;
-    const uint32_t k = in ? key_at(i + lane) & mask : 0u;
-    const uint32_t mg = __ballot_sync(0xffffffffu, in && k > prefix);
-    const uint32_t me = __ballot_sync(0xffffffffu, in && k == prefix);
-    const uint32_t below = (1u << lane) - 1u;
-    const int g = gt_at + __popc(mg & below), e = eq_at + __popc(me & below);
-    const bool tie = (me >> lane) & 1u;
-    if (((mg >> lane) & 1u) || (tie && e < want)) out[first + g + min(e, want)] = first + i + lane;
-    gt_at += __popc(mg);
-    eq_at += __popc(me);
+  for (int i = tid; i < n - end; i += kSelThreads) out[first + want + i] = end + i;
+  if (want == 0) return;
+  if (count <= kSelFew * kSelThreads) {
+    select_largest<kSelFew>(keys + first, count, want, first, out + first, s_sel);
+  } else {
+    select_largest<kSelMany>(keys + first, count, want, first, out + first, s_sel);
   }
 }
-
-struct SelectPlan {
-  int lanes, slice, slices;
-  size_t scratch_bytes, sync_bytes;
-};
 
 bool select_pdl() {
   static const bool on = env_switch_on("KL_DECODE_PDL");
@@ -363,11 +404,9 @@ bool select_pdl() {
 
 template <typename E, int LANES>
 cudaError_t launch_select(const SelectArgs& a, dim3 grid, cudaStream_t st) {
-  const size_t q_bytes = static_cast<size_t>(a.group) * (2 * LANES * 4 + 1) * sizeof(uint32_t);
-  const size_t key_bytes = static_cast<size_t>(std::min(a.max_pages, kSelKeys)) * sizeof(uint32_t);
-  const size_t smem = std::max(q_bytes, key_bytes);
+  const size_t smem = static_cast<size_t>(a.group) * (2 * LANES * 4 + 1) * sizeof(uint32_t);
   const auto kernel = block_select_kernel<E, LANES>;
-  if (smem > 46 * 1024) {  // 48 KB less the static part
+  if (smem > 40 * 1024) {  // 48 KB less the static part
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_shared_memory(kernel, 128 * 1024, done);
     if (e != cudaSuccess) return e;
