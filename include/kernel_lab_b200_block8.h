@@ -120,7 +120,8 @@ int kl_paged_decode_block8(int dtype, int code_type, void* out, const void* q, c
  * ties go to the lower column. selected [batch, num_kv_heads, num_selected] int32 receives the
  * min(num_selected, pages in use) block-table columns in ascending order, then -1. I is exact, so the
  * choice depends on no order of summation. Infinities count as the largest code, NaN as 0.
- * num_selected >= sink_pages + recent_pages; head_dim a multiple of 16 up to 256; q fp32, fp16 or bf16.
+ * num_selected >= sink_pages + recent_pages; head_dim a multiple of 16 up to 256; q fp32, fp16 or bf16; num_pages
+ * at least 1.
  * Scratch from kl_paged_block_select_workspace_size, under kl_paged_decode's rules.
  */
 int kl_paged_block_select_workspace_size(int batch, int num_kv_heads, int max_pages_per_seq, size_t* scratch_bytes,

@@ -4,15 +4,16 @@
 // page's key bounds lo <= hi (int8),
 //   I = sum_d max(qi_d lo_d, qi_d hi_d) = sum_d max(qi_d, 0) hi_d + min(qi_d, 0) lo_d
 //   score = fl(max over the group's query heads of fl(I * sq)) * fl(unit * k_scale)
-// I is a whole number below 2^24 (at most 2 * 127 * 127 * 256 / 2), formed by four-way integer dot
-// products, so the score is the same in whatever order it is summed, and so is the choice: the
+// I is a whole number below 2^24 (at most 127 * 127 * 256), formed by int8 matrix instructions with
+// 32-bit accumulation, so the score is the same in whatever order it is summed, and so is the choice: the
 // num_selected largest, ties to the lower page, the first and last pages first of all.
 //
 // Bound by reading the bounds: 2 * head_dim bytes a page and head, a sixteenth of the page's codes at
-// 16 tokens a page. A block takes a slice of one (sequence, KV head)'s pages: 16 bytes of lo and of hi
-// a lane, head_dim / 16 lanes (rounded up to a power of two) side by side on a page, four pages in
-// flight a lane; the group's q sits in shared memory and is read once for the four pages. The four
-// sums are reduced over the lanes by halving (each step exchanges half of the sums), then the score
+// 16 tokens a page. A block takes a slice of one (sequence, KV head)'s pages, a warp 16 of them at a
+// time as the rows of mma.m16n8k32 (8 query heads as columns): the contraction runs over the channels in
+// the order in which a lane's 16-byte reads deliver them, so bounds go from global memory straight
+// into the products, eight reads in flight a lane. (By four-way dot products the same took 55
+// instructions for each head and 16 pages, and those bound the kernel.) The score
 // goes to scratch as an order-preserving integer. The block that completes the row's count selects:
 // a radix selection over the keys in its registers (a digit of 8 bits a pass, from the first bit in
 // which they differ, ending when a digit's keys are all wanted), then a compaction in page order.
@@ -31,8 +32,9 @@ namespace {
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
-constexpr int kSelPages = 4;          // pages in flight a lane
-constexpr int kSelPasses = 2;         // passes of a block where the call has many
+constexpr int kSelTile = 16;          // pages of a warp's products
+constexpr int kSelPass = kSelWarps * kSelTile;
+constexpr int kSelPasses = 4;         // passes of kSelPass pages a block takes where the call has many
 constexpr int kSelFew = 8, kSelMany = 16;  // keys a thread holds: rows of up to 2048 pages, chunks of 4096
 
 struct SelectArgs {
@@ -48,6 +50,7 @@ struct SelectArgs {
   int num_kv_heads, group, head_dim, page_size, max_pages;
   int num_selected, sink, recent;
   int slice;        // pages a block scores
+  int q_aligned;    // q's rows start on 16 bytes
   float unit;       // codes a bound's unit stands for
 };
 
@@ -58,20 +61,31 @@ __device__ __forceinline__ uint32_t key_of(float s) {
 }
 
 __device__ __forceinline__ int pages_in_use(const SelectArgs& a, int b) {
-  const int64_t cap = static_cast<int64_t>(a.max_pages) * a.page_size;
-  const int64_t len = min(static_cast<int64_t>(a.seq_lens[b]), cap);
-  return len > 0 ? static_cast<int>((len - 1) / a.page_size + 1) : 0;
+  const int len = a.seq_lens[b];
+  return len > 0 ? min(static_cast<int>(static_cast<uint32_t>(len - 1) / static_cast<uint32_t>(a.page_size)) + 1, a.max_pages) : 0;
 }
 
 // This lane's 8 elements of a query head: channels 4 * lane .. + 3 and 128 more.
 template <typename E>
 __device__ __forceinline__ void load_q(const SelectArgs& a, int64_t head, float (&v)[8]) {
-  const E* q = static_cast<const E*>(a.q) + head * a.head_dim;
   const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int d = (i >> 2) * 128 + lane * 4 + (i & 3);
-    v[i] = d < a.head_dim ? Storage<E>::load(q[d]) : 0.0f;
+  for (int k = 0; k < 2; ++k) {
+    const int d = k * 128 + lane * 4;
+    const E* q = static_cast<const E*>(a.q) + head * a.head_dim + d;
+    Vec<E, 4> e;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) e.v[j] = Storage<E>::store(0.0f);
+    if (d < a.head_dim) {  // head_dim is a multiple of 16
+      if (a.q_aligned) {
+        e = *reinterpret_cast<const Vec<E, 4>*>(q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e.v[j] = q[j];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[k * 4 + j] = Storage<E>::load(e.v[j]);
   }
 }
 
@@ -101,6 +115,16 @@ __device__ __forceinline__ void quantise_q(const float (&v)[8], int row, uint32_
       words[row + w] = down;
     }
   }
+}
+
+// D += A (16 x 32, row) * B (32 x 8, col), int8, 32-bit accumulation.
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 struct SelectShared {
@@ -256,28 +280,27 @@ __device__ __forceinline__ void select_largest(const uint32_t* keys, int count, 
   }
 }
 
-// LANES: lanes side by side on a page (head_dim / 16 rounded up to a power of two).
-template <typename E, int LANES>
-__global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const SelectArgs a) {
-  constexpr int kRow = LANES * 4;           // words of one head's q part
-  constexpr int kAtOnce = kSelThreads / LANES;
-  extern __shared__ __align__(16) uint32_t s_dyn[];  // q words and scales
+// CHUNKS: 16-byte pieces of a bound a lane reads (head_dim / 64, rounded up to a power of two).
+template <typename E, int CHUNKS>
+__global__ void __launch_bounds__(kSelThreads, CHUNKS == 4 ? 2 : 4) block_select_kernel(const SelectArgs a) {
+  constexpr int kRow = CHUNKS * 16;         // words of one head's q part
+  extern __shared__ __align__(16) uint32_t s_dyn[];  // q words of whole groups of 8 heads, then scales
   __shared__ __align__(16) SelectShared s_sel;
   __shared__ int s_last;
 
   wait_prior_grid();
   allow_next_grid();
-  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5;
+  const int b = blockIdx.z, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, c = lane & 3;
   // What needs no length is asked for together with it: this warp's first query head and the first
   // pass's pages (entries past the length lie in the table and are not used).
-  const int sub = tid % LANES, col = tid / LANES;
   const int32_t* const table = a.block_table + b * a.bt_stride;
   const int lo = blockIdx.x * a.slice;
   const int64_t row = static_cast<int64_t>(b) * a.num_kv_heads + h;
-  int page[kSelPages];
+  int page[2];  // of rows g and g + 8
 #pragma unroll
-  for (int k = 0; k < kSelPages; ++k) {
-    const int p = lo + k * kAtOnce + col;
+  for (int k = 0; k < 2; ++k) {
+    const int p = lo + warp * kSelTile + g + 8 * k;
     page[k] = p < a.max_pages ? table[p] : -1;
   }
   float q_first[8];
@@ -293,79 +316,78 @@ __global__ void __launch_bounds__(kSelThreads, 4) block_select_kernel(const Sele
   if (lo >= n) return;
   uint32_t* const keys = a.keys + row * a.max_pages;
 
-  // ---- scores of pages [lo, hi), q's rounding under the first bounds' loads
+  // ---- scores of pages [lo, hi)
+  const int octets = (a.group + 7) / 8;
   uint32_t* const q_words = s_dyn;
-  float* const sq = reinterpret_cast<float*>(s_dyn + a.group * 2 * kRow);
+  float* const sq = reinterpret_cast<float*>(s_dyn + octets * 8 * 2 * kRow);
   const int hi = min(n, lo + a.slice);
-  const bool wide = sub * 16 < a.head_dim;
-  for (int p0 = lo; p0 < hi; p0 += kAtOnce * kSelPages) {
-    uint4 bl[kSelPages], bh[kSelPages];
-    float scale[kSelPages];
-    uint32_t bad = 0;  // pages outside the pool
+  const int8_t* const bounds = a.bounds + h * 2 * a.head_dim + c * 16;  // of page 0
+  const int64_t page_bytes = static_cast<int64_t>(a.num_kv_heads) * 2 * a.head_dim;
+  for (int m = warp; m < octets * 8; m += kSelWarps) {  // heads past the group: zeros
+    if (m != warp && m < a.group) load_q<E>(a, row * a.group + m, q_first);
+    if (m >= a.group) {
 #pragma unroll
-    for (int k = 0; k < kSelPages; ++k) {
-      const bool ok = p0 + k * kAtOnce + col < hi && page[k] >= 0 && page[k] < a.num_pages;
-      bad |= ok ? 0u : 1u << k;
-      const int64_t at = static_cast<int64_t>(ok ? page[k] : 0) * a.num_kv_heads + h;
-      bl[k] = bh[k] = make_uint4(0, 0, 0, 0);
-      scale[k] = 0.0f;
-      if (ok) {
-        const int8_t* from = a.bounds + at * 2 * a.head_dim + sub * 16;
-        if (wide) {
-          bl[k] = __ldg(reinterpret_cast<const uint4*>(from));
-          bh[k] = __ldg(reinterpret_cast<const uint4*>(from + a.head_dim));
+      for (int i = 0; i < 8; ++i) q_first[i] = 0.0f;
+    }
+    quantise_q(q_first, kRow, q_words + m * 2 * kRow, sq + m);
+  }
+  __syncthreads();
+  for (int p0 = lo; p0 < hi; p0 += kSelPass) {
+    uint4 bh[2][CHUNKS], bl[2][CHUNKS];
+    bool ok[2];
+    float scale[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // a page outside the pool, or past the end: page 0's, unused
+      ok[k] = page[k] >= 0 && page[k] < a.num_pages;
+      const int at = ok[k] ? page[k] : 0;
+      const int8_t* from = bounds + at * page_bytes;
+#pragma unroll
+      for (int j = 0; j < CHUNKS; ++j) {
+        bh[k][j] = bl[k][j] = make_uint4(0, 0, 0, 0);
+        if ((j * 4 + c) * 16 < a.head_dim) {
+          bl[k][j] = __ldg(reinterpret_cast<const uint4*>(from + j * 64));
+          bh[k][j] = __ldg(reinterpret_cast<const uint4*>(from + j * 64 + a.head_dim));
         }
-        scale[k] = __ldg(a.k_scale + at) * a.unit;
       }
+      scale[k] = __ldg(a.k_scale + static_cast<int64_t>(at) * a.num_kv_heads + h);
     }
 #pragma unroll
-    for (int k = 0; k < kSelPages; ++k) {  // the next pass's pages
-      const int p = p0 + (kSelPages + k) * kAtOnce + col;
+    for (int k = 0; k < 2; ++k) {  // the next pass's pages
+      const int p = p0 + kSelPass + warp * kSelTile + g + 8 * k;
       page[k] = p < hi ? table[p] : -1;
     }
-    if (p0 == lo) {
-      for (int m = warp; m < a.group; m += kSelWarps) {
-        if (m != warp) load_q<E>(a, row * a.group + m, q_first);
-        quantise_q(q_first, kRow, q_words + m * 2 * kRow, sq + m);
-      }
-      __syncthreads();
-    }
-    float best = -INFINITY;  // of the page this lane ends up with
-#pragma unroll 2
-    for (int m = 0; m < a.group; ++m) {
-      const uint4 up = *reinterpret_cast<const uint4*>(q_words + m * 2 * kRow + sub * 4);
-      const uint4 down = *reinterpret_cast<const uint4*>(q_words + m * 2 * kRow + kRow + sub * 4);
-      int s[kSelPages];
+    float best[2] = {-INFINITY, -INFINITY};
+    for (int m = 0; m < a.group; m += 8) {
+      const uint32_t* const q = q_words + (m + g) * 2 * kRow + c * 4;
+      int d[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int k = 0; k < kSelPages; ++k) {
-        int v = __dp4a(static_cast<int>(up.x), static_cast<int>(bh[k].x), 0);
-        v = __dp4a(static_cast<int>(up.y), static_cast<int>(bh[k].y), v);
-        v = __dp4a(static_cast<int>(up.z), static_cast<int>(bh[k].z), v);
-        v = __dp4a(static_cast<int>(up.w), static_cast<int>(bh[k].w), v);
-        v = __dp4a(static_cast<int>(down.x), static_cast<int>(bl[k].x), v);
-        v = __dp4a(static_cast<int>(down.y), static_cast<int>(bl[k].y), v);
-        v = __dp4a(static_cast<int>(down.z), static_cast<int>(bl[k].z), v);
-        s[k] = __dp4a(static_cast<int>(down.w), static_cast<int>(bl[k].w), v);
+      for (int j = 0; j < CHUNKS; ++j) {
+        const uint4 up = *reinterpret_cast<const uint4*>(q + j * 16);
+        const uint4 down = *reinterpret_cast<const uint4*>(q + kRow + j * 16);
+        mma_s8(d, bh[0][j].x, bh[1][j].x, bh[0][j].y, bh[1][j].y, up.x, up.y);
+        mma_s8(d, bh[0][j].z, bh[1][j].z, bh[0][j].w, bh[1][j].w, up.z, up.w);
+        mma_s8(d, bl[0][j].x, bl[1][j].x, bl[0][j].y, bl[1][j].y, down.x, down.y);
+        mma_s8(d, bl[0][j].z, bl[1][j].z, bl[0][j].w, bl[1][j].w, down.z, down.w);
       }
-      // Halving: lanes with bit LANES / 2 keep pages 2, 3, the others 0, 1; then bit LANES / 4.
-      const bool up1 = (sub & (LANES / 2)) != 0, up2 = (sub & (LANES / 4)) != 0;
-      const int k0 = up1 ? s[2] : s[0], k1 = up1 ? s[3] : s[1];
-      const int g0 = up1 ? s[0] : s[2], g1 = up1 ? s[1] : s[3];
-      const int a0 = k0 + __shfl_xor_sync(0xffffffffu, g0, LANES / 2);
-      const int a1 = k1 + __shfl_xor_sync(0xffffffffu, g1, LANES / 2);
-      int sum = (up2 ? a1 : a0) + __shfl_xor_sync(0xffffffffu, up2 ? a0 : a1, LANES / 4);
 #pragma unroll
-      for (int x = LANES / 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-      best = fmaxf(best, static_cast<float>(sum) * sq[m]);
+      for (int e = 0; e < 2; ++e) {  // heads m + 2c and m + 2c + 1
+        const int head = m + 2 * c + e;
+        const float s = sq[head];
+        if (head < a.group) {
+          best[0] = fmaxf(best[0], static_cast<float>(d[e]) * s);
+          best[1] = fmaxf(best[1], static_cast<float>(d[2 + e]) * s);
+        }
+      }
     }
-    // The lanes with sub % (LANES / 4) == 0 write the page of their two high bits.
-    const int k = sub / (LANES / 4);
-    const int p = p0 + k * kAtOnce + col;
-    if (sub % (LANES / 4) == 0 && p < hi) {
-      const float f = k == 0 ? scale[0] : k == 1 ? scale[1] : k == 2 ? scale[2] : scale[3];
-      const bool ok = (bad >> k & 1u) == 0;
-      if (!ok) atomicOr(a.sync, kStatusBadPage);
-      keys[p] = ok ? key_of(best * f) : key_of(-INFINITY);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      best[k] = fmaxf(best[k], __shfl_xor_sync(0xffffffffu, best[k], 1));
+      best[k] = fmaxf(best[k], __shfl_xor_sync(0xffffffffu, best[k], 2));
+      const int p = p0 + warp * kSelTile + g + 8 * k;
+      if (c == k && p < hi) {
+        if (!ok[k]) atomicOr(a.sync, kStatusBadPage);
+        keys[p] = ok[k] ? key_of(best[k] * (scale[k] * a.unit)) : key_of(-INFINITY);
+      }
     }
   }
 
@@ -402,10 +424,11 @@ bool select_pdl() {
   return on;
 }
 
-template <typename E, int LANES>
+template <typename E, int CHUNKS>
 cudaError_t launch_select(const SelectArgs& a, dim3 grid, cudaStream_t st) {
-  const size_t smem = static_cast<size_t>(a.group) * (2 * LANES * 4 + 1) * sizeof(uint32_t);
-  const auto kernel = block_select_kernel<E, LANES>;
+  const size_t heads = static_cast<size_t>((a.group + 7) / 8) * 8;
+  const size_t smem = heads * (2 * CHUNKS * 16 + 1) * sizeof(uint32_t);
+  const auto kernel = block_select_kernel<E, CHUNKS>;
   if (smem > 40 * 1024) {  // 48 KB less the static part
     static std::atomic<uint64_t> done{0};
     const cudaError_t e = allow_shared_memory(kernel, 128 * 1024, done);
@@ -415,11 +438,10 @@ cudaError_t launch_select(const SelectArgs& a, dim3 grid, cudaStream_t st) {
 }
 
 template <typename E>
-cudaError_t launch_lanes(const SelectArgs& a, dim3 grid, cudaStream_t st) {
-  const int units = a.head_dim / 16;
-  if (units <= 4) return launch_select<E, 4>(a, grid, st);
-  if (units <= 8) return launch_select<E, 8>(a, grid, st);
-  return launch_select<E, 16>(a, grid, st);
+cudaError_t launch_chunks(const SelectArgs& a, dim3 grid, cudaStream_t st) {
+  if (a.head_dim <= 64) return launch_select<E, 1>(a, grid, st);
+  if (a.head_dim <= 128) return launch_select<E, 2>(a, grid, st);
+  return launch_select<E, 4>(a, grid, st);
 }
 
 }  // namespace
@@ -447,7 +469,7 @@ extern "C" int kl_paged_block_select(int dtype, int code_type, int32_t* selected
   if (batch < 0 || batch > 65535 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads <= 0 ||
       num_q_heads % num_kv_heads != 0 || num_q_heads / num_kv_heads > 128 || head_dim <= 0 || head_dim % 16 != 0 ||
       head_dim > 256 || page_size <= 0 || max_pages_per_seq < 0 || block_table_stride < max_pages_per_seq ||
-      num_pages < 0 || num_pages > INT32_MAX || num_selected <= 0 || sink_pages < 0 || recent_pages < 0 ||
+      num_pages <= 0 || num_pages > INT32_MAX || num_selected <= 0 || sink_pages < 0 || recent_pages < 0 ||
       static_cast<int64_t>(sink_pages) + recent_pages > num_selected || !selected || !q || !k_bounds || !k_scale ||
       !block_table || !seq_lens || !sync || (reinterpret_cast<uintptr_t>(k_bounds) & 15u) != 0) {
     return kInvalid;
@@ -475,23 +497,21 @@ extern "C" int kl_paged_block_select(int dtype, int code_type, int32_t* selected
   a.num_selected = num_selected;
   a.sink = sink_pages;
   a.recent = recent_pages;
+  a.q_aligned = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
   a.unit = static_cast<float>(code_type == KL_CODE_E4M3 ? E4m3Code::kBoundUnit : Int8Code::kBoundUnit);
-  // A block scores kSelPasses passes (its threads' four pages each): the second pass's loads hide behind
-  // the first, and short rows leave no block idle for long.
-  const int units = head_dim / 16;
-  const int lanes = units <= 4 ? 4 : units <= 8 ? 8 : 16;
-  const int pass = kSelThreads / lanes * kSelPages;
-  const int64_t passes = std::max<int64_t>(1, (static_cast<int64_t>(max_pages_per_seq) + pass - 1) / pass);
+  // A block scores kSelPasses passes where the call has many: q is rounded once for them (1 pass a block
+  // 35 us, 2 32, 4 30 for 64 ragged sequences of up to 16384 tokens).
+  const int64_t passes = std::max<int64_t>(1, (static_cast<int64_t>(max_pages_per_seq) + kSelPass - 1) / kSelPass);
   const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
   const int64_t per = rows * passes <= 4 * static_cast<int64_t>(sm_count()) ? 1 : kSelPasses;
-  a.slice = static_cast<int>(std::min<int64_t>(per * pass, INT32_MAX));
+  a.slice = static_cast<int>(std::min<int64_t>(per * kSelPass, INT32_MAX));
   const dim3 grid(static_cast<unsigned>((passes + per - 1) / per), static_cast<unsigned>(num_kv_heads),
                   static_cast<unsigned>(batch));
   const auto st = static_cast<cudaStream_t>(stream);
   switch (dtype) {
-    case KL_FLOAT32: return static_cast<int>(launch_lanes<float>(a, grid, st));
-    case KL_FLOAT16: return static_cast<int>(launch_lanes<__half>(a, grid, st));
-    case KL_BFLOAT16: return static_cast<int>(launch_lanes<__nv_bfloat16>(a, grid, st));
+    case KL_FLOAT32: return static_cast<int>(launch_chunks<float>(a, grid, st));
+    case KL_FLOAT16: return static_cast<int>(launch_chunks<__half>(a, grid, st));
+    case KL_BFLOAT16: return static_cast<int>(launch_chunks<__nv_bfloat16>(a, grid, st));
     default: return kInvalid;
   }
 }
