@@ -303,3 +303,47 @@ def e4m3_scales(cache: torch.Tensor, margin: float = 1.0) -> torch.Tensor:
     x = cache.float()
     amax = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(dim=(0, 1, 3))
     return (amax.clamp_min(1e-12) * margin / 448.0).float().contiguous()
+
+
+@dataclass
+class Block8KV:
+    """A cache held in 8 bits with a float32 scale for each page and KV head, and (for the page
+    selection) each page's key bounds; the arguments of cuda_ops.paged_kv_append_block8 and
+    paged_decode_attention_block8."""
+
+    k_cache: torch.Tensor  # [num_pages, page_size, num_kv_heads, head_dim] codes, any order in memory
+    v_cache: torch.Tensor
+    k_scale: torch.Tensor  # [num_pages, num_kv_heads]
+    v_scale: torch.Tensor
+    k_bounds: torch.Tensor | None  # [num_pages, num_kv_heads, 2, head_dim] int8
+
+
+def block8_pool(
+    num_pages: int,
+    page_size: int,
+    num_kv_heads: int,
+    head_dim: int,
+    dtype: torch.dtype = torch.float8_e4m3fn,
+    device: str | torch.device = "cuda",
+    heads_first: bool = False,
+    bounds: bool = True,
+) -> Block8KV:
+    """An empty block-scaled pool. ``dtype`` is torch.float8_e4m3fn or torch.int8. ``heads_first`` stores
+    a page head by head ([num_pages, num_kv_heads, page_size, head_dim]; the tensors keep the usual
+    order of dimensions): the order for block-sparse decode, which reads single heads of a page, one
+    contiguous run each. ``bounds`` adds what the page selection reads."""
+    if dtype not in (torch.float8_e4m3fn, torch.int8):
+        raise ValueError("block-scaled caches are float8_e4m3fn or int8")
+
+    def codes() -> torch.Tensor:
+        if heads_first:
+            flat = torch.zeros(num_pages, num_kv_heads, page_size, head_dim, dtype=torch.int8, device=device)
+            return flat.view(dtype).permute(0, 2, 1, 3)
+        return torch.zeros(num_pages, page_size, num_kv_heads, head_dim, dtype=torch.int8, device=device).view(dtype)
+
+    def scales() -> torch.Tensor:
+        return torch.zeros(num_pages, num_kv_heads, dtype=torch.float32, device=device)
+
+    shape = (num_pages, num_kv_heads, 2, head_dim)
+    return Block8KV(codes(), codes(), scales(), scales(),
+                    torch.zeros(shape, dtype=torch.int8, device=device) if bounds else None)

@@ -137,3 +137,17 @@ def test_oracle_append_then_decode_recovers_the_tokens():
                 got = block8.decode_codes(codes[t][table[0]], kind) * scales[t][table[0]][:, None, :, None]
                 err = np.abs(got.reshape(-1, 2, 16)[:37] - x[t])
                 assert err.max() <= step * np.abs(x[t]).max()
+
+
+@pytest.mark.parametrize("heads_first", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+def test_block8_pool_layouts(heads_first, dtype):
+    from kernel_lab.kv_cache import block8_pool
+
+    pool = block8_pool(5, 16, 3, 32, dtype, device="cpu", heads_first=heads_first)
+    assert pool.k_cache.shape == (5, 16, 3, 32) and pool.k_cache.dtype == dtype
+    assert pool.k_cache.stride() == ((1536, 32, 512, 1) if heads_first else (1536, 96, 32, 1))
+    assert pool.k_scale.shape == (5, 3) and pool.k_bounds.shape == (5, 3, 2, 32)
+    assert block8_pool(5, 16, 3, 32, dtype, device="cpu", bounds=False).k_bounds is None
+    with pytest.raises(ValueError):
+        block8_pool(5, 16, 3, 32, torch.float16, device="cpu")

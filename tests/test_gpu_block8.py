@@ -549,3 +549,22 @@ def test_a_step_on_another_stream_and_in_a_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(kb, bounds)
+
+
+@pytest.mark.parametrize("dtype", [torch.float8_e4m3fn, torch.int8])
+def test_the_example_step_is_close_to_a_bf16_cache(dtype):
+    """e4m3 keeps 3 fraction bits (an element is off by at most 2^-4 of itself, about 2^-5.2 in the mean
+    square), int8 with a page's scale 1 / 254 of the page's largest: keys' and values' errors together
+    stay below 0.08 and 0.04 of the output; every page selected reads as the whole."""
+    import sys
+
+    from tests.conftest import REPO
+
+    sys.path.insert(0, str(REPO / "examples"))
+    import block8_step
+
+    whole, sparse = block8_step.run(hq=16, hkv=4, prompt=300, steps=3, pages=4, dtype=dtype)
+    assert whole < (0.08 if dtype is torch.float8_e4m3fn else 0.04)
+    assert whole < sparse < 2.0
+    whole, sparse = block8_step.run(hq=16, hkv=4, prompt=100, steps=2, pages=64, dtype=dtype)
+    assert abs(whole - sparse) < 0.01
