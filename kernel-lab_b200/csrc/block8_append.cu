@@ -30,10 +30,12 @@
 #include "kernel_lab_b200_block8.h"
 
 namespace klb {
-namespace {
+// A namespace with a name: an unnamed one's symbols carry a hash of the file's text, and with them the
+// compiler's register allocation would change with a comment.
+namespace block8_append {
 
 constexpr int kBlock8AppendThreads = 128;
-constexpr int kAppendBlocks = 6;  // resident an SM that the registers are held to (5: 51.8 us for 35k prompt tokens, 6: 50.0, 7: 62.3 with spills)
+constexpr int kAppendBlocks = 5;  // resident an SM that the registers are held to: the most without spills
 
 struct Block8AppendArgs {
   uint8_t* k_cache;
@@ -680,7 +682,7 @@ cudaError_t launch_elements(const Block8AppendArgs& a, int code_type, bool vec, 
 
 bool multiple_of(int64_t n, const void* p) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-}  // namespace
+}  // namespace block8_append
 }  // namespace klb
 
 extern "C" int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache, void* v_cache, float* k_scale,
@@ -691,6 +693,7 @@ extern "C" int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache
                                          int64_t block_table_stride, int max_pages_per_seq, int64_t num_pages,
                                          int64_t new_row_stride, uint32_t* status, void* stream) {
   using namespace klb;
+  using namespace klb::block8_append;
   constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
   if (batch == 0 || tokens == 0) return 0;
   if (batch < 0 || tokens < 0 || tokens > INT32_MAX || num_kv_heads <= 0 || num_kv_heads > 32767 || head_dim <= 0 ||

@@ -43,7 +43,9 @@
 #include "kernel_lab_b200_block8.h"
 
 namespace klb {
-namespace {
+// A namespace with a name: an unnamed one's symbols carry a hash of the file's text, and with them the
+// compiler's register allocation would change with a comment.
+namespace block8_decode {
 
 constexpr int kB8Warps = 8;
 constexpr int kB8Threads = 32 * kB8Warps;
@@ -903,6 +905,7 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   p.min_tiles = std::max(4, p.ts);
   const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + p.row_charge);
   p.grid = static_cast<int>(std::min<int64_t>(ctas, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
+  if (most / p.grid >= INT32_MAX - p.min_tiles) return false;  // positions within a piece are 32 bits
   const int stages = ring_stages(p.dp, p.hg);
   p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * step_tiles(p.dp) * (2 * kB8Tile * p.dp + kB8Meta);
   if (p.ts > 1) p.smem += static_cast<size_t>(kB8Warps / 2) * box_floats(p.dp) * 32 * sizeof(float);
@@ -952,7 +955,7 @@ cudaError_t launch_code(const Block8Args& a, const Block8Plan& p, cudaStream_t s
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-}  // namespace
+}  // namespace block8_decode
 }  // namespace klb
 
 extern "C" int kl_paged_decode_block8_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim,
@@ -962,8 +965,8 @@ extern "C" int kl_paged_decode_block8_workspace_size(int batch, int num_q_heads,
   *partial_bytes = 0;
   *sync_bytes = sizeof(uint32_t);
   if (batch == 0) return 0;
-  klb::Block8Plan p;
-  if (!klb::make_block8_plan(batch, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, num_selected, p)) {
+  klb::block8_decode::Block8Plan p;
+  if (!klb::block8_decode::make_block8_plan(batch, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, num_selected, p)) {
     return static_cast<int>(cudaErrorInvalidValue);
   }
   *partial_bytes = p.partial_bytes;
@@ -980,6 +983,7 @@ extern "C" int kl_paged_decode_block8(int dtype, int code_type, void* out, const
                                       int num_selected, float scale, void* partials, size_t partial_bytes, void* sync,
                                       size_t sync_bytes, void* stream) {
   using namespace klb;
+  using namespace klb::block8_decode;
   constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
   if (batch == 0) return 0;
   if ((dtype != KL_FLOAT16 && dtype != KL_BFLOAT16) || (code_type != KL_CODE_E4M3 && code_type != KL_CODE_INT8) ||

@@ -28,7 +28,9 @@
 #include "kernel_lab_b200_block8.h"
 
 namespace klb {
-namespace {
+// A namespace with a name: an unnamed one's symbols carry a hash of the file's text, and with them the
+// compiler's register allocation would change with a comment.
+namespace block8_select {
 
 constexpr int kSelThreads = 256;
 constexpr int kSelWarps = kSelThreads / 32;
@@ -444,7 +446,7 @@ cudaError_t launch_chunks(const SelectArgs& a, dim3 grid, cudaStream_t st) {
   return launch_select<E, 4>(a, grid, st);
 }
 
-}  // namespace
+}  // namespace block8_select
 }  // namespace klb
 
 extern "C" int kl_paged_block_select_workspace_size(int batch, int num_kv_heads, int max_pages_per_seq,
@@ -464,6 +466,7 @@ extern "C" int kl_paged_block_select(int dtype, int code_type, int32_t* selected
                                      int num_selected, int sink_pages, int recent_pages, void* scratch,
                                      size_t scratch_bytes, void* sync, size_t sync_bytes, void* stream) {
   using namespace klb;
+  using namespace klb::block8_select;
   constexpr int kInvalid = static_cast<int>(cudaErrorInvalidValue);
   if (batch == 0) return 0;
   if (batch < 0 || batch > 65535 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads <= 0 ||

@@ -27,7 +27,9 @@
 #include "kernel_lab_b200_block8.h"
 
 namespace klb {
-namespace {
+// A namespace with a name: an unnamed one's symbols carry a hash of the file's text, and with them the
+// compiler's register allocation would change with a comment.
+namespace rmsnorm_fp8 {
 
 constexpr float kE4m3Max = 448.0f;
 constexpr float kPerE4m3Max = 1.0f / 448.0f;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(512, 2) rmsnorm_fp8_row_regs(const NormFp8Args
     const uint4 none = make_uint4(0, 0, 0, 0);  // packs past the row add nothing
     a[i].load(pk < packs ? __ldcs(xr + pk) : none);
     if constexpr (RES) r[i].load(pk < packs ? __ldcs(rr + pk) : none);
-    w[i].load(pk < packs ? __ldg(wr + pk) : none);
+    if constexpr (!GROUPS) w[i].load(pk < packs ? __ldg(wr + pk) : none);
   }
 
   float s0 = 0.0f, s1 = 0.0f, top = 0.0f;
@@ -213,6 +215,13 @@ __global__ void __launch_bounds__(512, 2) rmsnorm_fp8_row_regs(const NormFp8Args
     }
   }
 
+  if constexpr (GROUPS) {  // needed only from here on: in the residual's registers, under the reduction
+#pragma unroll
+    for (int i = 0; i < NPT; ++i) {
+      const int pk = threadIdx.x + i * blockDim.x;
+      w[i].load(pk < packs ? __ldg(wr + pk) : make_uint4(0, 0, 0, 0));
+    }
+  }
   const SumMax all = block_allreduce(s0 + s1, top, red);
   const float rstd = 1.0f / sqrtf(all.sum / static_cast<float>(g.hidden) + g.eps);
   allow_next_grid();
@@ -352,13 +361,14 @@ cudaError_t launch_typed(const NormFp8Args& g, int rows, cudaStream_t st) {
                     : launch_rows(rmsnorm_fp8_row_general<T, false>, rows, threads, st, g);
 }
 
-}  // namespace
+}  // namespace rmsnorm_fp8
 }  // namespace klb
 
 extern "C" int kl_rms_norm_fp8(int dtype, void* codes, float* scales, void* residual_out, const void* x,
                                const void* residual, const void* weight, int rows, int hidden, int64_t x_row_stride,
                                int group_size, float eps, void* stream) {
   using namespace klb;
+  using namespace klb::rmsnorm_fp8;
   if (rows == 0) return 0;
   if (rows < 0 || hidden <= 0 || x_row_stride < 0 || group_size < 0 || !codes || !scales || !x || !weight ||
       (residual == nullptr) != (residual_out == nullptr)) {
