@@ -122,6 +122,12 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         if not (force or stale(obj, [CSRC / src, *HEADERS, *more])):
             continue
         rel_src = str(rel_csrc / src)
+        if BLOCK8_HEADERS[0] in more:
+            # Compiled in one part the allocation depends on the source alone (checked over object names) and
+            # spills nothing that counts; in 8 parts the same text got 151 or 202 registers in the decode kernel
+            # for groups of 8 (64 x 4096 tokens 98.5 or 94.1 us), by its object's name.
+            run([nvcc, *base, "-c", rel_src, "-o", str(obj)], verbose, cwd=REPO)
+            continue
         if src != "paged_decode.cu":
             run([nvcc, *base, "--split-compile=8", "-c", rel_src, "-o", str(obj)], verbose, cwd=REPO)
             continue
