@@ -13,14 +13,17 @@
 // whatever the page holds there (NaN codes included) never reaches a product.
 //
 // Warps of a CTA. Up to 8 * NT query heads of one KV head share a warp's products, so that codes are
-// widened once for them (NT = 1 for groups of at most 8, else 2 where the registers allow). Larger groups
-// take HG warps, which form a team: they share one ring, each copies 1/HG of a tile and meets the others
+// widened once for them: NT = 1 for groups of at most 8, 2 up to 16, 4 beyond for head_dim up to 64. (For 128 the
+// outputs of 32 query heads fill the registers: 168 us against 120 on 128 ragged int8 sequences, 101
+// against 70 for a group of 64. For 64 it is 47 against 55 us, 64 x 4000 tokens of 64/2 heads.) With NT = 4
+// a lane keeps its query fragments in shared memory. Larger groups take HG warps, which form a team: they share one ring, each copies 1/HG of a tile and meets the others
 // at a named barrier once a step. The CTA's teams are HB KV heads times TS parts of the token range; the
 // TS parts' states are joined through shared memory at the end of a
 // range. Many parallel KV heads and one part where there is work for every warp (fewest joins, and
 // a page's heads are read together), more parts of fewer heads where the whole call is small. A warp
-// takes two tiles a step (one for head_dim above 128, whose ring has no room for more): a tile is a
-// chain of dependent steps, and two of them fill each other's gaps.
+// takes two tiles a step: a tile is a chain of dependent steps, and two of them fill each other's gaps. One
+// for head_dim above 128, whose ring has no room for more, and for NT = 4, whose four products a
+// fragment are independent already (39.0 us against 41.2, 16 x 4000-8000 tokens of 128/2 heads of 64).
 //
 // Balance. Rows (sequence, block of HB heads) are laid end to end, each as long as its tiles plus a
 // fixed charge for starting it, and CTA c takes the c-th equal piece, found by every CTA alone from
@@ -29,11 +32,11 @@
 // them in chunk order, so the result does not depend on which came last, and sets the counter back to
 // zero. Nobody waits for another CTA.
 //
-// Measured (e4m3, 32/8 heads of 128, pages of 16): 64 x 4096 tokens 94-99 us on different GPUs (5.5-5.7
-// TB/s, 0.84-0.87 of the copy peak: about 12 us of launch, first loads and joins are the rest), 128 x 8192
-// of 64/8 heads 338-352 us (0.94-0.97). Groups above 8 are bound by the latency of a warp's dependent steps
-// with two warps a scheduler: 128 ragged sequences of one int8 KV head for 32 query heads 120-125 us (2.0
-// TB/s, 0.31; issue 42 % busy).
+// Measured (e4m3, 32/8 heads of 128, pages of 16): 64 x 4096 tokens 94.1 us (5.7 TB/s, 0.88
+// of the copy peak: about 12 us of launch, first loads and joins are the rest), 128 x 8192 of 64/8 heads 336
+// us (0.98). Groups above 8 are bound by the latency of a warp's dependent steps
+// with two warps a scheduler: 128 ragged sequences of one int8 KV head for 32 query heads 120 us (2.0
+// TB/s, 0.31; issue 46 % busy).
 //
 // Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
 // to f16 exactly, q is divided by a power of two so that f16 holds it, k_scale and that power enter
@@ -89,11 +92,13 @@ struct Block8Args {
 
 // Tiles of a step, and stages (of a step's tiles) of a team's ring: what 227 KB hold beside the boxes of
 // the joins.
-__host__ __device__ constexpr int step_tiles(int dp) { return dp == 256 ? 1 : 2; }
-__host__ __device__ constexpr int ring_stages(int dp, int hg) {
-  const int per_warp = dp == 64 ? 6 : 3;
+__host__ __device__ constexpr int step_tiles(int dp, int nt) { return dp == 256 || nt == 4 ? 1 : 2; }
+__host__ __device__ constexpr int ring_stages(int dp, int nt, int hg) {
+  const int per_warp = dp != 64 ? 3 : nt == 4 ? 8 : 6;
   return hg * per_warp < 12 ? hg * per_warp : 12;
 }
+// Bytes in which a warp keeps its 32 query heads' fragments (none where registers hold them).
+__host__ __device__ constexpr int query_bytes(int dp, int nt) { return nt == 4 ? 8 * nt * dp * 2 : 0; }
 // Floats a lane hands over at a time in a join: the maxima and sums of 8 query heads and half of their
 // outputs.
 __host__ __device__ constexpr int box_floats(int dp) { return 4 + dp / 8; }
@@ -272,8 +277,8 @@ __device__ __forceinline__ bool plan_piece(const Block8Args& a, PlanShared* ps, 
 // heads a warp. HG: warps a team.
 template <typename Code, int DP, int NT, int HG>
 __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Block8Args a) {
-  constexpr int kTiles = step_tiles(DP);
-  constexpr int kStages = ring_stages(DP, HG);
+  constexpr int kTiles = step_tiles(DP, NT);
+  constexpr int kStages = ring_stages(DP, NT, HG);
   constexpr int kTileBytes = kB8Tile * DP;
   constexpr int kPlace = 2 * kTileBytes + kB8Meta;  // a tile's codes (keys, values) and what goes with them
   constexpr int kStageBytes = kTiles * kPlace;
@@ -284,6 +289,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
   constexpr int kM = DP == 64 ? 4 : 8;        // value products (16 output channels) of a part
   constexpr int kSteps = DP / 16;             // score products (16 channels)
   constexpr int NH = 8 * NT;
+  constexpr bool kQRegs = query_bytes(DP, NT) == 0;
 
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ PlanShared s_plan;
@@ -304,7 +310,10 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
   // No block-wide barrier from here on: teams without a head leave.
 
   const uint32_t ring = smem_u32(smem) + team * (kStages * kStageBytes);
-  float* const joint = reinterpret_cast<float*>(smem + (kB8Warps / HG) * kStages * kStageBytes);
+  constexpr int kRings = (kB8Warps / HG) * kStages * kStageBytes;
+  // The lane's own query fragments, where they are not in registers: 16 bytes are two steps of one n.
+  const uint32_t q_at = smem_u32(smem) + kRings + warp * query_bytes(DP, NT) + lane * 16;
+  float* const joint = reinterpret_cast<float*>(smem + kRings + kB8Warps * query_bytes(DP, NT));
   const uint64_t policy = l2_policy_evict_first();
 
   // ---- loading side: the team's next tile
@@ -466,7 +475,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 
     // Q as the score product's B operand: lane (g, c) holds query head g of each group of 8. The
     // contraction runs over a row's codes in the order in which a lane's 16-byte reads deliver them.
-    uint32_t qf[NT][kSteps][2];
+    uint32_t qf[kQRegs ? NT : 1][kSteps][2];
     float q_mul[NT][2];  // scale of the scores of this lane's two heads (2c, 2c + 1)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -500,8 +509,15 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
 #pragma unroll
       for (int i = 0; i < kSteps; ++i) {
-        qf[n][i][0] = Storage<__half>::pack2(v[i][0] * down, v[i][1] * down);
-        qf[n][i][1] = Storage<__half>::pack2(v[i][2] * down, v[i][3] * down);
+        qf[kQRegs ? n : 0][i][0] = Storage<__half>::pack2(v[i][0] * down, v[i][1] * down);
+        qf[kQRegs ? n : 0][i][1] = Storage<__half>::pack2(v[i][2] * down, v[i][3] * down);
+      }
+      if constexpr (!kQRegs) {
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) {
+          sts128(q_at + (n * (kSteps / 2) + i) * 512,
+                 make_uint4(qf[0][2 * i][0], qf[0][2 * i][1], qf[0][2 * i + 1][0], qf[0][2 * i + 1][1]));
+        }
       }
       q_mul[n][0] = __shfl_sync(0xffffffffu, up, 8 * c);
       q_mul[n][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
@@ -545,8 +561,15 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
           k0[q] = lds128(at);
           k1[q] = lds128(at + 8 * DP);
         }
+        uint4 qs[NT];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+          if constexpr (!kQRegs) {
+            if (i % 2 == 0) {
+#pragma unroll
+              for (int n = 0; n < NT; ++n) qs[n] = lds128(q_at + (n * (kSteps / 2) + j * 2 + i / 2) * 512);
+            }
+          }
 #pragma unroll
           for (int q = 0; q < kTiles; ++q) {
             const uint32_t w0 = i == 0 ? k0[q].x : i == 1 ? k0[q].y : i == 2 ? k0[q].z : k0[q].w;
@@ -556,7 +579,11 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             widen<Code>(w1, a1, a3);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              Mma<__half>::run(sc[q][n], a0, a1, a2, a3, qf[n][j * 4 + i][0], qf[n][j * 4 + i][1]);
+              if constexpr (kQRegs) {
+                Mma<__half>::run(sc[q][n], a0, a1, a2, a3, qf[n][j * 4 + i][0], qf[n][j * 4 + i][1]);
+              } else {
+                Mma<__half>::run(sc[q][n], a0, a1, a2, a3, i % 2 ? qs[n].z : qs[n].x, i % 2 ? qs[n].w : qs[n].y);
+              }
             }
           }
         }
@@ -889,7 +916,7 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   const int group = hq / hkv;
   p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
   if (group > (p.dp == 256 ? 64 : 128)) return false;
-  p.nt = group <= 8 || p.dp == 256 ? 1 : 2;
+  p.nt = group <= 8 || p.dp == 256 ? 1 : group <= 16 || p.dp == 128 ? 2 : 4;
   p.hg = 1;
   while (p.hg * 8 * p.nt < group) p.hg *= 2;
   const int teams = kB8Warps / p.hg;
@@ -905,15 +932,20 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   while (p.hb > 1 && batch * static_cast<int64_t>((hkv + p.hb - 1) / p.hb) * 5 < ctas) p.hb /= 2;
   p.ts = teams / p.hb;
   p.units = (hkv + p.hb - 1) / p.hb;
+  const int least = std::max(4, step_tiles(p.dp, p.nt) * p.ts);
   // Starting a row costs a CTA a few microseconds whatever its heads, 8 tiles of every one of its TS
-  // parts; a short row, split or not, is not worth charging more than half of itself.
-  p.row_charge = static_cast<int>(std::min<int64_t>(8 * p.ts, std::max<int64_t>(4, tiles / 2)));
-  p.min_tiles = std::max(4, p.ts);
+  // parts; a short row, split or not, is not worth charging more than half of itself. No piece, and no row's
+  // charge, is less than a step of every warp: two short rows in one CTA, or a chunk that leaves half of the
+  // warps idle, cost more than the CTAs saved (us without the rule and with it: 1 x 16 tokens 13.9, 8.4; 1 x 256
+  // 10.8, 9.6; 8 x 1024 of 32/1 heads 19.8, 17.2).
+  p.row_charge = static_cast<int>(std::min<int64_t>(8 * p.ts, std::max<int64_t>(least, tiles / 2)));
+  p.min_tiles = least;
   const int64_t most = batch * static_cast<int64_t>(p.units) * (tiles + p.row_charge);
   p.grid = static_cast<int>(std::min<int64_t>(ctas, std::max<int64_t>(1, (most + p.min_tiles - 1) / p.min_tiles)));
   if (most / p.grid >= INT32_MAX - p.min_tiles) return false;  // positions within a piece are 32 bits
-  const int stages = ring_stages(p.dp, p.hg);
-  p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * step_tiles(p.dp) * (2 * kB8Tile * p.dp + kB8Meta);
+  const int stages = ring_stages(p.dp, p.nt, p.hg);
+  p.smem = static_cast<size_t>(kB8Warps / p.hg) * stages * step_tiles(p.dp, p.nt) * (2 * kB8Tile * p.dp + kB8Meta) +
+           static_cast<size_t>(kB8Warps) * query_bytes(p.dp, p.nt);
   if (p.ts > 1) p.smem += static_cast<size_t>(kB8Warps / 2) * box_floats(p.dp) * 32 * sizeof(float);
   const size_t rows = static_cast<size_t>(p.grid) * 2 * (kB8Warps / p.ts) * 8 * p.nt;
   p.partial_bytes = rows * (p.dp * sizeof(float) + sizeof(float2));
@@ -945,18 +977,17 @@ cudaError_t launch_heads(const Block8Args& a, const Block8Plan& p, cudaStream_t 
   }
 }
 
-// Groups of up to 8 query heads are one warp's.
-template <typename Code, int DP>
-cudaError_t launch_narrow(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
-  if (p.nt == 1) return launch_block8<Code, DP, 1, 1>(a, p, st);
-  return launch_heads<Code, DP, 2>(a, p, st);
-}
-
 template <typename Code>
 cudaError_t launch_code(const Block8Args& a, const Block8Plan& p, cudaStream_t st) {
-  if (p.dp == 64) return launch_narrow<Code, 64>(a, p, st);
-  if (p.dp == 128) return launch_narrow<Code, 128>(a, p, st);
-  return launch_heads<Code, 256, 1>(a, p, st);
+  if (p.dp == 256) return launch_heads<Code, 256, 1>(a, p, st);
+  if (p.nt == 1) return p.dp == 64 ? launch_block8<Code, 64, 1, 1>(a, p, st) : launch_block8<Code, 128, 1, 1>(a, p, st);
+  if (p.dp == 128) return launch_heads<Code, 128, 2>(a, p, st);
+  if (p.nt == 2) return launch_block8<Code, 64, 2, 1>(a, p, st);
+  switch (p.hg) {  // up to 128 query heads are four warps of 32
+    case 1: return launch_block8<Code, 64, 4, 1>(a, p, st);
+    case 2: return launch_block8<Code, 64, 4, 2>(a, p, st);
+    default: return launch_block8<Code, 64, 4, 4>(a, p, st);
+  }
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -248,6 +248,21 @@ def test_decode_heads(kind, hq, hkv, dim, page):
         check_decode(pool, q, got, dim**-0.5)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,dim,page", [(17, 1, 64, 16), (32, 1, 48, 8), (66, 2, 64, 16), (64, 1, 32, 32),
+                                             (65, 1, 64, 8), (96, 3, 16, 16), (256, 2, 64, 16)])
+def test_decode_many_heads_of_small_dim(kind, hq, hkv, dim, page):
+    """Groups of 17 to 128 query heads for head_dim up to 64, short rows beside rows of several CTAs."""
+    from kernel_lab import cuda_ops
+
+    pool = Pool(kind, [3, 2100, 0, page, 5000, 1, 130], hkv, dim, page, "padded", seed=31)
+    q = make_q(pool, hq, torch.bfloat16)
+    table, lens = pool.tables()
+    got = cuda_ops.paged_decode_attention_block8(q, **pool.gpu(), block_table=table, seq_lens=lens)
+    assert (got[2] == 0).all()
+    check_decode(pool, q, got, dim**-0.5)
+
+
 @pytest.mark.parametrize("layout", ["nhd", "hnd", "padded"])
 @pytest.mark.parametrize("lens", [[1], [15], [4096], [1025, 3, 700], [64] * 40, [2000, 1] * 8])
 def test_decode_lengths_and_layouts(layout, lens):
