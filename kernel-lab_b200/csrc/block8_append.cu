@@ -5,17 +5,19 @@
 // new elements gives the scale, so a unit is a reduction and then an elementwise pass over the same
 // elements. A team of one warp (pages of up to 4096 elements a head) or of four warps takes a unit
 // and copies its new elements to shared memory, all in flight at once and without registers, so that
-// it reads them once; larger pages re-read theirs from L2. A team takes several parts of a page (keys
-// or values of a head) in turn where the call is large: finding the page costs about as many instructions as a unit's elements. HBM-bound for prompts (the new rows in, half or a quarter of their bytes out),
-// latency-bound for single tokens, where the chain is indptr / position, block-table entry, new row.
-// Measured: 33.4k prompt tokens of 8 heads of 128, e4m3 with bounds, 51.8 us (4.0 TB/s of the 210 MB it has to
-// move, 0.62 of the copy peak: a part's packs arrive, then are reduced, then quantised, and only other
-// warps' loads run beside that; issue 63 % busy); 37 int8 chunks of up to 257 tokens 23.9 us; one token
-// of each of 64 sequences 5.3 us in a graph.
+// it reads them once; larger pages re-read theirs from L2. HBM-bound for prompts (the new rows in, half
+// or a quarter of their bytes out), latency-bound for single tokens, where the chain is indptr / position,
+// block-table entry, new row.
+// Measured: 33.4k prompt tokens of 8 heads of 128, e4m3 with bounds, 42.0 us (5.0 TB/s of the 210 MB it has to
+// move, 0.76 of the copy peak); 37 int8 chunks of up to 257 tokens 20.9 us; one token of each of 64 sequences
+// 5.0 us in a graph.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
-// tokens and looks for the tokens in it that are the first of their sequence in a page; the window
-// is a page's length when sequences bring many tokens and one token when they bring one each.
+// tokens and looks for the tokens in it that are the first of their sequence in a page; the window is
+// one token when sequences bring one each, else one page's length, or up to four pages' in a large call:
+// the sequence is found once for them, and while a page filled whole is quantised the next one's rows are
+// on their way (one page at a time 51.4 us, two 46, four 42.0; eight 49.6, too few teams). The parts of
+// a page lie side by side in the grid, so that neighbouring heads are read and written together (1.1 us).
 //
 // Bounds: rounding is monotone, so the least and largest code of a channel are the codes of the
 // least and largest scaled element, and only those two are rounded; they are combined over the
@@ -39,8 +41,9 @@ namespace klb {
 namespace block8_append {
 
 constexpr int kBlock8AppendThreads = 128;
-// Blocks an SM that the registers are held to. 35k prompt tokens with 4, 5, 6: 53.4, 51.8, 56.5 us; 37 int8
-// chunks 23.0, 23.9, 29.5 us (6 spills).
+constexpr int kMaxGridY = 65535;
+// Blocks an SM that the registers are held to. Before a team took several pages, 33.4k prompt tokens with 4, 5,
+// 6: 53.4, 51.8, 56.5 us; 37 int8 chunks 23.0, 23.9, 29.5 us (6 spills).
 constexpr int kAppendBlocks = 5;
 
 struct Block8AppendArgs {
@@ -69,7 +72,7 @@ struct Block8AppendArgs {
 };
 
 // Last b with indptr[b] <= t, by all lanes of a warp (32 samples a step).
-__device__ __forceinline__ int sequence_of(const int32_t* indptr, int batch, int64_t t) {
+__device__ __forceinline__ int sequence_of(const int32_t* indptr, int batch, int t) {
   const int lane = threadIdx.x & 31;
   int lo = 0, n = batch;
   while (n > 1) {
@@ -104,8 +107,7 @@ struct Sequences {
     const int got = w == 0 ? v[0] : w == 1 ? v[1] : w == 2 ? v[2] : v[3];
     return __shfl_sync(0xffffffffu, got, i & 31);
   }
-  __device__ __forceinline__ void find(const Block8AppendArgs& a, int64_t t, int& b, int64_t& begin, int64_t& end,
-                                       int& start) const {
+  __device__ __forceinline__ void find(const Block8AppendArgs& a, int t, int& b, int& begin, int& end, int& start) const {
     if (whole) {
       int count = 0;
 #pragma unroll
@@ -120,12 +122,12 @@ struct Sequences {
       end = a.indptr[b + 1];
       start = a.positions[b];
     } else {
-      b = static_cast<int>(t);
+      b = t;
       begin = t;
       end = t + 1;
       start = a.positions[b];
     }
-    end = min(end, a.tokens);
+    end = min(end, static_cast<int>(a.tokens));
   }
 };
 
@@ -348,21 +350,25 @@ __device__ __forceinline__ float team_max(float v, float* red) {
 }
 
 // Eight packs a lane of a page that is filled whole by one call (the bulk of a prompt): straight-line,
-// from registers. Returns false, with nothing written, when the page holds a NaN or an infinity.
+// in registers. `staged` holds the lane's packs; `next` is called when they have been read, to ask for the
+// next part's in their place. Returns false, with nothing written or asked for, when the page holds a
+// NaN or an infinity.
 constexpr int kWhole = 8;
-template <typename E, typename Code>
-__device__ __forceinline__ bool append_whole_page(const E* src, int64_t src_step, uint8_t* dst, int64_t dst_step,
-                                                  float* scale_at, int8_t* bounds, int head_dim, int across) {
+template <typename E, typename Code, typename Next>
+__device__ __forceinline__ bool append_whole_page(const NewPack<E, 8>* staged, uint8_t* dst, int64_t dst_step,
+                                                  float* scale_at, int8_t* bounds, int head_dim, int across,
+                                                  Next&& next) {
   using Pack = NewPack<E, 8>;
   Pack p[kWhole];
 #pragma unroll
-  for (int i = 0; i < kWhole; ++i, src += src_step) p[i].load(src);
+  for (int i = 0; i < kWhole; ++i) p[i].load(staged[i * 32].v);
   Magnitude<E, 8> mag;
   mag.reset();
 #pragma unroll
   for (int i = 0; i < kWhole; ++i) mag.add(p[i]);
   float amax = mag.get();
-  if (!__all_sync(0xffffffffu, amax <= FLT_MAX)) return false;
+  if (!__all_sync(0xffffffffu, amax <= FLT_MAX)) return false;  // every lane has its packs
+  next();
   amax = warp_allreduce_max(amax);
   const float scale = Code::scale_for(amax);
   const float inv = reciprocal_scale(scale);
@@ -414,8 +420,13 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, kAppendBlocks) kv_append
   float* const s_hi = s_lo + TEAM * VEC;
   wait_prior_grid();
   allow_next_grid();
-  const int first_part = blockIdx.y * kTeams + team;  // part 2 * head + (0: keys, 1: values) of a page
-  if (first_part >= 2 * a.num_kv_heads) return;  // whole warps; with TEAM 128 there is one team a block
+  const int part = blockIdx.x * kTeams + team;  // 2 * head + (0: keys, 1: values)
+  if (part >= 2 * a.num_kv_heads) return;       // whole warps; with TEAM 128 there is one team a block
+  const int64_t window = static_cast<int64_t>(blockIdx.z) * kMaxGridY + blockIdx.y;
+  if (window * a.window >= a.tokens) return;
+  const int h = part >> 1;
+  const bool keys = (part & 1) == 0;
+  const bool bounds = keys && a.k_bounds != nullptr;
 
   const int units = a.head_dim / VEC;
   const int across = a.across, down = a.down;
@@ -427,24 +438,26 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, kAppendBlocks) kv_append
 
   Sequences seqs;
   seqs.read(a);
-  const int64_t w1 = min(a.tokens, (static_cast<int64_t>(blockIdx.x) + 1) * a.window);
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * a.window; t < w1;) {
-    int64_t begin, end;
-    int b, start;
-    seqs.find(a, t, b, begin, end, start);
+  const int w1 = static_cast<int>(min(a.tokens, (window + 1) * a.window));
+  int begin, end = -1;  // rows of sequence b, whose first position is start
+  int b, start;
+  bool asked = false;  // the new packs of the page at t are on their way to s_new
+  for (int t = static_cast<int>(window * a.window); t < w1;) {
+    if (t >= end) seqs.find(a, t, b, begin, end, start);
     if (t < begin || t >= end) {  // a row of no sequence
       ++t;
+      end = -1;
       continue;
     }
     if (start < 0) {
       t = end;
       continue;
     }
-    const uint32_t pos = static_cast<uint32_t>(start) + static_cast<uint32_t>(t - begin);  // below 2^32
+    const uint32_t pos = static_cast<uint32_t>(start) + static_cast<uint32_t>(t) - static_cast<uint32_t>(begin);  // below 2^32
     const uint32_t col = pos / static_cast<uint32_t>(a.page_size);
     const int s0 = static_cast<int>(pos - col * static_cast<uint32_t>(a.page_size));
-    const int n = static_cast<int>(min(static_cast<int64_t>(a.page_size - s0), end - t));
-    const int64_t first = t;
+    const int n = min(a.page_size - s0, end - t);
+    const int first = t;
     t += n;
     if (first != begin && s0 != 0) continue;  // not the sequence's first token in this page
 
@@ -461,184 +474,193 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, kAppendBlocks) kv_append
     const bool staged = VEC == 8 && units <= across && s0 <= a.keep * down;
     // The whole page at once, eight packs a lane, channel units a power of two.
     const bool whole = VEC == 8 && n == a.page_size && n == kWhole * down && across * down == 32 && units == across;
-    const int64_t row = (first + my_tok) * a.new_stride + my_unit * VEC;
+    const int64_t row = static_cast<int64_t>(first + my_tok) * a.new_stride + my_unit * VEC;
     const int64_t place = page * a.page_stride + my_tok * a.token_stride + my_unit * VEC;
 
-    for (int part = first_part; part < 2 * a.num_kv_heads; part += gridDim.y * kTeams) {
-      const int h = part >> 1;
-      const bool keys = (part & 1) == 0;
-      const bool bounds = keys && a.k_bounds != nullptr;
-      const E* const src = static_cast<const E*>(keys ? a.k_new : a.v_new) + row + h * a.head_dim;
-      if constexpr (TEAM == 32 && PackExtremes<E, VEC>::kPairs) {
-        if (whole && page >= 0 && page < a.num_pages) {
-          uint8_t* const to = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
-          float* const scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
-          int8_t* const out = bounds ? a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim : nullptr;
-          if (append_whole_page<E, Code>(src, src_step, to, dst_step, scale_at, out, a.head_dim, across)) continue;
-        }
-      }
-      // The new packs first (they need no page), then the page, its present scale and its codes.
-      if constexpr (VEC == 8) {
-        if (kept) {
-          const uint8_t* from = reinterpret_cast<const uint8_t*>(src);
-          uint32_t to = smem_u32(s_new + tid);
-#pragma unroll 4
-          for (int i = 0; i < my_new; ++i) {
+    const bool have = asked;
+    const bool more = t < w1 && end - t >= a.page_size;  // the window's next page is filled whole too
+    asked = false;
+    const E* const src = static_cast<const E*>(keys ? a.k_new : a.v_new) + row + h * a.head_dim;
+    if constexpr (TEAM == 32 && PackExtremes<E, VEC>::kPairs) {
+      if (whole && page >= 0 && page < a.num_pages) {
+        uint8_t* const to = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
+        float* const scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
+        int8_t* const out = bounds ? a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim : nullptr;
+        const auto ask = [&](const E* from) {
+          const uint32_t at = smem_u32(s_new + tid);
 #pragma unroll
-            for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) cp_async16(to + k, from + k);
-            from += src_step * static_cast<int64_t>(sizeof(E));
-            to += TEAM * sizeof(Pack);
-          }
+          for (int i = 0; i < kWhole; ++i) cp_async16(at + i * TEAM * sizeof(Pack), from + i * src_step);
+        };
+        if (!have) ask(src);
+        cp_async_wait_all();
+        const auto next = [&] {
+          if (more) ask(src + a.page_size * a.new_stride);
+          asked = more;
+        };
+        if (append_whole_page<E, Code>(s_new + tid, to, dst_step, scale_at, out, a.head_dim, across, next)) continue;
+      }
+    }
+    // The new packs first (they need no page), then the page, its present scale and its codes.
+    if constexpr (VEC == 8) {
+      if (kept && !have) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(src);
+        uint32_t to = smem_u32(s_new + tid);
+#pragma unroll 4
+        for (int i = 0; i < my_new; ++i) {
+#pragma unroll
+          for (int k = 0; k < static_cast<int>(sizeof(Pack)); k += 16) cp_async16(to + k, from + k);
+          from += src_step * static_cast<int64_t>(sizeof(E));
+          to += TEAM * sizeof(Pack);
         }
       }
-      if (page < 0 || page >= a.num_pages) {
-        if (tid == 0 && a.status) atomicOr(a.status, kStatusBadPage);
-        cp_async_wait_all();  // the next unit's copies may take the same places
-        break;
-      }
-      float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
-      const float old = s0 > 0 ? *scale_at : 0.0f;
-      // This thread's first slot; slot s0 + my_tok is its first new one.
-      uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
-      if (staged) {
-        uint32_t to = smem_u32(s_codes) + tid * VEC;
-        const uint8_t* from = dst;
+    }
+    if (page < 0 || page >= a.num_pages) {
+      if (tid == 0 && a.status) atomicOr(a.status, kStatusBadPage);
+      cp_async_wait_all();  // the next unit's copies may take the same places
+      continue;
+    }
+    float* scale_at = (keys ? a.k_scale : a.v_scale) + page * a.num_kv_heads + h;
+    const float old = s0 > 0 ? *scale_at : 0.0f;
+    // This thread's first slot; slot s0 + my_tok is its first new one.
+    uint8_t* const dst = (keys ? a.k_cache : a.v_cache) + place + h * a.head_stride;
+    if (staged) {
+      uint32_t to = smem_u32(s_codes) + tid * VEC;
+      const uint8_t* from = dst;
 #pragma unroll 4
-        for (int i = 0; i < my_old; ++i, from += dst_step, to += TEAM * VEC) cp_async8(to, from);
-      }
-      cp_async_wait_all();  // each thread reads back what it copied itself
+      for (int i = 0; i < my_old; ++i, from += dst_step, to += TEAM * VEC) cp_async8(to, from);
+    }
+    cp_async_wait_all();  // each thread reads back what it copied itself
 
-      // f(pack) over this thread's new packs of channel units c0, c0 + 1, ..., in token order.
-      const auto for_new = [&](int c0, auto&& f) {
-        if (kept) {
-          const Pack* at = s_new + tid;
+    // f(pack) over this thread's new packs of channel units c0, c0 + 1, ..., in token order.
+    const auto for_new = [&](int c0, auto&& f) {
+      if (kept) {
+        const Pack* at = s_new + tid;
 #pragma unroll 4
-          for (int i = 0; i < my_new; ++i, at += TEAM) {
-            Pack p;
-            p.load(at->v);
-            f(p);
-          }
-        } else if (c0 + my_unit < units) {
-          const E* at = src + c0 * VEC;
+        for (int i = 0; i < my_new; ++i, at += TEAM) {
+          Pack p;
+          p.load(at->v);
+          f(p);
+        }
+      } else if (c0 + my_unit < units) {
+        const E* at = src + c0 * VEC;
 #pragma unroll 1
-          for (int i = 0; i < my_new; ++i, at += src_step) {
-            Pack p;
-            p.load(at);
-            f(p);
+        for (int i = 0; i < my_new; ++i, at += src_step) {
+          Pack p;
+          p.load(at);
+          f(p);
+        }
+      }
+    };
+
+    Magnitude<E, VEC> mag;
+    mag.reset();
+    for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p) { mag.add(p); });
+    float amax = mag.get();
+    const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
+    if (!plain) {
+      amax = 0.0f;
+      for (int c0 = 0; c0 < units; c0 += across) {
+        for_new(c0, [&](const Pack& p) {
+          float f[VEC];
+          p.unpack(f);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            if (fabsf(f[j]) <= FLT_MAX) amax = fmaxf(amax, fabsf(f[j]));
           }
+        });
+      }
+    }
+    amax = team_max<TEAM>(amax, s_red);
+    const float scale = fmaxf(old, Code::scale_for(amax));
+    const float inv = reciprocal_scale(scale);
+    const bool grew = s0 > 0 && scale > old;
+    const float ratio = grew ? old / scale : 1.0f;
+    barrier();  // every thread has read the old scale
+    if (tid == 0) *scale_at = scale;
+
+    for (int c0 = 0; c0 < units; c0 += across) {
+      Extremes<VEC> ext;
+      ext.reset();
+      uint8_t* put = dst + c0 * VEC + s0 * a.token_stride;
+      const auto quantise = [&](const Pack& p) {
+        float y[VEC];
+        p.unpack(y);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) y[j] *= inv;
+        store_codes<Code, VEC>(put, y, plain);  // plain: |y| is at most a rounding above kMax
+        put += dst_step;
+      };
+      if (bounds) {
+        PackExtremes<E, VEC> raw;
+        raw.reset();
+        for_new(c0, [&](const Pack& p) {
+          quantise(p);
+          raw.add(p);
+        });
+        if (plain && my_new > 0) {  // this thread's own extremes, scaled
+          raw.get(ext.lo, ext.hi);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) ext.lo[j] *= inv, ext.hi[j] *= inv;
+        }
+      } else {
+        for_new(c0, quantise);
+      }
+      // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
+      const auto for_codes = [&](int count, uint8_t* at, float by, bool write, bool in_shared) {
+        if (c0 + my_unit >= units) return;
+        const uint8_t* in = in_shared ? s_codes + tid * VEC : at;
+        const int64_t in_step = in_shared ? TEAM * VEC : dst_step;
+#pragma unroll 2
+        for (int i = 0; i < count; ++i, at += dst_step, in += in_step) {
+          float y[VEC];
+          load_codes<Code, VEC>(in, y);
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) y[j] *= by;
+          if (write) store_codes<Code, VEC>(at, y, false);
+          if (bounds) ext.add(y);
         }
       };
-
-      Magnitude<E, VEC> mag;
-      mag.reset();
-      for (int c0 = 0; c0 < units; c0 += across) for_new(c0, [&](const Pack& p) { mag.add(p); });
-      float amax = mag.get();
-      const bool plain = team_all<TEAM>(amax <= FLT_MAX);  // no NaN, no infinity in the unit
-      if (!plain) {
-        amax = 0.0f;
-        for (int c0 = 0; c0 < units; c0 += across) {
-          for_new(c0, [&](const Pack& p) {
-            float f[VEC];
-            p.unpack(f);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              if (fabsf(f[j]) <= FLT_MAX) amax = fmaxf(amax, fabsf(f[j]));
-            }
-          });
-        }
+      if (grew || bounds) for_codes(my_old, dst + c0 * VEC, ratio, grew, staged);
+      if (bounds && !plain) {
+        barrier();
+        for_codes(my_new, dst + c0 * VEC + s0 * a.token_stride, 1.0f, false, false);
       }
-      amax = team_max<TEAM>(amax, s_red);
-      const float scale = fmaxf(old, Code::scale_for(amax));
-      const float inv = reciprocal_scale(scale);
-      const bool grew = s0 > 0 && scale > old;
-      const float ratio = grew ? old / scale : 1.0f;
-      barrier();  // every thread has read the old scale
-      if (tid == 0) *scale_at = scale;
-
-      for (int c0 = 0; c0 < units; c0 += across) {
-        Extremes<VEC> ext;
-        ext.reset();
-        uint8_t* put = dst + c0 * VEC + s0 * a.token_stride;
-        const auto quantise = [&](const Pack& p) {
-          float y[VEC];
-          p.unpack(y);
+      if (bounds) {
+        const int width = across * VEC;
+        barrier();
+        if (active) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) y[j] *= inv;
-          store_codes<Code, VEC>(put, y, plain);  // plain: |y| is at most a rounding above kMax
-          put += dst_step;
-        };
-        if (bounds) {
-          PackExtremes<E, VEC> raw;
-          raw.reset();
-          for_new(c0, [&](const Pack& p) {
-            quantise(p);
-            raw.add(p);
-          });
-          if (plain && my_new > 0) {  // this thread's own extremes, scaled
-            raw.get(ext.lo, ext.hi);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) ext.lo[j] *= inv, ext.hi[j] *= inv;
+          for (int j = 0; j < VEC; ++j) {
+            s_lo[my_tok * width + my_unit * VEC + j] = ext.lo[j];
+            s_hi[my_tok * width + my_unit * VEC + j] = ext.hi[j];
           }
-        } else {
-          for_new(c0, quantise);
         }
-        // Codes of the slots in use: those kept, and the new ones where the packs' extremes do not serve.
-        const auto for_codes = [&](int count, uint8_t* at, float by, bool write, bool in_shared) {
-          if (c0 + my_unit >= units) return;
-          const uint8_t* in = in_shared ? s_codes + tid * VEC : at;
-          const int64_t in_step = in_shared ? TEAM * VEC : dst_step;
-#pragma unroll 2
-          for (int i = 0; i < count; ++i, at += dst_step, in += in_step) {
-            float y[VEC];
-            load_codes<Code, VEC>(in, y);
+        barrier();
+        int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim + c0 * VEC;
+        const int here = min(width, a.head_dim - c0 * VEC);
+        constexpr int kAtOnce = VEC == 8 ? 4 : 1;  // channels a thread writes
+        for (int i = tid * kAtOnce; i < here; i += TEAM * kAtOnce) {
+          float l[kAtOnce], m[kAtOnce];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) y[j] *= by;
-            if (write) store_codes<Code, VEC>(at, y, false);
-            if (bounds) ext.add(y);
-          }
-        };
-        if (grew || bounds) for_codes(my_old, dst + c0 * VEC, ratio, grew, staged);
-        if (bounds && !plain) {
-          barrier();
-          for_codes(my_new, dst + c0 * VEC + s0 * a.token_stride, 1.0f, false, false);
-        }
-        if (bounds) {
-          const int width = across * VEC;
-          barrier();
-          if (active) {
+          for (int j = 0; j < kAtOnce; ++j) l[j] = FLT_MAX, m[j] = -FLT_MAX;
+          for (int k = 0; k < down; ++k) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-              s_lo[my_tok * width + my_unit * VEC + j] = ext.lo[j];
-              s_hi[my_tok * width + my_unit * VEC + j] = ext.hi[j];
+            for (int j = 0; j < kAtOnce; ++j) {
+              l[j] = fminf(l[j], s_lo[k * width + i + j]);
+              m[j] = fmaxf(m[j], s_hi[k * width + i + j]);
             }
           }
-          barrier();
-          int8_t* out = a.k_bounds + ((page * a.num_kv_heads + h) * 2) * a.head_dim + c0 * VEC;
-          const int here = min(width, a.head_dim - c0 * VEC);
-          constexpr int kAtOnce = VEC == 8 ? 4 : 1;  // channels a thread writes
-          for (int i = tid * kAtOnce; i < here; i += TEAM * kAtOnce) {
-            float l[kAtOnce], m[kAtOnce];
-#pragma unroll
-            for (int j = 0; j < kAtOnce; ++j) l[j] = FLT_MAX, m[j] = -FLT_MAX;
-            for (int k = 0; k < down; ++k) {
-#pragma unroll
-              for (int j = 0; j < kAtOnce; ++j) {
-                l[j] = fminf(l[j], s_lo[k * width + i + j]);
-                m[j] = fmaxf(m[j], s_hi[k * width + i + j]);
-              }
-            }
-            if constexpr (VEC == 8) {
-              *reinterpret_cast<uint32_t*>(out + i) = bound_codes<Code, false, 4>(l, 1.0f);
-              *reinterpret_cast<uint32_t*>(out + a.head_dim + i) = bound_codes<Code, true, 4>(m, 1.0f);
-            } else {
-              out[i] = static_cast<int8_t>(bound_codes<Code, false, 1>(l, 1.0f));
-              out[a.head_dim + i] = static_cast<int8_t>(bound_codes<Code, true, 1>(m, 1.0f));
-            }
+          if constexpr (VEC == 8) {
+            *reinterpret_cast<uint32_t*>(out + i) = bound_codes<Code, false, 4>(l, 1.0f);
+            *reinterpret_cast<uint32_t*>(out + a.head_dim + i) = bound_codes<Code, true, 4>(m, 1.0f);
+          } else {
+            out[i] = static_cast<int8_t>(bound_codes<Code, false, 1>(l, 1.0f));
+            out[a.head_dim + i] = static_cast<int8_t>(bound_codes<Code, true, 1>(m, 1.0f));
           }
         }
       }
-      barrier();  // another unit may follow: the extremes' place is free again
     }
+    barrier();  // another unit may follow: the extremes' place is free again
   }
 }
 
@@ -657,12 +679,14 @@ cudaError_t launch_team(Block8AppendArgs a, cudaStream_t st) {
   const int64_t packs = (static_cast<int64_t>(a.page_size) + a.down - 1) / a.down;
   a.keep = VEC == 8 ? static_cast<int>(std::min<int64_t>(packs, 16)) : 0;
   constexpr int kTeams = kBlock8AppendThreads / TEAM;
-  const int64_t windows = (a.tokens + a.window - 1) / a.window;
-  // Parts of a page that a team takes in turn: up to four, as many as leave about four waves of blocks.
   const int blocks = (2 * a.num_kv_heads + kTeams - 1) / kTeams;
-  const int64_t waves = windows * blocks / (static_cast<int64_t>(sm_count()) * kAppendBlocks);
-  const int turns = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(waves / 4, 4)));
-  const dim3 grid(static_cast<unsigned>(windows), static_cast<unsigned>((blocks + turns - 1) / turns));
+  // Up to four pages a window, as many as leave 2.5 waves of blocks, and no more than a sequence brings.
+  const int64_t waves = (a.tokens + a.window - 1) / a.window * blocks / (static_cast<int64_t>(sm_count()) * kAppendBlocks);
+  a.window = static_cast<int>(std::min<int64_t>(a.window * std::max<int64_t>(1, std::min<int64_t>(waves * 2 / 5, 4)),
+                                                std::max<int64_t>(1, a.tokens / a.batch)));
+  const int64_t windows = (a.tokens + a.window - 1) / a.window;
+  const unsigned y = static_cast<unsigned>(std::min<int64_t>(windows, kMaxGridY));
+  const dim3 grid(static_cast<unsigned>(blocks), y, static_cast<unsigned>((windows + kMaxGridY - 1) / kMaxGridY));
   const int bytes = kTeams * team_bytes<E, VEC, TEAM>(a.keep);
   const auto kernel = kv_append_block8<E, Code, VEC, TEAM>;
   if (bytes > 48 * 1024 - 64) {

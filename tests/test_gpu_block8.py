@@ -209,6 +209,22 @@ def test_append_ignores_rows_of_no_sequence():
     np.testing.assert_array_equal(state["v_scale"].cpu().numpy(), pool.v_scale)
 
 
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("heads,dim,page,new", [(64, 64, 32, [2200, 900, 800]), (64, 8, 4, [500, 300, 250])])
+def test_append_large_calls(kind, heads, dim, page, new):
+    """Enough pages that a team takes several in turn: NaN and infinities inside, a page id outside the pool
+    between good ones, sequences that begin within a page, rows of no sequence after the last."""
+    start = [page // 2 + 1, 0, 3 * page]
+    pool = Pool(kind, [s + n for s, n in zip(start, new)], heads, dim, page, seed=32)
+    pool.table[0, 5] = 1 << 30
+    g = torch.Generator().manual_seed(33)
+    rows = [torch.randn(sum(new) + 9, heads, dim, generator=g).to(torch.bfloat16) for _ in range(2)]
+    for at, value in [(3 * page, float("nan")), (7 * page + 1, float("inf")), (8 * page + 2, -float("inf"))]:
+        rows[0][at, ::2, 1], rows[1][at, 1::3, 2] = value, value
+    new_rows = [*new, 9]
+    assert run_append(pool, new_rows, start, torch.bfloat16, True, np.cumsum([0, *new]).tolist(), *rows)[1] == 1
+
+
 # ---------------------------------------------------------------- decode
 
 
