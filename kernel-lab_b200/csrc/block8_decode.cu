@@ -40,9 +40,12 @@
 //
 // Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
 // to f16 exactly, q is divided by a power of two so that f16 holds it, k_scale and that power enter
-// with the softmax scale. P is at most 2^8 (the running maximum is only raised when a score passes it
-// by 8) and rounded to f16; v_scale enters P relative to the largest one met so far, so that P stays
-// in f16's range whatever the scales' magnitude.
+// with the softmax scale. p is at most 2^8 (the running maximum is only raised when a score passes it
+// by 8). What is rounded to f16 is P = p * v_scale / w: w, a power of two, is the head's own measure of its
+// largest p * v_scale so far, so that neither the scales' magnitude nor a page of large values and
+// vanishing probability takes bits from the tokens that count. It is taken anew whenever the maximum is raised
+// (the weights before shrink with it) and when a step's v_scale passes w by 2^7, which keeps P at most 2^15
+// between. A token's P is thus off by 2^-11 of itself or by 2^-25 of the largest p * v_scale.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -62,6 +65,8 @@ constexpr int kB8Tile = 16;
 constexpr int kB8Meta = 32;        // bytes of a stage after its codes: scales (k, v) of its octets, valid counts
 constexpr float kRaiseBy = 8.0f;   // the running maximum is raised when a score passes it by this (base 2)
 constexpr float kNoMax = -1e30f;   // running maximum before the first score
+constexpr float kLeastWeight = 0x1p-126f, kMostWeight = 0x1p126f;  // w and 1 / w are normal numbers
+constexpr float kWeightRange = 128.0f;  // w is taken anew when a v_scale passes it by this
 constexpr int kMaxShared = 227 * 1024 - 128;  // dynamic, beside the plan's static part
 constexpr int kTeamBarrier = 1, kGroupBarrier = 8;  // named barriers: 1.. teams, 8.. groups
 
@@ -102,6 +107,12 @@ __host__ __device__ constexpr int query_bytes(int dp, int nt) { return nt == 4 ?
 // Floats a lane hands over at a time in a join: the maxima and sums of 8 query heads and half of their
 // outputs.
 __host__ __device__ constexpr int box_floats(int dp) { return 4 + dp / 8; }
+
+// The power of two at or below v, kept to where its reciprocal is a normal number too.
+__device__ __forceinline__ float weight_unit(float v) {
+  return __uint_as_float(__float_as_uint(fminf(fmaxf(v, kLeastWeight), kMostWeight)) & 0x7f800000u);
+}
+__device__ __forceinline__ float reciprocal_of_power(float w) { return __uint_as_float(0x7f000000u - __float_as_uint(w)); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -525,10 +536,11 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 
     float acc[NT][kHalves][kM][4];
     float m[NT][2], l[NT][2];
-    float v_ref = 0.0f, v_inv = 0.0f;  // the largest value scale so far, its reciprocal
+    float w[NT][2];  // acc is in units of w
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = kNoMax;
+      w[n][0] = w[n][1] = kLeastWeight;
       l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
       for (int f = 0; f < kHalves; ++f)
@@ -602,19 +614,6 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
         there[q][0] = g < static_cast<int>(valid & 0xffffu);
         there[q][1] = g < static_cast<int>(valid >> 16);
       }
-      if (v_top > v_ref && v_top >= kLeastScale) {  // the same for the whole warp
-        const float f = v_ref / v_top;
-        v_ref = v_top;
-        v_inv = 1.0f / v_top;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int x = 0; x < kHalves; ++x)
-#pragma unroll
-            for (int i = 0; i < kM; ++i)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][x][i][e] *= f;
-      }
 
       // Scores less the running maximum, in base 2; rows past the end at -infinity.
       float x[kTiles][NT][4];
@@ -629,7 +628,12 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             x[q][n][e] = there[q][e >> 1] ? v : -INFINITY;
             most = fmaxf(most, x[q][n][e]);
           }
-      if (__any_sync(0xffffffffu, most > kRaiseBy)) {
+      bool raise = most > kRaiseBy;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) raise |= v_top * reciprocal_of_power(w[n][e]) > kWeightRange;
+      if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -648,18 +652,27 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             const float next = fmaxf(m[n][e], top);
             const float f = exp2_fast(m[n][e] - next);
             m[n][e] = next;
+            float heaviest = w[n][e] * f;
+            const float before = heaviest;
 #pragma unroll
-            for (int q = 0; q < kTiles; ++q) {
-              x[q][n][e] -= next;
-              x[q][n][2 + e] -= next;
-            }
+            for (int q = 0; q < kTiles; ++q)
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                x[q][n][2 * o + e] -= next;
+                heaviest = fmaxf(heaviest, exp2_fast(x[q][n][2 * o + e]) * fabsf(vs[q][o]));
+              }
+            heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 4));
+            heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 8));
+            heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 16));
+            w[n][e] = weight_unit(heaviest);
+            const float k = before * reciprocal_of_power(w[n][e]);  // below 2
             l[n][e] *= f;
 #pragma unroll
             for (int y = 0; y < kHalves; ++y)
 #pragma unroll
               for (int i = 0; i < kM; ++i) {
-                acc[n][y][i][e] *= f;
-                acc[n][y][i][2 + e] *= f;
+                acc[n][y][i][e] *= k;
+                acc[n][y][i][2 + e] *= k;
               }
           }
         }
@@ -668,18 +681,19 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       // P^T as the value product's B operand.
       uint32_t p0[kTiles][NT], p1[kTiles][NT];
 #pragma unroll
-      for (int q = 0; q < kTiles; ++q) {
-        const float r0 = vs[q][0] * v_inv, r1 = vs[q][1] * v_inv;
+      for (int n = 0; n < NT; ++n) {
+        const float per[2] = {reciprocal_of_power(w[n][0]), reciprocal_of_power(w[n][1])};
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
+        for (int q = 0; q < kTiles; ++q) {
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             p[e] = exp2_fast(x[q][n][e]);
             l[n][e & 1] += p[e];
+            p[e] *= vs[q][e >> 1] * per[e & 1];
           }
-          p0[q][n] = movmatrix_trans(Storage<__half>::pack2(p[0] * r0, p[1] * r0));
-          p1[q][n] = movmatrix_trans(Storage<__half>::pack2(p[2] * r1, p[3] * r1));
+          p0[q][n] = movmatrix_trans(Storage<__half>::pack2(p[0], p[1]));
+          p1[q][n] = movmatrix_trans(Storage<__half>::pack2(p[2], p[3]));
         }
       }
 
@@ -732,7 +746,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 #pragma unroll
         for (int i = 0; i < kM; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= v_ref;
+          for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= w[n][e & 1];
     }
     // Join the TS parts: the upper half hands its state to the lower half, fragment by fragment, half
     // of the outputs of 8 query heads at a time.
