@@ -92,8 +92,8 @@ int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache, void* v_c
  * q and out are fp16 or bf16 ([batch, num_q_heads, head_dim], 16-byte aligned); head_dim is a
  * multiple of 16 up to 256; page_size is 8 or a multiple of 16; the caches and their strides are
  * 16-byte aligned, the strides below 2^31; at most 128 query heads a KV head (64 for head_dim above 128). Others return
- * cudaErrorInvalidValue. The products run in fp16 (codes exactly; q scaled by a power of two and
- * rounded to fp16, which is exact for fp16 and for bf16 within 2^-14 of a head's largest element)
+ * cudaErrorInvalidValue. The products run in fp16 (codes exactly; an fp16 q as it is; a bf16 q scaled by a
+ * power of two, exact for elements down to 2^-31 of their head's largest, others off by at most 2^-39 of it)
  * and accumulate in fp32. A token's probability times its value scale is rounded to fp16: it is off by at
  * most 2^-11 of itself or 2^-25 of the query head's largest such product, whatever the scales of the other pages.
  *

@@ -39,7 +39,7 @@
 // TB/s, 0.31; issue 46 % busy).
 //
 // Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
-// to f16 exactly, q is divided by a power of two so that f16 holds it, k_scale and that power enter
+// to f16 exactly, a bf16 q is divided by a power of two so that f16 holds it, k_scale and that power enter
 // with the softmax scale. p is at most 2^8 (the running maximum is only raised when a score passes it
 // by 8). What is rounded to f16 is P = p * v_scale / w: w, a power of two, is the head's own measure of its
 // largest p * v_scale so far, so that neither the scales' magnitude nor a page of large values and
@@ -514,8 +514,9 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e just below the largest element; kept to where 2^-e is a normal number too.
-      const int e = max(-126, min(126, static_cast<int>(__float_as_uint(top) >> 23) - 127));
+      // An fp16 q goes in as it is. A bf16 q is divided by the 2^e that puts its largest element between 2^14 and
+      // 2^15, so that f16's bits reach 2^-31 of it without loss; e is kept to where 2^-e is a normal number too.
+      const int e = a.q_bf16 ? max(-126, min(113, static_cast<int>(__float_as_uint(top) >> 23) - 127 - 14)) : 0;
       const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23) * a.scale_log2;
 #pragma unroll

@@ -1,4 +1,4 @@
-"""Block-scaled decode where the numbers spread widely: value scales of unlike size.
+"""Block-scaled decode where the numbers spread widely: value scales and elements of q of unlike size.
 
 Tolerance of an output element, from the definition's roundings: a token's weight p * v_scale is rounded to fp16
 (2^-11 of itself, or 2^-25 of the head's largest weight where that is more), 2^-14 for ex2, the products and the
@@ -115,3 +115,26 @@ def test_selected_pages_of_unlike_scales():
     got = cuda_ops.paged_decode_attention_block8(q, **pool.gpu(), block_table=table, seq_lens=seq, scale=float(np.log(2.0)),
                                                  selected=torch.from_numpy(chosen).cuda())
     check(pool, q, got, float(np.log(2.0)), chosen)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("hq,hkv,dim", [(8, 1, 64), (32, 1, 64), (16, 1, 128), (4, 1, 256)])
+@pytest.mark.parametrize(
+    "dtype,largest,small", [(torch.float16, 8.0, 1e-4), (torch.float16, 3e4, 2.0**-22), (torch.bfloat16, 1.0, 2.0**-20), (torch.bfloat16, 2.0**100, 2.0**70), (torch.bfloat16, 2.0**-110, 2.0**-130)]
+)
+def test_small_elements_of_q_beside_a_large_one(kind, hq, hkv, dim, dtype, largest, small):
+    """The large element meets keys of zero, so the scores are the small ones': none of their bits may be lost."""
+    from kernel_lab import cuda_ops
+
+    pool = Pool(kind, [200, 31], hkv, dim, 16, seed=46)
+    pool.k_scale[:] = 1.0
+    x = block8.decode_codes(pool.k, kind).copy()
+    x[..., 3] = 0
+    pool.k = block8.encode(x, kind)
+    q = small * (1 + np.random.RandomState(47).rand(2, hq, dim))
+    q[..., 3] = largest
+    q = torch.from_numpy(q).to(dtype).cuda()
+    scale = 0.02 / small
+    table, seq = pool.tables()
+    got = cuda_ops.paged_decode_attention_block8(q, **pool.gpu(), block_table=table, seq_lens=seq, scale=scale)
+    check(pool, q, got, scale)
