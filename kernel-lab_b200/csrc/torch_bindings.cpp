@@ -16,17 +16,32 @@
 // paged_kv_append_block8, paged_decode_attention_block8 and paged_block_select.
 //
 // Decode scratch (split partials and arrival counters) is owned here, one pair of
-// buffers per (device, stream), allocated through PyTorch's caching allocator and grown
-// on demand. The counters are zeroed once at allocation; every call leaves them zero.
-// Entries live as long as the process (a stream that is destroyed keeps its entry, so a
-// host that creates streams per request should reuse a pool of them).
+// buffers per (device, stream), grown on demand. The counters are zeroed once at allocation; every call
+// leaves them zero. Entries live as long as the process (a stream that is destroyed keeps its entry, so a
+// host that creates streams per request should reuse a pool of them), and so do outgrown buffers, each
+// less than 4/5 of the next: kernels in flight or another thread's launch may still use them.
+//
+// Calls that are captured into a CUDA graph have scratch of their own, one pair per capture and
+// stream: a graph may be replayed on any stream, at the same time as other graphs and eager calls,
+// and after the capturing stream's own buffers have grown. It is zeroed at once, outside of
+// the capture (a recorded memset would clear the status word at each replay), and is the graph's until
+// that is destroyed (a CUDA user object says when; it costs 2 to 3 us a replay, whatever the graph's size); then
+// a later capture may have it.
+//
+// The buffers come from cudaMalloc, not from PyTorch's allocator: whichever pool serves the calling thread or
+// stream there (a graph's private pool, torch.compile's) would count them as its own and could outlive or
+// refuse them.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <utility>
+#include <vector>
 
 #include "kernel_lab_b200.h"
 #include "kernel_lab_b200_block8.h"
@@ -91,21 +106,162 @@ struct Scratch {
   at::Tensor sync;      // uint8, zero at rest
 };
 
-std::mutex g_scratch_mu;
-std::map<std::pair<int, cudaStream_t>, Scratch> g_scratch;
+size_t scratch_size(size_t bytes) { return std::max<size_t>(bytes, 256) * 5 / 4; }
+bool holds(const at::Tensor& t, size_t bytes) { return t.defined() && static_cast<size_t>(t.numel()) >= bytes; }
 
-Scratch& scratch_for(const at::Device& dev, cudaStream_t stream, size_t partial_bytes, size_t sync_bytes) {
-  std::lock_guard<std::mutex> lock(g_scratch_mu);
-  Scratch& s = g_scratch[{dev.index(), stream}];
+// Scratch of one capture's calls on one stream; what was outgrown during the capture stays, for the nodes
+// recorded with it.
+struct GraphScratch {
+  int device;
+  cudaStream_t stream;
+  unsigned long long capture;
+  std::vector<Scratch> grown;  // the last is in use
+};
+
+struct ScratchPool {
+  std::mutex mu;
+  std::map<std::pair<int, cudaStream_t>, Scratch> streams;
+  std::vector<at::Tensor> outgrown;
+  std::vector<std::unique_ptr<GraphScratch>> graphs;
+  std::map<int, std::vector<Scratch>> spare;  // of graphs that are gone
+  std::map<int, uint32_t> spare_status;       // their status bits
+  std::map<int, cudaStream_t> side;           // a stream of our own per device, for work outside of captures
+  // Filled by the driver when a graph is gone; no CUDA call may be made there.
+  std::mutex ended_mu;
+  std::vector<GraphScratch*> ended;
+  std::atomic<bool> any_ended{false};
+};
+
+// Never destroyed: a graph may outlive the other statics.
+ScratchPool& scratch_pool() {
+  static ScratchPool* const pool = new ScratchPool;
+  return *pool;
+}
+
+void CUDART_CB graph_ended(void* scratch) {
+  ScratchPool& pool = scratch_pool();
+  const std::lock_guard<std::mutex> lock(pool.ended_mu);
+  pool.ended.push_back(static_cast<GraphScratch*>(scratch));
+  pool.any_ended.store(true, std::memory_order_release);
+}
+
+// The functions below hold pool.mu, with the device current and the thread's capture mode relaxed: while any
+// stream captures, others forbid allocations and waits. Nothing here touches a capturing stream.
+cudaStream_t side_stream(ScratchPool& pool, int device) {
+  cudaStream_t& st = pool.side[device];
+  if (st == nullptr) C10_CUDA_CHECK(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
+  return st;
+}
+
+at::Tensor scratch_buffer(ScratchPool& pool, const at::Device& dev, size_t bytes) {
+  const auto size = static_cast<int64_t>(scratch_size(bytes));
   const auto opts = at::TensorOptions().dtype(at::kByte).device(dev);
-  if (!s.partials.defined() || static_cast<size_t>(s.partials.numel()) < partial_bytes) {
-    s.partials = at::empty({static_cast<int64_t>(std::max<size_t>(partial_bytes, 256) * 5 / 4)}, opts);
+  void* p = nullptr;
+  if (cudaMalloc(&p, static_cast<size_t>(size)) == cudaSuccess) return at::from_blob(p, {size}, opts);
+  (void)cudaGetLastError();  // PyTorch may hold the memory that is left
+  const c10::cuda::CUDAStreamGuard guard(c10::cuda::getStreamFromExternal(side_stream(pool, dev.index()), dev.index()));
+  return at::empty({size}, opts);
+}
+
+// Takes back the scratch of graphs that are gone.
+void collect_ended_graphs(ScratchPool& pool) {
+  if (!pool.any_ended.load(std::memory_order_acquire)) return;
+  std::vector<GraphScratch*> ended;
+  {
+    const std::lock_guard<std::mutex> lock(pool.ended_mu);
+    ended.swap(pool.ended);
+    pool.any_ended.store(false, std::memory_order_release);
   }
-  if (!s.sync.defined() || static_cast<size_t>(s.sync.numel()) < sync_bytes) {
-    at::Tensor grown = at::zeros({static_cast<int64_t>(std::max<size_t>(sync_bytes, 256) * 5 / 4)}, opts);
-    // Status word 0 is sticky until decode_status(clear=True): carry it into the larger buffer
-    // (stream-ordered after every earlier call on this stream; the counters are zero at rest).
-    if (s.sync.defined()) grown.narrow(0, 0, 4).copy_(s.sync.narrow(0, 0, 4), /*non_blocking=*/true);
+  for (GraphScratch* g : ended) {
+    const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(g->device));
+    for (const Scratch& s : g->grown) {
+      uint32_t status = 0;
+      check_status(kl_paged_decode_read_status(s.sync.data_ptr(), &status, 1, side_stream(pool, g->device)), "scratch");
+      pool.spare_status[g->device] |= status;
+      pool.spare[g->device].push_back(s);
+    }
+    for (auto& p : pool.graphs) {
+      if (p.get() == g) {
+        std::swap(p, pool.graphs.back());
+        pool.graphs.pop_back();
+        break;
+      }
+    }
+  }
+}
+
+// Scratch for a call that is being captured into `graph`.
+Scratch graph_scratch(ScratchPool& pool, const at::Device& dev, cudaStream_t stream, unsigned long long capture,
+                      cudaGraph_t graph, size_t partial_bytes, size_t sync_bytes) {
+  const auto serves = [&](const Scratch& s) { return holds(s.partials, partial_bytes) && holds(s.sync, sync_bytes); };
+  GraphScratch* own = nullptr;
+  for (const auto& p : pool.graphs) {
+    if (p->capture == capture && p->stream == stream && p->device == dev.index()) own = p.get();
+  }
+  if (own && serves(own->grown.back())) return own->grown.back();
+  collect_ended_graphs(pool);
+  Scratch s;
+  std::vector<Scratch>& spare = pool.spare[dev.index()];
+  for (Scratch& t : spare) {
+    if (!serves(t)) continue;
+    s = t;
+    std::swap(t, spare.back());
+    spare.pop_back();
+    break;
+  }
+  if (!s.sync.defined()) {
+    s.partials = scratch_buffer(pool, dev, partial_bytes);
+    s.sync = scratch_buffer(pool, dev, sync_bytes);
+    const cudaStream_t side = side_stream(pool, dev.index());
+    C10_CUDA_CHECK(cudaMemsetAsync(s.sync.data_ptr(), 0, s.sync.numel(), side));
+    C10_CUDA_CHECK(cudaStreamSynchronize(side));
+  }
+  if (own) {
+    own->grown.push_back(s);
+    return s;
+  }
+  pool.graphs.push_back(std::unique_ptr<GraphScratch>(new GraphScratch{dev.index(), stream, capture, {s}}));
+  cudaUserObject_t object = nullptr;
+  cudaError_t e = cudaUserObjectCreate(&object, pool.graphs.back().get(), graph_ended, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    pool.graphs.pop_back();
+  } else {
+    e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+    if (e != cudaSuccess) cudaUserObjectRelease(object, 1);  // graph_ended takes it from here
+  }
+  C10_CUDA_CHECK(e);
+  return s;
+}
+
+// The buffers for a call on `stream`, the current one of `dev`.
+Scratch scratch_for(const at::Device& dev, cudaStream_t stream, size_t partial_bytes, size_t sync_bytes) {
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &capturing, &capture, &graph, nullptr, nullptr));
+  ScratchPool& pool = scratch_pool();
+  const std::lock_guard<std::mutex> lock(pool.mu);
+  if (capturing != cudaStreamCaptureStatusNone) {
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    return graph_scratch(pool, dev, stream, capture, graph, partial_bytes, sync_bytes);
+  }
+  Scratch& s = pool.streams[{dev.index(), stream}];
+  if (holds(s.partials, partial_bytes) && holds(s.sync, sync_bytes)) return s;
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  if (!holds(s.partials, partial_bytes)) {
+    const at::Tensor grown = scratch_buffer(pool, dev, partial_bytes);
+    if (s.partials.defined()) pool.outgrown.push_back(s.partials);
+    s.partials = grown;
+  }
+  if (!holds(s.sync, sync_bytes)) {
+    const at::Tensor grown = scratch_buffer(pool, dev, sync_bytes);
+    C10_CUDA_CHECK(cudaMemsetAsync(grown.data_ptr(), 0, grown.numel(), stream));
+    if (s.sync.defined()) {
+      // Status word 0 is sticky until decode_status(clear=True): carry it into the larger buffer
+      // (stream-ordered after every earlier call on this stream; the counters are zero at rest).
+      C10_CUDA_CHECK(cudaMemcpyAsync(grown.data_ptr(), s.sync.data_ptr(), 4, cudaMemcpyDeviceToDevice, stream));
+      pool.outgrown.push_back(s.sync);
+    }
     s.sync = grown;
   }
   return s;
@@ -152,7 +308,7 @@ void paged_decode_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor& k
                                               max_pages, static_cast<int>(num_splits), &partial_bytes,
                                               &sync_bytes),
                "paged_decode_attention (workspace)");
-  Scratch& s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(kl_paged_decode(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch, num_q_heads,
                                num_kv_heads, head_dim, page_size, block_table.stride(0), max_pages,
@@ -207,7 +363,7 @@ void paged_kv_append(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor&
   if (batch == 0) return;
   const c10::cuda::CUDAGuard guard(k_new.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  Scratch& s = scratch_for(k_new.device(), stream, 0, 4);
+  const Scratch s = scratch_for(k_new.device(), stream, 0, 4);
   check_status(kl_paged_kv_append(to_dtype(k_cache.scalar_type()), k_cache.data_ptr(), v_cache.data_ptr(),
                                   k_new.data_ptr(), v_new.data_ptr(), block_table.data_ptr<int32_t>(),
                                   positions.data_ptr<int32_t>(), static_cast<int>(batch),
@@ -265,7 +421,7 @@ void paged_decode_attention_fp8(at::Tensor& out, const at::Tensor& q, const at::
   check_status(kl_paged_decode_workspace_size(dtype, batch, num_q_heads, num_kv_heads, head_dim, page_size,
                                               max_pages, 0, &partial_bytes, &sync_bytes),
                "paged_decode_attention_fp8 (workspace)");
-  Scratch& s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(kl_paged_decode_fp8(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                    k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
                                    block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch,
@@ -307,7 +463,7 @@ void paged_kv_append_fp8(at::Tensor& k_cache, at::Tensor& v_cache, const at::Ten
   if (batch == 0) return;
   const c10::cuda::CUDAGuard guard(k_new.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  Scratch& s = scratch_for(k_new.device(), stream, 0, 4);
+  const Scratch s = scratch_for(k_new.device(), stream, 0, 4);
   check_status(kl_paged_kv_append_fp8(to_dtype(k_new.scalar_type()), k_cache.data_ptr(), v_cache.data_ptr(),
                                       k_new.data_ptr(), v_new.data_ptr(), k_scale.data_ptr<float>(),
                                       v_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
@@ -377,7 +533,7 @@ void paged_decode_attention_cascade(at::Tensor& out, const at::Tensor& q, const 
                                                       num_kv_heads, head_dim, page_size, max_pages, max_prefix_pages,
                                                       &partial_bytes, &sync_bytes),
                "paged_decode_attention_cascade (workspace)");
-  Scratch& s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(
       kl_paged_decode_cascade(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                               fp8 ? k_scale->data_ptr<float>() : nullptr, fp8 ? v_scale->data_ptr<float>() : nullptr,
@@ -520,7 +676,7 @@ void paged_kv_append_block8(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor
   const int64_t row_stride = tokens == 1 ? num_kv_heads * head_dim : k_new.stride(0);
   const c10::cuda::CUDAGuard guard(k_cache.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  Scratch& s = scratch_for(k_cache.device(), stream, 0, 4);
+  const Scratch s = scratch_for(k_cache.device(), stream, 0, 4);
   check_status(
       kl_paged_kv_append_block8(to_dtype(k_new.scalar_type()), code_type, k_cache.data_ptr(), v_cache.data_ptr(),
                                 k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
@@ -570,7 +726,7 @@ void paged_decode_attention_block8(at::Tensor& out, const at::Tensor& q, const a
                                                      static_cast<int>(num_kv_heads), d, page, max_pages, num_selected,
                                                      &partial_bytes, &sync_bytes),
                "paged_decode_attention_block8 (workspace)");
-  Scratch& s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(
       kl_paged_decode_block8(to_dtype(q.scalar_type()), code_type, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
                              v_cache.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
@@ -613,7 +769,7 @@ void paged_block_select(at::Tensor& selected, const at::Tensor& q, const at::Ten
   check_status(kl_paged_block_select_workspace_size(static_cast<int>(batch), static_cast<int>(num_kv_heads), max_pages,
                                                     &scratch_bytes, &sync_bytes),
                "paged_block_select (workspace)");
-  Scratch& s = scratch_for(q.device(), stream, scratch_bytes, sync_bytes);
+  const Scratch s = scratch_for(q.device(), stream, scratch_bytes, sync_bytes);
   check_status(
       kl_paged_block_select(to_dtype(q.scalar_type()), code_type, selected.data_ptr<int32_t>(), q.data_ptr(),
                             k_bounds.data_ptr(), k_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
@@ -627,19 +783,33 @@ void paged_block_select(at::Tensor& selected, const at::Tensor& q, const at::Ten
       "paged_block_select");
 }
 
-// Status bits (KL_STATUS_*) left by decode calls on the current device and stream.
+// Status bits (KL_STATUS_*) left by decode calls on the current device and stream and by the graphs
+// captured on the device.
 int64_t decode_status(bool clear) {
   const at::Device dev(at::kCUDA, c10::cuda::current_device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  at::Tensor sync;
-  {
-    std::lock_guard<std::mutex> lock(g_scratch_mu);
-    auto it = g_scratch.find({dev.index(), stream});
-    if (it == g_scratch.end() || !it->second.sync.defined()) return 0;
-    sync = it->second.sync;
-  }
+  std::vector<at::Tensor> words;
   uint32_t status = 0;
-  check_status(kl_paged_decode_read_status(sync.data_ptr(), &status, clear ? 1 : 0, stream), "decode_status");
+  {
+    ScratchPool& pool = scratch_pool();
+    const std::lock_guard<std::mutex> lock(pool.mu);
+    const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    collect_ended_graphs(pool);
+    const auto it = pool.streams.find({dev.index(), stream});
+    if (it != pool.streams.end() && it->second.sync.defined()) words.push_back(it->second.sync);
+    for (const auto& p : pool.graphs) {
+      if (p->device != dev.index()) continue;
+      for (const Scratch& s : p->grown) words.push_back(s.sync);
+    }
+    uint32_t& gone = pool.spare_status[dev.index()];
+    status = gone;
+    if (clear) gone = 0;
+  }
+  for (const at::Tensor& sync : words) {
+    uint32_t bits = 0;
+    check_status(kl_paged_decode_read_status(sync.data_ptr(), &bits, clear ? 1 : 0, stream), "decode_status");
+    status |= bits;
+  }
   return status;
 }
 
@@ -798,7 +968,7 @@ TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
 // Importing kernel_lab._C runs the registrations above.
 PYBIND11_MODULE(_C, m) {
   m.def("decode_status", &decode_status, pybind11::arg("clear") = false,
-        "Status bits left by paged_decode_attention on the current device and stream.");
+        "Status bits left by calls on the current device and stream and by the graphs captured on the device.");
   m.def("rms_norm_fp8", &rms_norm_fp8_new);
   m.def("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8_new);
   m.def("paged_kv_append_block8", &paged_kv_append_block8);

@@ -278,7 +278,7 @@ def paged_block_select(
 
 
 def decode_status(clear: bool = False) -> int:
-    """KL_STATUS_* bits left by decode and append calls on the current device and stream
-    (synchronises)."""
+    """KL_STATUS_* bits left by decode, append and selection calls on the current device and stream, and
+    by those of CUDA graphs captured on the device (synchronises)."""
     _require()
     return int(_C.decode_status(clear))
