@@ -34,6 +34,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <ATen/record_function.h>
 #include <torch/extension.h>
 
 #include <atomic>
@@ -720,6 +721,8 @@ void paged_decode_attention_block8(at::Tensor& out, const at::Tensor& q, const a
   const int d = static_cast<int>(q.size(2)), page = static_cast<int>(k_cache.size(1));
   const int max_pages = static_cast<int>(block_table.size(1));
   const c10::cuda::CUDAGuard guard(q.device());
+  // A view may start anywhere; the kernel reads q 16 bytes at a time.
+  const at::Tensor rows = reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 ? q : q.clone();
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   size_t partial_bytes = 0, sync_bytes = 0;
   check_status(kl_paged_decode_block8_workspace_size(static_cast<int>(batch), static_cast<int>(num_q_heads),
@@ -728,7 +731,7 @@ void paged_decode_attention_block8(at::Tensor& out, const at::Tensor& q, const a
                "paged_decode_attention_block8 (workspace)");
   const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(
-      kl_paged_decode_block8(to_dtype(q.scalar_type()), code_type, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+      kl_paged_decode_block8(to_dtype(q.scalar_type()), code_type, out.data_ptr(), rows.data_ptr(), k_cache.data_ptr(),
                              v_cache.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
                              block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(),
                              selected ? selected->data_ptr<int32_t>() : nullptr, static_cast<int>(batch),
@@ -813,9 +816,28 @@ int64_t decode_status(bool clear) {
   return status;
 }
 
-// Functional forms of the 8-bit ops for eager callers (kernel_lab.cuda_ops): outputs allocated here and
-// the implementation called directly, which costs a host 4-8 us less a call than allocating in Python
-// and going through the dispatcher. Traced code takes the torch.ops, which have Meta kernels.
+// Whether a call on these tensors (or None) may go past the dispatcher without anyone's noticing: plain CUDA tensors, and no
+// dispatch mode, transform or profiler that would see the operator.
+bool direct(const pybind11::args& tensors) {
+  c10::DispatchKeySet keys;
+  for (const pybind11::handle& t : tensors) {
+    if (t.is_none()) continue;
+    if (!THPVariable_Check(t.ptr())) return false;
+    const at::Tensor& tensor = THPVariable_Unpack(t.ptr());
+    if (!tensor.is_cuda()) return false;
+    keys = keys | tensor.key_set();
+  }
+  const auto tls = c10::impl::tls_local_dispatch_key_set();
+  // Keys that these operators fall through: no kernels for them.
+  const c10::DispatchKeySet through = c10::autograd_dispatch_keyset_with_ADInplaceOrView | c10::autocast_dispatch_keyset |
+                                      c10::DispatchKeySet(c10::DispatchKey::BackendSelect);
+  const c10::DispatchKeySet seen = ((keys | tls.included_) - tls.excluded_) - through;
+  return seen.highestPriorityTypeId() == c10::DispatchKey::CUDA && !at::hasCallbacks();
+}
+
+// Functional forms of the 8-bit ops for eager callers (kernel_lab.cuda_ops) whose call is direct(): outputs
+// allocated here and the implementation called directly, which costs a host 4-8 us less a call than
+// allocating in Python and going through the dispatcher. Others take the torch.ops, which have Meta kernels.
 std::pair<at::Tensor, at::Tensor> fp8_outputs(const at::Tensor& x, int64_t group_size) {
   TORCH_CHECK(group_size >= 0, "group_size must be >= 0");
   TORCH_CHECK(x.dim() >= 1 && x.is_cuda(), "x must be rows on CUDA");
@@ -846,10 +868,8 @@ at::Tensor paged_decode_attention_block8_new(const at::Tensor& q, const at::Tens
                                              const at::Tensor& k_scale, const at::Tensor& v_scale,
                                              const at::Tensor& block_table, const at::Tensor& seq_lens, double scale,
                                              const std::optional<at::Tensor>& selected) {
-  at::Tensor rows = q.contiguous();
-  if (reinterpret_cast<uintptr_t>(rows.data_ptr()) % 16 != 0) rows = rows.clone();  // a view may start anywhere
   at::Tensor out = at::empty(q.sizes(), q.options());
-  paged_decode_attention_block8(out, rows, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected);
+  paged_decode_attention_block8(out, q.contiguous(), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected);
   return out;
 }
 
@@ -969,6 +989,7 @@ TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
 PYBIND11_MODULE(_C, m) {
   m.def("decode_status", &decode_status, pybind11::arg("clear") = false,
         "Status bits left by calls on the current device and stream and by the graphs captured on the device.");
+  m.def("direct", &direct);
   m.def("rms_norm_fp8", &rms_norm_fp8_new);
   m.def("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8_new);
   m.def("paged_kv_append_block8", &paged_kv_append_block8);

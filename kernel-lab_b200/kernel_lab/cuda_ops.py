@@ -157,6 +157,11 @@ def paged_decode_attention_cascade(
     return out
 
 
+def _direct(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call may go past the dispatcher: real CUDA tensors, and nothing traces, transforms or watches it."""
+    return not torch.compiler.is_compiling() and not torch.overrides.has_torch_function(tensors) and _C.direct(*tensors)
+
+
 def rms_norm_fp8(
     x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, group_size: int = 0
 ) -> tuple[torch.Tensor, torch.Tensor]:
@@ -164,7 +169,7 @@ def rms_norm_fp8(
     a scale (0: a whole row); codes are torch.float8_e4m3fn in x's shape, scales float32
     [..., ceil(hidden / group_size)]. A scale is its group's largest magnitude / 448."""
     _require()
-    if not torch.compiler.is_compiling():
+    if _direct(x, weight):
         return _C.rms_norm_fp8(x, weight, eps, group_size)
     codes, scales = _fp8_outputs(x, group_size)
     torch.ops.kernel_lab.rms_norm_fp8(codes, scales, x, weight, eps, group_size)
@@ -177,7 +182,7 @@ def fused_add_rms_norm_fp8(
     """Functional form: (codes, scales, new_residual) of x + residual, ``residual`` left untouched.
     Call torch.ops.kernel_lab.fused_add_rms_norm_fp8 with residual_out = residual to update in place."""
     _require()
-    if not torch.compiler.is_compiling():
+    if _direct(x, residual, weight):
         return _C.fused_add_rms_norm_fp8(x, residual, weight, eps, group_size)
     codes, scales = _fp8_outputs(x, group_size)
     new_residual = torch.empty_like(x, memory_format=torch.contiguous_format)
@@ -215,10 +220,9 @@ def paged_kv_append_block8(
     :func:`paged_block_select`. Two sequences must not append to one page. Page ids outside the pool
     are skipped and reported by :func:`decode_status`."""
     _require()
-    append = torch.ops.kernel_lab.paged_kv_append_block8 if torch.compiler.is_compiling() else _C.paged_kv_append_block8
-    append(
-        k_cache, v_cache, k_scale, v_scale, k_bounds, k_new, v_new, block_table, positions, indptr
-    )
+    tensors = (k_cache, v_cache, k_scale, v_scale, k_bounds, k_new, v_new, block_table, positions, indptr)
+    append = _C.paged_kv_append_block8 if _direct(*tensors) else torch.ops.kernel_lab.paged_kv_append_block8
+    append(*tensors)
 
 
 def paged_decode_attention_block8(
@@ -238,7 +242,7 @@ def paged_decode_attention_block8(
     columns of its block-table row (each at most once; -1 selects nothing)."""
     _require()
     scale = q.shape[-1] ** -0.5 if scale is None else scale
-    if not torch.compiler.is_compiling():
+    if _direct(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, selected):
         return _C.paged_decode_attention_block8(
             q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale, selected
         )
@@ -266,7 +270,7 @@ def paged_block_select(
     them. Scores are sums of whole numbers (q rounded to int8 per head), ties go to the lower column:
     the choice is the same on every run and rank."""
     _require()
-    if not torch.compiler.is_compiling():
+    if _direct(q, k_cache, k_scale, k_bounds, block_table, seq_lens):
         return _C.paged_block_select(
             q, k_cache, k_scale, k_bounds, block_table, seq_lens, num_selected, sink_pages, recent_pages
         )
