@@ -342,7 +342,8 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
   const auto read_entry = [&](int e, int& page, int& col) {
     page = -1;
     col = e;
-    const int used = (l_len + a.page_size - 1) / a.page_size;
+    const uint32_t page_size = static_cast<uint32_t>(a.page_size);  // the sum may pass 31 bits
+    const int used = static_cast<int>((static_cast<uint32_t>(l_len) + page_size - 1u) / page_size);
     if (a.selected) {
       col = -1;
       if (e < a.num_selected) {

@@ -138,3 +138,23 @@ def test_small_elements_of_q_beside_a_large_one(kind, hq, hkv, dim, dtype, large
     table, seq = pool.tables()
     got = cuda_ops.paged_decode_attention_block8(q, **pool.gpu(), block_table=table, seq_lens=seq, scale=scale)
     check(pool, q, got, scale)
+
+
+@pytest.mark.parametrize("page", [16, 144, 4096])
+def test_lengths_near_the_end_of_32_bits(page):
+    """A table of nearly 2^31 tokens over three pages of the pool: the pages in use are counted without a sum that
+    passes 31 bits, and the last one ends inside a tile."""
+    from kernel_lab import cuda_ops
+
+    pool = Pool("int8", [3 * page], 1, 16, page, seed=48)
+    width = (2**31 - 1 - 64) // page
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    order = torch.from_numpy(pool.table[0].copy()).cuda()
+    columns = torch.tensor([0, width // 2, width - 1], dtype=torch.int32, device="cuda")
+    table[0, columns.long()] = order
+    length = width * page - 5
+    q = torch.randn(1, 4, 16, generator=torch.Generator().manual_seed(3)).to(torch.float16).cuda()
+    got = cuda_ops.paged_decode_attention_block8(q, **pool.gpu(), block_table=table, scale=0.02, selected=columns.view(1, 1, 3),
+                                                 seq_lens=torch.tensor([length], dtype=torch.int32, device="cuda"))
+    pool.lens = np.array([3 * page - 5])
+    check(pool, q, got, 0.02)
