@@ -212,3 +212,52 @@ def test_torch_compile_with_graphs():
         torch.compiler.cudagraph_mark_step_begin()
         got = [t.clone() for t in compiled(*args)]
         same(got, want)
+
+
+def test_a_captured_step_reads_what_each_replay_finds():
+    """norm -> append -> selection -> decode, captured once and replayed with other activations and positions: outputs,
+    caches, scales and bounds are the eager step's every time."""
+    from kernel_lab import cuda_ops
+
+    hq, hkv, dim, group = 16, 4, 128, 128
+    pool = Pool("e4m3", [4000, 2500, 40], hkv, dim, 16, "hnd", seed=70)
+    table, _ = pool.tables()
+    width = (hq + 2 * hkv) * dim
+    weight = torch.randn(width, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+
+    def start():
+        return {**pool.gpu(), "k_bounds": torch.from_numpy(pool.bounds).cuda(),
+                "residual": torch.randn(3, width, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()}
+
+    def step(s, x, position):
+        codes, scales, residual = cuda_ops.fused_add_rms_norm_fp8(x, s["residual"], weight, 1e-5, group_size=group)
+        s["residual"].copy_(residual)
+        rows = (codes.float().unflatten(-1, (-1, group)) * scales[..., None]).to(torch.bfloat16).view(3, hq + 2 * hkv, dim)
+        q, k, v = rows[:, :hq], rows[:, hq : hq + hkv], rows[:, hq + hkv :]
+        cache = {name: s[name] for name in ("k_cache", "v_cache", "k_scale", "v_scale")}
+        cuda_ops.paged_kv_append_block8(*cache.values(), k, v, table, position, k_bounds=s["k_bounds"])
+        lens = position + 1
+        chosen = cuda_ops.paged_block_select(q, s["k_cache"], s["k_scale"], s["k_bounds"], table, lens, 20)
+        sparse = cuda_ops.paged_decode_attention_block8(q, **cache, block_table=table, seq_lens=lens, selected=chosen)
+        return [codes.view(torch.uint8), scales, chosen, sparse,
+                cuda_ops.paged_decode_attention_block8(q, **cache, block_table=table, seq_lens=lens)]
+
+    xs = [torch.randn(3, width, generator=torch.Generator().manual_seed(10 + t)).to(torch.bfloat16).cuda() for t in range(5)]
+    positions = [torch.tensor(p, dtype=torch.int32, device="cuda") for p in
+                 ([3990, 2490, 0], [3991, 2491, 1], [3992, 30, 2], [100, 2492, 31], [3993, 0, 39])]
+    step(start(), xs[0], positions[0])
+    eager, captured = start(), start()
+    x, position = xs[0].clone(), positions[0].clone()
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        got = step(captured, x, position)
+    for t in range(5):
+        want = step(eager, xs[t], positions[t])
+        x.copy_(xs[t])
+        position.copy_(positions[t])
+        graph.replay()
+        same(got, want)
+        for name in eager:
+            a, b = (s[name].view(torch.uint8) if s[name].dtype == torch.float8_e4m3fn else s[name] for s in (captured, eager))
+            assert torch.equal(a, b), name
