@@ -12,7 +12,6 @@ constexpr float kLeastScale = 0x1p-126f;
 constexpr float kPer127 = 1.0f / 127.0f;  // int8 scales are products with this, one rounding, no division
 
 struct E4m3Code {
-  static constexpr float kMax = 448.0f;
   static constexpr int kBoundUnit = 4;  // 448 / 4 = 112 fits int8
   // The least power of two 2^k, k >= -126, with a <= 448 * 2^k: powers of two lose nothing (a code's
   // relative precision does not depend on the scale) and make a later growth exact. From the bits
@@ -42,7 +41,6 @@ struct E4m3Code {
 };
 
 struct Int8Code {
-  static constexpr float kMax = 127.0f;
   static constexpr int kBoundUnit = 1;
   static __device__ __forceinline__ float scale_for(float amax) {
     return amax > 0.0f ? fmaxf(amax * kPer127, kLeastScale) : 0.0f;

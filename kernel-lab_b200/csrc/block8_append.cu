@@ -587,7 +587,7 @@ __global__ void __launch_bounds__(kBlock8AppendThreads, kAppendBlocks) kv_append
         p.unpack(y);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) y[j] *= inv;
-        store_codes<Code, VEC>(put, y, plain);  // plain: |y| is at most a rounding above kMax
+        store_codes<Code, VEC>(put, y, plain);  // plain: |y| is at most a rounding above the largest code
         put += dst_step;
       };
       if (bounds) {

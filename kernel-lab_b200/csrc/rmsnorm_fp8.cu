@@ -28,7 +28,7 @@
 
 #include <cuda_runtime.h>
 
-#include "common.cuh"
+#include "block8.cuh"
 #include "kernel_lab_b200_block8.h"
 
 namespace klb {
@@ -126,12 +126,6 @@ __device__ __forceinline__ float largest(const float (&t)[N], float top) {
 #pragma unroll
   for (int j = 0; j < N; ++j) top = fmaxf(top, fabsf(t[j]));
   return top;
-}
-
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
 }
 
 // What a group's t are multiplied by for its codes, and the scale that undoes it for y.
@@ -256,7 +250,7 @@ __global__ void __launch_bounds__(512, 2) rmsnorm_fp8_row_regs(const NormFp8Args
       uint32_t c[P::N / 4];
 #pragma unroll
       for (int j = 0; j < P::N; j += 4) {
-        c[j / 4] = pack_e4m3x4(t[j] * inv, t[j + 1] * inv, t[j + 2] * inv, t[j + 3] * inv);
+        c[j / 4] = E4m3Code::code4(t[j] * inv, t[j + 1] * inv, t[j + 2] * inv, t[j + 3] * inv);
       }
       if constexpr (P::N == 8) {
         *reinterpret_cast<uint2*>(codes + pk * 8) = make_uint2(c[0], c[1]);
@@ -299,7 +293,7 @@ __global__ void __launch_bounds__(1024) rmsnorm_fp8_row_general(const NormFp8Arg
   const T* src = RES ? ro : xr;
   const auto t = [&](int i) { return Storage<T>::load(src[i]) * Storage<T>::load(w[i]); };
   const auto put = [&](int i, float inv) {
-    codes[i] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(t(i) * inv, __NV_SATFINITE, __NV_E4M3));
+    codes[i] = static_cast<uint8_t>(E4m3Code::code(t(i) * inv));
   };
   if (g.groups == 1) {
     float top = 0.0f;
