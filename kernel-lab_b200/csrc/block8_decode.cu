@@ -538,11 +538,12 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 
     float acc[NT][kHalves][kM][4];
     float m[NT][2], l[NT][2];
-    float w[NT][2];  // acc is in units of w
+    float per[NT][2];              // 1 / w: acc is in units of w
+    float most_per = 1.0f / kLeastWeight;  // the largest of this lane's
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       m[n][0] = m[n][1] = kNoMax;
-      w[n][0] = w[n][1] = kLeastWeight;
+      per[n][0] = per[n][1] = 1.0f / kLeastWeight;
       l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
       for (int f = 0; f < kHalves; ++f)
@@ -630,12 +631,8 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             x[q][n][e] = there[q][e >> 1] ? v : -INFINITY;
             most = fmaxf(most, x[q][n][e]);
           }
-      bool raise = most > kRaiseBy;
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) raise |= v_top * reciprocal_of_power(w[n][e]) > kWeightRange;
-      if (__any_sync(0xffffffffu, raise)) {
+      if (__any_sync(0xffffffffu, most > kRaiseBy || v_top * most_per > kWeightRange)) {
+        most_per = 0.0f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -654,7 +651,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             const float next = fmaxf(m[n][e], top);
             const float f = exp2_fast(m[n][e] - next);
             m[n][e] = next;
-            float heaviest = w[n][e] * f;
+            float heaviest = reciprocal_of_power(per[n][e]) * f;
             const float before = heaviest;
 #pragma unroll
             for (int q = 0; q < kTiles; ++q)
@@ -666,8 +663,9 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
             heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 4));
             heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 8));
             heaviest = fmaxf(heaviest, __shfl_xor_sync(0xffffffffu, heaviest, 16));
-            w[n][e] = weight_unit(heaviest);
-            const float k = before * reciprocal_of_power(w[n][e]);  // below 2
+            per[n][e] = reciprocal_of_power(weight_unit(heaviest));
+            most_per = fmaxf(most_per, per[n][e]);
+            const float k = before * per[n][e];  // below 2
             l[n][e] *= f;
 #pragma unroll
             for (int y = 0; y < kHalves; ++y)
@@ -684,7 +682,6 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
       uint32_t p0[kTiles][NT], p1[kTiles][NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const float per[2] = {reciprocal_of_power(w[n][0]), reciprocal_of_power(w[n][1])};
 #pragma unroll
         for (int q = 0; q < kTiles; ++q) {
           float p[4];
@@ -692,7 +689,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
           for (int e = 0; e < 4; ++e) {
             p[e] = exp2_fast(x[q][n][e]);
             l[n][e & 1] += p[e];
-            p[e] *= vs[q][e >> 1] * per[e & 1];
+            p[e] *= vs[q][e >> 1] * per[n][e & 1];
           }
           p0[q][n] = movmatrix_trans(Storage<__half>::pack2(p[0], p[1]));
           p1[q][n] = movmatrix_trans(Storage<__half>::pack2(p[2], p[3]));
@@ -748,7 +745,7 @@ __global__ void __launch_bounds__(kB8Threads, 1) decode_block8_kernel(const Bloc
 #pragma unroll
         for (int i = 0; i < kM; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= w[n][e & 1];
+          for (int e = 0; e < 4; ++e) acc[n][y][i][e] *= reciprocal_of_power(per[n][e & 1]);
     }
     // Join the TS parts: the upper half hands its state to the lower half, fragment by fragment, half
     // of the outputs of 8 query heads at a time.
