@@ -5,8 +5,8 @@
 Produces, inside ``kernel-lab_b200/kernel_lab/``:
 
 * ``libkernel_lab_b200.so`` -- the kernels and the C ABI declared in
-  ``include/kernel_lab_b200.h`` and ``include/kernel_lab_b200_block8.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
-  CUDA runtime linked statically, no PyTorch);
+  ``include/kernel_lab_b200.h``, ``include/kernel_lab_b200_block8.h`` and ``include/kernel_lab_b200_chunk.h``
+  (nvcc, ``-gencode arch=compute_100a,code=sm_100a``, CUDA runtime linked statically, no PyTorch);
 * ``_C<ext-suffix>.so`` -- the ``torch.ops.kernel_lab`` registrations, a thin C++
   layer over the C ABI, linked against the library above (rpath ``$ORIGIN``).
 
@@ -35,6 +35,7 @@ LIB = OUT_DIR / "libkernel_lab_b200.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 BLOCK8_HEADERS = [CSRC / "block8.cuh", INCLUDE / "kernel_lab_b200_block8.h"]
+CHUNK_HEADERS = [INCLUDE / "kernel_lab_b200_chunk.h", INCLUDE / "kernel_lab_b200_block8.h"]
 # Source -> the headers it includes beyond HEADERS.
 CU_SOURCES = {
     "rmsnorm.cu": [],
@@ -44,6 +45,9 @@ CU_SOURCES = {
     "block8_append.cu": BLOCK8_HEADERS,
     "block8_decode.cu": BLOCK8_HEADERS,
     "block8_select.cu": BLOCK8_HEADERS,
+    "chunk_append.cu": CHUNK_HEADERS,
+    "chunk_attention.cu": CHUNK_HEADERS,
+    "page_pool.cu": CHUNK_HEADERS,
 }
 HEADERS = [CSRC / "common.cuh", INCLUDE / "kernel_lab_b200.h"]
 
@@ -122,7 +126,7 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
         if not (force or stale(obj, [CSRC / src, *HEADERS, *more])):
             continue
         rel_src = str(rel_csrc / src)
-        if BLOCK8_HEADERS[0] in more:
+        if more:
             # Compiled in one part the allocation depends on the source alone (checked over object names) and
             # spills nothing that counts; in 8 parts the same text got 151 or 202 registers in the decode kernel
             # for groups of 8 (64 x 4096 tokens 98.5 or 94.1 us), by its object's name.

@@ -1,0 +1,332 @@
+// Attention of chunks of new tokens over a paged cache: sequence b's n new tokens are its last n, and token i
+// sees the keys up to its own position (causal) or all of them.
+//
+//   out[i, h] = sum_j p_ij V_j,   p_ij = exp(s_ij - max_j s_ij) / sum_j exp(s_ij - max_j s_ij),   s_ij = scale q_i.K_j
+//
+// The rows of one product are the (token, query head) pairs of a KV head: its query heads share keys and values.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "kernel_lab_b200.h"
+#include "kernel_lab_b200_chunk.h"
+
+namespace klb {
+namespace chunk_attention {
+
+struct Args {
+  void* out;
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* indptr;
+  int64_t tokens;
+  int64_t q_stride, page_stride, token_stride, head_stride;  // elements
+  int64_t scale_stride;                                      // of a page's scales
+  int64_t bt_stride, num_pages;
+  int batch, hq, hkv, group, dim, page_size, max_pages, causal;
+  float scale_log2;  // scale * log2(e)
+  uint32_t* status;
+};
+
+// Sequence b of the call: its rows first .. first + n - 1, its length.
+struct Seq {
+  int64_t first;
+  int n, len;
+};
+
+__device__ __forceinline__ Seq read_seq(const Args& a, int b, bool report) {
+  const int64_t lo = min(max(static_cast<int64_t>(__ldcg(a.indptr + b)), int64_t(0)), a.tokens);
+  const int64_t hi = min(max(static_cast<int64_t>(__ldcg(a.indptr + b + 1)), int64_t(0)), a.tokens);
+  Seq s{lo, static_cast<int>(max(hi - lo, int64_t(0))), max(0, __ldcg(a.seq_lens + b))};
+  const int room = a.max_pages * a.page_size;
+  if (s.len > room) {
+    s.len = room;
+    if (report) atomicOr(a.status, kStatusLenClamped);
+  }
+  return s;
+}
+
+// Keys that token i of the sequence sees.
+__device__ __forceinline__ int keys_of(const Args& a, const Seq& s, int i) {
+  return a.causal ? max(0, s.len - s.n + i + 1) : s.len;
+}
+
+// ----------------------------------------------------------------- CUDA-core kernel
+//
+// Any dtype, cache, group, head_dim up to 256, page size and stride. A CTA takes kRows rows of one KV head and
+// walks their keys kKeys at a time: K and V widened to fp32 in shared memory, a thread per four scores, eight
+// threads a row for the softmax and for the row's output.
+
+constexpr int kRows = 16, kKeys = 32, kThreads = 128, kMaxDim = 256;
+
+template <typename C>
+struct Code {  // an element of a cache, as fp32
+  static __device__ __forceinline__ float load(C v) { return Storage<C>::load(v); }
+};
+template <>
+struct Code<__nv_fp8_e4m3> {
+  static __device__ __forceinline__ float load(__nv_fp8_e4m3 v) { return static_cast<float>(v); }
+};
+template <>
+struct Code<int8_t> {
+  static __device__ __forceinline__ float load(int8_t v) { return static_cast<float>(v); }
+};
+
+size_t generic_smem(int dim) { return sizeof(float) * (static_cast<size_t>(kRows) * dim + kKeys * (2 * dim + 1) + kRows * kKeys); }
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant__ Args a) {
+  extern __shared__ float smem[];
+  __shared__ int s_found[2];
+  __shared__ int s_scan[kThreads / 32];
+  __shared__ int64_t s_page[kKeys];  // a key's page, -1: not to be attended to
+  __shared__ int s_slot[kKeys];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.dim;
+  float* sq = smem;                  // [kRows][dim]
+  float* sk = sq + kRows * dim;      // [kKeys][dim + 1]
+  float* sv = sk + kKeys * (dim + 1);
+  float* sp = sv + kKeys * dim;      // [kRows][kKeys]; -1: masked
+  wait_prior_grid();
+  allow_next_grid();
+
+  // Row block blockIdx.x of KV head blockIdx.y: whose it is.
+  const int target = blockIdx.x, kvh = blockIdx.y;
+  if (tid == 0) s_found[0] = -1;
+  long long run = 0;
+  for (int base = 0; base < a.batch; base += kThreads) {
+    const int b = base + tid;
+    int mine = 0;
+    if (b < a.batch) {
+      const Seq s = read_seq(a, b, false);
+      mine = static_cast<int>((static_cast<int64_t>(s.n) * a.group + kRows - 1) / kRows);
+    }
+    int inc = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, m);
+      if (lane >= m) inc += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    long long before = run;
+    for (int w = 0; w < warp; ++w) before += s_scan[w];
+    for (int w = 0; w < kThreads / 32; ++w) run += s_scan[w];
+    const long long first = before + inc - mine;
+    if (target >= first && target < first + mine) {
+      s_found[0] = b;
+      s_found[1] = static_cast<int>(target - first);
+    }
+    if (run > target) break;
+  }
+  __syncthreads();
+  const int b = s_found[0];
+  if (b < 0) return;
+  const Seq s = read_seq(a, b, tid == 0);
+  const int64_t row0 = static_cast<int64_t>(s_found[1]) * kRows, rows = static_cast<int64_t>(s.n) * a.group;
+
+  for (int i = tid; i < kRows * dim; i += kThreads) {
+    const int64_t r = row0 + i / dim;
+    float x = 0.0f;
+    if (r < rows) {
+      const int64_t token = s.first + r / a.group;
+      x = Storage<T>::load(static_cast<const T*>(a.q)[token * a.q_stride + (kvh * a.group + r % a.group) * static_cast<int64_t>(dim) + i % dim]);
+    }
+    sq[i] = x;
+  }
+  const int r = tid >> 3, part = tid & 7;  // this thread's row, and its eighth of the row
+  const int64_t my_row = row0 + r;
+  const int limit = my_row < rows ? keys_of(a, s, static_cast<int>(my_row / a.group)) : 0;
+  const int last_limit = keys_of(a, s, static_cast<int>((min(rows, row0 + kRows) - 1) / a.group));
+  float acc[kMaxDim / 8];
+#pragma unroll
+  for (int i = 0; i < kMaxDim / 8; ++i) acc[i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+
+  for (int k0 = 0; k0 < last_limit; k0 += kKeys) {
+    __syncthreads();
+    if (tid < kKeys) {
+      const int j = k0 + tid;
+      int64_t page = -1;
+      if (j < s.len) {
+        page = __ldcg(a.block_table + b * a.bt_stride + j / a.page_size);
+        if (page < 0 || page >= a.num_pages) {
+          page = -1;
+          atomicOr(a.status, kStatusBadPage);
+        }
+      }
+      s_page[tid] = page;
+      s_slot[tid] = j % a.page_size;
+    }
+    __syncthreads();
+    for (int i = tid; i < kKeys * dim; i += kThreads) {
+      const int j = i / dim, d = i - j * dim;
+      const int64_t page = s_page[j];
+      float x = 0.0f, y = 0.0f;
+      if (page >= 0) {
+        const int64_t at = page * a.page_stride + s_slot[j] * a.token_stride + kvh * a.head_stride + d;
+        x = Code<C>::load(static_cast<const C*>(a.k)[at]);
+        y = Code<C>::load(static_cast<const C*>(a.v)[at]);
+        if (!std::is_same<C, T>::value) {
+          x *= __ldcg(a.k_scale + page * a.scale_stride + kvh);
+          y *= __ldcg(a.v_scale + page * a.scale_stride + kvh);
+        }
+      }
+      sk[j * (dim + 1) + d] = x;
+      sv[i] = y;
+    }
+    __syncthreads();
+    float x[kKeys / 8];
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i) x[i] = 0.0f;
+    for (int d = 0; d < dim; ++d) {
+      const float qd = sq[r * dim + d];
+#pragma unroll
+      for (int i = 0; i < kKeys / 8; ++i) x[i] = fmaf(qd, sk[(part + 8 * i) * (dim + 1) + d], x[i]);
+    }
+    float mc = -INFINITY;
+    bool seen[kKeys / 8];
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i) {
+      const int j = part + 8 * i;
+      seen[i] = k0 + j < limit && s_page[j] >= 0;
+      x[i] *= a.scale_log2;
+      if (seen[i]) mc = fmaxf(mc, x[i]);
+    }
+#pragma unroll
+    for (int w = 4; w > 0; w >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, w));
+    const float mn = fmaxf(m, mc), shift = mn == -INFINITY ? 0.0f : mn;
+    const float alpha = exp2f(m - shift);
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kKeys / 8; ++i) {
+      const float p = exp2f(x[i] - shift);
+      if (seen[i]) sum += p;
+      sp[r * kKeys + part + 8 * i] = seen[i] ? p : -1.0f;
+    }
+#pragma unroll
+    for (int w = 4; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    m = mn;
+    l = l * alpha + sum;
+    __syncwarp();  // a row's eight threads are in one warp
+#pragma unroll
+    for (int i = 0; i < kMaxDim / 8; ++i) acc[i] *= alpha;
+    for (int j = 0; j < kKeys; ++j) {
+      const float p = sp[r * kKeys + j];
+      if (p < 0.0f) continue;  // masked, whatever V holds
+#pragma unroll
+      for (int i = 0; i < kMaxDim / 8; ++i) {
+        const int d = part + 8 * i;
+        if (d < dim) acc[i] = fmaf(p, sv[j * dim + d], acc[i]);
+      }
+    }
+  }
+  if (my_row >= rows) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(a.out) + ((s.first + my_row / a.group) * a.hq + kvh * a.group + my_row % a.group) * dim;
+#pragma unroll
+  for (int i = 0; i < kMaxDim / 8; ++i) {
+    const int d = part + 8 * i;
+    if (d < dim) out[d] = Storage<T>::store(acc[i] * inv);
+  }
+}
+
+template <typename T, typename C>
+cudaError_t launch_generic(const Args& a, cudaStream_t st) {
+  const size_t smem = generic_smem(a.dim);
+  cudaError_t e = cudaFuncSetAttribute(generic_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (e != cudaSuccess) return e;
+  // At most this many blocks of rows: each sequence's last one may be short.
+  const int64_t blocks = a.tokens * a.group / kRows + std::min<int64_t>(a.batch, a.tokens);
+  if (blocks > INT_MAX) return cudaErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.hkv));
+  return launch_kernel(true, generic_kernel<T, C>, grid, dim3(kThreads), smem, st, a);
+}
+
+}  // namespace chunk_attention
+}  // namespace klb
+
+extern "C" int kl_paged_chunk_attention_workspace_size(int dtype, int code_type, int64_t tokens, int batch,
+                                                       int num_q_heads, int num_kv_heads, int head_dim,
+                                                       size_t* partial_bytes, size_t* sync_bytes) {
+  if (!partial_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  *partial_bytes = 0;
+  *sync_bytes = 256;
+  return 0;
+}
+
+extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, const void* q, const void* k_cache,
+                                        const void* v_cache, const float* k_scale, const float* v_scale,
+                                        const int32_t* block_table, const int32_t* seq_lens, const int32_t* indptr,
+                                        int batch, int64_t tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                                        int page_size, int64_t q_row_stride, int64_t page_stride, int64_t token_stride,
+                                        int64_t head_stride, int64_t scale_page_stride, int64_t block_table_stride,
+                                        int max_pages_per_seq, int64_t num_pages, int causal, float scale,
+                                        void* partials, size_t partial_bytes, void* sync, size_t sync_bytes,
+                                        void* stream) {
+  using namespace klb::chunk_attention;
+  const int invalid = static_cast<int>(cudaErrorInvalidValue);
+  if (batch < 0 || tokens < 0) return invalid;
+  if (batch == 0 || tokens == 0) return 0;
+  if (dtype != KL_FLOAT32 && dtype != KL_FLOAT16 && dtype != KL_BFLOAT16) return invalid;
+  const bool coded = code_type != KL_CODE_NONE;
+  if (coded && code_type != KL_CODE_E4M3 && code_type != KL_CODE_INT8) return invalid;
+  if (coded && (dtype == KL_FLOAT32 || !k_scale || !v_scale || scale_page_stride < 0)) return invalid;
+  if (batch > 65535 || tokens > INT_MAX || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+      head_dim <= 0 || head_dim > kMaxDim || page_size <= 0 || max_pages_per_seq < 0 || block_table_stride < max_pages_per_seq ||
+      num_pages < 1 || static_cast<int64_t>(max_pages_per_seq) * page_size > INT_MAX - 256 ||
+      q_row_stride < static_cast<int64_t>(num_q_heads) * head_dim || page_stride < 0 || token_stride < 0 || head_stride < 0) {
+    return invalid;
+  }
+  if (!out || !q || !k_cache || !v_cache || !block_table || !seq_lens || !indptr || !sync || sync_bytes < 256) return invalid;
+  Args a{};
+  a.out = out;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.k_scale = k_scale;
+  a.v_scale = v_scale;
+  a.block_table = block_table;
+  a.seq_lens = seq_lens;
+  a.indptr = indptr;
+  a.tokens = tokens;
+  a.q_stride = q_row_stride;
+  a.page_stride = page_stride;
+  a.token_stride = token_stride;
+  a.head_stride = head_stride;
+  a.scale_stride = scale_page_stride;
+  a.bt_stride = block_table_stride;
+  a.num_pages = num_pages;
+  a.batch = batch;
+  a.hq = num_q_heads;
+  a.hkv = num_kv_heads;
+  a.group = num_q_heads / num_kv_heads;
+  a.dim = head_dim;
+  a.page_size = page_size;
+  a.max_pages = max_pages_per_seq;
+  a.causal = causal != 0;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.status = static_cast<uint32_t*>(sync);
+  const auto st = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (!coded) {
+    e = dtype == KL_FLOAT32   ? launch_generic<float, float>(a, st)
+        : dtype == KL_FLOAT16 ? launch_generic<__half, __half>(a, st)
+                              : launch_generic<__nv_bfloat16, __nv_bfloat16>(a, st);
+  } else if (dtype == KL_FLOAT16) {
+    e = code_type == KL_CODE_E4M3 ? launch_generic<__half, __nv_fp8_e4m3>(a, st) : launch_generic<__half, int8_t>(a, st);
+  } else {
+    e = code_type == KL_CODE_E4M3 ? launch_generic<__nv_bfloat16, __nv_fp8_e4m3>(a, st)
+                                  : launch_generic<__nv_bfloat16, int8_t>(a, st);
+  }
+  return static_cast<int>(e);
+}

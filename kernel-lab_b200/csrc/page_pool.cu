@@ -1,0 +1,632 @@
+// The pages of a paged cache: copied, given to growing and forked sequences (reserve), compacted.
+//
+// No counts are kept: a page is in use if the first ceil(len / page_size) entries of some row name it. A call
+// marks every page that its rows name in an array of one word a page, finds the free ones by a scan over that
+// array in the order of the ids, and writes the new table; what has to move goes on a list of (source,
+// destination) pages that the copy kernel works off. Everything follows from the inputs alone (marks by
+// atomic maximum, ranks by scans), so two runs give the same table.
+//
+// Bookkeeping: one cluster of kClusterCtas CTAs of kPlanThreads threads, phases divided by cluster barriers: one
+// launch, the CTAs of a cluster being resident together by definition. It is bound by latency: table and marks
+// are a few hundred KB that stay in L2.
+// Copies: HBM-bound, 2 * bytes. CTAs take 16 KB slices of a page, all loads of a slice before its stores.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+
+#include "common.cuh"
+#include "kernel_lab_b200.h"
+#include "kernel_lab_b200_chunk.h"
+
+namespace klb {
+namespace page_pool {
+
+namespace cg = cooperative_groups;
+
+constexpr uint32_t kStatusNoPages = KL_STATUS_NO_PAGES;
+
+// ----------------------------------------------------------------- copies
+
+constexpr int kCopyThreads = 256;
+constexpr int kSlice = 16384;     // bytes of a page that a CTA takes at a time
+constexpr int kMaxTensors = 64;   // of one launch
+
+struct CopyArgs {
+  uint8_t* base[kMaxTensors];
+  int64_t stride[kMaxTensors];
+  int64_t bytes[kMaxTensors];
+  int64_t slice_end[kMaxTensors];  // slices of a page in the tensors up to this one
+  uint8_t unit[kMaxTensors];       // bytes of a load: 16, 4 or 1
+  int count;
+  const int32_t* src;
+  const int32_t* dst;
+  int64_t pairs;
+  const int32_t* pairs_on_device;  // if non-null, their number
+  int64_t num_pages;
+  uint32_t* status;
+};
+
+template <typename U>
+__device__ __forceinline__ void copy_slice(uint8_t* to, const uint8_t* from, int bytes) {
+  constexpr int K = kSlice / 16 / kCopyThreads;
+  const U* s = reinterpret_cast<const U*>(from);
+  U* d = reinterpret_cast<U*>(to);
+  const int n = bytes / static_cast<int>(sizeof(U));
+  for (int base = threadIdx.x; base < n; base += K * kCopyThreads) {
+    U v[K];
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      if (base + u * kCopyThreads < n) v[u] = s[base + u * kCopyThreads];
+    }
+#pragma unroll
+    for (int u = 0; u < K; ++u) {
+      if (base + u * kCopyThreads < n) d[base + u * kCopyThreads] = v[u];
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) copy_pages(const __grid_constant__ CopyArgs a) {
+  wait_prior_grid();
+  allow_next_grid();
+  const int64_t pairs = a.pairs_on_device ? __ldcg(a.pairs_on_device) : a.pairs;
+  const int64_t per_page = a.slice_end[a.count - 1];
+  for (int64_t item = blockIdx.x; item < pairs * per_page; item += gridDim.x) {
+    const int64_t i = item / per_page, s = item - i * per_page;
+    const int from = __ldcg(a.src + i), to = __ldcg(a.dst + i);
+    if (from < 0 || to < 0) continue;
+    if (from >= a.num_pages || to >= a.num_pages) {
+      if (threadIdx.x == 0 && a.status) atomicOr(a.status, kStatusBadPage);
+      continue;
+    }
+    int t = 0, hi = a.count - 1;  // the first tensor with slice_end > s
+    while (t < hi) {
+      const int mid = (t + hi) >> 1;
+      if (a.slice_end[mid] > s) hi = mid; else t = mid + 1;
+    }
+    const int64_t off = (s - (t ? a.slice_end[t - 1] : 0)) * kSlice;
+    const int bytes = static_cast<int>(min(static_cast<int64_t>(kSlice), a.bytes[t] - off));
+    const uint8_t* p = a.base[t] + from * a.stride[t] + off;
+    uint8_t* q = a.base[t] + to * a.stride[t] + off;
+    if (a.unit[t] == 16) copy_slice<uint4>(q, p, bytes);
+    else if (a.unit[t] == 4) copy_slice<uint32_t>(q, p, bytes);
+    else copy_slice<uint8_t>(q, p, bytes);
+  }
+}
+
+bool valid(const kl_page_pools_t* pools) {
+  if (!pools || pools->count < 0 || (pools->count > 0 && (!pools->base || !pools->stride || !pools->bytes))) return false;
+  for (int t = 0; t < pools->count; ++t) {
+    if (!pools->base[t] || pools->bytes[t] < 0 || pools->stride[t] < pools->bytes[t]) return false;
+  }
+  return true;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return n;
+}
+
+// `pairs`: their number, or with pairs_on_device the most that there can be.
+cudaError_t launch_copies(const kl_page_pools_t* pools, const int32_t* src, const int32_t* dst, int64_t pairs,
+                          const int32_t* pairs_on_device, int64_t num_pages, uint32_t* status, cudaStream_t st) {
+  if (pairs == 0) return cudaSuccess;
+  for (int first = 0; first < pools->count; first += kMaxTensors) {
+    CopyArgs a{};
+    int64_t slices = 0;
+    for (int t = first; t < pools->count && t < first + kMaxTensors; ++t) {
+      if (pools->bytes[t] == 0) continue;
+      const int k = a.count++;
+      a.base[k] = static_cast<uint8_t*>(pools->base[t]);
+      a.stride[k] = pools->stride[t];
+      a.bytes[k] = pools->bytes[t];
+      slices += (a.bytes[k] + kSlice - 1) / kSlice;
+      a.slice_end[k] = slices;
+      const int64_t bits = static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.base[k])) | a.stride[k] | a.bytes[k];
+      a.unit[k] = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+    }
+    if (a.count == 0) continue;
+    a.src = src;
+    a.dst = dst;
+    a.pairs = pairs;
+    a.pairs_on_device = pairs_on_device;
+    a.num_pages = num_pages;
+    a.status = status;
+    const int64_t most = pairs > INT64_MAX / slices ? INT64_MAX : pairs * slices;
+    const int64_t grid = std::min<int64_t>(most, static_cast<int64_t>(sm_count()) * 8);
+    const cudaError_t e = launch_kernel(true, copy_pages, dim3(static_cast<unsigned>(grid)), dim3(kCopyThreads), 0, st, a);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+// ----------------------------------------------------------------- bookkeeping
+
+constexpr int kClusterCtas = 8;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kHeld = INT_MAX;  // the mark of a page that a row holds and is not about to write
+
+struct PlanArgs {
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* new_tokens;  // reserve
+  const int32_t* parents;     // reserve; may be null
+  int32_t* out_table;
+  int32_t* out_lens;          // reserve
+  uint8_t* served;            // reserve
+  int32_t* used;              // compact
+  int64_t bt_stride;
+  int64_t num_pages;
+  int batch, rows, width, page_size;
+  // scratch
+  int32_t* mark;       // [num_pages, rounded up to 4]
+  int32_t* pool_list;  // [num_pages]: free ids in order (reserve), sources of moves (compact)
+  int32_t* src;        // pairs to copy
+  int32_t* dst;
+  int32_t* count;      // their number
+  int64_t* begin;      // [rows]: the row's first page among those given out
+  int32_t* copy_begin; // [rows]: its copy's place on the list
+  int64_t* totals;     // [0]: pages needed
+  uint32_t* status;
+};
+
+struct Shared {
+  long long warp_a[kPlanWarps], warp_b[kPlanWarps];
+  long long total_a, total_b;
+  long long cta_count;  // read by the other CTAs
+};
+
+// Exclusive block-wide prefix sums of two numbers a thread; the totals in sh.total_a and sh.total_b.
+__device__ __forceinline__ void scan_two(Shared& sh, long long& a, long long& b) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long ia = a, ib = b;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const long long ya = __shfl_up_sync(0xffffffffu, ia, m), yb = __shfl_up_sync(0xffffffffu, ib, m);
+    if (lane >= m) {
+      ia += ya;
+      ib += yb;
+    }
+  }
+  __syncthreads();  // the previous use of the arrays is over
+  if (lane == 31) {
+    sh.warp_a[warp] = ia;
+    sh.warp_b[warp] = ib;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const long long wa = sh.warp_a[lane], wb = sh.warp_b[lane];
+    long long xa = wa, xb = wb;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const long long ya = __shfl_up_sync(0xffffffffu, xa, m), yb = __shfl_up_sync(0xffffffffu, xb, m);
+      if (lane >= m) {
+        xa += ya;
+        xb += yb;
+      }
+    }
+    sh.warp_a[lane] = xa - wa;
+    sh.warp_b[lane] = xb - wb;
+    if (lane == 31) {
+      sh.total_a = xa;
+      sh.total_b = xb;
+    }
+  }
+  __syncthreads();
+  a = ia - a + sh.warp_a[warp];
+  b = ib - b + sh.warp_b[warp];
+}
+
+struct Row {
+  int parent;  // -1: empty
+  int len, have;
+};
+
+__device__ __forceinline__ Row read_row(const PlanArgs& a, int r, bool report) {
+  Row x{r, 0, 0};
+  if (a.parents) x.parent = __ldcg(a.parents + r);
+  if (x.parent < 0 || x.parent >= a.batch) {
+    x.parent = -1;
+    return x;
+  }
+  x.len = max(0, __ldcg(a.seq_lens + x.parent));
+  const long long room = static_cast<long long>(a.width) * a.page_size;
+  if (x.len > room) {
+    x.len = static_cast<int>(room);
+    if (report && a.status) atomicOr(a.status, kStatusLenClamped);
+  }
+  x.have = (x.len + a.page_size - 1) / a.page_size;  // room < 2^31 - page_size
+  return x;
+}
+
+__device__ __forceinline__ void store_mark(int32_t* p, int v) {
+  asm volatile("st.relaxed.gpu.global.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+
+// This CTA's pages: a multiple of 4 of them, so that marks are read 16 bytes at a time.
+__device__ __forceinline__ void own_pages(const PlanArgs& a, int cta, int64_t& lo, int64_t& hi) {
+  const int64_t quads = (a.num_pages + 3) / 4, per = (quads + kClusterCtas - 1) / kClusterCtas;
+  lo = min(quads, cta * per) * 4;
+  hi = min(quads, (cta + 1) * per) * 4;
+}
+
+__device__ __forceinline__ int4 marks_at(const PlanArgs& a, int64_t p) {
+  int4 m = __ldcg(reinterpret_cast<const int4*>(a.mark + p));
+  // Places past the last page count as held.
+  if (p + 1 >= a.num_pages) m.y = kHeld;
+  if (p + 2 >= a.num_pages) m.z = kHeld;
+  if (p + 3 >= a.num_pages) m.w = kHeld;
+  return m;
+}
+
+__device__ __forceinline__ void clear_marks(const PlanArgs& a, int cta) {
+  int64_t lo, hi;
+  own_pages(a, cta, lo, hi);
+  for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
+    __stcg(reinterpret_cast<int4*>(a.mark + p), make_int4(0, 0, 0, 0));
+  }
+}
+
+__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPlanThreads)
+reserve_plan(const __grid_constant__ PlanArgs a) {
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cta = static_cast<int>(cluster.block_rank());
+  const int lane = threadIdx.x & 31, warp = cta * kPlanWarps + (threadIdx.x >> 5);
+  constexpr int kWarps = kClusterCtas * kPlanWarps;
+  wait_prior_grid();
+  allow_next_grid();
+  clear_marks(a, cta);
+  cluster.sync();
+
+  // Marks, and the rows' entries taken over. A row that is to write its last page marks it with rows - r (of
+  // several the lowest has the largest), any other holder with kHeld.
+  for (int r = warp; r < a.rows; r += kWarps) {
+    const Row x = read_row(a, r, lane == 0);
+    const int add = max(0, __ldcg(a.new_tokens + r));
+    const bool writes = x.parent >= 0 && add > 0 && x.len % a.page_size != 0;
+    const int32_t* in = a.block_table + (x.parent < 0 ? 0 : x.parent) * a.bt_stride;
+    int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
+    for (int c = lane; c < a.width; c += 32) {
+      int e = 0;
+      if (c < x.have) {
+        e = __ldcg(in + c);
+        if (e < 0 || e >= a.num_pages) {
+          if (a.status) atomicOr(a.status, kStatusBadPage);
+        } else if (writes && c == x.have - 1) {
+          atomicMax(a.mark + e, a.rows - r);
+        } else {
+          store_mark(a.mark + e, kHeld);
+        }
+      }
+      out[c] = e;
+    }
+    if (lane == 0) a.out_lens[r] = x.len;
+  }
+  cluster.sync();
+
+  // What each row needs, summed in order (CTA 0); the free pages of each CTA's part.
+  int64_t lo, hi;
+  own_pages(a, cta, lo, hi);
+  long long mine = 0, none = 0;
+  for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
+    const int4 m = marks_at(a, p);
+    mine += (m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0);
+  }
+  scan_two(sh, mine, none);
+  if (threadIdx.x == 0) sh.cta_count = sh.total_a;
+  if (cta == 0) {
+    long long need_before = 0, copies_before = 0;
+    for (int base = 0; base < a.rows; base += kPlanThreads) {
+      const int r = base + threadIdx.x;
+      long long need = 0, copy = 0;
+      if (r < a.rows) {
+        const Row x = read_row(a, r, false);
+        const long long add = x.parent < 0 ? 0 : max(0, __ldcg(a.new_tokens + r));
+        if (x.len + add <= static_cast<long long>(a.width) * a.page_size) {
+          if (add > 0 && x.len % a.page_size != 0) {
+            const int last = __ldcg(a.block_table + x.parent * a.bt_stride + x.have - 1);
+            if (last >= 0 && last < a.num_pages) copy = __ldcg(a.mark + last) != a.rows - r;
+          }
+          need = copy + (x.len + add + a.page_size - 1) / a.page_size - x.have;
+        } else {
+          need = -1;  // does not fit
+        }
+      }
+      const bool fits = need >= 0;
+      long long n = fits ? need : 0, k = copy;
+      scan_two(sh, n, k);
+      if (r < a.rows) {
+        a.begin[r] = fits ? need_before + n : -1;
+        a.copy_begin[r] = copy ? static_cast<int32_t>(copies_before + k) : -1;
+      }
+      need_before += sh.total_a;
+      copies_before += sh.total_b;
+    }
+    if (threadIdx.x == 0) {
+      a.totals[0] = need_before;
+      *a.count = static_cast<int32_t>(copies_before);
+    }
+  }
+  cluster.sync();
+
+  // The lowest free pages in order, as many as are needed.
+  long long before = 0, all = 0;
+  for (int c = 0; c < kClusterCtas; ++c) {
+    const long long n = cluster.map_shared_rank(&sh, c)->cta_count;
+    if (c < cta) before += n;
+    all += n;
+  }
+  const long long wanted = min(static_cast<long long>(__ldcg(a.totals)), all);
+  for (int64_t p0 = lo; p0 < hi && before < wanted; p0 += kPlanThreads * 4) {
+    const int64_t p = p0 + threadIdx.x * 4;
+    int4 m = make_int4(kHeld, kHeld, kHeld, kHeld);
+    if (p < hi) m = marks_at(a, p);
+    long long at = (m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0), unused = 0;
+    scan_two(sh, at, unused);
+    at += before;
+    const int marks[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (marks[u] == 0) {
+        if (at < wanted) __stcg(a.pool_list + at, static_cast<int32_t>(p + u));
+        ++at;
+      }
+    }
+    before += sh.total_a;
+  }
+  cluster.sync();  // also: no CTA has left while another reads its count
+
+  for (int r = warp; r < a.rows; r += kWarps) {
+    const Row x = read_row(a, r, false);
+    const long long add = x.parent < 0 ? 0 : max(0, __ldcg(a.new_tokens + r));
+    const long long begin = __ldcg(a.begin + r);
+    const int copy_at = __ldcg(a.copy_begin + r);
+    const int grown = begin < 0 ? 0 : static_cast<int>((x.len + add + a.page_size - 1) / a.page_size - x.have);
+    const int copies = copy_at >= 0;
+    const bool ok = begin >= 0 && (grown + copies == 0 || begin + grown + copies <= all);
+    int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
+    if (lane == 0) {
+      a.served[r] = ok;
+      if (!ok && a.status) atomicOr(a.status, kStatusNoPages);
+      if (copies) {
+        int from = -1, to = -1;
+        if (ok) {
+          from = __ldcg(a.block_table + x.parent * a.bt_stride + x.have - 1);
+          to = __ldcg(a.pool_list + begin);
+          out[x.have - 1] = to;
+        }
+        a.src[copy_at] = from;
+        a.dst[copy_at] = to;
+      }
+    }
+    for (int i = lane; ok && i < grown; i += 32) out[x.have + i] = __ldcg(a.pool_list + begin + copies + i);
+  }
+}
+
+__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPlanThreads)
+compact_plan(const __grid_constant__ PlanArgs a) {
+  __shared__ Shared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int cta = static_cast<int>(cluster.block_rank());
+  const int lane = threadIdx.x & 31, warp = cta * kPlanWarps + (threadIdx.x >> 5);
+  constexpr int kWarps = kClusterCtas * kPlanWarps;
+  wait_prior_grid();
+  allow_next_grid();
+  clear_marks(a, cta);
+  cluster.sync();
+  for (int r = warp; r < a.rows; r += kWarps) {
+    const Row x = read_row(a, r, lane == 0);
+    const int32_t* in = a.block_table + static_cast<int64_t>(r) * a.bt_stride;
+    for (int c = lane; c < x.have; c += 32) {
+      const int e = __ldcg(in + c);
+      if (e >= 0 && e < a.num_pages) {
+        store_mark(a.mark + e, kHeld);
+      } else if (a.status) {
+        atomicOr(a.status, kStatusBadPage);
+      }
+    }
+  }
+  cluster.sync();
+
+  int64_t lo, hi;
+  own_pages(a, cta, lo, hi);
+  long long mine = 0, none = 0;
+  for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
+    const int4 m = marks_at(a, p);
+    mine += min(a.num_pages, p + 4) - p - ((m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0));
+  }
+  scan_two(sh, mine, none);
+  if (threadIdx.x == 0) sh.cta_count = sh.total_a;
+  cluster.sync();
+  long long before = 0, used = 0;
+  for (int c = 0; c < kClusterCtas; ++c) {
+    const long long n = cluster.map_shared_rank(&sh, c)->cta_count;
+    if (c < cta) before += n;
+    used += n;
+  }
+  // Page p with L(p) pages in use below it. The free ones below `used` come in order as number p - L(p), the
+  // ones in use from `used` on, counted down from the last, as number used - 1 - L(p): as many as the former.
+  // In ascending order they are number L(p) - L(used), and L(used) = used - (free ones below it).
+  for (int64_t p0 = lo; p0 < hi; p0 += kPlanThreads * 4) {
+    const int64_t p = p0 + threadIdx.x * 4;
+    int4 m = make_int4(0, 0, 0, 0);
+    if (p < hi) m = marks_at(a, p);
+    const int marks[4] = {m.x, m.y, m.z, m.w};
+    long long at = 0, unused = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at += marks[u] != 0 && p + u < a.num_pages && p < hi;
+    scan_two(sh, at, unused);
+    at += before;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int64_t id = p + u;
+      if (p >= hi || id >= a.num_pages) continue;
+      const bool in_use = marks[u] != 0;
+      if (in_use && id >= used) a.pool_list[used - 1 - at] = static_cast<int32_t>(id);  // last first
+      if (!in_use && id < used) __stcg(a.dst + (id - at), static_cast<int32_t>(id));
+      if (id == used - 1) *a.count = static_cast<int32_t>(used - at - in_use);  // free ones below `used`
+      at += in_use;
+    }
+    before += sh.total_a;
+  }
+  if (cta == 0 && threadIdx.x == 0) {
+    *a.used = static_cast<int32_t>(used);
+    if (used == 0) *a.count = 0;
+  }
+  cluster.sync();  // also: no CTA has left while another reads its count
+  const int moves = __ldcg(a.count);
+  for (int i = cta * kPlanThreads + threadIdx.x; i < moves; i += kClusterCtas * kPlanThreads) {
+    const int from = __ldcg(a.pool_list + (moves - 1 - i)), to = __ldcg(a.dst + i);
+    a.src[i] = from;
+    __stcg(a.mark + from, to + 1);  // where the page goes; its mark is not needed any more
+  }
+  cluster.sync();
+  for (int r = warp; r < a.rows; r += kWarps) {
+    const Row x = read_row(a, r, false);
+    const int32_t* in = a.block_table + static_cast<int64_t>(r) * a.bt_stride;
+    int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
+    for (int c = lane; c < a.width; c += 32) {
+      int e = c < x.have ? __ldcg(in + c) : 0;
+      if (c < x.have && e >= used && e < a.num_pages) e = __ldcg(a.mark + e) - 1;
+      out[c] = e;
+    }
+  }
+}
+
+size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
+
+// The scratch of a call, cut into its arrays; returns its size.
+size_t cut(PlanArgs& a, uint8_t* p, int64_t num_pages, int64_t rows, int64_t pairs) {
+  size_t off = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* at = p + off;
+    off += rounded(bytes);
+    return at;
+  };
+  const size_t pages = static_cast<size_t>(num_pages + 3) / 4 * 4;
+  a.totals = reinterpret_cast<int64_t*>(take(16));
+  a.count = reinterpret_cast<int32_t*>(take(4));
+  a.mark = reinterpret_cast<int32_t*>(take(pages * 4));
+  a.pool_list = reinterpret_cast<int32_t*>(take(pages * 4));
+  a.src = reinterpret_cast<int32_t*>(take(static_cast<size_t>(pairs) * 4));
+  a.dst = reinterpret_cast<int32_t*>(take(static_cast<size_t>(pairs) * 4));
+  a.begin = reinterpret_cast<int64_t*>(take(static_cast<size_t>(rows) * 8));
+  a.copy_begin = reinterpret_cast<int32_t*>(take(static_cast<size_t>(rows) * 4));
+  return off;
+}
+
+constexpr int kMaxRows = 1 << 24;
+
+bool sizes_ok(int batch, int rows, int width, int page_size, int64_t bt_stride, int64_t num_pages) {
+  return batch >= 0 && rows >= 0 && rows <= kMaxRows && width >= 0 && page_size > 0 && bt_stride >= width && num_pages >= 0 &&
+         num_pages <= INT32_MAX - 8 && static_cast<int64_t>(width) * page_size <= INT32_MAX - page_size;
+}
+
+bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
+}
+
+bool tables_overlap(const PlanArgs& a) {
+  const int64_t in = a.batch > 0 ? ((a.batch - 1) * a.bt_stride + a.width) * 4 : 0;
+  return overlap(a.out_table, static_cast<int64_t>(a.rows) * a.width * 4, a.block_table, in);
+}
+
+}  // namespace page_pool
+}  // namespace klb
+
+extern "C" int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const int32_t* dst, int64_t pairs,
+                                   int64_t num_pages, uint32_t* status, void* stream) {
+  using namespace klb::page_pool;
+  if (!valid(pools) || pairs < 0 || pairs > INT32_MAX || num_pages < 0 || num_pages > INT32_MAX || (pairs > 0 && (!src || !dst))) {
+    return static_cast<int>(cudaErrorInvalidValue);
+  }
+  if (pairs == 0) return 0;
+  return static_cast<int>(launch_copies(pools, src, dst, pairs, nullptr, num_pages, status, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes) {
+  using namespace klb::page_pool;
+  if (num_pages < 0 || num_pages > INT32_MAX - 8 || rows < 0 || rows > kMaxRows || !scratch_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  PlanArgs a{};
+  *scratch_bytes = cut(a, nullptr, num_pages, rows, rows);
+  return 0;
+}
+
+extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table, int32_t* out_lens, uint8_t* served,
+                                const int32_t* block_table, const int32_t* seq_lens, const int32_t* new_tokens,
+                                const int32_t* parents, int batch, int rows, int width, int page_size,
+                                int64_t block_table_stride, int64_t num_pages, void* scratch, size_t scratch_bytes,
+                                uint32_t* status, void* stream) {
+  using namespace klb::page_pool;
+  const int invalid = static_cast<int>(cudaErrorInvalidValue);
+  if (!valid(pools) || !sizes_ok(batch, rows, width, page_size, block_table_stride, num_pages)) return invalid;
+  if (!parents && rows != batch) return invalid;
+  if (rows == 0) return 0;
+  if (!out_lens || !served || !new_tokens || (batch > 0 && !seq_lens) || (width > 0 && (!out_table || (batch > 0 && !block_table)))) return invalid;
+  PlanArgs a{};
+  const size_t need = cut(a, static_cast<uint8_t*>(scratch), num_pages, rows, rows);
+  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) return invalid;
+  a.block_table = block_table;
+  a.seq_lens = seq_lens;
+  a.new_tokens = new_tokens;
+  a.parents = parents;
+  a.out_table = out_table;
+  a.out_lens = out_lens;
+  a.served = served;
+  a.bt_stride = block_table_stride;
+  a.num_pages = num_pages;
+  a.batch = batch;
+  a.rows = rows;
+  a.width = width;
+  a.page_size = page_size;
+  a.status = status;
+  if (tables_overlap(a)) return invalid;
+  const auto st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = klb::launch_kernel(true, reserve_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return static_cast<int>(launch_copies(pools, a.src, a.dst, rows, a.count, num_pages, status, st));
+}
+
+extern "C" int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes) {
+  using namespace klb::page_pool;
+  if (num_pages < 0 || num_pages > INT32_MAX - 8 || !scratch_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  PlanArgs a{};
+  *scratch_bytes = cut(a, nullptr, num_pages, 0, num_pages);
+  return 0;
+}
+
+extern "C" int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table, int32_t* used,
+                                const int32_t* block_table, const int32_t* seq_lens, int batch, int width,
+                                int page_size, int64_t block_table_stride, int64_t num_pages, void* scratch,
+                                size_t scratch_bytes, uint32_t* status, void* stream) {
+  using namespace klb::page_pool;
+  const int invalid = static_cast<int>(cudaErrorInvalidValue);
+  if (!valid(pools) || !sizes_ok(batch, batch, width, page_size, block_table_stride, num_pages) || !used) return invalid;
+  if (batch > 0 && (!seq_lens || (width > 0 && (!out_table || !block_table)))) return invalid;
+  PlanArgs a{};
+  const size_t need = cut(a, static_cast<uint8_t*>(scratch), num_pages, 0, num_pages);
+  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) return invalid;
+  a.block_table = block_table;
+  a.seq_lens = seq_lens;
+  a.out_table = out_table;
+  a.used = used;
+  a.bt_stride = block_table_stride;
+  a.num_pages = num_pages;
+  a.batch = batch;
+  a.rows = batch;
+  a.width = width;
+  a.page_size = page_size;
+  a.status = status;
+  if (tables_overlap(a)) return invalid;
+  const auto st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = klb::launch_kernel(true, compact_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  // Pages with ids of `used` and more that go below it: at most half of them.
+  return static_cast<int>(launch_copies(pools, a.src, a.dst, num_pages / 2, a.count, num_pages, status, st));
+}

@@ -14,6 +14,8 @@
 //
 // The 8-bit serving step (kernel_lab_b200_block8.h): rms_norm_fp8, fused_add_rms_norm_fp8,
 // paged_kv_append_block8, paged_decode_attention_block8 and paged_block_select.
+// The chunked step (kernel_lab_b200_chunk.h): paged_kv_append_chunks(_fp8), paged_chunk_attention(_fp8,
+// _block8), paged_copy_pages, paged_reserve and paged_compact.
 //
 // Decode scratch (split partials and arrival counters) is owned here, one pair of
 // buffers per (device, stream), grown on demand. The counters are zeroed once at allocation; every call
@@ -37,6 +39,7 @@
 #include <ATen/record_function.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <memory>
@@ -46,6 +49,7 @@
 
 #include "kernel_lab_b200.h"
 #include "kernel_lab_b200_block8.h"
+#include "kernel_lab_b200_chunk.h"
 
 namespace {
 
@@ -786,6 +790,270 @@ void paged_block_select(at::Tensor& selected, const at::Tensor& q, const at::Ten
       "paged_block_select");
 }
 
+// Rows of chunks: sequence b's are indptr[b] .. indptr[b + 1] - 1.
+void check_indptr(const at::Tensor& indptr, int64_t batch, const at::Device& dev) {
+  TORCH_CHECK(indptr.scalar_type() == at::kInt && indptr.is_contiguous() && indptr.dim() == 1 && indptr.numel() == batch + 1 &&
+                  indptr.device() == dev,
+              "indptr is contiguous int32 [batch + 1] on the caches' device");
+}
+
+// Append of chunks (kl_paged_kv_append_chunks; with scales kl_paged_kv_append_chunks_fp8).
+void append_chunks_impl(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& k_new, const at::Tensor& v_new,
+                        const at::Tensor* k_scale, const at::Tensor* v_scale, const at::Tensor& block_table,
+                        const at::Tensor& positions, const at::Tensor& indptr, const char* what) {
+  TORCH_CHECK(k_cache.is_cuda() && v_cache.is_cuda() && k_new.is_cuda() && v_new.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.is_contiguous() && v_cache.is_contiguous() && k_cache.sizes() == v_cache.sizes() &&
+                  k_cache.scalar_type() == v_cache.scalar_type(),
+              "caches are contiguous [num_pages, page_size, num_kv_heads, head_dim] of one shape and dtype");
+  const int64_t num_kv_heads = k_cache.size(2), head_dim = k_cache.size(3);
+  TORCH_CHECK(k_new.sizes() == v_new.sizes() && k_new.strides() == v_new.strides() && k_new.scalar_type() == v_new.scalar_type(),
+              "k_new and v_new must have one shape, layout and dtype");
+  TORCH_CHECK((k_new.dim() == 3 && k_new.size(1) == num_kv_heads && k_new.size(2) == head_dim && k_new.stride(2) == 1 &&
+               (k_new.stride(1) == head_dim || num_kv_heads == 1)) ||
+                  (k_new.dim() == 2 && k_new.size(1) == num_kv_heads * head_dim && k_new.stride(1) == 1),
+              "k_new is [tokens, num_kv_heads, head_dim] (or [tokens, num_kv_heads*head_dim]) with contiguous rows");
+  const at::Device dev = k_cache.device();
+  const int64_t tokens = k_new.size(0), batch = positions.numel();
+  check_tables(block_table, positions, batch, dev, "positions");
+  check_indptr(indptr, batch, dev);
+  TORCH_CHECK(v_cache.device() == dev && k_new.device() == dev && v_new.device() == dev, "tensors must be on one device");
+  for (int64_t d : k_cache.sizes()) TORCH_CHECK(d <= INT32_MAX, "cache dimensions must fit 32 bits");
+  TORCH_CHECK(batch <= INT32_MAX && block_table.size(1) <= INT32_MAX, "too many sequences or pages");
+  if (k_scale) {
+    TORCH_CHECK(is_e4m3(k_cache), "caches must be float8_e4m3fn (or uint8 e4m3 codes)");
+    check_scales(*k_scale, *v_scale, num_kv_heads, dev);
+  } else {
+    TORCH_CHECK(k_new.scalar_type() == k_cache.scalar_type(), "new rows and caches must share a dtype");
+  }
+  if (batch == 0 || tokens == 0) return;
+  // A row stride is arbitrary where there is one row.
+  const int64_t row_stride = tokens == 1 ? num_kv_heads * head_dim : k_new.stride(0);
+  const c10::cuda::CUDAGuard guard(dev);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  const Scratch s = scratch_for(dev, stream, 0, 4);
+  uint32_t* const status = static_cast<uint32_t*>(s.sync.data_ptr());
+  const int dtype = to_dtype(k_new.scalar_type()), heads = static_cast<int>(num_kv_heads), dim = static_cast<int>(head_dim);
+  const int page = static_cast<int>(k_cache.size(1)), width = static_cast<int>(block_table.size(1)), b = static_cast<int>(batch);
+  check_status(
+      k_scale ? kl_paged_kv_append_chunks_fp8(dtype, k_cache.data_ptr(), v_cache.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+                                              k_scale->data_ptr<float>(), v_scale->data_ptr<float>(),
+                                              block_table.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
+                                              indptr.data_ptr<int32_t>(), b, tokens, heads, dim, page, block_table.stride(0),
+                                              width, k_cache.size(0), row_stride, status, stream)
+              : kl_paged_kv_append_chunks(dtype, k_cache.data_ptr(), v_cache.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+                                          block_table.data_ptr<int32_t>(), positions.data_ptr<int32_t>(),
+                                          indptr.data_ptr<int32_t>(), b, tokens, heads, dim, page, block_table.stride(0), width,
+                                          k_cache.size(0), row_stride, status, stream),
+      what);
+}
+
+void paged_kv_append_chunks(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& k_new, const at::Tensor& v_new,
+                            const at::Tensor& block_table, const at::Tensor& positions, const at::Tensor& indptr) {
+  append_chunks_impl(k_cache, v_cache, k_new, v_new, nullptr, nullptr, block_table, positions, indptr, "paged_kv_append_chunks");
+}
+
+void paged_kv_append_chunks_fp8(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& k_new, const at::Tensor& v_new,
+                                const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                                const at::Tensor& positions, const at::Tensor& indptr) {
+  append_chunks_impl(k_cache, v_cache, k_new, v_new, &k_scale, &v_scale, block_table, positions, indptr,
+                     "paged_kv_append_chunks_fp8");
+}
+
+// Attention of chunks of new tokens (kl_paged_chunk_attention). Without scales the caches are q's dtype; scales are
+// [num_kv_heads], or per page [num_pages, num_kv_heads].
+void chunk_attention_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                          const at::Tensor* k_scale, const at::Tensor* v_scale, const at::Tensor& block_table,
+                          const at::Tensor& seq_lens, const at::Tensor& indptr, double scale, bool causal, int code_type,
+                          bool per_page, const char* what) {
+  TORCH_CHECK(q.is_cuda() && out.is_cuda() && k_cache.is_cuda() && v_cache.is_cuda(), "tensors must be on CUDA");
+  TORCH_CHECK(q.dim() == 3 && k_cache.dim() == 4, "q is [tokens, heads, dim]; caches are 4-D");
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.strides() == v_cache.strides() &&
+                  k_cache.scalar_type() == v_cache.scalar_type() && k_cache.size(3) > 0 && k_cache.stride(3) == 1,
+              "caches are [num_pages, page_size, num_kv_heads, head_dim] of one shape, layout and dtype, head_dim contiguous");
+  const int64_t tokens = q.size(0), hq = q.size(1), dim = q.size(2), hkv = k_cache.size(2);
+  TORCH_CHECK(dim == k_cache.size(3), "cache head_dim differs from q");
+  TORCH_CHECK(hkv > 0 && hq > 0 && hq % hkv == 0, "num_q_heads must be a multiple of num_kv_heads");
+  TORCH_CHECK(q.stride(2) == 1 && (q.stride(1) == dim || hq == 1), "a row of q must be contiguous");
+  TORCH_CHECK(out.is_contiguous() && out.sizes() == q.sizes() && out.scalar_type() == q.scalar_type(),
+              "out must be contiguous and match q");
+  if (code_type == KL_CODE_NONE) {
+    TORCH_CHECK(q.scalar_type() == k_cache.scalar_type(), "q and caches must share a dtype");
+  } else {
+    TORCH_CHECK(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16, "q and out are fp16 or bf16");
+  }
+  const at::Device dev = q.device();
+  TORCH_CHECK(out.device() == dev && k_cache.device() == dev && v_cache.device() == dev, "tensors must be on one device");
+  const int64_t batch = seq_lens.numel();
+  check_tables(block_table, seq_lens, batch, dev, "seq_lens");
+  check_indptr(indptr, batch, dev);
+  for (int64_t d : k_cache.sizes()) TORCH_CHECK(d <= INT32_MAX, "cache dimensions must fit 32 bits");
+  TORCH_CHECK(batch <= 65535 && tokens <= INT32_MAX && hq <= INT32_MAX && block_table.size(1) <= INT32_MAX,
+              "too many sequences, tokens, heads or pages");
+  if (batch == 0 || tokens == 0) return;
+  const c10::cuda::CUDAGuard guard(dev);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  const int dtype = to_dtype(q.scalar_type()), b = static_cast<int>(batch), d = static_cast<int>(dim);
+  size_t partial_bytes = 0, sync_bytes = 0;
+  check_status(kl_paged_chunk_attention_workspace_size(dtype, code_type, tokens, b, static_cast<int>(hq), static_cast<int>(hkv), d,
+                                                       &partial_bytes, &sync_bytes),
+               what);
+  const Scratch s = scratch_for(dev, stream, partial_bytes, sync_bytes);
+  check_status(
+      kl_paged_chunk_attention(dtype, code_type, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                               k_scale ? k_scale->data_ptr<float>() : nullptr, v_scale ? v_scale->data_ptr<float>() : nullptr,
+                               block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), indptr.data_ptr<int32_t>(), b, tokens,
+                               static_cast<int>(hq), static_cast<int>(hkv), d, static_cast<int>(k_cache.size(1)),
+                               tokens == 1 ? hq * dim : q.stride(0), stride_of(k_cache, 0), stride_of(k_cache, 1),
+                               stride_of(k_cache, 2), per_page ? hkv : 0, block_table.stride(0),
+                               static_cast<int>(block_table.size(1)), k_cache.size(0), causal, static_cast<float>(scale),
+                               s.partials.data_ptr(), static_cast<size_t>(s.partials.numel()), s.sync.data_ptr(),
+                               static_cast<size_t>(s.sync.numel()), stream),
+      what);
+}
+
+void paged_chunk_attention(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& indptr, double scale,
+                           bool causal) {
+  chunk_attention_impl(out, q, k_cache, v_cache, nullptr, nullptr, block_table, seq_lens, indptr, scale, causal, KL_CODE_NONE,
+                       false, "paged_chunk_attention");
+}
+
+void paged_chunk_attention_fp8(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                               const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                               const at::Tensor& seq_lens, const at::Tensor& indptr, double scale, bool causal) {
+  TORCH_CHECK(k_cache.dim() == 4 && is_e4m3(k_cache), "caches must be float8_e4m3fn (or uint8 e4m3 codes)");
+  check_scales(k_scale, v_scale, k_cache.size(2), k_cache.device());
+  chunk_attention_impl(out, q, k_cache, v_cache, &k_scale, &v_scale, block_table, seq_lens, indptr, scale, causal, KL_CODE_E4M3,
+                       false, "paged_chunk_attention_fp8");
+}
+
+void paged_chunk_attention_block8(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                  const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                                  const at::Tensor& seq_lens, const at::Tensor& indptr, double scale, bool causal) {
+  check_block8_cache(k_cache, v_cache, k_scale, v_scale);
+  chunk_attention_impl(out, q, k_cache, v_cache, &k_scale, &v_scale, block_table, seq_lens, indptr, scale, causal,
+                       code_type_of(k_cache), true, "paged_chunk_attention_block8");
+}
+
+// The pools of the page operators: tensors whose first dimension is the page, each page's elements filling one
+// piece of memory (in any order of its dimensions).
+struct Pools {
+  std::vector<void*> base;
+  std::vector<int64_t> stride, bytes;
+  int64_t num_pages = 0;
+  at::Device device = at::kCPU;
+  kl_page_pools_t c() const { return {static_cast<int>(base.size()), base.data(), stride.data(), bytes.data()}; }
+};
+
+Pools check_pools(at::TensorList caches) {
+  TORCH_CHECK(!caches.empty(), "there must be at least one cache");
+  Pools p;
+  p.num_pages = caches[0].dim() > 0 ? caches[0].size(0) : 0;
+  p.device = caches[0].device();
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (const at::Tensor& t : caches) {
+    TORCH_CHECK(t.is_cuda() && t.device() == p.device, "caches must be on one CUDA device");
+    TORCH_CHECK(t.dim() >= 1 && t.size(0) == p.num_pages && p.num_pages <= INT32_MAX - 8, "caches must have one number of pages");
+    dims.clear();
+    int64_t elements = 1;
+    for (int64_t i = 1; i < t.dim(); ++i) {
+      elements *= t.size(i);
+      if (t.size(i) > 1) dims.emplace_back(t.stride(i), t.size(i));
+    }
+    std::sort(dims.begin(), dims.end());
+    int64_t filled = 1;
+    for (const auto& d : dims) {
+      TORCH_CHECK(elements == 0 || d.first == filled, "a page of a cache must fill one piece of memory");
+      filled *= d.second;
+    }
+    const int64_t e = t.element_size();
+    TORCH_CHECK(p.num_pages <= 1 || t.stride(0) >= elements, "pages of a cache must not overlap");
+    if (elements == 0 || p.num_pages == 0) continue;
+    p.base.push_back(t.data_ptr());
+    p.stride.push_back((p.num_pages > 1 ? t.stride(0) : elements) * e);
+    p.bytes.push_back(elements * e);
+  }
+  return p;
+}
+
+bool is_index(const at::Tensor& t, const at::Device& dev) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous() && t.device() == dev;
+}
+
+void paged_copy_pages(at::TensorList caches, const at::Tensor& src, const at::Tensor& dst) {
+  const Pools p = check_pools(caches);
+  TORCH_CHECK(is_index(src, p.device) && is_index(dst, p.device) && src.numel() == dst.numel() && src.numel() <= INT32_MAX,
+              "src and dst are contiguous int32 of one length on the caches' device");
+  if (src.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(p.device);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  const Scratch s = scratch_for(p.device, stream, 0, 4);
+  const kl_page_pools_t pools = p.c();
+  check_status(kl_paged_copy_pages(&pools, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.numel(), p.num_pages,
+                                   static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+               "paged_copy_pages");
+}
+
+void check_page_table(const at::Tensor& out_table, const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t rows,
+                      const at::Device& dev) {
+  check_tables(block_table, seq_lens, seq_lens.numel(), dev, "seq_lens");
+  TORCH_CHECK(out_table.scalar_type() == at::kInt && out_table.is_contiguous() && out_table.dim() == 2 && out_table.size(0) == rows &&
+                  out_table.size(1) == block_table.size(1) && out_table.device() == dev,
+              "out_table is contiguous int32 [rows, width of block_table] on the caches' device");
+  TORCH_CHECK(seq_lens.numel() <= INT32_MAX && rows <= (1 << 24) && block_table.size(1) <= INT32_MAX, "too many sequences or pages");
+}
+
+// Pages for new tokens, and forks (kl_paged_reserve).
+void paged_reserve(at::Tensor& out_table, at::Tensor& out_lens, at::Tensor& served, at::TensorList caches,
+                   const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& new_tokens,
+                   const std::optional<at::Tensor>& parents, int64_t page_size) {
+  const Pools p = check_pools(caches);
+  const int64_t batch = seq_lens.numel(), rows = parents ? parents->numel() : batch;
+  check_page_table(out_table, block_table, seq_lens, rows, p.device);
+  TORCH_CHECK(page_size > 0 && page_size <= INT32_MAX, "page_size must be positive");
+  TORCH_CHECK(is_index(new_tokens, p.device) && new_tokens.numel() == rows && (!parents || is_index(*parents, p.device)),
+              "new_tokens and parents are contiguous int32 [rows] on the caches' device");
+  TORCH_CHECK(is_index(out_lens, p.device) && out_lens.numel() == rows && served.scalar_type() == at::kBool && served.dim() == 1 &&
+                  served.is_contiguous() && served.numel() == rows && served.device() == p.device,
+              "out_lens is int32 [rows] and served bool [rows] on the caches' device");
+  if (rows == 0) return;
+  const c10::cuda::CUDAGuard guard(p.device);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  size_t bytes = 0;
+  check_status(kl_paged_reserve_workspace_size(p.num_pages, static_cast<int>(rows), &bytes), "paged_reserve (workspace)");
+  const Scratch s = scratch_for(p.device, stream, bytes, 4);
+  const kl_page_pools_t pools = p.c();
+  check_status(kl_paged_reserve(&pools, out_table.data_ptr<int32_t>(), out_lens.data_ptr<int32_t>(),
+                                reinterpret_cast<uint8_t*>(served.data_ptr<bool>()), block_table.data_ptr<int32_t>(),
+                                seq_lens.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(),
+                                parents ? parents->data_ptr<int32_t>() : nullptr, static_cast<int>(batch), static_cast<int>(rows),
+                                static_cast<int>(block_table.size(1)), static_cast<int>(page_size), block_table.stride(0), p.num_pages,
+                                s.partials.data_ptr(), static_cast<size_t>(s.partials.numel()),
+                                static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+               "paged_reserve");
+}
+
+// The pages in use moved to the lowest ids (kl_paged_compact).
+void paged_compact(at::Tensor& out_table, at::Tensor& used, at::TensorList caches, const at::Tensor& block_table,
+                   const at::Tensor& seq_lens, int64_t page_size) {
+  const Pools p = check_pools(caches);
+  const int64_t batch = seq_lens.numel();
+  check_page_table(out_table, block_table, seq_lens, batch, p.device);
+  TORCH_CHECK(page_size > 0 && page_size <= INT32_MAX, "page_size must be positive");
+  TORCH_CHECK(used.scalar_type() == at::kInt && used.numel() == 1 && used.device() == p.device, "used is one int32 on the caches' device");
+  const c10::cuda::CUDAGuard guard(p.device);
+  const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+  size_t bytes = 0;
+  check_status(kl_paged_compact_workspace_size(p.num_pages, &bytes), "paged_compact (workspace)");
+  const Scratch s = scratch_for(p.device, stream, bytes, 4);
+  const kl_page_pools_t pools = p.c();
+  check_status(kl_paged_compact(&pools, out_table.data_ptr<int32_t>(), used.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(),
+                                seq_lens.data_ptr<int32_t>(), static_cast<int>(batch), static_cast<int>(block_table.size(1)),
+                                static_cast<int>(page_size), block_table.stride(0), p.num_pages, s.partials.data_ptr(),
+                                static_cast<size_t>(s.partials.numel()), static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+               "paged_compact");
+}
+
 // Status bits (KL_STATUS_*) left by decode calls on the current device and stream and by the graphs
 // captured on the device.
 int64_t decode_status(bool clear) {
@@ -885,6 +1153,56 @@ at::Tensor paged_block_select_new(const at::Tensor& q, const at::Tensor& k_cache
   return selected;
 }
 
+// The chunked step's functional forms, under the same rule.
+at::Tensor rows_of_q(const at::Tensor& q) {
+  return q.dim() == 3 && q.stride(2) == 1 && (q.stride(1) == q.size(2) || q.size(1) == 1) ? q : q.contiguous();
+}
+
+at::Tensor paged_chunk_attention_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                     const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& indptr,
+                                     double scale, bool causal) {
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  paged_chunk_attention(out, rows_of_q(q), k_cache, v_cache, block_table, seq_lens, indptr, scale, causal);
+  return out;
+}
+
+at::Tensor paged_chunk_attention_fp8_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                         const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                                         const at::Tensor& seq_lens, const at::Tensor& indptr, double scale, bool causal) {
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  paged_chunk_attention_fp8(out, rows_of_q(q), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr, scale, causal);
+  return out;
+}
+
+at::Tensor paged_chunk_attention_block8_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                            const at::Tensor& k_scale, const at::Tensor& v_scale, const at::Tensor& block_table,
+                                            const at::Tensor& seq_lens, const at::Tensor& indptr, double scale, bool causal) {
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  paged_chunk_attention_block8(out, rows_of_q(q), k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr, scale, causal);
+  return out;
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> paged_reserve_new(const std::vector<at::Tensor>& caches,
+                                                                 const at::Tensor& block_table, const at::Tensor& seq_lens,
+                                                                 const at::Tensor& new_tokens,
+                                                                 const std::optional<at::Tensor>& parents, int64_t page_size) {
+  TORCH_CHECK(block_table.dim() == 2, "block_table is [batch, width]");
+  const int64_t rows = parents ? parents->numel() : seq_lens.numel();
+  at::Tensor table = at::empty({rows, block_table.size(1)}, block_table.options().dtype(at::kInt));
+  at::Tensor lens = at::empty({rows}, table.options()), served = at::empty({rows}, table.options().dtype(at::kBool));
+  paged_reserve(table, lens, served, caches, block_table, seq_lens, new_tokens, parents, page_size);
+  return {table, lens, served};
+}
+
+std::tuple<at::Tensor, at::Tensor> paged_compact_new(const std::vector<at::Tensor>& caches, const at::Tensor& block_table,
+                                                     const at::Tensor& seq_lens, int64_t page_size) {
+  TORCH_CHECK(block_table.dim() == 2, "block_table is [batch, width]");
+  at::Tensor table = at::empty({seq_lens.numel(), block_table.size(1)}, block_table.options().dtype(at::kInt));
+  at::Tensor used = at::empty({}, table.options());
+  paged_compact(table, used, caches, block_table, seq_lens, page_size);
+  return {table, used};
+}
+
 void noop_rms_norm(at::Tensor&, const at::Tensor&, const at::Tensor&, double) {}
 void noop_fused(at::Tensor&, const at::Tensor&, at::Tensor&, const at::Tensor&, double) {}
 void noop_decode(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
@@ -912,6 +1230,18 @@ void noop_decode_block8(at::Tensor&, const at::Tensor&, const at::Tensor&, const
                         const std::optional<at::Tensor>&) {}
 void noop_select(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
                  const at::Tensor&, const at::Tensor&, int64_t, int64_t) {}
+void noop_append_chunks(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                        const at::Tensor&) {}
+void noop_append_chunks_fp8(at::Tensor&, at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                            const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&) {}
+void noop_chunk(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                const at::Tensor&, double, bool) {}
+void noop_chunk8(at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                 const at::Tensor&, const at::Tensor&, const at::Tensor&, double, bool) {}
+void noop_copy_pages(at::TensorList, const at::Tensor&, const at::Tensor&) {}
+void noop_reserve(at::Tensor&, at::Tensor&, at::Tensor&, at::TensorList, const at::Tensor&, const at::Tensor&,
+                  const at::Tensor&, const std::optional<at::Tensor>&, int64_t) {}
+void noop_compact(at::Tensor&, at::Tensor&, at::TensorList, const at::Tensor&, const at::Tensor&, int64_t) {}
 
 }  // namespace
 
@@ -951,6 +1281,28 @@ TORCH_LIBRARY(kernel_lab, m) {
   m.def(
       "paged_block_select(Tensor! selected, Tensor q, Tensor k_cache, Tensor k_scale, Tensor k_bounds, "
       "Tensor block_table, Tensor seq_lens, int sink_pages, int recent_pages) -> ()");
+  m.def(
+      "paged_kv_append_chunks(Tensor! k_cache, Tensor! v_cache, Tensor k_new, Tensor v_new, Tensor block_table, "
+      "Tensor positions, Tensor indptr) -> ()");
+  m.def(
+      "paged_kv_append_chunks_fp8(Tensor! k_cache, Tensor! v_cache, Tensor k_new, Tensor v_new, Tensor k_scale, "
+      "Tensor v_scale, Tensor block_table, Tensor positions, Tensor indptr) -> ()");
+  m.def(
+      "paged_chunk_attention(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, "
+      "Tensor seq_lens, Tensor indptr, float scale, bool causal) -> ()");
+  m.def(
+      "paged_chunk_attention_fp8(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, "
+      "Tensor block_table, Tensor seq_lens, Tensor indptr, float scale, bool causal) -> ()");
+  m.def(
+      "paged_chunk_attention_block8(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor k_scale, "
+      "Tensor v_scale, Tensor block_table, Tensor seq_lens, Tensor indptr, float scale, bool causal) -> ()");
+  m.def("paged_copy_pages(Tensor(a!)[] caches, Tensor src, Tensor dst) -> ()");
+  m.def(
+      "paged_reserve(Tensor! out_table, Tensor! out_lens, Tensor! served, Tensor(a!)[] caches, Tensor block_table, "
+      "Tensor seq_lens, Tensor new_tokens, Tensor? parents, int page_size) -> ()");
+  m.def(
+      "paged_compact(Tensor! out_table, Tensor! used, Tensor(a!)[] caches, Tensor block_table, Tensor seq_lens, "
+      "int page_size) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
@@ -967,6 +1319,14 @@ TORCH_LIBRARY_IMPL(kernel_lab, CUDA, m) {
   m.impl("paged_kv_append_block8", &paged_kv_append_block8);
   m.impl("paged_decode_attention_block8", &paged_decode_attention_block8);
   m.impl("paged_block_select", &paged_block_select);
+  m.impl("paged_kv_append_chunks", &paged_kv_append_chunks);
+  m.impl("paged_kv_append_chunks_fp8", &paged_kv_append_chunks_fp8);
+  m.impl("paged_chunk_attention", &paged_chunk_attention);
+  m.impl("paged_chunk_attention_fp8", &paged_chunk_attention_fp8);
+  m.impl("paged_chunk_attention_block8", &paged_chunk_attention_block8);
+  m.impl("paged_copy_pages", &paged_copy_pages);
+  m.impl("paged_reserve", &paged_reserve);
+  m.impl("paged_compact", &paged_compact);
 }
 
 TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
@@ -983,6 +1343,14 @@ TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
   m.impl("paged_kv_append_block8", &noop_append_block8);
   m.impl("paged_decode_attention_block8", &noop_decode_block8);
   m.impl("paged_block_select", &noop_select);
+  m.impl("paged_kv_append_chunks", &noop_append_chunks);
+  m.impl("paged_kv_append_chunks_fp8", &noop_append_chunks_fp8);
+  m.impl("paged_chunk_attention", &noop_chunk);
+  m.impl("paged_chunk_attention_fp8", &noop_chunk8);
+  m.impl("paged_chunk_attention_block8", &noop_chunk8);
+  m.impl("paged_copy_pages", &noop_copy_pages);
+  m.impl("paged_reserve", &noop_reserve);
+  m.impl("paged_compact", &noop_compact);
 }
 
 // Importing kernel_lab._C runs the registrations above.
@@ -995,5 +1363,15 @@ PYBIND11_MODULE(_C, m) {
   m.def("paged_kv_append_block8", &paged_kv_append_block8);
   m.def("paged_decode_attention_block8", &paged_decode_attention_block8_new);
   m.def("paged_block_select", &paged_block_select_new);
+  m.def("paged_kv_append_chunks", &paged_kv_append_chunks);
+  m.def("paged_kv_append_chunks_fp8", &paged_kv_append_chunks_fp8);
+  m.def("paged_chunk_attention", &paged_chunk_attention_new);
+  m.def("paged_chunk_attention_fp8", &paged_chunk_attention_fp8_new);
+  m.def("paged_chunk_attention_block8", &paged_chunk_attention_block8_new);
+  m.def("paged_copy_pages", [](const std::vector<at::Tensor>& caches, const at::Tensor& src, const at::Tensor& dst) {
+    paged_copy_pages(caches, src, dst);
+  });
+  m.def("paged_reserve", &paged_reserve_new);
+  m.def("paged_compact", &paged_compact_new);
   m.attr("version") = kl_version();
 }

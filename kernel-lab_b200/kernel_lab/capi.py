@@ -85,6 +85,41 @@ SIGNATURES = {
     "kl_ipc_free": (_c_int, [_c_vp]),
 }
 
+
+class PagePools(ctypes.Structure):
+    """kl_page_pools_t."""
+
+    _fields_ = [("count", ctypes.c_int), ("base", ctypes.POINTER(ctypes.c_void_p)), ("stride", ctypes.POINTER(ctypes.c_int64)),
+                ("bytes", ctypes.POINTER(ctypes.c_int64))]
+
+
+_c_poolsp = ctypes.POINTER(PagePools)
+
+# The same for include/kernel_lab_b200_chunk.h.
+CHUNK_SIGNATURES = {
+    "kl_paged_kv_append_chunks": (
+        _c_int, [_c_int] + [_c_vp] * 7 + [_c_int, _c_i64] + [_c_int] * 3 + [_c_i64, _c_int, _c_i64, _c_i64, _c_vp, _c_vp],
+    ),
+    "kl_paged_kv_append_chunks_fp8": (
+        _c_int, [_c_int] + [_c_vp] * 9 + [_c_int, _c_i64] + [_c_int] * 3 + [_c_i64, _c_int, _c_i64, _c_i64, _c_vp, _c_vp],
+    ),
+    "kl_paged_chunk_attention_workspace_size": (_c_int, [_c_int, _c_int, _c_i64] + [_c_int] * 4 + [_c_szp, _c_szp]),
+    "kl_paged_chunk_attention": (
+        _c_int,
+        [_c_int, _c_int] + [_c_vp] * 9 + [_c_int, _c_i64] + [_c_int] * 4 + [_c_i64] * 6
+        + [_c_int, _c_i64, _c_int, _c_float, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
+    ),
+    "kl_paged_copy_pages": (_c_int, [_c_poolsp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp]),
+    "kl_paged_reserve_workspace_size": (_c_int, [_c_i64, _c_int, _c_szp]),
+    "kl_paged_reserve": (
+        _c_int, [_c_poolsp] + [_c_vp] * 7 + [_c_int] * 4 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp],
+    ),
+    "kl_paged_compact_workspace_size": (_c_int, [_c_i64, _c_szp]),
+    "kl_paged_compact": (
+        _c_int, [_c_poolsp] + [_c_vp] * 4 + [_c_int] * 3 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp],
+    ),
+}
+
 # The same for include/kernel_lab_b200_block8.h.
 BLOCK8_SIGNATURES = {
     "kl_rms_norm_fp8": (_c_int, [_c_int] + [_c_vp] * 6 + [_c_int, _c_int, _c_i64, _c_int, _c_float, _c_vp]),
@@ -142,7 +177,7 @@ def load() -> ctypes.CDLL:
         if not LIB_PATH.exists():
             raise RuntimeError(f"{LIB_PATH.name} is not built; run `python kernel-lab_b200/build.py`")
         lib = ctypes.CDLL(str(LIB_PATH))
-        for name, (res, args) in (SIGNATURES | BLOCK8_SIGNATURES).items():
+        for name, (res, args) in (SIGNATURES | BLOCK8_SIGNATURES | CHUNK_SIGNATURES).items():
             fn = getattr(lib, name)
             fn.restype = res
             fn.argtypes = args

@@ -3,11 +3,14 @@
 Same API as kernel-lab's ``kernel_lab/cuda_ops.py:11-61`` (``available``,
 ``why_unavailable``, ``rms_norm``, ``fused_add_rms_norm``, ``paged_decode_attention``),
 plus ``num_splits`` on ``paged_decode_attention``, ``decode_status`` and the serving step around decode
-(append, e4m3 and block-scaled 8-bit caches, page selection, e4m3 norms). There is no
+(append, e4m3 and block-scaled 8-bit caches, page selection, e4m3 norms) and the chunked step (appends and attention
+of chunks of new tokens, the pages that they need). There is no
 fallback: if the extension is not built these functions raise RuntimeError.
 """
 
 from __future__ import annotations
+
+from collections.abc import Sequence
 
 import torch
 
@@ -85,11 +88,18 @@ def paged_kv_append(
     v_new: torch.Tensor,
     block_table: torch.Tensor,
     positions: torch.Tensor,
+    indptr: torch.Tensor | None = None,
 ) -> None:
     """Write each sequence's new token's K/V rows ([batch, num_kv_heads, head_dim], rows may be a
     strided view) into its pages at token index ``positions[b]`` (in place; negative skips).
+    With ``indptr`` (int32 [batch + 1]) sequence b's new tokens are the rows ``indptr[b]`` .. ``indptr[b + 1] - 1``
+    and take the positions from ``positions[b]`` on.
     Page ids outside the pool are skipped and reported by :func:`decode_status`."""
     _require()
+    if indptr is not None:
+        tensors = (k_cache, v_cache, k_new, v_new, block_table, positions, indptr)
+        (_C if _direct(*tensors) else torch.ops.kernel_lab).paged_kv_append_chunks(*tensors)
+        return
     torch.ops.kernel_lab.paged_kv_append(k_cache, v_cache, k_new, v_new, block_table, positions)
 
 
@@ -123,10 +133,15 @@ def paged_kv_append_fp8(
     v_scale: torch.Tensor,
     block_table: torch.Tensor,
     positions: torch.Tensor,
+    indptr: torch.Tensor | None = None,
 ) -> None:
     """paged_kv_append into an e4m3 cache: rows are quantised per KV head as
     e4m3(x / scale) (round to nearest-even, saturating to +-448)."""
     _require()
+    if indptr is not None:
+        tensors = (k_cache, v_cache, k_new, v_new, k_scale, v_scale, block_table, positions, indptr)
+        (_C if _direct(*tensors) else torch.ops.kernel_lab).paged_kv_append_chunks_fp8(*tensors)
+        return
     torch.ops.kernel_lab.paged_kv_append_fp8(k_cache, v_cache, k_new, v_new, k_scale, v_scale, block_table, positions)
 
 
@@ -279,6 +294,149 @@ def paged_block_select(
         selected, q.contiguous(), k_cache, k_scale, k_bounds, block_table, seq_lens, sink_pages, recent_pages
     )
     return selected
+
+
+def _rows_of_q(q: torch.Tensor) -> torch.Tensor:
+    """q as rows of contiguous heads, any distance apart."""
+    return q if q.stride(-1) == 1 and (q.stride(1) == q.shape[2] or q.shape[1] == 1) else q.contiguous()
+
+
+def paged_chunk_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    indptr: torch.Tensor,
+    scale: float | None = None,
+    causal: bool = True,
+) -> torch.Tensor:
+    """Attention of chunks of new tokens over a paged cache (prompts, chunks of them, draft tokens, single
+    tokens, in one call). q is [tokens, num_q_heads, head_dim] (rows may be a strided view); sequence b's new tokens are its
+    rows ``indptr[b]`` .. ``indptr[b + 1] - 1`` (indptr: int32 [batch + 1]) and the last of the ``seq_lens[b]`` tokens in its
+    pages: append them first (:func:`paged_kv_append`). A token attends to the tokens up to itself, without
+    ``causal`` to all ``seq_lens[b]`` (cross attention over an encoder's states). What is masked does not count,
+    whatever it holds; a token that has none to attend to gets zeros. The rows of the result that are no sequence's are
+    undefined. Caches as in :func:`paged_decode_attention`, or views with any order of pages, tokens and heads in memory."""
+    _require()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    tensors = (k_cache, v_cache, block_table, seq_lens, indptr)
+    if _direct(q, *tensors):
+        return _C.paged_chunk_attention(q, *tensors, scale, causal)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    torch.ops.kernel_lab.paged_chunk_attention(out, _rows_of_q(q), *tensors, scale, causal)
+    return out
+
+
+def paged_chunk_attention_fp8(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    indptr: torch.Tensor,
+    scale: float | None = None,
+    causal: bool = True,
+) -> torch.Tensor:
+    """:func:`paged_chunk_attention` over an e4m3 cache with per-KV-head float32 scales (as
+    :func:`paged_decode_attention_fp8`). q is fp16 or bf16."""
+    _require()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    tensors = (k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr)
+    if _direct(q, *tensors):
+        return _C.paged_chunk_attention_fp8(q, *tensors, scale, causal)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    torch.ops.kernel_lab.paged_chunk_attention_fp8(out, _rows_of_q(q), *tensors, scale, causal)
+    return out
+
+
+def paged_chunk_attention_block8(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    indptr: torch.Tensor,
+    scale: float | None = None,
+    causal: bool = True,
+) -> torch.Tensor:
+    """:func:`paged_chunk_attention` over an 8-bit cache with a scale for each page and KV head (as
+    :func:`paged_decode_attention_block8`). q is fp16 or bf16."""
+    _require()
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    tensors = (k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, indptr)
+    if _direct(q, *tensors):
+        return _C.paged_chunk_attention_block8(q, *tensors, scale, causal)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    torch.ops.kernel_lab.paged_chunk_attention_block8(out, _rows_of_q(q), *tensors, scale, causal)
+    return out
+
+
+def paged_copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """Copy page ``src[i]`` to page ``dst[i]`` (int32 [n]; negative skips) in every tensor of ``caches``, in one launch for
+    up to 64 of them: keys, values, scales and bounds of any number of layers, whose first dimension is the page
+    and whose pages each fill one piece of memory. No page may be a destination twice, or both a source and a
+    destination. Page ids outside the pool are skipped and reported by :func:`decode_status`."""
+    _require()
+    caches = list(caches)
+    if _direct(*caches, src, dst):
+        _C.paged_copy_pages(caches, src, dst)
+    else:
+        torch.ops.kernel_lab.paged_copy_pages(caches, src, dst)
+
+
+def paged_reserve(
+    caches: Sequence[torch.Tensor],
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    new_tokens: torch.Tensor,
+    parents: torch.Tensor | None = None,
+    page_size: int | None = None,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages for the tokens to come, on the device: (block_table, seq_lens, served), new tensors. Without ``parents`` the
+    rows are the sequences; with it (int32 [rows]) row r is a fork of sequence ``parents[r]`` (negative: an empty row) and
+    shares its pages, and sequences that no row names are dropped. A page is free if no row's first
+    ceil(len / page_size) entries name it, so dropping or shortening a sequence frees its pages, and whatever is to keep
+    pages (a stored prefix, say) has to be a row. In the order of the rows each takes the free pages with the
+    lowest ids: a copy of its last page if ``new_tokens[r]`` > 0, that page is partly filled and others hold
+    it too (copied in every tensor of ``caches``; of several that only write to it the lowest row keeps it), then pages
+    for the ``new_tokens[r]`` tokens that are to be appended at ``seq_lens[r]``. ``served[r]`` is False, and the row
+    gets nothing, where the table is too narrow or the free pages run out (then
+    :func:`decode_status` has bit 32). The returned lengths do not count the new tokens."""
+    _require()
+    caches = list(caches)
+    page_size = caches[0].shape[1] if page_size is None else page_size
+    if _direct(*caches, block_table, seq_lens, new_tokens, parents):
+        return _C.paged_reserve(caches, block_table, seq_lens, new_tokens, parents, page_size)
+    rows = (seq_lens if parents is None else parents).shape[0]
+    table = torch.empty((rows, block_table.shape[1]), dtype=torch.int32, device=block_table.device)
+    lens = torch.empty((rows,), dtype=torch.int32, device=block_table.device)
+    served = torch.empty((rows,), dtype=torch.bool, device=block_table.device)
+    torch.ops.kernel_lab.paged_reserve(
+        table, lens, served, caches, block_table, seq_lens, new_tokens, parents, page_size
+    )
+    return table, lens, served
+
+
+def paged_compact(
+    caches: Sequence[torch.Tensor], block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int | None = None
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Move the pages in use to the lowest ids: (block_table, used), new tensors. ``used`` (int32 scalar) pages are
+    named by the rows' first ceil(len / page_size) entries; those with ids of ``used`` and more go, in order, to the free
+    ids below, in every tensor of ``caches``. Afterwards the pages from ``used`` on are free."""
+    _require()
+    caches = list(caches)
+    page_size = caches[0].shape[1] if page_size is None else page_size
+    if _direct(*caches, block_table, seq_lens):
+        return _C.paged_compact(caches, block_table, seq_lens, page_size)
+    table = torch.empty((seq_lens.shape[0], block_table.shape[1]), dtype=torch.int32, device=block_table.device)
+    used = torch.empty((), dtype=torch.int32, device=block_table.device)
+    torch.ops.kernel_lab.paged_compact(table, used, caches, block_table, seq_lens, page_size)
+    return table, used
 
 
 def decode_status(clear: bool = False) -> int:
