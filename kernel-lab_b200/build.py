@@ -46,7 +46,8 @@ CU_SOURCES = {
     "block8_decode.cu": BLOCK8_HEADERS,
     "block8_select.cu": BLOCK8_HEADERS,
     "chunk_append.cu": CHUNK_HEADERS,
-    "chunk_attention.cu": CHUNK_HEADERS,
+    "chunk_attention.cu": [*CHUNK_HEADERS, CSRC / "chunk_attention.cuh"],
+    "chunk_attention_tc.cu": [*CHUNK_HEADERS, CSRC / "chunk_attention.cuh"],
     "page_pool.cu": CHUNK_HEADERS,
 }
 HEADERS = [CSRC / "common.cuh", INCLUDE / "kernel_lab_b200.h"]

@@ -11,54 +11,10 @@
 #include <cstdint>
 #include <type_traits>
 
-#include "common.cuh"
-#include "kernel_lab_b200.h"
-#include "kernel_lab_b200_chunk.h"
+#include "chunk_attention.cuh"
 
 namespace klb {
 namespace chunk_attention {
-
-struct Args {
-  void* out;
-  const void* q;
-  const void* k;
-  const void* v;
-  const float* k_scale;
-  const float* v_scale;
-  const int32_t* block_table;
-  const int32_t* seq_lens;
-  const int32_t* indptr;
-  int64_t tokens;
-  int64_t q_stride, page_stride, token_stride, head_stride;  // elements
-  int64_t scale_stride;                                      // of a page's scales
-  int64_t bt_stride, num_pages;
-  int batch, hq, hkv, group, dim, page_size, max_pages, causal;
-  float scale_log2;  // scale * log2(e)
-  uint32_t* status;
-};
-
-// Sequence b of the call: its rows first .. first + n - 1, its length.
-struct Seq {
-  int64_t first;
-  int n, len;
-};
-
-__device__ __forceinline__ Seq read_seq(const Args& a, int b, bool report) {
-  const int64_t lo = min(max(static_cast<int64_t>(__ldcg(a.indptr + b)), int64_t(0)), a.tokens);
-  const int64_t hi = min(max(static_cast<int64_t>(__ldcg(a.indptr + b + 1)), int64_t(0)), a.tokens);
-  Seq s{lo, static_cast<int>(max(hi - lo, int64_t(0))), max(0, __ldcg(a.seq_lens + b))};
-  const int room = a.max_pages * a.page_size;
-  if (s.len > room) {
-    s.len = room;
-    if (report) atomicOr(a.status, kStatusLenClamped);
-  }
-  return s;
-}
-
-// Keys that token i of the sequence sees.
-__device__ __forceinline__ int keys_of(const Args& a, const Seq& s, int i) {
-  return a.causal ? max(0, s.len - s.n + i + 1) : s.len;
-}
 
 // ----------------------------------------------------------------- CUDA-core kernel
 //
@@ -252,6 +208,15 @@ cudaError_t launch_generic(const Args& a, cudaStream_t st) {
   return launch_kernel(true, generic_kernel<T, C>, grid, dim3(kThreads), smem, st, a);
 }
 
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  return n;
+}
+
 }  // namespace chunk_attention
 }  // namespace klb
 
@@ -259,8 +224,9 @@ extern "C" int kl_paged_chunk_attention_workspace_size(int dtype, int code_type,
                                                        int num_q_heads, int num_kv_heads, int head_dim,
                                                        size_t* partial_bytes, size_t* sync_bytes) {
   if (!partial_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
-  *partial_bytes = 0;
-  *sync_bytes = 256;
+  const int sms = klb::chunk_attention::sm_count();
+  *partial_bytes = klb::chunk_attention::tc_partial_bytes(head_dim, sms);
+  *sync_bytes = klb::chunk_attention::tc_sync_bytes(sms);
   return 0;
 }
 
@@ -318,6 +284,13 @@ extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, con
   a.status = static_cast<uint32_t*>(sync);
   const auto st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
+  const int sms = sm_count();
+  if (partials && partial_bytes >= tc_partial_bytes(head_dim, sms) && sync_bytes >= tc_sync_bytes(sms) &&
+      tc_fits(a, dtype, code_type)) {
+    a.partials = static_cast<float*>(partials);
+    a.counters = static_cast<uint32_t*>(sync) + 64;
+    return static_cast<int>(launch_tc(a, dtype, code_type, sms, st));
+  }
   if (!coded) {
     e = dtype == KL_FLOAT32   ? launch_generic<float, float>(a, st)
         : dtype == KL_FLOAT16 ? launch_generic<__half, __half>(a, st)

@@ -1,0 +1,972 @@
+// Chunk attention on the 5th-generation tensor cores: fp16 and bf16, head_dim up to 128, pages of a multiple of
+// 8 tokens, groups of up to 128 query heads.
+//
+// Rows are the (token, query head) pairs of one KV head, 128 a tile (128 / group tokens), two tiles a block. A
+// unit of work is a block and 128 of its keys:
+//   S_t = Q_t K^T (M = 128 rows, N = 128 keys) into tensor memory, by one thread, for the tiles t = 0, 1;
+//   a warpgroup a tile, one thread a row: the row's maximum, P_t = exp2(S_t - max) back into tensor memory over
+//   S_t, in 16 bits; O_t is rescaled in place only when a row's maximum has grown by more than 2^8;
+//   O_t += P_t V (A from tensor memory, V as an MN-major operand), by the same thread.
+// The two tiles alternate: one's softmax runs under the other's products, which complete in the order of issue, so
+// that S_t of the next unit says that O_t += P_t V of this one is done.
+// K and V tiles come by TMA through a ring of 128-key stages: a box per page (or 128 keys of it), zeros past the
+// sequence's end and for pages outside the pool.
+//
+// Units are numbered over sequences, KV heads, blocks and keys; every CTA takes an equal run of them, so causal
+// triangles, ragged lengths and few rows over long contexts are all balanced the same way. A block that the runs
+// cut leaves pieces (O in fp32, maximum, sum) in scratch; of each 32 rows the warp that arrives last joins them in
+// the pieces' order.
+//
+// What is masked does not count whatever it holds: scores are replaced, not added to; two warps clear the V rows
+// past the sequence's end and look for infinities and NaN in rows that some row of the block does not see, in which
+// case the softmax threads add that unit's P V themselves, key by key.
+#include <cuda.h>
+
+#include <algorithm>
+#include <climits>
+#include <mutex>
+#include <type_traits>
+
+#include "chunk_attention.cuh"
+
+namespace klb {
+namespace chunk_attention {
+
+namespace {
+
+constexpr int kBN = 128;                 // keys of a unit
+constexpr int kTcThreads = 384;          // two softmax warpgroups, then: load, products, two warps on V
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 * 208 + 128 * 88 <= 384 * 168, the launch's
+constexpr float kLazy = 8.0f;            // log2 by which a maximum may be passed before O is rescaled
+constexpr uint64_t kWaitCycles = 2000000000ull;  // about one second
+constexpr int kFixSlots = 4, kBadSlots = 8;
+constexpr int kCountersPerCta = 8;       // a counter for each warp's 32 rows of the two tiles
+
+template <int DP>
+struct Layout {
+  static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a row
+  static constexpr uint32_t kHalf = 128u * 128u;            // 128 rows of one
+  static constexpr uint32_t kTile = kHalves * kHalf;
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr uint32_t kRing = 2 * kTile;              // Q's two tiles first
+  static constexpr uint32_t kBars = kRing + kStages * kTile;
+  static constexpr uint32_t kWords = kBars + 256;           // ints
+  static constexpr uint32_t kBytes = kWords + 256 + 1024;   // slack to align the base to 1024 bytes
+};
+
+// Barriers, 8 bytes each from Layout::kBars on.
+enum Bar { kQFull0, kQFull1, kQEmpty, kSFull0, kSFull1, kPReady0, kPReady1, kOFull0, kOFull1, kDrain, kFix0, kRingFull = kFix0 + kFixSlots };
+
+// Words from Layout::kWords on.
+enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kTotalLo, kTotalHi, kVFlag, kBad = kVFlag + 2 * kFixSlots, kScan = kBad + kBadSlots };
+
+struct Smem {
+  uint32_t base;        // shared address
+  uint8_t* ptr;
+  uint32_t bars;
+  volatile int* words;
+  uint32_t* status;
+  __device__ uint32_t bar(int i) const { return bars + 8u * i; }
+};
+
+// False when the wait ran out or another one of the CTA has: the role then leaves its loops.
+__device__ __forceinline__ bool wait_for(const Smem& sm, uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i) {
+      if (mbar_try_wait(bar, parity)) return true;
+    }
+    if (sm.words[kDead]) return false;
+    if (static_cast<uint64_t>(clock64()) - start > kWaitCycles) {
+      atomicOr(sm.status, kStatusWaitTimeout);
+      sm.words[kDead] = 1;
+      return false;
+    }
+  }
+}
+
+// ----------------------------------------------------------------- plan
+
+// Units of row block k of sequence s: the keys that its last row sees, at least one unit.
+__device__ __forceinline__ int block_units(const Args& a, const Seq& s, int k) {
+  const int rows_end = min(s.n, (k + 1) * 2 * a.tile_tokens);
+  return max(1, (keys_of(a, s, rows_end - 1) + kBN - 1) / kBN);
+}
+
+__device__ __forceinline__ int blocks_of(const Args& a, const Seq& s) { return (s.n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens); }
+
+// The same summed over a sequence's blocks. Causal, all but the last block, step = tokens of a block:
+//   max(1, ceil((base + (k + 1) step) / 128)), base = len - n,
+// is 1 while base + (k + 1) step <= 128 and floor((A + i step) / 128) after that. The sum of the latter is that of the
+// terms less that of their remainders, over 128; the remainders run through the residues of A mod g, g = gcd(step, 128).
+__device__ __forceinline__ int64_t head_units(const Args& a, const Seq& s) {
+  const int nb = blocks_of(a, s);
+  if (nb == 0) return 0;
+  if (!a.causal) return static_cast<int64_t>(nb) * max(1, (s.len + kBN - 1) / kBN);
+  const int step = 2 * a.tile_tokens, base = s.len - s.n;
+  int64_t total = max(1, (s.len + kBN - 1) / kBN);
+  const int ones = min(nb - 1, base <= kBN - step ? (kBN - base) / step : 0);
+  const int64_t m = nb - 1 - ones;
+  total += ones;
+  if (m > 0) {
+    const int64_t A = base + static_cast<int64_t>(ones + 1) * step + kBN - 1;
+    const int g = min(step & -step, kBN), p = kBN / g;
+    int64_t rest = (m / p) * (p * (A % g) + static_cast<int64_t>(g) * p * (p - 1) / 2);
+    int r = static_cast<int>(A % kBN);
+    for (int i = 0; i < m % p; ++i) {
+      rest += r;
+      r = (r + step) % kBN;
+    }
+    total += (m * A + step * (m * (m - 1) / 2) - rest) / kBN;
+  }
+  return total;
+}
+
+struct Segment {
+  Seq s;
+  int b, h, blk;   // sequence, KV head, row block
+  int j0, j1, nt;  // its units of this segment, and how many the block has
+  int64_t first;   // number of the block's first unit
+};
+
+struct Walk {
+  Seq s;
+  int b, h, blk, j, nb;
+  int64_t u, u1;
+
+  // By a whole warp. Run c of `runs` of the total units begins at total * c / runs.
+  __device__ void init(const Args& a, const Smem& sm, int lane, int64_t u_first, int64_t u_end) {
+    u = u_first;
+    u1 = u_end;
+    b = sm.words[kStartSeq];
+    int64_t off = static_cast<int64_t>(static_cast<uint32_t>(sm.words[kStartLo])) | (static_cast<int64_t>(sm.words[kStartHi]) << 32);
+    s = read_seq(a, b, false);
+    nb = blocks_of(a, s);
+    const int64_t per_head = head_units(a, s);
+    h = static_cast<int>(off / per_head);
+    off -= h * per_head;
+    blk = 0;
+    for (;;) {  // 32 blocks at a time
+      const int k = blk + lane;
+      int inc = k < nb ? block_units(a, s, k) : 0;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, inc, m);
+        if (lane >= m) inc += y;
+      }
+      const int passed = __popc(__ballot_sync(0xffffffffu, inc <= off && k < nb));
+      if (passed < 32 || blk + 32 >= nb) {
+        const int before = __shfl_sync(0xffffffffu, inc, max(0, passed - 1));
+        if (passed > 0) off -= before;
+        blk += passed;
+        break;
+      }
+      off -= __shfl_sync(0xffffffffu, inc, 31);
+      blk += 32;
+    }
+    j = static_cast<int>(off);
+  }
+
+  __device__ bool next(const Args& a, Segment& g) {
+    if (u >= u1) return false;
+    const int nt = block_units(a, s, blk);
+    const int take = static_cast<int>(min(u1 - u, static_cast<int64_t>(nt - j)));
+    g = Segment{s, b, h, blk, j, j + take, nt, u - j};
+    u += take;
+    j += take;
+    if (j == nt && u < u1) {
+      j = 0;
+      if (++blk == nb) {
+        blk = 0;
+        if (++h == a.hkv) {
+          h = 0;
+          do {
+            s = read_seq(a, ++b, false);
+          } while (s.n == 0 && b + 1 < a.batch);
+          nb = blocks_of(a, s);
+        }
+      }
+    }
+    return true;
+  }
+};
+
+// What a block's tile t has to do within a segment: units [j0, end(t)).
+struct Tiles {
+  int tok0[2];     // first token of the tile
+  int end[2];      // end of its units in the segment
+  int seen_first;  // keys that the block's first row sees
+  __device__ Tiles(const Args& a, const Segment& g) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      tok0[t] = (2 * g.blk + t) * a.tile_tokens;
+      int nt = 0;
+      if (tok0[t] < g.s.n) nt = max(1, (keys_of(a, g.s, min(g.s.n, tok0[t] + a.tile_tokens) - 1) + kBN - 1) / kBN);
+      end[t] = max(g.j0, min(g.j1, nt));
+    }
+    seen_first = keys_of(a, g.s, tok0[0]);
+  }
+  // Units in which some row does not see every key.
+  __device__ bool special(int j) const { return (j + 1) * kBN > seen_first; }
+};
+
+// ----------------------------------------------------------------- PTX
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar), "l"(policy)
+      : "memory");
+}
+
+// D[tmem] (+)= A[tmem] . B[smem]; A's row i is lane i, two 16-bit elements a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  const uint32_t none = 0u;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(none)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, float (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const float (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "f"(r[0]), "f"(r[1]),
+               "f"(r[2]), "f"(r[3]), "f"(r[4]), "f"(r[5]), "f"(r[6]), "f"(r[7])
+               : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 32 bytes a lane in one store: a whole sector.
+__device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// ----------------------------------------------------------------- pieces of cut blocks
+
+// CTA c's piece of a block that an earlier CTA began lies in slot 2c, of one that it began itself in slot 2c + 1.
+// A slot: for each tile O [DP][128] fp32 (a warp's rows side by side), then maxima [128] and sums [128].
+template <int DP>
+__device__ __forceinline__ float* piece_at(const Args& a, int64_t slot, int t) {
+  return a.partials + (slot * 2 + t) * (static_cast<int64_t>(DP) + 2) * 128;
+}
+
+// ----------------------------------------------------------------- roles
+
+struct Plan {
+  int64_t total;
+  int runs;
+  __device__ int64_t begin(int c) const { return total * c / runs; }
+  __device__ int run_of(int64_t u) const { return static_cast<int>(((u + 1) * runs - 1) / total); }
+};
+
+template <typename T, int DP>
+__device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w, int lane, const CUtensorMap* mq, const CUtensorMap* mk,
+                                          const CUtensorMap* mv) {
+  using L = Layout<DP>;
+  const uint64_t keep = l2_policy_evict_normal(), once = l2_policy_evict_first();
+  const int boxes = kBN / a.box_rows;
+  const uint32_t box_bytes = a.box_rows * 128u;
+  uint32_t slot = 0, phase = 0, issued = 0, unit = 0;
+  uint32_t q_phase = 0;
+  bool ok = true, first_segment = true;
+  Segment g;
+  while (ok && w.next(a, g)) {
+    const Tiles tiles(a, g);
+    for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
+      // Lane i looks up box i: its page, or one past the pool's for zeros.
+      const int tok = j * kBN + lane * a.box_rows;
+      int64_t page = a.num_pages;
+      bool bad = false;
+      if (lane < boxes && tok < g.s.len) {
+        page = __ldcg(a.block_table + g.b * a.bt_stride + tok / a.page_size);
+        bad = page < 0 || page >= a.num_pages;
+        if (bad) page = a.num_pages;
+      }
+      const uint32_t bad_boxes = __ballot_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        sm.words[kBad + unit % kBadSlots] = static_cast<int>(bad_boxes);
+        if (bad_boxes) atomicOr(sm.status, kStatusBadPage);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t full = sm.bar(kRingFull + slot), empty = sm.bar(kRingFull + L::kStages + slot);
+        if (issued >= L::kStages) ok = wait_for(sm, empty, phase ^ 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
+        __syncwarp();
+        if (lane < boxes) {
+#pragma unroll
+          for (int c = 0; c < L::kHalves; ++c) {
+            tma_load_4d(sm.base + L::kRing + slot * L::kTile + c * L::kHalf + lane * box_bytes, kv ? mv : mk, c * 64, g.h, tok % a.page_size,
+                        static_cast<int>(page), full, keep);
+          }
+        }
+        ++issued;
+        if (++slot == L::kStages) {
+          slot = 0;
+          phase ^= 1;
+        }
+        if (kv == 0 && j == g.j0) {  // behind the segment's first keys, which need not wait for Q's room
+          if (!first_segment) {
+            ok = wait_for(sm, sm.bar(kQEmpty), q_phase);
+            q_phase ^= 1;
+          }
+          first_segment = false;
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane < 2 && tiles.end[lane] > g.j0) {
+            mbar_arrive_expect_tx(sm.bar(kQFull0 + lane), L::kHalves * a.tile_tokens * a.group * 128u);
+#pragma unroll
+            for (int c = 0; c < L::kHalves; ++c) {
+              tma_load_3d(sm.base + lane * L::kTile + c * L::kHalf, mq, c * 64, g.h * a.group, static_cast<int>(g.s.first) + tiles.tok0[lane],
+                          sm.bar(kQFull0 + lane), once);
+            }
+          }
+        }
+      }
+    }
+  }
+  // Nothing may be in flight into this CTA's shared memory when it ends; normally it has long landed.
+  if (lane == 0) {
+    for (uint32_t k = 0; k < min(issued, static_cast<uint32_t>(L::kStages)); ++k) {
+      const uint32_t i = issued - 1 - k, s = i % L::kStages;
+      const uint64_t start = clock64();
+      while (!mbar_try_wait(sm.bar(kRingFull + s), (i / L::kStages) & 1) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
+      }
+    }
+  }
+  __syncwarp();
+}
+
+// One thread.
+template <typename T, int DP>
+__device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, uint32_t tmem) {
+  using L = Layout<DP>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16, 128, DP, true);
+  const int ksteps = (a.dim + 15) / 16;
+  uint32_t slot = 0, phase = 0, unit = 0;
+  uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+  bool ok = true;
+  Segment g;
+  auto ring_wait = [&] { ok = ok && wait_for(sm, sm.bar(kRingFull + slot), phase); };
+  auto ring_next = [&] {
+    umma_commit(sm.bar(kRingFull + L::kStages + slot));
+    if (++slot == L::kStages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  };
+  auto scores = [&](int t, uint32_t k_slot) {
+    const uint32_t sq = sm.base + t * L::kTile, sk = sm.base + L::kRing + k_slot * L::kTile;
+    for (int ks = 0; ks < ksteps; ++ks) {
+      const uint32_t off = (ks / 4) * L::kHalf + (ks % 4) * 32u;
+      umma_f16(tmem + t * 128, umma_desc_sw128(sq + off, 16u, 1024u), umma_desc_sw128(sk + off, 16u, 1024u), IDESC_S, ks > 0);
+    }
+    umma_commit(sm.bar(kSFull0 + t));
+  };
+  while (ok && w.next(a, g)) {
+    const Tiles tiles(a, g);
+    // The first unit's scores.
+    ring_wait();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (!ok || tiles.end[t] <= g.j0) continue;
+      ok = wait_for(sm, sm.bar(kQFull0 + t), q_phase[t]);
+      q_phase[t] ^= 1;
+      if (!ok) break;
+      tcgen05_fence_after();
+      scores(t, slot);
+    }
+    if (!ok) break;
+    ring_next();
+    if (g.j1 == g.j0 + 1) umma_commit(sm.bar(kQEmpty));
+    for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
+      ring_wait();
+      const uint32_t v_slot = slot;
+      const uint32_t sv = sm.base + L::kRing + v_slot * L::kTile;
+      // V's stage is given back after the last product that reads it, then the next unit's K is in the next stage.
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (ok && j < tiles.end[t]) {
+          ok = wait_for(sm, sm.bar(kPReady0 + t), p_phase[t]);
+          p_phase[t] ^= 1;
+          if (!ok) break;
+          tcgen05_fence_after();
+          const bool by_hand = tiles.special(j) && (sm.words[kVFlag + 2 * (unit % kFixSlots)] | sm.words[kVFlag + 2 * (unit % kFixSlots) + 1]);
+          if (!by_hand) {
+#pragma unroll
+            for (int ks = 0; ks < kBN / 16; ++ks) {
+              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, umma_desc_sw128(sv + ks * 16u * 128u, L::kHalf, 1024u), IDESC_O,
+                          j > g.j0 || ks > 0);
+            }
+          }
+          if (j + 1 == tiles.end[t]) umma_commit(sm.bar(kOFull0 + t));
+        }
+        if (t == 1) ring_next();  // V
+        if (ok && j + 1 < tiles.end[t]) {
+          // The next unit's K: the stage after V's.
+          const uint32_t k_slot = v_slot + 1 == L::kStages ? 0 : v_slot + 1;
+          const uint32_t k_phase = v_slot + 1 == L::kStages ? (t == 1 ? phase : phase ^ 1) : phase;
+          ok = wait_for(sm, sm.bar(kRingFull + k_slot), k_phase);
+          if (!ok) break;
+          tcgen05_fence_after();
+          scores(t, k_slot);
+        }
+      }
+      if (!ok) break;
+      if (j + 1 < g.j1) {
+        ring_next();  // K
+        if (j + 2 == g.j1) umma_commit(sm.bar(kQEmpty));
+      }
+    }
+  }
+  // Every product has ended before the CTA does.
+  umma_commit(sm.bar(kDrain));
+  const uint64_t start = clock64();
+  while (!mbar_try_wait(sm.bar(kDrain), 0) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
+  }
+}
+
+// Two warps: the V rows of special units.
+template <typename T, int DP>
+__device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, int tid) {
+  using L = Layout<DP>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
+  uint32_t unit = 0;
+  bool ok = true;
+  Segment g;
+  while (ok && w.next(a, g)) {
+    const Tiles tiles(a, g);
+    for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
+      // Every stage is waited for and given back: a wait by parity must not be more than a phase off.
+      uint32_t slot = 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint32_t i = 2 * unit + kv;
+        slot = i % L::kStages;
+        ok = ok && wait_for(sm, sm.bar(kRingFull + slot), (i / L::kStages) & 1);
+        if (kv == 0 && (tid & 31) == 0) mbar_arrive(sm.bar(kRingFull + L::kStages + slot));
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const uint32_t empty = sm.bar(kRingFull + L::kStages + slot);
+      if (!tiles.special(j)) {
+        if ((tid & 31) == 0) mbar_arrive(empty);
+        continue;
+      }
+      const uint32_t sv = sm.base + L::kRing + slot * L::kTile;
+      const int held = max(0, min(kBN, g.s.len - j * kBN));                            // rows of tokens
+      const int boxed = min(kBN, (held + a.box_rows - 1) / a.box_rows * a.box_rows);   // zeros from here on
+      const int unseen = max(0, min(held, tiles.seen_first - j * kBN));                // seen by all below
+      for (int k = tid; k < (boxed - held) * L::kHalves * 8; k += 64) {
+        const int row = held + k / (L::kHalves * 8), c = k / 8 % L::kHalves, u = k % 8;
+        sts128(sv + c * L::kHalf + row * 128u + u * 16u, make_uint4(0u, 0u, 0u, 0u));
+      }
+      uint32_t odd = 0;
+      for (int k = tid; k < (held - unseen) * L::kHalves * 8; k += 64) {
+        const int row = unseen + k / (L::kHalves * 8), c = k / 8 % L::kHalves, u = k % 8;
+        const uint4 v = lds128(sv + c * L::kHalf + row * 128u + u * 16u);
+        odd |= ((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne);
+      }
+      odd = __any_sync(0xffffffffu, (odd & 0x80008000u) != 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if ((tid & 31) == 0) {
+        sm.words[kVFlag + 2 * (unit % kFixSlots) + (tid >> 5)] = static_cast<int>(odd);
+        mbar_arrive(sm.bar(kFix0 + unit % kFixSlots));
+        mbar_arrive(empty);
+      }
+      __syncwarp();
+    }
+  }
+}
+
+template <typename T, int DP>
+__device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk w, const Plan& plan, int t, int warp, int lane, uint32_t tmem) {
+  using L = Layout<DP>;
+  const int row = warp * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
+  const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
+  const float sl = a.scale_log2;
+  const uint64_t sl2 = pair(sl, sl);
+  uint32_t unit = 0, s_phase = 0, o_phase = 0, fix_phases = 0;
+  bool ok = true;
+  Segment g;
+  while (ok && w.next(a, g)) {
+    const Tiles tiles(a, g);
+    const int tok = row / a.group, head = row - tok * a.group;
+    const bool valid = row < a.tile_tokens * a.group && tiles.tok0[t] + tok < g.s.n;
+    const int limit = valid ? keys_of(a, g.s, tiles.tok0[t] + tok) : 0;
+    float m = -INFINITY, l = 0.0f;
+    uint32_t u = unit;
+    for (int j = g.j0; j < g.j1; ++j, ++u) {
+      const bool special = tiles.special(j);
+      const uint32_t fix = u % kFixSlots;
+      if (j >= tiles.end[t]) {  // the other tile's units: only the count of special ones goes on
+        if (special) fix_phases ^= 1u << fix;
+        continue;
+      }
+      ok = wait_for(sm, sm.bar(kSFull0 + t), s_phase);
+      s_phase ^= 1;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+      uint32_t sr[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
+      const uint32_t bad = static_cast<uint32_t>(sm.words[kBad + u % kBadSlots]);
+      tmem_wait_ld();
+      const int cols = limit - j * kBN;  // columns that this row sees
+      if (special || bad) {
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          const bool seen = c < cols && !(bad >> (c >> a.box_shift) & 1u);
+          if (!seen) sr[c / 32][c % 32] = 0xff800000u;  // -inf
+        }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          mx[k] = max3(mx[k], __uint_as_float(sr[(c + 2 * k) / 32][(c + 2 * k) % 32]), __uint_as_float(sr[(c + 2 * k + 1) / 32][(c + 2 * k + 1) % 32]));
+        }
+      }
+      const float mc = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl;
+      float alpha = 1.0f;
+      if (mc > m + kLazy) {
+        alpha = exp2_approx(m - mc);  // 0 where m is -inf
+        m = mc;
+        l *= alpha;
+      }
+      if (j > g.j0 && __any_sync(0xffffffffu, alpha < 1.0f)) {
+        // S of this unit is complete, and so is O += P V of the one before.
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 8) {
+          float o[8];
+          tmem_ld8(tO + c, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] *= alpha;
+          tmem_st8(tO + c, o);
+        }
+      }
+      const float shift = m == -INFINITY ? 0.0f : m;
+      const uint64_t sh2 = pair(-shift, -shift);
+      uint64_t sum[2] = {0, 0};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t p[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          uint32_t& s0 = sr[half * 2 + i / 16][(2 * i) % 32];
+          uint32_t& s1 = sr[half * 2 + i / 16][(2 * i + 1) % 32];
+          float x0, x1;
+          unpair(fma2(pair(__uint_as_float(s0), __uint_as_float(s1)), sl2, sh2), x0, x1);
+          x0 = exp2_approx(x0);
+          x1 = exp2_approx(x1);
+          sum[i & 1] = add2(sum[i & 1], pair(x0, x1));
+          p[i] = Storage<T>::pack2(x0, x1);
+          s0 = __float_as_uint(x0);
+          s1 = __float_as_uint(x1);
+        }
+        tmem_st32(tS + half * 32, p);
+      }
+      {
+        float x0, x1;
+        unpair(add2(sum[0], sum[1]), x0, x1);
+        l += x0 + x1;
+      }
+      if (special) {
+        ok = wait_for(sm, sm.bar(kFix0 + fix), (fix_phases >> fix) & 1u);
+        fix_phases ^= 1u << fix;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (sm.words[kVFlag + 2 * fix] | sm.words[kVFlag + 2 * fix + 1]) {
+          // Infinities or NaN in rows of V that not every row sees: P V key by key.
+          const uint32_t sv = sm.base + L::kRing + (2 * u + 1) % L::kStages * L::kTile;
+#pragma unroll 1
+          for (int c8 = 0; c8 < DP / 8; ++c8) {
+            float o[8];
+            tmem_ld8(tO + c8 * 8, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = j > g.j0 ? o[i] : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 128; ++c) {
+              const uint4 v = lds128(sv + (c8 / 8) * L::kHalf + c * 128u + static_cast<uint32_t>(((c8 & 7) ^ (c & 7)) * 16));
+              const bool seen = c < cols && !(bad >> (c >> a.box_shift) & 1u);
+              const float p = __uint_as_float(sr[c / 32][c % 32]);
+              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float2 f = Storage<T>::unpack2(vw[i]);
+                if (seen) {
+                  o[2 * i] = fmaf(p, f.x, o[2 * i]);
+                  o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1]);
+                }
+              }
+            }
+            tmem_st8(tO + c8 * 8, o);
+          }
+        }
+      }
+      tmem_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sm.bar(kPReady0 + t));
+    }
+    unit += g.j1 - g.j0;
+    if (!ok) break;
+
+    // ---- the segment's rows: final, or a piece of a cut block
+    const bool active = tiles.end[t] > g.j0;
+    if (active) {
+      ok = wait_for(sm, sm.bar(kOFull0 + t), o_phase);
+      o_phase ^= 1;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tcgen05_fence_after();
+    }
+    if (tiles.tok0[t] >= g.s.n) continue;  // no rows in this tile, in any piece
+    T* const out = static_cast<T*>(a.out) + ((g.s.first + tiles.tok0[t] + tok) * a.hq + g.h * a.group + head) * static_cast<int64_t>(a.dim);
+    const bool wide = a.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+    auto put = [&](int c, const float (&o)[32], float inv) {  // columns c .. c + 31
+      if (wide) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 16) {
+          if (c + i >= a.dim) break;
+          uint32_t r[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) r[k] = Storage<T>::pack2(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
+          store32(out + c + i, r);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {  // head_dim is a multiple of 8, out 4-byte aligned
+          if (c + i < a.dim) *reinterpret_cast<uint32_t*>(out + c + i) = Storage<T>::pack2(o[i] * inv, o[i + 1] * inv);
+        }
+      }
+    };
+    if (g.j0 == 0 && g.j1 == g.nt) {
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tO + c, o);
+        tmem_wait_ld();
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
+        if (valid) put(c, f, inv);
+      }
+      continue;
+    }
+    const int run0 = plan.run_of(g.first), run1 = plan.run_of(g.first + g.nt - 1), run = static_cast<int>(blockIdx.x);
+    float* const mine = piece_at<DP>(a, 2 * static_cast<int64_t>(run) + (run == run0 ? 1 : 0), t);
+    if (active) {
+#pragma unroll
+      for (int c = 0; c < DP; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tO + c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          if (valid) __stcg(mine + (c + i) * 128 + row, __uint_as_float(o[i]));
+        }
+      }
+    }
+    __stcg(mine + DP * 128 + row, m);
+    __stcg(mine + (DP + 1) * 128 + row, l);
+    __syncwarp();
+    uint32_t* const counter = a.counters + run0 * kCountersPerCta + t * 4 + warp;
+    uint32_t before = 0;
+    if (lane == 0) before = atom_add_acq_rel_gpu(counter, 1u);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    if (before != static_cast<uint32_t>(run1 - run0)) continue;
+    // Last: the pieces' sum, weighted by their maxima, in their order.
+    fence_acq_rel_gpu();
+    __syncwarp();
+    float top = -INFINITY;
+    for (int r = run0; r <= run1; ++r) {
+      const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + DP * 128 + row;
+      if (__ldcg(pc + 128) != 0.0f) top = fmaxf(top, __ldcg(pc));
+    }
+    float total = 0.0f;
+    for (int r = run0; r <= run1; ++r) {
+      const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + DP * 128 + row;
+      const float pl = __ldcg(pc + 128);
+      if (pl != 0.0f) total += pl * exp2_approx(__ldcg(pc) - top);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 32) {
+      if (c >= a.dim) break;
+      float o[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+#pragma unroll 1
+      for (int r = run0; r <= run1; ++r) {
+        const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + row;
+        const float pl = __ldcg(pc + (DP + 1) * 128);
+        if (valid && pl != 0.0f) {
+          const float f = exp2_approx(__ldcg(pc + DP * 128) - top);
+          float x[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x[i] = __ldcg(pc + (c + i) * 128);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = fmaf(f, x[i], o[i]);
+        }
+      }
+      if (valid) put(c, o, inv);
+    }
+    if (lane == 0) __stcg(counter, 0u);
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                                                           const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
+  using L = Layout<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  Smem sm;
+  sm.ptr = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  sm.base = smem_u32(sm.ptr);
+  sm.bars = sm.base + L::kBars;
+  sm.words = reinterpret_cast<volatile int*>(sm.ptr + L::kWords);
+  sm.status = a.status;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    for (int i = 0; i < kRingFull + 2 * L::kStages; ++i) {
+      const bool per_warp = i == kPReady0 || i == kPReady1;
+      const bool fix = i >= kFix0 && i < kFix0 + kFixSlots;
+      // A stage is given back by the products that read it and by the two warps on V, which follow every one.
+      mbar_init(sm.bar(i), per_warp ? 4 : fix ? 2 : i >= kRingFull + L::kStages ? 3 : 1);
+    }
+    fence_barrier_init();
+    sm.words[kDead] = 0;
+    tma_prefetch_descriptor(&mq);
+    tma_prefetch_descriptor(&mk);
+    tma_prefetch_descriptor(&mv);
+  }
+  wait_prior_grid();
+  allow_next_grid();
+  __syncwarp();
+  if (warp == 0) {  // not before the previous grid has ended: a CTA of it could wait for these columns
+    tmem_alloc(sm.base + L::kWords + 4 * kTmem, 512);
+    tmem_relinquish();
+  }
+
+  // The sequences' units, a run of sequences a thread; every CTA's run of units, and the sequence where this one's begins.
+  const int per = (a.batch + kTcThreads - 1) / kTcThreads;
+  const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
+  int64_t mine = 0;
+  for (int b = lo; b < hi; ++b) {
+    const Seq s = read_seq(a, b, blockIdx.x == 0);
+    mine += s.n > 0 ? head_units(a, s) * a.hkv : 0;
+  }
+  int64_t inc = mine;
+#pragma unroll
+  for (int k = 1; k < 32; k <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, k);
+    if (lane >= k) inc += y;
+  }
+  volatile int64_t* const scan = reinterpret_cast<volatile int64_t*>(sm.ptr + L::kWords + 4 * ((kScan + 1) / 2 * 2));
+  if (lane == 31) scan[warp] = inc;
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  int64_t before = inc - mine;
+  Plan plan{0, 0};
+  for (int k = 0; k < kTcThreads / 32; ++k) {
+    if (k < warp) before += scan[k];
+    plan.total += scan[k];
+  }
+  plan.runs = static_cast<int>(min(static_cast<int64_t>(gridDim.x), plan.total));
+  const bool busy = static_cast<int>(blockIdx.x) < plan.runs;
+  int64_t u0 = 0, u1 = 0;
+  if (busy) {
+    u0 = plan.begin(blockIdx.x);
+    u1 = plan.begin(blockIdx.x + 1);
+    if (u0 >= before && u0 < before + mine) {
+      int64_t off = u0 - before;
+      for (int b = lo; b < hi; ++b) {
+        const Seq s = read_seq(a, b, false);
+        const int64_t n = s.n > 0 ? head_units(a, s) * a.hkv : 0;
+        if (off < n) {
+          sm.words[kStartSeq] = b;
+          sm.words[kStartLo] = static_cast<int>(off & 0xffffffff);
+          sm.words[kStartHi] = static_cast<int>(off >> 32);
+          break;
+        }
+        off -= n;
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = static_cast<uint32_t>(sm.words[kTmem]);
+  if (busy) {
+    Walk w;
+    w.init(a, sm, lane, u0, u1);
+    if (warp < 8) {
+      more_registers<kSoftmaxRegs>();
+      softmax_role<T, DP>(a, sm, w, plan, warp >> 2, warp & 3, lane, tmem);
+    } else {
+      fewer_registers<kOtherRegs>();
+      if (warp == kLoadWarp) {
+        load_role<T, DP>(a, sm, w, lane, &mq, &mk, &mv);
+      } else if (warp == kMmaWarp) {
+        if (lane == 0) mma_role<T, DP>(a, sm, w, tmem);
+        __syncwarp();
+      } else {
+        fix_role<T, DP>(a, sm, w, tid - kFixWarp * 32);
+      }
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ----------------------------------------------------------------- host
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+  static Encode fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) == cudaSuccess &&
+        found == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<Encode>(p);
+    }
+  });
+  return fn;
+}
+
+// `bytes` between two entries of a dimension; one of one entry may have any.
+cuuint64_t stride_bytes(int64_t elements, int64_t extent) { return extent == 1 ? 16 : static_cast<cuuint64_t>(elements) * 2; }
+
+template <typename T, int DP>
+cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
+  using L = Layout<DP>;
+  const Encode enc = encoder();
+  if (!enc) return cudaErrorNotSupported;
+  const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  CUtensorMap mq, mk, mv;
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  {
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hq), static_cast<cuuint64_t>(a.tokens)};
+    const cuuint64_t strides[2] = {stride_bytes(a.dim, a.hq), stride_bytes(a.q_stride, a.tokens)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(a.tile_tokens)};
+    if (enc(&mq, type, 3, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      return cudaErrorInvalidValue;
+    }
+  }
+  for (int i = 0; i < 2; ++i) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hkv), static_cast<cuuint64_t>(a.page_size),
+                                static_cast<cuuint64_t>(a.num_pages)};
+    const cuuint64_t strides[3] = {stride_bytes(a.head_stride, a.hkv), stride_bytes(a.token_stride, a.page_size),
+                                   stride_bytes(a.page_stride, a.num_pages)};
+    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(a.box_rows), 1};
+    if (enc(i ? &mv : &mk, type, 4, const_cast<void*>(i ? a.v : a.k), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+      return cudaErrorInvalidValue;
+    }
+  }
+  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  if (e != cudaSuccess) return e;
+  return launch_kernel(true, tc_kernel<T, DP>, dim3(sms), dim3(kTcThreads), L::kBytes, st, mq, mk, mv, a);
+}
+
+bool fits_map(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * 2)) % 16 == 0; }
+
+}  // namespace
+
+// A box: tokens of one page within 128, a multiple of 8.
+static int box_rows_of(int page_size) {
+  int r = page_size & -page_size;
+  return std::min(r, kBN);
+}
+
+bool tc_fits(const Args& a, int dtype, int code_type) {
+  if (dtype == KL_FLOAT32 || code_type != KL_CODE_NONE) return false;
+  if (a.dim % 8 != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
+  const auto stride_ok = [](int64_t stride, int64_t extent) { return extent == 1 || (stride > 0 && stride % 8 == 0 && stride < (int64_t(1) << 38)); };
+  return fits_map(a.q, 0) && fits_map(a.k, 0) && fits_map(a.v, 0) && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 &&
+         stride_ok(a.q_stride, a.tokens) && stride_ok(a.head_stride, a.hkv) && stride_ok(a.token_stride, a.page_size) &&
+         stride_ok(a.page_stride, a.num_pages) && a.num_pages < INT_MAX;
+}
+
+size_t tc_partial_bytes(int head_dim, int sms) {
+  if (head_dim > 128) return 0;
+  const size_t dp = head_dim <= 64 ? 64 : 128;
+  return static_cast<size_t>(sms) * 2 * 2 * (dp + 2) * 128 * sizeof(float);
+}
+
+size_t tc_sync_bytes(int sms) { return 256 + static_cast<size_t>(sms) * kCountersPerCta * sizeof(uint32_t); }
+
+cudaError_t launch_tc(Args a, int dtype, int code_type, int sms, cudaStream_t st) {
+  a.tile_tokens = 128 / a.group;
+  a.box_rows = box_rows_of(a.page_size);
+  while ((1 << a.box_shift) < a.box_rows) ++a.box_shift;
+  if (dtype == KL_FLOAT16) return a.dim <= 64 ? launch<__half, 64>(a, sms, st) : launch<__half, 128>(a, sms, st);
+  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, sms, st) : launch<__nv_bfloat16, 128>(a, sms, st);
+}
+
+}  // namespace chunk_attention
+}  // namespace klb
