@@ -35,28 +35,40 @@ namespace chunk_attention {
 namespace {
 
 constexpr int kBN = 128;                 // keys of a unit
-constexpr int kTcThreads = 384;          // two softmax warpgroups, then: load, products, two warps on V
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10;
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;  // 256 * 208 + 128 * 88 <= 384 * 168, the launch's
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10, kWidenWarp = 12;
 constexpr float kLazy = 8.0f;            // log2 by which a maximum may be passed before O is rescaled
 constexpr uint64_t kWaitCycles = 2000000000ull;  // about one second
 constexpr int kFixSlots = 4, kBadSlots = 8;
 constexpr int kCountersPerCta = 8;       // a counter for each warp's 32 rows of the two tiles
 
-template <int DP>
+template <int DP, int CODE>
 struct Layout {
-  static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a row
+  static constexpr bool kCoded = CODE != KL_CODE_NONE;
+  // Two softmax warpgroups; load, products, two warps on V; over an 8-bit cache four warps that widen its codes.
+  static constexpr int kThreads = kCoded ? 512 : 384;
+  // Registers: 256 * 192 + 256 * 64 = 512 * 128, 256 * 208 + 128 * 88 = 384 * 168, the launch's.
+  static constexpr int kSoftmaxRegs = kCoded ? 192 : 208, kOtherRegs = kCoded ? 64 : 88;
+  static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a 16-bit row
   static constexpr uint32_t kHalf = 128u * 128u;            // 128 rows of one
   static constexpr uint32_t kTile = kHalves * kHalf;
-  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kStages = kCoded ? (DP == 128 ? 3 : 4) : (DP == 128 ? 5 : 8);
+  static constexpr int kRawStages = kCoded ? (DP == 128 ? 4 : 6) : 0;
+  static constexpr uint32_t kRawTile = 128u * DP;           // codes, a row after the other
   static constexpr uint32_t kRing = 2 * kTile;              // Q's two tiles first
-  static constexpr uint32_t kBars = kRing + kStages * kTile;
-  static constexpr uint32_t kWords = kBars + 256;           // ints
-  static constexpr uint32_t kBytes = kWords + 256 + 1024;   // slack to align the base to 1024 bytes
+  static constexpr uint32_t kRaw = kRing + kStages * kTile;
+  static constexpr uint32_t kBars = kRaw + kRawStages * kRawTile;
+  static constexpr uint32_t kWords = kBars + 320;           // ints
+  static constexpr uint32_t kScales = kWords + 256;         // [kBadSlots][K, V][16]: a scale for every 8 keys
+  static constexpr uint32_t kBytes = kScales + (kCoded ? 1024 : 0) + 1024;  // slack to align the base to 1024 bytes
+  // Barriers of the rings.
+  static constexpr int kFull = 14, kEmpty = kFull + kStages, kRawFull = kEmpty + kStages, kRawEmpty = kRawFull + kRawStages;
+  static constexpr int kBarCount = kRawEmpty + kRawStages;
+  static_assert(kBarCount * 8 <= 320 && kBytes <= 232448, "shared memory");
 };
 
 // Barriers, 8 bytes each from Layout::kBars on.
-enum Bar { kQFull0, kQFull1, kQEmpty, kSFull0, kSFull1, kPReady0, kPReady1, kOFull0, kOFull1, kDrain, kFix0, kRingFull = kFix0 + kFixSlots };
+enum Bar { kQFull0, kQFull1, kQEmpty, kSFull0, kSFull1, kPReady0, kPReady1, kOFull0, kOFull1, kDrain, kFix0, kFixEnd = kFix0 + kFixSlots };
+static_assert(kFixEnd == 14, "the rings' barriers follow");
 
 // Words from Layout::kWords on.
 enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kTotalLo, kTotalHi, kVFlag, kBad = kVFlag + 2 * kFixSlots, kScan = kBad + kBadSlots };
@@ -266,6 +278,11 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -301,52 +318,72 @@ struct Plan {
   __device__ int run_of(int64_t u) const { return static_cast<int>(((u + 1) * runs - 1) / total); }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, int CODE>
 __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w, int lane, const CUtensorMap* mq, const CUtensorMap* mk,
                                           const CUtensorMap* mv) {
-  using L = Layout<DP>;
+  using L = Layout<DP, CODE>;
   const uint64_t keep = l2_policy_evict_normal(), once = l2_policy_evict_first();
+  constexpr int kDepth = L::kCoded ? L::kRawStages : L::kStages;
+  constexpr int kFull = L::kCoded ? L::kRawFull : L::kFull, kEmpty = L::kCoded ? L::kRawEmpty : L::kEmpty;
   const int boxes = kBN / a.box_rows;
-  const uint32_t box_bytes = a.box_rows * 128u;
+  const uint32_t box_bytes = a.box_rows * (L::kCoded ? DP : 128u);
   uint32_t slot = 0, phase = 0, issued = 0, unit = 0;
   uint32_t q_phase = 0;
   bool ok = true, first_segment = true;
-  Segment g;
+  Segment g{};
+  // Lane i looks after box i of a unit: its page, num_pages (for zeros) past the sequence's end or where the id is
+  // no page's. Ids are asked for two units ahead, scales one.
+  auto page_of = [&](int j) -> int64_t {
+    const int tok = j * kBN + lane * a.box_rows;
+    return j < g.j1 && lane < boxes && tok < g.s.len ? __ldcg(a.block_table + g.b * a.bt_stride + tok / a.page_size) : a.num_pages;
+  };
+  auto scale_of = [&](const float* scales, int64_t page) {
+    return L::kCoded && page >= 0 && page < a.num_pages ? __ldcg(scales + page * a.scale_stride + g.h) : 0.0f;
+  };
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
+    int64_t page = page_of(g.j0), page1 = page_of(g.j0 + 1);
+    float ks = scale_of(a.k_scale, page), vs = scale_of(a.v_scale, page);
     for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
-      // Lane i looks up box i: its page, or one past the pool's for zeros.
+      const int64_t page2 = page_of(j + 2);
+      const float ks1 = scale_of(a.k_scale, page1), vs1 = scale_of(a.v_scale, page1);
       const int tok = j * kBN + lane * a.box_rows;
-      int64_t page = a.num_pages;
-      bool bad = false;
-      if (lane < boxes && tok < g.s.len) {
-        page = __ldcg(a.block_table + g.b * a.bt_stride + tok / a.page_size);
-        bad = page < 0 || page >= a.num_pages;
-        if (bad) page = a.num_pages;
-      }
+      const bool bad = lane < boxes && tok < g.s.len && (page < 0 || page >= a.num_pages);
+      if (bad) page = a.num_pages;
       const uint32_t bad_boxes = __ballot_sync(0xffffffffu, bad);
       if (lane == 0) {
         sm.words[kBad + unit % kBadSlots] = static_cast<int>(bad_boxes);
         if (bad_boxes) atomicOr(sm.status, kStatusBadPage);
       }
+      if constexpr (L::kCoded) {
+        const int from = (lane & 15) * 8 >> a.box_shift;
+        const float x = __shfl_sync(0xffffffffu, ks, from), y = __shfl_sync(0xffffffffu, vs, from);
+        float* const to = reinterpret_cast<float*>(sm.ptr + L::kScales) + unit % kBadSlots * 32 + lane;
+        *to = lane < 16 ? x * a.scale_log2 : y;
+      }
       __syncwarp();
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
-        const uint32_t full = sm.bar(kRingFull + slot), empty = sm.bar(kRingFull + L::kStages + slot);
-        if (issued >= L::kStages) ok = wait_for(sm, empty, phase ^ 1);
+        const uint32_t full = sm.bar(kFull + slot), empty = sm.bar(kEmpty + slot);
+        if (issued >= kDepth) ok = wait_for(sm, empty, phase ^ 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (lane == 0) mbar_arrive_expect_tx(full, L::kTile);
+        if (lane == 0) mbar_arrive_expect_tx(full, L::kCoded ? L::kRawTile : L::kTile);
         __syncwarp();
         if (lane < boxes) {
-#pragma unroll
-          for (int c = 0; c < L::kHalves; ++c) {
-            tma_load_4d(sm.base + L::kRing + slot * L::kTile + c * L::kHalf + lane * box_bytes, kv ? mv : mk, c * 64, g.h, tok % a.page_size,
+          if constexpr (L::kCoded) {
+            tma_load_4d(sm.base + L::kRaw + slot * L::kRawTile + lane * box_bytes, kv ? mv : mk, 0, g.h, tok % a.page_size,
                         static_cast<int>(page), full, keep);
+          } else {
+#pragma unroll
+            for (int c = 0; c < L::kHalves; ++c) {
+              tma_load_4d(sm.base + L::kRing + slot * L::kTile + c * L::kHalf + lane * box_bytes, kv ? mv : mk, c * 64, g.h,
+                          tok % a.page_size, static_cast<int>(page), full, keep);
+            }
           }
         }
         ++issued;
-        if (++slot == L::kStages) {
+        if (++slot == kDepth) {
           slot = 0;
           phase ^= 1;
         }
@@ -368,34 +405,122 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
           }
         }
       }
+      page = page1;
+      page1 = page2;
+      ks = ks1;
+      vs = vs1;
     }
   }
   // Nothing may be in flight into this CTA's shared memory when it ends; normally it has long landed.
   if (lane == 0) {
-    for (uint32_t k = 0; k < min(issued, static_cast<uint32_t>(L::kStages)); ++k) {
-      const uint32_t i = issued - 1 - k, s = i % L::kStages;
+    for (uint32_t k = 0; k < min(issued, static_cast<uint32_t>(kDepth)); ++k) {
+      const uint32_t i = issued - 1 - k, s = i % kDepth;
       const uint64_t start = clock64();
-      while (!mbar_try_wait(sm.bar(kRingFull + s), (i / L::kStages) & 1) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
+      while (!mbar_try_wait(sm.bar(kFull + s), (i / kDepth) & 1) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
       }
     }
   }
   __syncwarp();
 }
 
+// ----------------------------------------------------------------- codes to 16 bits
+
+// Two codes, the bytes 2 * HI and 2 * HI + 1 of a word, as a pair of TO; exact: e4m3 has 4 significant bits, int8 7.
+template <typename TO, int CODE, int HI>
+__device__ __forceinline__ uint32_t widen_pair(uint32_t w) {
+  if constexpr (CODE == KL_CODE_E4M3) {
+    const uint32_t h = HI ? e4m3x2_hi_to_f16x2(w) : e4m3x2_lo_to_f16x2(w);
+    if constexpr (std::is_same<TO, __half>::value) return h;
+    const float2 f = Storage<__half>::unpack2(h);
+    return Storage<__nv_bfloat16>::pack2(f.x, f.y);
+  } else if constexpr (std::is_same<TO, __half>::value) {
+    // The code with its sign bit turned over, as the last bits of 1024 + (code + 128).
+    const uint32_t x = __byte_perm(w ^ 0x80808080u, 0x64646464u, HI ? 0x7372 : 0x7170);
+    const __half2 bias = __floats2half2_rn(1152.0f, 1152.0f);
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), bias);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    // 128 + the low seven bits, less 256 for a negative code and 128 for another.
+    const uint32_t x = __byte_perm(w, 0u, HI ? 0x4342 : 0x4140);
+    const uint32_t p = (x & 0x007f007fu) | 0x43004300u, n = (x & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&p), *reinterpret_cast<const __nv_bfloat162*>(&n));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// One row of a tile: codes in, 16-bit elements in the 128-byte swizzle out. The rows of a warp start at different
+// places of their row, which leaves neither side with bank conflicts.
+template <typename TO, int DP, int CODE>
+__device__ __forceinline__ void widen_row(uint32_t raw, uint32_t tile, int row) {
+  using L = Layout<DP, CODE>;
+  constexpr int kUnits = DP / 16;
+#pragma unroll
+  for (int k = 0; k < kUnits; ++k) {
+    const int u = (k + row) & (kUnits - 1);
+    const uint4 v = lds128(raw + row * DP + u * 16);
+    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+    uint32_t out[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      out[2 * i] = widen_pair<TO, CODE, 0>(in[i]);
+      out[2 * i + 1] = widen_pair<TO, CODE, 1>(in[i]);
+    }
+    const uint32_t at = tile + (u >> 2) * L::kHalf + row * 128u;
+    const uint32_t c = (2 * u) & 7, s = row & 7;
+    sts128(at + ((c ^ s) << 4), make_uint4(out[0], out[1], out[2], out[3]));
+    sts128(at + (((c + 1) ^ s) << 4), make_uint4(out[4], out[5], out[6], out[7]));
+  }
+}
+
+// Four warps, a thread a row: K into q's dtype, V into bf16.
+template <typename T, int DP, int CODE>
+__device__ __forceinline__ void widen_role(const Args& a, const Smem& sm, Walk w, int row) {
+  using L = Layout<DP, CODE>;
+  uint32_t raw_slot = 0, raw_phase = 0, slot = 0, phase = 0;
+  const int64_t items = 2 * (w.u1 - w.u);
+  for (int64_t i = 0; i < items; ++i) {
+    bool ok = wait_for(sm, sm.bar(L::kRawFull + raw_slot), raw_phase);
+    if (i >= L::kStages) ok = ok && wait_for(sm, sm.bar(L::kEmpty + slot), phase ^ 1);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return;
+    const uint32_t raw = sm.base + L::kRaw + raw_slot * L::kRawTile, tile = sm.base + L::kRing + slot * L::kTile;
+    if (i & 1) {
+      widen_row<__nv_bfloat16, DP, CODE>(raw, tile, row);
+    } else {
+      widen_row<T, DP, CODE>(raw, tile, row);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if ((row & 31) == 0) {
+      mbar_arrive(sm.bar(L::kFull + slot));
+      mbar_arrive(sm.bar(L::kRawEmpty + raw_slot));
+    }
+    if (++raw_slot == L::kRawStages) {
+      raw_slot = 0;
+      raw_phase ^= 1;
+    }
+    if (++slot == L::kStages) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+}
+
 // One thread.
-template <typename T, int DP>
+template <typename T, int DP, int CODE>
 __device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, uint32_t tmem) {
-  using L = Layout<DP>;
+  using L = Layout<DP, CODE>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16, 128, DP, true);
+  // Over codes P V runs in bf16, whose range holds a probability times any scale.
+  constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16 || L::kCoded, 128, DP, true);
   const int ksteps = (a.dim + 15) / 16;
   uint32_t slot = 0, phase = 0, unit = 0;
   uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
   bool ok = true;
-  Segment g;
-  auto ring_wait = [&] { ok = ok && wait_for(sm, sm.bar(kRingFull + slot), phase); };
+  Segment g{};
+  auto ring_wait = [&] { ok = ok && wait_for(sm, sm.bar(L::kFull + slot), phase); };
   auto ring_next = [&] {
-    umma_commit(sm.bar(kRingFull + L::kStages + slot));
+    umma_commit(sm.bar(L::kEmpty + slot));
     if (++slot == L::kStages) {
       slot = 0;
       phase ^= 1;
@@ -452,7 +577,7 @@ __device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, 
           // The next unit's K: the stage after V's.
           const uint32_t k_slot = v_slot + 1 == L::kStages ? 0 : v_slot + 1;
           const uint32_t k_phase = v_slot + 1 == L::kStages ? (t == 1 ? phase : phase ^ 1) : phase;
-          ok = wait_for(sm, sm.bar(kRingFull + k_slot), k_phase);
+          ok = wait_for(sm, sm.bar(L::kFull + k_slot), k_phase);
           if (!ok) break;
           tcgen05_fence_after();
           scores(t, k_slot);
@@ -473,14 +598,14 @@ __device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, 
 }
 
 // Two warps: the V rows of special units.
-template <typename T, int DP>
+template <typename T, int DP, int CODE>
 __device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, int tid) {
-  using L = Layout<DP>;
-  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+  using L = Layout<DP, CODE>;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value || L::kCoded;
   constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
   uint32_t unit = 0;
   bool ok = true;
-  Segment g;
+  Segment g{};
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
     for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
@@ -490,12 +615,12 @@ __device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, 
       for (int kv = 0; kv < 2; ++kv) {
         const uint32_t i = 2 * unit + kv;
         slot = i % L::kStages;
-        ok = ok && wait_for(sm, sm.bar(kRingFull + slot), (i / L::kStages) & 1);
-        if (kv == 0 && (tid & 31) == 0) mbar_arrive(sm.bar(kRingFull + L::kStages + slot));
+        ok = ok && wait_for(sm, sm.bar(L::kFull + slot), (i / L::kStages) & 1);
+        if (kv == 0 && (tid & 31) == 0) mbar_arrive(sm.bar(L::kEmpty + slot));
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      const uint32_t empty = sm.bar(kRingFull + L::kStages + slot);
+      const uint32_t empty = sm.bar(L::kEmpty + slot);
       if (!tiles.special(j)) {
         if ((tid & 31) == 0) mbar_arrive(empty);
         continue;
@@ -527,17 +652,18 @@ __device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, 
   }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, int CODE>
 __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk w, const Plan& plan, int t, int warp, int lane, uint32_t tmem) {
-  using L = Layout<DP>;
+  using L = Layout<DP, CODE>;
   const int row = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
   const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
+  using TV = std::conditional_t<L::kCoded, __nv_bfloat16, T>;  // of P and V
   const float sl = a.scale_log2;
   const uint64_t sl2 = pair(sl, sl);
   uint32_t unit = 0, s_phase = 0, o_phase = 0, fix_phases = 0;
   bool ok = true;
-  Segment g;
+  Segment g{};
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
     const int tok = row / a.group, head = row - tok * a.group;
@@ -563,6 +689,21 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       const uint32_t bad = static_cast<uint32_t>(sm.words[kBad + u % kBadSlots]);
       tmem_wait_ld();
       const int cols = limit - j * kBN;  // columns that this row sees
+      const float4* const scales = reinterpret_cast<const float4*>(sm.ptr + L::kScales) + u % kBadSlots * 8;
+      if constexpr (L::kCoded) {  // in units of log2 from here on
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float4 f4 = scales[q];
+          const float f[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float x0, x1;
+            unpair(mul2(pair(__uint_as_float(sr[q][c]), __uint_as_float(sr[q][c + 1])), pair(f[c / 8], f[c / 8])), x0, x1);
+            sr[q][c] = __float_as_uint(x0);
+            sr[q][c + 1] = __float_as_uint(x1);
+          }
+        }
+      }
       if (special || bad) {
 #pragma unroll
         for (int c = 0; c < 128; ++c) {
@@ -578,7 +719,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           mx[k] = max3(mx[k], __uint_as_float(sr[(c + 2 * k) / 32][(c + 2 * k) % 32]), __uint_as_float(sr[(c + 2 * k + 1) / 32][(c + 2 * k + 1) % 32]));
         }
       }
-      const float mc = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sl;
+      const float mc = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * (L::kCoded ? 1.0f : sl);
       float alpha = 1.0f;
       if (mc > m + kLazy) {
         alpha = exp2_approx(m - mc);  // 0 where m is -inf
@@ -603,16 +744,31 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t p[32];
+        float half_scales[8];
+        if constexpr (L::kCoded) {
+          const float4 f0 = scales[4 + 2 * half], f1 = scales[5 + 2 * half];
+          half_scales[0] = f0.x, half_scales[1] = f0.y, half_scales[2] = f0.z, half_scales[3] = f0.w;
+          half_scales[4] = f1.x, half_scales[5] = f1.y, half_scales[6] = f1.z, half_scales[7] = f1.w;
+        }
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
           uint32_t& s0 = sr[half * 2 + i / 16][(2 * i) % 32];
           uint32_t& s1 = sr[half * 2 + i / 16][(2 * i + 1) % 32];
           float x0, x1;
-          unpair(fma2(pair(__uint_as_float(s0), __uint_as_float(s1)), sl2, sh2), x0, x1);
+          const uint64_t s = pair(__uint_as_float(s0), __uint_as_float(s1));
+          unpair(L::kCoded ? add2(s, sh2) : fma2(s, sl2, sh2), x0, x1);
           x0 = exp2_approx(x0);
           x1 = exp2_approx(x1);
           sum[i & 1] = add2(sum[i & 1], pair(x0, x1));
-          p[i] = Storage<T>::pack2(x0, x1);
+          if constexpr (L::kCoded) {
+            const float f = half_scales[i / 4];
+            unpair(mul2(pair(x0, x1), pair(f, f)), x0, x1);
+            if (special) {  // a masked key's scale does not count either
+              if (half * 64 + 2 * i >= cols) x0 = 0.0f;
+              if (half * 64 + 2 * i + 1 >= cols) x1 = 0.0f;
+            }
+          }
+          p[i] = Storage<TV>::pack2(x0, x1);
           s0 = __float_as_uint(x0);
           s1 = __float_as_uint(x1);
         }
@@ -646,7 +802,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
               const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const float2 f = Storage<T>::unpack2(vw[i]);
+                const float2 f = Storage<TV>::unpack2(vw[i]);
                 if (seen) {
                   o[2 * i] = fmaf(p, f.x, o[2 * i]);
                   o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1]);
@@ -770,10 +926,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
   }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+template <typename T, int DP, int CODE>
+__global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                                                            const __grid_constant__ CUtensorMap mv, const __grid_constant__ Args a) {
-  using L = Layout<DP>;
+  using L = Layout<DP, CODE>;
   extern __shared__ uint8_t smem_raw[];
   Smem sm;
   sm.ptr = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -784,11 +940,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < kRingFull + 2 * L::kStages; ++i) {
-      const bool per_warp = i == kPReady0 || i == kPReady1;
-      const bool fix = i >= kFix0 && i < kFix0 + kFixSlots;
-      // A stage is given back by the products that read it and by the two warps on V, which follow every one.
-      mbar_init(sm.bar(i), per_warp ? 4 : fix ? 2 : i >= kRingFull + L::kStages ? 3 : 1);
+    for (int i = 0; i < L::kBarCount; ++i) {
+      // P by a tile's four warps, special units by two; a stage is filled by TMA or the four widening warps and given
+      // back by the products that read it and the two warps on V, which follow every one.
+      int count = 1;
+      if (i == kPReady0 || i == kPReady1) count = 4;
+      if (i >= kFix0 && i < kFixEnd) count = 2;
+      if (i >= L::kFull && i < L::kEmpty) count = L::kCoded ? 4 : 1;
+      if (i >= L::kEmpty && i < L::kRawFull) count = 3;
+      if (i >= L::kRawEmpty) count = 4;
+      mbar_init(sm.bar(i), count);
     }
     fence_barrier_init();
     sm.words[kDead] = 0;
@@ -805,7 +966,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant
   }
 
   // The sequences' units, a run of sequences a thread; every CTA's run of units, and the sequence where this one's begins.
-  const int per = (a.batch + kTcThreads - 1) / kTcThreads;
+  const int per = (a.batch + L::kThreads - 1) / L::kThreads;
   const int lo = min(a.batch, tid * per), hi = min(a.batch, lo + per);
   int64_t mine = 0;
   for (int b = lo; b < hi; ++b) {
@@ -825,7 +986,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant
   tcgen05_fence_after();
   int64_t before = inc - mine;
   Plan plan{0, 0};
-  for (int k = 0; k < kTcThreads / 32; ++k) {
+  for (int k = 0; k < L::kThreads / 32; ++k) {
     if (k < warp) before += scan[k];
     plan.total += scan[k];
   }
@@ -856,17 +1017,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_kernel(const __grid_constant
     Walk w;
     w.init(a, sm, lane, u0, u1);
     if (warp < 8) {
-      more_registers<kSoftmaxRegs>();
-      softmax_role<T, DP>(a, sm, w, plan, warp >> 2, warp & 3, lane, tmem);
+      more_registers<L::kSoftmaxRegs>();
+      softmax_role<T, DP, CODE>(a, sm, w, plan, warp >> 2, warp & 3, lane, tmem);
     } else {
-      fewer_registers<kOtherRegs>();
+      fewer_registers<L::kOtherRegs>();
       if (warp == kLoadWarp) {
-        load_role<T, DP>(a, sm, w, lane, &mq, &mk, &mv);
+        load_role<T, DP, CODE>(a, sm, w, lane, &mq, &mk, &mv);
       } else if (warp == kMmaWarp) {
-        if (lane == 0) mma_role<T, DP>(a, sm, w, tmem);
+        if (lane == 0) mma_role<T, DP, CODE>(a, sm, w, tmem);
         __syncwarp();
-      } else {
-        fix_role<T, DP>(a, sm, w, tid - kFixWarp * 32);
+      } else if (warp < kWidenWarp) {
+        fix_role<T, DP, CODE>(a, sm, w, tid - kFixWarp * 32);
+      } else if constexpr (L::kCoded) {
+        widen_role<T, DP, CODE>(a, sm, w, tid - kWidenWarp * 32);
       }
     }
   }
@@ -898,11 +1061,11 @@ Encode encoder() {
 }
 
 // `bytes` between two entries of a dimension; one of one entry may have any.
-cuuint64_t stride_bytes(int64_t elements, int64_t extent) { return extent == 1 ? 16 : static_cast<cuuint64_t>(elements) * 2; }
+cuuint64_t stride_bytes(int64_t elements, int64_t extent, int size) { return extent == 1 ? 16 : static_cast<cuuint64_t>(elements) * size; }
 
-template <typename T, int DP>
+template <typename T, int DP, int CODE>
 cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
-  using L = Layout<DP>;
+  using L = Layout<DP, CODE>;
   const Encode enc = encoder();
   if (!enc) return cudaErrorNotSupported;
   const auto type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -910,7 +1073,7 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   {
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hq), static_cast<cuuint64_t>(a.tokens)};
-    const cuuint64_t strides[2] = {stride_bytes(a.dim, a.hq), stride_bytes(a.q_stride, a.tokens)};
+    const cuuint64_t strides[2] = {stride_bytes(a.dim, a.hq, 2), stride_bytes(a.q_stride, a.tokens, 2)};
     const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(a.tile_tokens)};
     if (enc(&mq, type, 3, const_cast<void*>(a.q), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
@@ -920,20 +1083,33 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
   for (int i = 0; i < 2; ++i) {
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hkv), static_cast<cuuint64_t>(a.page_size),
                                 static_cast<cuuint64_t>(a.num_pages)};
-    const cuuint64_t strides[3] = {stride_bytes(a.head_stride, a.hkv), stride_bytes(a.token_stride, a.page_size),
-                                   stride_bytes(a.page_stride, a.num_pages)};
-    const cuuint32_t box[4] = {64, 1, static_cast<cuuint32_t>(a.box_rows), 1};
-    if (enc(i ? &mv : &mk, type, 4, const_cast<void*>(i ? a.v : a.k), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+    constexpr int size = L::kCoded ? 1 : 2;
+    const cuuint64_t strides[3] = {stride_bytes(a.head_stride, a.hkv, size), stride_bytes(a.token_stride, a.page_size, size),
+                                   stride_bytes(a.page_stride, a.num_pages, size)};
+    const cuuint32_t box[4] = {L::kCoded ? DP : 64, 1, static_cast<cuuint32_t>(a.box_rows), 1};
+    if (enc(i ? &mv : &mk, L::kCoded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, 4, const_cast<void*>(i ? a.v : a.k), dims, strides, box, ones,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, L::kCoded ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
       return cudaErrorInvalidValue;
     }
   }
-  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
+  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, DP, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return e;
-  return launch_kernel(true, tc_kernel<T, DP>, dim3(sms), dim3(kTcThreads), L::kBytes, st, mq, mk, mv, a);
+  return launch_kernel(true, tc_kernel<T, DP, CODE>, dim3(sms), dim3(L::kThreads), L::kBytes, st, mq, mk, mv, a);
 }
 
-bool fits_map(const void* p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | static_cast<uintptr_t>(stride * 2)) % 16 == 0; }
+template <typename T, int CODE>
+cudaError_t launch_dim(const Args& a, int sms, cudaStream_t st) {
+  return a.dim <= 64 ? launch<T, 64, CODE>(a, sms, st) : launch<T, 128, CODE>(a, sms, st);
+}
+
+template <typename T>
+cudaError_t launch_for(const Args& a, int code_type, int sms, cudaStream_t st) {
+  if (code_type == KL_CODE_E4M3) return launch_dim<T, KL_CODE_E4M3>(a, sms, st);
+  if (code_type == KL_CODE_INT8) return launch_dim<T, KL_CODE_INT8>(a, sms, st);
+  return launch_dim<T, KL_CODE_NONE>(a, sms, st);
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 }  // namespace
 
@@ -944,12 +1120,15 @@ static int box_rows_of(int page_size) {
 }
 
 bool tc_fits(const Args& a, int dtype, int code_type) {
-  if (dtype == KL_FLOAT32 || code_type != KL_CODE_NONE) return false;
-  if (a.dim % 8 != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
-  const auto stride_ok = [](int64_t stride, int64_t extent) { return extent == 1 || (stride > 0 && stride % 8 == 0 && stride < (int64_t(1) << 38)); };
-  return fits_map(a.q, 0) && fits_map(a.k, 0) && fits_map(a.v, 0) && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 &&
-         stride_ok(a.q_stride, a.tokens) && stride_ok(a.head_stride, a.hkv) && stride_ok(a.token_stride, a.page_size) &&
-         stride_ok(a.page_stride, a.num_pages) && a.num_pages < INT_MAX;
+  if (dtype == KL_FLOAT32) return false;
+  const int unit = code_type == KL_CODE_NONE ? 8 : 16;  // elements of a cache in 16 bytes
+  if (a.dim % unit != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
+  const auto stride_ok = [](int64_t stride, int64_t extent, int u) {
+    return extent == 1 || (stride > 0 && stride % u == 0 && stride < (int64_t(1) << 38));
+  };
+  return aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 &&
+         stride_ok(a.q_stride, a.tokens, 8) && stride_ok(a.head_stride, a.hkv, unit) && stride_ok(a.token_stride, a.page_size, unit) &&
+         stride_ok(a.page_stride, a.num_pages, unit) && a.num_pages < INT_MAX;
 }
 
 size_t tc_partial_bytes(int head_dim, int sms) {
@@ -964,8 +1143,8 @@ cudaError_t launch_tc(Args a, int dtype, int code_type, int sms, cudaStream_t st
   a.tile_tokens = 128 / a.group;
   a.box_rows = box_rows_of(a.page_size);
   while ((1 << a.box_shift) < a.box_rows) ++a.box_shift;
-  if (dtype == KL_FLOAT16) return a.dim <= 64 ? launch<__half, 64>(a, sms, st) : launch<__half, 128>(a, sms, st);
-  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, sms, st) : launch<__nv_bfloat16, 128>(a, sms, st);
+  if (dtype == KL_FLOAT16) return launch_for<__half>(a, code_type, sms, st);
+  return launch_for<__nv_bfloat16>(a, code_type, sms, st);
 }
 
 }  // namespace chunk_attention
