@@ -33,6 +33,11 @@ struct Args {
   int tile_tokens;     // tokens of a 128-row tile
   int box_rows;        // token rows of a TMA box, a power of two: 1 << box_shift
   int box_shift;
+  // A 16-bit tile in shared memory: groups of 8 tokens group_bytes apart, a row's 128-byte halves half_bytes apart. With
+  // `merged` a TMA box has both halves: its coordinates are head * head_halves in halves and
+  // page * page_groups + head * head_groups + token / 8 in groups, total_groups (and more) giving zeros.
+  uint32_t group_bytes, half_bytes;
+  int merged, head_halves, head_groups, page_groups, total_groups;
   float* partials;     // pieces of split row blocks
   uint32_t* counters;  // arrivals at a split block's rows
 };

@@ -17,8 +17,8 @@
 // cut leaves pieces (O in fp32, maximum, sum) in scratch; of each 32 rows the warp that arrives last joins them in
 // the pieces' order.
 //
-// What is masked does not count whatever it holds: scores are replaced, not added to; two warps clear the V rows
-// past the sequence's end and look for infinities and NaN in rows that some row of the block does not see, in which
+// What is masked does not count whatever it holds: scores are replaced, not added to; a warp clears the V rows
+// past the sequence's end and looks for infinities and NaN in rows that some row of the block does not see, in which
 // case the softmax threads add that unit's P V themselves, key by key.
 #include <cuda.h>
 
@@ -35,16 +35,20 @@ namespace chunk_attention {
 namespace {
 
 constexpr int kBN = 128;                 // keys of a unit
-constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 10, kWidenWarp = 12;
+constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 11, kWidenWarp = 12;
+constexpr int kByFma = 3;                // of 8 exponentials, those on the multiply-add pipes
 constexpr float kLazy = 8.0f;            // log2 by which a maximum may be passed before O is rescaled
 constexpr uint64_t kWaitCycles = 2000000000ull;  // about one second
-constexpr int kFixSlots = 4, kBadSlots = 8;
+// Units whose marks are told apart. A tile passes over the special units that it has no part in: that no wait of it is a phase
+// off takes slots for more units than the ring holds.
+constexpr uint32_t kOddScales = 1u << 16;  // beside the bits of the unit's bad boxes
+constexpr int kFixSlots = 8, kBadSlots = 8;
 constexpr int kCountersPerCta = 8;       // a counter for each warp's 32 rows of the two tiles
 
 template <int DP, int CODE>
 struct Layout {
   static constexpr bool kCoded = CODE != KL_CODE_NONE;
-  // Two softmax warpgroups; load, products, two warps on V; over an 8-bit cache four warps that widen its codes.
+  // Two softmax warpgroups; load, each tile's products, V; over an 8-bit cache four warps that widen its codes.
   static constexpr int kThreads = kCoded ? 512 : 384;
   // Registers: 256 * 192 + 256 * 64 = 512 * 128, 256 * 208 + 128 * 88 = 384 * 168, the launch's.
   static constexpr int kSoftmaxRegs = kCoded ? 192 : 208, kOtherRegs = kCoded ? 64 : 88;
@@ -57,21 +61,21 @@ struct Layout {
   static constexpr uint32_t kRing = 2 * kTile;              // Q's two tiles first
   static constexpr uint32_t kRaw = kRing + kStages * kTile;
   static constexpr uint32_t kBars = kRaw + kRawStages * kRawTile;
-  static constexpr uint32_t kWords = kBars + 320;           // ints
+  static constexpr uint32_t kWords = kBars + 384;           // ints
   static constexpr uint32_t kScales = kWords + 256;         // [kBadSlots][K, V][16]: a scale for every 8 keys
   static constexpr uint32_t kBytes = kScales + (kCoded ? 1024 : 0) + 1024;  // slack to align the base to 1024 bytes
   // Barriers of the rings.
-  static constexpr int kFull = 14, kEmpty = kFull + kStages, kRawFull = kEmpty + kStages, kRawEmpty = kRawFull + kRawStages;
+  static constexpr int kFull = 24, kEmpty = kFull + kStages, kRawFull = kEmpty + kStages, kRawEmpty = kRawFull + kRawStages;
   static constexpr int kBarCount = kRawEmpty + kRawStages;
-  static_assert(kBarCount * 8 <= 320 && kBytes <= 232448, "shared memory");
+  static_assert(kBarCount * 8 <= 384 && kBytes <= 232448, "shared memory");
 };
 
 // Barriers, 8 bytes each from Layout::kBars on.
-enum Bar { kQFull0, kQFull1, kQEmpty, kSFull0, kSFull1, kPReady0, kPReady1, kOFull0, kOFull1, kDrain, kFix0, kFixEnd = kFix0 + kFixSlots };
-static_assert(kFixEnd == 14, "the rings' barriers follow");
+enum Bar { kQFull0, kQFull1, kQEmpty0, kQEmpty1, kSFull0, kSFull1, kPReady0, kPReady1, kPRest0, kPRest1, kOFull0, kOFull1, kDrain0, kDrain1, kTurn0, kTurn1, kFix0, kFixEnd = kFix0 + kFixSlots };
+static_assert(kFixEnd == 24, "the rings' barriers follow");
 
 // Words from Layout::kWords on.
-enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kTotalLo, kTotalHi, kVFlag, kBad = kVFlag + 2 * kFixSlots, kScan = kBad + kBadSlots };
+enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kStartHead, kStartBlock, kStartUnit, kVFlag, kBad = kVFlag + kFixSlots, kScan = kBad + kBadSlots };
 
 struct Smem {
   uint32_t base;        // shared address
@@ -149,37 +153,16 @@ struct Walk {
   int b, h, blk, j, nb;
   int64_t u, u1;
 
-  // By a whole warp. Run c of `runs` of the total units begins at total * c / runs.
-  __device__ void init(const Args& a, const Smem& sm, int lane, int64_t u_first, int64_t u_end) {
+  // At the place that find_start left.
+  __device__ void init(const Args& a, const Smem& sm, int64_t u_first, int64_t u_end) {
     u = u_first;
     u1 = u_end;
     b = sm.words[kStartSeq];
-    int64_t off = static_cast<int64_t>(static_cast<uint32_t>(sm.words[kStartLo])) | (static_cast<int64_t>(sm.words[kStartHi]) << 32);
+    h = sm.words[kStartHead];
+    blk = sm.words[kStartBlock];
+    j = sm.words[kStartUnit];
     s = read_seq(a, b, false);
     nb = blocks_of(a, s);
-    const int64_t per_head = head_units(a, s);
-    h = static_cast<int>(off / per_head);
-    off -= h * per_head;
-    blk = 0;
-    for (;;) {  // 32 blocks at a time
-      const int k = blk + lane;
-      int inc = k < nb ? block_units(a, s, k) : 0;
-#pragma unroll
-      for (int m = 1; m < 32; m <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, inc, m);
-        if (lane >= m) inc += y;
-      }
-      const int passed = __popc(__ballot_sync(0xffffffffu, inc <= off && k < nb));
-      if (passed < 32 || blk + 32 >= nb) {
-        const int before = __shfl_sync(0xffffffffu, inc, max(0, passed - 1));
-        if (passed > 0) off -= before;
-        blk += passed;
-        break;
-      }
-      off -= __shfl_sync(0xffffffffu, inc, 31);
-      blk += 32;
-    }
-    j = static_cast<int>(off);
   }
 
   __device__ bool next(const Args& a, Segment& g) {
@@ -205,6 +188,39 @@ struct Walk {
     return true;
   }
 };
+
+// Where unit `off` of sequence b lies, by a whole warp.
+__device__ __forceinline__ void find_start(const Args& a, const Smem& sm, int lane) {
+  const Seq s = read_seq(a, sm.words[kStartSeq], false);
+  int64_t off = static_cast<int64_t>(static_cast<uint32_t>(sm.words[kStartLo])) | (static_cast<int64_t>(sm.words[kStartHi]) << 32);
+  const int64_t per_head = head_units(a, s);
+  const int h = static_cast<int>(off / per_head), nb = blocks_of(a, s);
+  off -= h * per_head;
+  int blk = 0;
+  for (;;) {  // 32 blocks at a time
+    const int k = blk + lane;
+    int inc = k < nb ? block_units(a, s, k) : 0;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, m);
+      if (lane >= m) inc += y;
+    }
+    const int passed = __popc(__ballot_sync(0xffffffffu, inc <= off && k < nb));
+    if (passed < 32 || blk + 32 >= nb) {
+      const int before = __shfl_sync(0xffffffffu, inc, max(0, passed - 1));
+      if (passed > 0) off -= before;
+      blk += passed;
+      break;
+    }
+    off -= __shfl_sync(0xffffffffu, inc, 31);
+    blk += 32;
+  }
+  if (lane == 0) {
+    sm.words[kStartHead] = h;
+    sm.words[kStartBlock] = blk;
+    sm.words[kStartUnit] = static_cast<int>(off);
+  }
+}
 
 // What a block's tile t has to do within a segment: units [j0, end(t)).
 struct Tiles {
@@ -235,6 +251,17 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* map, int x
       : "memory");
 }
 
+// The products are issued by one thread, and a chain of 64-bit shifts before each of them would hold them up: a
+// descriptor's low word moves by the offset in 16-byte units, its high word is a constant.
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4 << 16); }
+// Bytes between groups of 8 rows, version, 128-byte swizzle.
+__device__ __forceinline__ uint32_t desc_hi(uint32_t sbo) { return sbo >> 4 | (1u << 14) | (2u << 29); }
+
 // D[tmem] (+)= A[tmem] . B[smem]; A's row i is lane i, two 16-bit elements a column.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   const uint32_t none = 0u;
@@ -257,14 +284,29 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const float (&r)[8]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 __device__ __forceinline__ uint64_t pair(float lo, float hi) {
@@ -287,6 +329,34 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// 2^x of a pair on the multiply-add pipes, x <= 8 (NaN is not kept): 2^n 2^f with n the nearest whole number, f in [-1/2, 1/2],
+// and 2^f by 1 + c1 f + c2 f^2 + ..., the coefficients of least relative error (by linear programming over [-1/2, 1/2]):
+// 1.02e-4 with three of them (P in bf16, half a step 2^-8), 3.0e-6 with four (fp16, 2^-11). Zero from x = -127 down, exactly.
+template <int DEGREE>
+__device__ __forceinline__ void exp2_pair(uint64_t x2, float& p0, float& p1) {
+  float x0, x1;
+  unpair(x2, x0, x1);
+  const uint64_t x = pair(fmaxf(x0, -127.0f), fmaxf(x1, -127.0f));
+  const uint64_t shifter = pair(12582912.0f, 12582912.0f), back = pair(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
+  const uint64_t n = add2(x, shifter);  // n in the low bits
+  const uint64_t minus = pair(-1.0f, -1.0f);
+  const uint64_t f = fma2(add2(n, back), minus, x);
+  uint64_t y;
+  if (DEGREE == 3) {
+    y = fma2(pair(0.05500893294811249f, 0.05500893294811249f), f, pair(0.2422109693288803f, 0.2422109693288803f));
+    y = fma2(y, f, pair(0.6932829022407532f, 0.6932829022407532f));
+  } else {
+    y = fma2(pair(0.009585382416844368f, 0.009585382416844368f), f, pair(0.05590662732720375f, 0.05590662732720375f));
+    y = fma2(y, f, pair(0.24024038016796112f, 0.24024038016796112f));
+    y = fma2(y, f, pair(0.6931241750717163f, 0.6931241750717163f));
+  }
+  y = fma2(y, f, pair(1.0f, 1.0f));
+  float n0, n1, y0, y1;
+  unpair(n, n0, n1);
+  unpair(y, y0, y1);
+  p0 = __uint_as_float((__float_as_uint(n0) << 23) + __float_as_uint(y0));
+  p1 = __uint_as_float((__float_as_uint(n1) << 23) + __float_as_uint(y1));
 }
 // 32 bytes a lane in one store: a whole sector.
 __device__ __forceinline__ void store32(void* p, const uint32_t (&r)[8]) {
@@ -328,8 +398,8 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
   const int boxes = kBN / a.box_rows;
   const uint32_t box_bytes = a.box_rows * (L::kCoded ? DP : 128u);
   uint32_t slot = 0, phase = 0, issued = 0, unit = 0;
-  uint32_t q_phase = 0;
-  bool ok = true, first_segment = true;
+  uint32_t q_loads = 0;
+  bool ok = true;
   Segment g{};
   // Lane i looks after box i of a unit: its page, num_pages (for zeros) past the sequence's end or where the id is
   // no page's. Ids are asked for two units ahead, scales one.
@@ -351,8 +421,10 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
       const bool bad = lane < boxes && tok < g.s.len && (page < 0 || page >= a.num_pages);
       if (bad) page = a.num_pages;
       const uint32_t bad_boxes = __ballot_sync(0xffffffffu, bad);
+      // Scales that are negative, infinite or NaN.
+      const bool odd = L::kCoded && __any_sync(0xffffffffu, !(ks >= 0.0f && ks < INFINITY && vs >= 0.0f && vs < INFINITY));
       if (lane == 0) {
-        sm.words[kBad + unit % kBadSlots] = static_cast<int>(bad_boxes);
+        sm.words[kBad + unit % kBadSlots] = static_cast<int>(bad_boxes | (odd ? kOddScales : 0u));
         if (bad_boxes) atomicOr(sm.status, kStatusBadPage);
       }
       if constexpr (L::kCoded) {
@@ -375,10 +447,17 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
             tma_load_4d(sm.base + L::kRaw + slot * L::kRawTile + lane * box_bytes, kv ? mv : mk, 0, g.h, tok % a.page_size,
                         static_cast<int>(page), full, keep);
           } else {
+            const uint32_t to = sm.base + L::kRing + slot * L::kTile;
+            if (a.merged) {
+              const int group = page < a.num_pages ? static_cast<int>(page) * a.page_groups + g.h * a.head_groups + tok % a.page_size / 8
+                                                   : a.total_groups;
+              tma_load_4d(to + (lane << a.box_shift >> 3) * a.group_bytes, kv ? mv : mk, 0, 0, g.h * a.head_halves, group, full, keep);
+            } else {
 #pragma unroll
-            for (int c = 0; c < L::kHalves; ++c) {
-              tma_load_4d(sm.base + L::kRing + slot * L::kTile + c * L::kHalf + lane * box_bytes, kv ? mv : mk, c * 64, g.h,
-                          tok % a.page_size, static_cast<int>(page), full, keep);
+              for (int c = 0; c < L::kHalves; ++c) {
+                tma_load_4d(to + c * L::kHalf + lane * box_bytes, kv ? mv : mk, c * 64, g.h, tok % a.page_size, static_cast<int>(page), full,
+                            keep);
+              }
             }
           }
         }
@@ -387,22 +466,21 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
           slot = 0;
           phase ^= 1;
         }
-        if (kv == 0 && j == g.j0) {  // behind the segment's first keys, which need not wait for Q's room
-          if (!first_segment) {
-            ok = wait_for(sm, sm.bar(kQEmpty), q_phase);
-            q_phase ^= 1;
-          }
-          first_segment = false;
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+        if (kv == 0 && j == g.j0) {  // behind the segment's first keys, which need not wait for Q's room; lane t: tile t
           if (lane < 2 && tiles.end[lane] > g.j0) {
-            mbar_arrive_expect_tx(sm.bar(kQFull0 + lane), L::kHalves * a.tile_tokens * a.group * 128u);
+            if (q_loads > 0) ok = wait_for(sm, sm.bar(kQEmpty0 + lane), (q_loads - 1) & 1);
+            ++q_loads;
+            if (ok) {
+              mbar_arrive_expect_tx(sm.bar(kQFull0 + lane), L::kHalves * a.tile_tokens * a.group * 128u);
 #pragma unroll
-            for (int c = 0; c < L::kHalves; ++c) {
-              tma_load_3d(sm.base + lane * L::kTile + c * L::kHalf, mq, c * 64, g.h * a.group, static_cast<int>(g.s.first) + tiles.tok0[lane],
-                          sm.bar(kQFull0 + lane), once);
+              for (int c = 0; c < L::kHalves; ++c) {
+                tma_load_3d(sm.base + lane * L::kTile + c * L::kHalf, mq, c * 64, g.h * a.group, static_cast<int>(g.s.first) + tiles.tok0[lane],
+                            sm.bar(kQFull0 + lane), once);
+              }
             }
           }
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
         }
       }
       page = page1;
@@ -412,6 +490,11 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
     }
   }
   // Nothing may be in flight into this CTA's shared memory when it ends; normally it has long landed.
+  if (lane < 2 && q_loads > 0) {
+    const uint64_t start = clock64();
+    while (!mbar_try_wait(sm.bar(kQFull0 + lane), (q_loads - 1) & 1) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
+    }
+  }
   if (lane == 0) {
     for (uint32_t k = 0; k < min(issued, static_cast<uint32_t>(kDepth)); ++k) {
       const uint32_t i = issued - 1 - k, s = i % kDepth;
@@ -454,7 +537,7 @@ template <typename TO, int DP, int CODE>
 __device__ __forceinline__ void widen_row(uint32_t raw, uint32_t tile, int row) {
   using L = Layout<DP, CODE>;
   constexpr int kUnits = DP / 16;
-#pragma unroll
+#pragma unroll 2
   for (int k = 0; k < kUnits; ++k) {
     const int u = (k + row) & (kUnits - 1);
     const uint4 v = lds128(raw + row * DP + u * 16);
@@ -465,7 +548,7 @@ __device__ __forceinline__ void widen_row(uint32_t raw, uint32_t tile, int row) 
       out[2 * i] = widen_pair<TO, CODE, 0>(in[i]);
       out[2 * i + 1] = widen_pair<TO, CODE, 1>(in[i]);
     }
-    const uint32_t at = tile + (u >> 2) * L::kHalf + row * 128u;
+    const uint32_t at = tile + (u >> 2) * L::kHalf + row * 128u;  // groups of 8 rows 1024 bytes apart, halves kHalf
     const uint32_t c = (2 * u) & 7, s = row & 7;
     sts128(at + ((c ^ s) << 4), make_uint4(out[0], out[1], out[2], out[3]));
     sts128(at + (((c + 1) ^ s) << 4), make_uint4(out[4], out[5], out[6], out[7]));
@@ -506,100 +589,139 @@ __device__ __forceinline__ void widen_role(const Args& a, const Smem& sm, Walk w
   }
 }
 
-// One thread.
+// A value that is the same in all lanes, known to be so: operands of the products live in uniform registers, and moving
+// them there one by one for a lone thread took as long as the products (a unit's 4 products of 128 x 128 x 128: 3500 cycles).
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
+
+// A warp for each tile t; one thread of it issues.
 template <typename T, int DP, int CODE>
-__device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, uint32_t tmem) {
+__device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, int t, uint32_t tmem) {
   using L = Layout<DP, CODE>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   // Over codes P V runs in bf16, whose range holds a probability times any scale.
   constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16 || L::kCoded, 128, DP, true);
   const int ksteps = (a.dim + 15) / 16;
-  uint32_t slot = 0, phase = 0, unit = 0;
-  uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+  const uint32_t sq = uniform(desc_lo(sm.base + t * L::kTile, 16)), ring = uniform(desc_lo(sm.base + L::kRing, 0));
+  const uint32_t hi = desc_hi(a.group_bytes);
+  const uint32_t s_at = uniform(tmem + t * 128), o_at = uniform(tmem + 256 + t * 128);
+  uint32_t slot = 0, phase = 0, unit = 0, q_phase = 0, p_phase = 0, turn = 0;
   bool ok = true;
   Segment g{};
-  auto ring_wait = [&] { ok = ok && wait_for(sm, sm.bar(L::kFull + slot), phase); };
+  auto wait = [&](uint32_t bar, uint32_t parity) {
+    ok = ok && wait_for(sm, bar, parity);
+    ok = __all_sync(0xffffffffu, ok);
+  };
+  auto commit = [&](uint32_t bar) {
+    if (elect_one()) umma_commit(bar);
+  };
+  // Waits for a stage; gives it back when the products issued so far are done.
+  auto ring_wait = [&] { wait(sm.bar(L::kFull + slot), phase); };
   auto ring_next = [&] {
-    umma_commit(sm.bar(L::kEmpty + slot));
+    commit(sm.bar(L::kEmpty + slot));
     if (++slot == L::kStages) {
       slot = 0;
       phase ^= 1;
     }
   };
-  auto scores = [&](int t, uint32_t k_slot) {
-    const uint32_t sq = sm.base + t * L::kTile, sk = sm.base + L::kRing + k_slot * L::kTile;
-    for (int ks = 0; ks < ksteps; ++ks) {
-      const uint32_t off = (ks / 4) * L::kHalf + (ks % 4) * 32u;
-      umma_f16(tmem + t * 128, umma_desc_sw128(sq + off, 16u, 1024u), umma_desc_sw128(sk + off, 16u, 1024u), IDESC_S, ks > 0);
+  // The tiles take turns, unit by unit: two threads' products would share the tensor cores evenly, and both tiles' softmax
+  // would then run at once and wait at once.
+  auto my_turn = [&] {
+    if (t == 1 || turn > 0) wait(sm.bar(kTurn0 + t), (t == 1 ? turn : turn - 1) & 1);
+  };
+  auto scores = [&](uint32_t k_slot) {
+    const uint32_t sk = uniform(ring + k_slot * (L::kTile >> 4) + (1u << 16));
+    if (elect_one()) {
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ++ks) {
+        const uint32_t in_half = (ks % 4) * 32u >> 4;
+        if (ks < ksteps) {
+          umma_f16(s_at, desc_of(sq + ((ks / 4) * L::kHalf >> 4) + in_half, desc_hi(1024)), desc_of(sk + (ks / 4) * (a.half_bytes >> 4) + in_half, hi),
+                   IDESC_S, ks > 0);
+        }
+      }
+      umma_commit(sm.bar(kSFull0 + t));
     }
-    umma_commit(sm.bar(kSFull0 + t));
+    __syncwarp();
   };
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
-    // The first unit's scores.
+    const int end = tiles.end[t];
     ring_wait();
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (!ok || tiles.end[t] <= g.j0) continue;
-      ok = wait_for(sm, sm.bar(kQFull0 + t), q_phase[t]);
-      q_phase[t] ^= 1;
+    if (end > g.j0) {
+      wait(sm.bar(kQFull0 + t), q_phase);
+      q_phase ^= 1;
       if (!ok) break;
       tcgen05_fence_after();
-      scores(t, slot);
+      scores(slot);
+      if (end == g.j0 + 1) commit(sm.bar(kQEmpty0 + t));
     }
     if (!ok) break;
     ring_next();
-    if (g.j1 == g.j0 + 1) umma_commit(sm.bar(kQEmpty));
     for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
+      // V of this unit and K of the next one before P: what follows P is then issued without a pause.
+      const uint32_t v_slot = slot, k_slot = v_slot + 1 == L::kStages ? 0 : v_slot + 1;
+      const bool more_keys = j + 1 < g.j1;
       ring_wait();
-      const uint32_t v_slot = slot;
-      const uint32_t sv = sm.base + L::kRing + v_slot * L::kTile;
-      // V's stage is given back after the last product that reads it, then the next unit's K is in the next stage.
+      if (more_keys) wait(sm.bar(L::kFull + k_slot), k_slot == 0 ? phase ^ 1 : phase);
+      if (j < end) {
+        const uint32_t sv = uniform(ring + v_slot * (L::kTile >> 4) + (a.half_bytes >> 4 << 16)), again = uniform(j > g.j0);
+        const bool special = tiles.special(j);
+        bool by_hand = false;
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (ok && j < tiles.end[t]) {
-          ok = wait_for(sm, sm.bar(kPReady0 + t), p_phase[t]);
-          p_phase[t] ^= 1;
+        for (int half = 0; half < 2; ++half) {
+          wait(sm.bar((half ? kPRest0 : kPReady0) + t), p_phase);
+          if (half == 0) my_turn();
           if (!ok) break;
           tcgen05_fence_after();
-          const bool by_hand = tiles.special(j) && (sm.words[kVFlag + 2 * (unit % kFixSlots)] | sm.words[kVFlag + 2 * (unit % kFixSlots) + 1]);
-          if (!by_hand) {
+          if (half == 0) by_hand = special && sm.words[kVFlag + unit % kFixSlots];
+          if (!by_hand && elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < kBN / 16; ++ks) {
-              umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + ks * 8, umma_desc_sw128(sv + ks * 16u * 128u, L::kHalf, 1024u), IDESC_O,
-                          j > g.j0 || ks > 0);
+            for (int ks = half * kBN / 32; ks < (half + 1) * kBN / 32; ++ks) {
+              umma_f16_ts(o_at, s_at + ks * 8, desc_of(sv + ks * (a.group_bytes >> 3), hi), IDESC_O, ks > 0 ? 1u : again);
             }
           }
-          if (j + 1 == tiles.end[t]) umma_commit(sm.bar(kOFull0 + t));
+          __syncwarp();
         }
-        if (t == 1) ring_next();  // V
-        if (ok && j + 1 < tiles.end[t]) {
-          // The next unit's K: the stage after V's.
-          const uint32_t k_slot = v_slot + 1 == L::kStages ? 0 : v_slot + 1;
-          const uint32_t k_phase = v_slot + 1 == L::kStages ? (t == 1 ? phase : phase ^ 1) : phase;
-          ok = wait_for(sm, sm.bar(L::kFull + k_slot), k_phase);
-          if (!ok) break;
-          tcgen05_fence_after();
-          scores(t, k_slot);
+        p_phase ^= 1;
+        if (!ok) break;
+        if (j + 1 < end) {
+          scores(k_slot);
+          if (j + 2 == end) commit(sm.bar(kQEmpty0 + t));
+        } else {
+          commit(sm.bar(kOFull0 + t));
         }
+      } else {
+        my_turn();
       }
       if (!ok) break;
-      if (j + 1 < g.j1) {
-        ring_next();  // K
-        if (j + 2 == g.j1) umma_commit(sm.bar(kQEmpty));
-      }
+      if (elect_one()) mbar_arrive(sm.bar(kTurn0 + (1 - t)));
+      ++turn;
+      ring_next();  // V and, if there are more keys, K
+      if (more_keys) ring_next();
     }
   }
   // Every product has ended before the CTA does.
-  umma_commit(sm.bar(kDrain));
+  commit(sm.bar(kDrain0 + t));
   const uint64_t start = clock64();
-  while (!mbar_try_wait(sm.bar(kDrain), 0) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
+  while (!mbar_try_wait(sm.bar(kDrain0 + t), 0) && static_cast<uint64_t>(clock64()) - start < kWaitCycles) {
   }
+  __syncwarp();
 }
 
-// Two warps: the V rows of special units.
+// Where half `half` of row `row` lies in a tile.
+__device__ __forceinline__ uint32_t row_at(const Args& a, int row, int half) {
+  return (row >> 3) * a.group_bytes + half * a.half_bytes + (row & 7) * 128u;
+}
+
+// One warp: the V rows of special units.
 template <typename T, int DP, int CODE>
-__device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, int tid) {
+__device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, int lane) {
   using L = Layout<DP, CODE>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value || L::kCoded;
   constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
@@ -616,34 +738,35 @@ __device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, 
         const uint32_t i = 2 * unit + kv;
         slot = i % L::kStages;
         ok = ok && wait_for(sm, sm.bar(L::kFull + slot), (i / L::kStages) & 1);
-        if (kv == 0 && (tid & 31) == 0) mbar_arrive(sm.bar(L::kEmpty + slot));
+        if (kv == 0 && lane == 0) mbar_arrive(sm.bar(L::kEmpty + slot));
       }
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const uint32_t empty = sm.bar(L::kEmpty + slot);
       if (!tiles.special(j)) {
-        if ((tid & 31) == 0) mbar_arrive(empty);
+        if (lane == 0) mbar_arrive(empty);
         continue;
       }
       const uint32_t sv = sm.base + L::kRing + slot * L::kTile;
       const int held = max(0, min(kBN, g.s.len - j * kBN));                            // rows of tokens
       const int boxed = min(kBN, (held + a.box_rows - 1) / a.box_rows * a.box_rows);   // zeros from here on
       const int unseen = max(0, min(held, tiles.seen_first - j * kBN));                // seen by all below
-      for (int k = tid; k < (boxed - held) * L::kHalves * 8; k += 64) {
+      for (int k = lane; k < (boxed - held) * L::kHalves * 8; k += 32) {
         const int row = held + k / (L::kHalves * 8), c = k / 8 % L::kHalves, u = k % 8;
-        sts128(sv + c * L::kHalf + row * 128u + u * 16u, make_uint4(0u, 0u, 0u, 0u));
+        sts128(sv + row_at(a, row, c) + u * 16u, make_uint4(0u, 0u, 0u, 0u));
       }
       uint32_t odd = 0;
-      for (int k = tid; k < (held - unseen) * L::kHalves * 8; k += 64) {
+      for (int k = lane; k < (held - unseen) * L::kHalves * 8; k += 32) {
         const int row = unseen + k / (L::kHalves * 8), c = k / 8 % L::kHalves, u = k % 8;
-        const uint4 v = lds128(sv + c * L::kHalf + row * 128u + u * 16u);
+        const uint4 v = lds128(sv + row_at(a, row, c) + u * 16u);
         odd |= ((v.x & kExp) + kOne) | ((v.y & kExp) + kOne) | ((v.z & kExp) + kOne) | ((v.w & kExp) + kOne);
       }
       odd = __any_sync(0xffffffffu, (odd & 0x80008000u) != 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if ((tid & 31) == 0) {
-        sm.words[kVFlag + 2 * (unit % kFixSlots) + (tid >> 5)] = static_cast<int>(odd);
+      if (lane == 0) {
+        // Scales that are no numbers are taken by hand, too: a masked probability times one would be NaN.
+        sm.words[kVFlag + unit % kFixSlots] = static_cast<int>(odd | (static_cast<uint32_t>(sm.words[kBad + unit % kBadSlots]) & kOddScales));
         mbar_arrive(sm.bar(kFix0 + unit % kFixSlots));
         mbar_arrive(empty);
       }
@@ -683,50 +806,55 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tcgen05_fence_after();
-      uint32_t sr[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, sr[c]);
-      const uint32_t bad = static_cast<uint32_t>(sm.words[kBad + u % kBadSlots]);
-      tmem_wait_ld();
+      const uint32_t marks = static_cast<uint32_t>(sm.words[kBad + u % kBadSlots]);
       const int cols = limit - j * kBN;  // columns that this row sees
-      const float4* const scales = reinterpret_cast<const float4*>(sm.ptr + L::kScales) + u % kBadSlots * 8;
-      if constexpr (L::kCoded) {  // in units of log2 from here on
+      const float* const scales = reinterpret_cast<const float*>(sm.ptr + L::kScales) + u % kBadSlots * 32;
+      const bool plain = !special && marks == 0;
+      if (!plain) {
+        // S is put back as scaled, and -inf where masked: what follows need not ask.
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t s[32];
+          tmem_ld32(tS + c, s);
+          tmem_wait_ld();
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f4 = scales[q];
-          const float f[4] = {f4.x, f4.y, f4.z, f4.w};
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float x0, x1;
-            unpair(mul2(pair(__uint_as_float(sr[q][c]), __uint_as_float(sr[q][c + 1])), pair(f[c / 8], f[c / 8])), x0, x1);
-            sr[q][c] = __float_as_uint(x0);
-            sr[q][c + 1] = __float_as_uint(x1);
+          for (int i = 0; i < 32; ++i) {
+            if (L::kCoded) s[i] = __float_as_uint(__uint_as_float(s[i]) * scales[(c + i) / 8]);
+            if (c + i >= cols || (marks >> ((c + i) >> a.box_shift) & 1u)) s[i] = 0xff800000u;
           }
+          tmem_st32(tS + c, s);
         }
+        tmem_wait_st();
       }
-      if (special || bad) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          const bool seen = c < cols && !(bad >> (c >> a.box_shift) & 1u);
-          if (!seen) sr[c / 32][c % 32] = 0xff800000u;  // -inf
-        }
-      }
+      // The row's maximum, 32 columns at a time, the next ones on their way.
+      // The row's maximum. Rolled loops here and below: longer code would not stay in the instruction caches.
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 64) {
+        uint32_t s[2][32];
+        tmem_ld32(tS + c, s[0]);
+        tmem_ld32(tS + c + 32, s[1]);
+        tmem_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 128; c += 8) {
+        for (int q = 0; q < 8; ++q) {
+          float top = L::kCoded ? -INFINITY : mx[q & 3];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          mx[k] = max3(mx[k], __uint_as_float(sr[(c + 2 * k) / 32][(c + 2 * k) % 32]), __uint_as_float(sr[(c + 2 * k + 1) / 32][(c + 2 * k + 1) % 32]));
+          for (int i = 0; i < 8; i += 2) {
+            top = max3(top, __uint_as_float(s[q / 4][q % 4 * 8 + i]), __uint_as_float(s[q / 4][q % 4 * 8 + i + 1]));
+          }
+          if constexpr (L::kCoded) top = max3(mx[q & 3], mx[q & 3], top * (plain ? scales[c / 8 + q] : 1.0f));  // no scale is negative here
+          mx[q & 3] = top;
         }
       }
-      const float mc = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * (L::kCoded ? 1.0f : sl);
+      const float mc = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * (L::kCoded ? 1.0f : sl);
       float alpha = 1.0f;
-      if (mc > m + kLazy) {
-        alpha = exp2_approx(m - mc);  // 0 where m is -inf
-        m = mc;
+      if (!(mc <= m + kLazy)) {
+        // 0 where m is -inf. An infinite or NaN score makes the row NaN, by way of m: exp2_pair does not keep NaN.
+        alpha = mc < INFINITY ? exp2_approx(m - mc) : NAN;
+        m = mc < INFINITY ? mc : NAN;
         l *= alpha;
       }
-      if (j > g.j0 && __any_sync(0xffffffffu, alpha < 1.0f)) {
+      if (j > g.j0 && __any_sync(0xffffffffu, !(alpha >= 1.0f))) {
         // S of this unit is complete, and so is O += P V of the one before.
 #pragma unroll 1
         for (int c = 0; c < DP; c += 8) {
@@ -741,39 +869,52 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       const float shift = m == -INFINITY ? 0.0f : m;
       const uint64_t sh2 = pair(-shift, -shift);
       uint64_t sum[2] = {0, 0};
+      // P, 32 columns at a time, over columns of S that have been read; the products with the first 64 keys may begin
+      // before the rest is done.
+      auto put_p = [&](const uint32_t(&s)[16], int c) {
+        uint32_t p[8];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t p[32];
-        float half_scales[8];
-        if constexpr (L::kCoded) {
-          const float4 f0 = scales[4 + 2 * half], f1 = scales[5 + 2 * half];
-          half_scales[0] = f0.x, half_scales[1] = f0.y, half_scales[2] = f0.z, half_scales[3] = f0.w;
-          half_scales[4] = f1.x, half_scales[5] = f1.y, half_scales[6] = f1.z, half_scales[7] = f1.w;
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          uint32_t& s0 = sr[half * 2 + i / 16][(2 * i) % 32];
-          uint32_t& s1 = sr[half * 2 + i / 16][(2 * i + 1) % 32];
+        for (int i = 0; i < 8; ++i) {
+          const uint64_t x2 = pair(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+          float f = 1.0f;
+          if constexpr (L::kCoded) f = plain ? scales[c / 8 + i / 4] : 1.0f;
           float x0, x1;
-          const uint64_t s = pair(__uint_as_float(s0), __uint_as_float(s1));
-          unpair(L::kCoded ? add2(s, sh2) : fma2(s, sl2, sh2), x0, x1);
-          x0 = exp2_approx(x0);
-          x1 = exp2_approx(x1);
-          sum[i & 1] = add2(sum[i & 1], pair(x0, x1));
+          const uint64_t e2 = fma2(x2, L::kCoded ? pair(f, f) : sl2, sh2);
+          if (i * kByFma % 8 < kByFma) {
+            exp2_pair<std::is_same<TV, __half>::value ? 4 : 3>(e2, x0, x1);
+          } else {
+            unpair(e2, x0, x1);
+            x0 = exp2_approx(x0);
+            x1 = exp2_approx(x1);
+          }
+          const uint64_t p2 = pair(x0, x1);
+          sum[i & 1] = add2(sum[i & 1], p2);
           if constexpr (L::kCoded) {
-            const float f = half_scales[i / 4];
-            unpair(mul2(pair(x0, x1), pair(f, f)), x0, x1);
-            if (special) {  // a masked key's scale does not count either
-              if (half * 64 + 2 * i >= cols) x0 = 0.0f;
-              if (half * 64 + 2 * i + 1 >= cols) x1 = 0.0f;
-            }
+            const float v = scales[16 + c / 8 + i / 4];
+            unpair(mul2(p2, pair(v, v)), x0, x1);
           }
           p[i] = Storage<TV>::pack2(x0, x1);
-          s0 = __float_as_uint(x0);
-          s1 = __float_as_uint(x1);
         }
-        tmem_st32(tS + half * 32, p);
+        tmem_st8(tS + c / 2, p);
+      };
+      uint32_t s0[16], s1[16];
+      tmem_ld16(tS, s0);
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        tmem_wait_ld();
+        tmem_ld16(tS + c + 16, s1);
+        put_p(s0, c);
+        tmem_wait_ld();
+        tmem_ld16(tS + (c + 32) % 128, s0);  // the last round's is not used
+        put_p(s1, c + 16);
+        if (c == 32 && !special) {
+          tmem_wait_st();
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sm.bar(kPReady0 + t));
+        }
       }
+      tmem_wait_ld();
       {
         float x0, x1;
         unpair(add2(sum[0], sum[1]), x0, x1);
@@ -784,9 +925,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
         fix_phases ^= 1u << fix;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (sm.words[kVFlag + 2 * fix] | sm.words[kVFlag + 2 * fix + 1]) {
+        if (sm.words[kVFlag + fix]) {
           // Infinities or NaN in rows of V that not every row sees: P V key by key.
           const uint32_t sv = sm.base + L::kRing + (2 * u + 1) % L::kStages * L::kTile;
+          tmem_wait_st();
 #pragma unroll 1
           for (int c8 = 0; c8 < DP / 8; ++c8) {
             float o[8];
@@ -794,18 +936,26 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
             tmem_wait_ld();
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = j > g.j0 ? o[i] : 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < kBN; c0 += 16) {
+              float pp[8];  // 16 keys' probabilities, in pairs
+              tmem_ld8(tS + c0 / 2, pp);
+              tmem_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 128; ++c) {
-              const uint4 v = lds128(sv + (c8 / 8) * L::kHalf + c * 128u + static_cast<uint32_t>(((c8 & 7) ^ (c & 7)) * 16));
-              const bool seen = c < cols && !(bad >> (c >> a.box_shift) & 1u);
-              const float p = __uint_as_float(sr[c / 32][c % 32]);
-              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+              for (int k = 0; k < 16; ++k) {
+                const int c = c0 + k;
+                const uint4 v = lds128(sv + row_at(a, c, c8 / 8) + static_cast<uint32_t>(((c8 & 7) ^ (c & 7)) * 16));
+                const bool seen = c < cols && !(marks >> (c >> a.box_shift) & 1u);
+                const float2 p2 = Storage<TV>::unpack2(__float_as_uint(pp[k / 2]));
+                const float p = k & 1 ? p2.y : p2.x;
+                const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 f = Storage<TV>::unpack2(vw[i]);
-                if (seen) {
-                  o[2 * i] = fmaf(p, f.x, o[2 * i]);
-                  o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) {
+                  const float2 f = Storage<TV>::unpack2(vw[i]);
+                  if (seen) {
+                    o[2 * i] = fmaf(p, f.x, o[2 * i]);
+                    o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1]);
+                  }
                 }
               }
             }
@@ -816,7 +966,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       tmem_wait_st();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(sm.bar(kPReady0 + t));
+      if (lane == 0) {
+        if (special) mbar_arrive(sm.bar(kPReady0 + t));
+        mbar_arrive(sm.bar(kPRest0 + t));
+      }
     }
     unit += g.j1 - g.j0;
     if (!ok) break;
@@ -941,11 +1094,10 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
 
   if (tid == 0) {
     for (int i = 0; i < L::kBarCount; ++i) {
-      // P by a tile's four warps, special units by two; a stage is filled by TMA or the four widening warps and given
-      // back by the products that read it and the two warps on V, which follow every one.
+      // P comes from a tile's four warps; a stage is filled by TMA or the four widening warps and given back by both
+      // tiles' products and by the warp on V, which follows every one.
       int count = 1;
-      if (i == kPReady0 || i == kPReady1) count = 4;
-      if (i >= kFix0 && i < kFixEnd) count = 2;
+      if (i >= kPReady0 && i <= kPRest1) count = 4;
       if (i >= L::kFull && i < L::kEmpty) count = L::kCoded ? 4 : 1;
       if (i >= L::kEmpty && i < L::kRawFull) count = 3;
       if (i >= L::kRawEmpty) count = 4;
@@ -1012,10 +1164,12 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
     }
   }
   __syncthreads();
+  if (busy && warp == 0) find_start(a, sm, lane);
+  __syncthreads();
   const uint32_t tmem = static_cast<uint32_t>(sm.words[kTmem]);
   if (busy) {
     Walk w;
-    w.init(a, sm, lane, u0, u1);
+    w.init(a, sm, u0, u1);
     if (warp < 8) {
       more_registers<L::kSoftmaxRegs>();
       softmax_role<T, DP, CODE>(a, sm, w, plan, warp >> 2, warp & 3, lane, tmem);
@@ -1023,11 +1177,10 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
       fewer_registers<L::kOtherRegs>();
       if (warp == kLoadWarp) {
         load_role<T, DP, CODE>(a, sm, w, lane, &mq, &mk, &mv);
-      } else if (warp == kMmaWarp) {
-        if (lane == 0) mma_role<T, DP, CODE>(a, sm, w, tmem);
-        __syncwarp();
+      } else if (warp < kFixWarp) {
+        mma_role<T, DP, CODE>(a, sm, w, warp - kMmaWarp, tmem);
       } else if (warp < kWidenWarp) {
-        fix_role<T, DP, CODE>(a, sm, w, tid - kFixWarp * 32);
+        fix_role<T, DP, CODE>(a, sm, w, lane);
       } else if constexpr (L::kCoded) {
         widen_role<T, DP, CODE>(a, sm, w, tid - kWidenWarp * 32);
       }
@@ -1081,16 +1234,29 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
     }
   }
   for (int i = 0; i < 2; ++i) {
-    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hkv), static_cast<cuuint64_t>(a.page_size),
-                                static_cast<cuuint64_t>(a.num_pages)};
+    void* const base = const_cast<void*>(i ? a.v : a.k);
     constexpr int size = L::kCoded ? 1 : 2;
-    const cuuint64_t strides[3] = {stride_bytes(a.head_stride, a.hkv, size), stride_bytes(a.token_stride, a.page_size, size),
-                                   stride_bytes(a.page_stride, a.num_pages, size)};
-    const cuuint32_t box[4] = {L::kCoded ? DP : 64, 1, static_cast<cuuint32_t>(a.box_rows), 1};
-    if (enc(i ? &mv : &mk, L::kCoded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, 4, const_cast<void*>(i ? a.v : a.k), dims, strides, box, ones,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, L::kCoded ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
-      return cudaErrorInvalidValue;
+    CUtensorMap* const map = i ? &mv : &mk;
+    CUresult r;
+    if (a.merged) {
+      const cuuint64_t token = stride_bytes(a.token_stride, 0, size);
+      const cuuint64_t dims[4] = {64, 8, static_cast<cuuint64_t>(a.head_halves ? a.hkv * L::kHalves : L::kHalves),
+                                  static_cast<cuuint64_t>(a.total_groups)};
+      const cuuint64_t strides[3] = {token, 128, 8 * token};
+      const cuuint32_t box[4] = {64, 8, L::kHalves, static_cast<cuuint32_t>(a.box_rows / 8)};
+      r = enc(map, type, 4, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    } else {
+      const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(a.hkv), static_cast<cuuint64_t>(a.page_size),
+                                  static_cast<cuuint64_t>(a.num_pages)};
+      const cuuint64_t strides[3] = {stride_bytes(a.head_stride, a.hkv, size), stride_bytes(a.token_stride, a.page_size, size),
+                                     stride_bytes(a.page_stride, a.num_pages, size)};
+      const cuuint32_t box[4] = {L::kCoded ? DP : 64, 1, static_cast<cuuint32_t>(a.box_rows), 1};
+      r = enc(map, L::kCoded ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : type, 4, base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              L::kCoded ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     }
+    if (r != CUDA_SUCCESS) return cudaErrorInvalidValue;
   }
   const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, DP, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes);
   if (e != cudaSuccess) return e;
@@ -1119,10 +1285,34 @@ static int box_rows_of(int page_size) {
   return std::min(r, kBN);
 }
 
+// One TMA box for both halves of a row, where head_dim is whole halves and the strides let a head and a page be found
+// by halves and groups of 8 tokens; else a box a half. A box takes its warp about 90 cycles to issue, and with pages of
+// 16 tokens 32 of them a unit took longer than the unit's products.
+static void place_tiles(Args& a, int code_type) {
+  const int halves = a.dim <= 64 ? 1 : 2;
+  a.group_bytes = 1024;
+  a.half_bytes = 128 * 128;
+  if (code_type != KL_CODE_NONE || a.dim != 64 * halves) return;
+  const int64_t group = 8 * a.token_stride;
+  const int64_t page = a.num_pages == 1 ? 0 : a.page_stride, head = a.hkv == 1 ? 0 : a.head_stride;
+  if (group <= 0 || page % group != 0) return;
+  const bool in_row = head == 64 * halves;  // heads of a token side by side
+  if (!in_row && head % group != 0) return;
+  const int64_t total = (a.num_pages - 1) * (page / group) + (in_row ? 0 : (a.hkv - 1) * (head / group)) + a.page_size / 8;
+  if (total >= INT_MAX) return;
+  a.merged = 1;
+  a.head_halves = in_row ? halves : 0;
+  a.head_groups = in_row ? 0 : static_cast<int>(head / group);
+  a.page_groups = static_cast<int>(page / group);
+  a.total_groups = static_cast<int>(total);
+  a.group_bytes = halves * 1024;
+  a.half_bytes = 1024;
+}
+
 bool tc_fits(const Args& a, int dtype, int code_type) {
   if (dtype == KL_FLOAT32) return false;
   const int unit = code_type == KL_CODE_NONE ? 8 : 16;  // elements of a cache in 16 bytes
-  if (a.dim % unit != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
+  if (a.dim % 8 != 0 || a.dim % unit != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
   const auto stride_ok = [](int64_t stride, int64_t extent, int u) {
     return extent == 1 || (stride > 0 && stride % u == 0 && stride < (int64_t(1) << 38));
   };
@@ -1143,6 +1333,7 @@ cudaError_t launch_tc(Args a, int dtype, int code_type, int sms, cudaStream_t st
   a.tile_tokens = 128 / a.group;
   a.box_rows = box_rows_of(a.page_size);
   while ((1 << a.box_shift) < a.box_rows) ++a.box_shift;
+  place_tiles(a, code_type);
   if (dtype == KL_FLOAT16) return launch_for<__half>(a, code_type, sms, st);
   return launch_for<__nv_bfloat16>(a, code_type, sms, st);
 }
