@@ -31,6 +31,7 @@ struct Args {
   uint32_t* status;
   // Tensor-core kernel:
   int tile_tokens;     // tokens of a 128-row tile
+  int block_tokens;    // of a block of one or two tiles
   int box_rows;        // token rows of a TMA box, a power of two: 1 << box_shift
   int box_shift;
   // A 16-bit tile in shared memory: groups of 8 tokens group_bytes apart, a row's 128-byte halves half_bytes apart. With

@@ -1,7 +1,7 @@
-// Chunk attention on the 5th-generation tensor cores: fp16 and bf16, head_dim up to 128, pages of a multiple of
+// Chunk attention on the 5th-generation tensor cores: fp16, bf16 and 8-bit caches, head_dim up to 256, pages of a multiple of
 // 8 tokens, groups of up to 128 query heads.
 //
-// Rows are the (token, query head) pairs of one KV head, 128 a tile (128 / group tokens), two tiles a block. A
+// Rows are the (token, query head) pairs of one KV head, 128 a tile (128 / group tokens), two tiles a block (one for head_dim above 128). A
 // unit of work is a block and 128 of its keys:
 //   S_t = Q_t K^T (M = 128 rows, N = 128 keys) into tensor memory, by one thread, for the tiles t = 0, 1;
 //   a warpgroup a tile, one thread a row: the row's maximum, P_t = exp2(S_t - max) back into tensor memory over
@@ -45,6 +45,9 @@ constexpr uint32_t kOddScales = 1u << 16;  // beside the bits of the unit's bad 
 constexpr int kFixSlots = 8, kBadSlots = 8;
 constexpr int kCountersPerCta = 8;       // a counter for each warp's 32 rows of the two tiles
 
+// Tiles of a block: S and O of one take 128 + DP of the 512 columns of tensor memory.
+__host__ __device__ constexpr int tiles_of(int dp) { return dp == 256 ? 1 : 2; }
+
 template <int DP, int CODE>
 struct Layout {
   static constexpr bool kCoded = CODE != KL_CODE_NONE;
@@ -52,13 +55,14 @@ struct Layout {
   static constexpr int kThreads = kCoded ? 512 : 384;
   // Registers: 256 * 192 + 256 * 64 = 512 * 128, 256 * 208 + 128 * 88 = 384 * 168, the launch's.
   static constexpr int kSoftmaxRegs = kCoded ? 192 : 208, kOtherRegs = kCoded ? 64 : 88;
+  static constexpr int kTiles = tiles_of(DP);
   static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a 16-bit row
   static constexpr uint32_t kHalf = 128u * 128u;            // 128 rows of one
   static constexpr uint32_t kTile = kHalves * kHalf;
-  static constexpr int kStages = kCoded ? (DP == 128 ? 3 : 4) : (DP == 128 ? 5 : 8);
-  static constexpr int kRawStages = kCoded ? (DP == 128 ? 4 : 6) : 0;
+  static constexpr int kStages = DP == 256 ? 2 : kCoded ? (DP == 128 ? 3 : 4) : (DP == 128 ? 5 : 8);
+  static constexpr int kRawStages = !kCoded ? 0 : DP == 256 ? 1 : DP == 128 ? 4 : 6;
   static constexpr uint32_t kRawTile = 128u * DP;           // codes, a row after the other
-  static constexpr uint32_t kRing = 2 * kTile;              // Q's two tiles first
+  static constexpr uint32_t kRing = kTiles * kTile;         // Q's tiles first
   static constexpr uint32_t kRaw = kRing + kStages * kTile;
   static constexpr uint32_t kBars = kRaw + kRawStages * kRawTile;
   static constexpr uint32_t kWords = kBars + 384;           // ints
@@ -75,7 +79,7 @@ enum Bar { kQFull0, kQFull1, kQEmpty0, kQEmpty1, kSFull0, kSFull1, kPReady0, kPR
 static_assert(kFixEnd == 24, "the rings' barriers follow");
 
 // Words from Layout::kWords on.
-enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kStartHead, kStartBlock, kStartUnit, kVFlag, kBad = kVFlag + kFixSlots, kScan = kBad + kBadSlots };
+enum Word { kTmem, kDead, kStartSeq, kStartLo, kStartHi, kStartHead, kStartBlock, kStartUnit, kStartFirst, kStartN, kStartLen, kVFlag, kBad = kVFlag + kFixSlots, kScan = kBad + kBadSlots };
 
 struct Smem {
   uint32_t base;        // shared address
@@ -108,11 +112,11 @@ __device__ __forceinline__ bool wait_for(const Smem& sm, uint32_t bar, uint32_t 
 
 // Units of row block k of sequence s: the keys that its last row sees, at least one unit.
 __device__ __forceinline__ int block_units(const Args& a, const Seq& s, int k) {
-  const int rows_end = min(s.n, (k + 1) * 2 * a.tile_tokens);
+  const int rows_end = min(s.n, (k + 1) * a.block_tokens);
   return max(1, (keys_of(a, s, rows_end - 1) + kBN - 1) / kBN);
 }
 
-__device__ __forceinline__ int blocks_of(const Args& a, const Seq& s) { return (s.n + 2 * a.tile_tokens - 1) / (2 * a.tile_tokens); }
+__device__ __forceinline__ int blocks_of(const Args& a, const Seq& s) { return (s.n + a.block_tokens - 1) / a.block_tokens; }
 
 // The same summed over a sequence's blocks. Causal, all but the last block, step = tokens of a block:
 //   max(1, ceil((base + (k + 1) step) / 128)), base = len - n,
@@ -122,7 +126,7 @@ __device__ __forceinline__ int64_t head_units(const Args& a, const Seq& s) {
   const int nb = blocks_of(a, s);
   if (nb == 0) return 0;
   if (!a.causal) return static_cast<int64_t>(nb) * max(1, (s.len + kBN - 1) / kBN);
-  const int step = 2 * a.tile_tokens, base = s.len - s.n;
+  const int step = a.block_tokens, base = s.len - s.n;
   int64_t total = max(1, (s.len + kBN - 1) / kBN);
   const int ones = min(nb - 1, base <= kBN - step ? (kBN - base) / step : 0);
   const int64_t m = nb - 1 - ones;
@@ -148,6 +152,10 @@ struct Segment {
   int64_t first;   // number of the block's first unit
 };
 
+__device__ __forceinline__ Seq start_seq(const Smem& sm) {
+  return Seq{sm.words[kStartFirst], sm.words[kStartN], sm.words[kStartLen]};
+}
+
 struct Walk {
   Seq s;
   int b, h, blk, j, nb;
@@ -161,7 +169,7 @@ struct Walk {
     h = sm.words[kStartHead];
     blk = sm.words[kStartBlock];
     j = sm.words[kStartUnit];
-    s = read_seq(a, b, false);
+    s = start_seq(sm);
     nb = blocks_of(a, s);
   }
 
@@ -191,7 +199,7 @@ struct Walk {
 
 // Where unit `off` of sequence b lies, by a whole warp.
 __device__ __forceinline__ void find_start(const Args& a, const Smem& sm, int lane) {
-  const Seq s = read_seq(a, sm.words[kStartSeq], false);
+  const Seq s = start_seq(sm);
   int64_t off = static_cast<int64_t>(static_cast<uint32_t>(sm.words[kStartLo])) | (static_cast<int64_t>(sm.words[kStartHi]) << 32);
   const int64_t per_head = head_units(a, s);
   const int h = static_cast<int>(off / per_head), nb = blocks_of(a, s);
@@ -224,18 +232,20 @@ __device__ __forceinline__ void find_start(const Args& a, const Smem& sm, int la
 
 // What a block's tile t has to do within a segment: units [j0, end(t)).
 struct Tiles {
-  int tok0[2];     // first token of the tile
-  int end[2];      // end of its units in the segment
+  int tok0_, end0, end1;
+  int step;        // tokens of a tile
   int seen_first;  // keys that the block's first row sees
-  __device__ Tiles(const Args& a, const Segment& g) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      tok0[t] = (2 * g.blk + t) * a.tile_tokens;
-      int nt = 0;
-      if (tok0[t] < g.s.n) nt = max(1, (keys_of(a, g.s, min(g.s.n, tok0[t] + a.tile_tokens) - 1) + kBN - 1) / kBN);
-      end[t] = max(g.j0, min(g.j1, nt));
-    }
-    seen_first = keys_of(a, g.s, tok0[0]);
+  __device__ Tiles(const Args& a, const Segment& g) : tok0_(g.blk * a.block_tokens), step(a.tile_tokens) {
+    end0 = end_of(a, g, 0);
+    end1 = a.block_tokens > step ? end_of(a, g, 1) : g.j0;
+    seen_first = keys_of(a, g.s, tok0_);
+  }
+  __device__ int tok0(int t) const { return tok0_ + t * step; }    // first token of the tile
+  __device__ int end(int t) const { return t ? end1 : end0; }      // end of its units in the segment
+  __device__ int end_of(const Args& a, const Segment& g, int t) const {
+    int nt = 0;
+    if (tok0(t) < g.s.n) nt = max(1, (keys_of(a, g.s, min(g.s.n, tok0(t) + step) - 1) + kBN - 1) / kBN);
+    return max(g.j0, min(g.j1, nt));
   }
   // Units in which some row does not see every key.
   __device__ bool special(int j) const { return (j + 1) * kBN > seen_first; }
@@ -373,10 +383,23 @@ __device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec
 // ----------------------------------------------------------------- pieces of cut blocks
 
 // CTA c's piece of a block that an earlier CTA began lies in slot 2c, of one that it began itself in slot 2c + 1.
-// A slot: for each tile O [DP][128] fp32 (a warp's rows side by side), then maxima [128] and sums [128].
+// A slot: for each tile O [128][DP] fp32, then maxima [128] and sums [128].
 template <int DP>
 __device__ __forceinline__ float* piece_at(const Args& a, int64_t slot, int t) {
-  return a.partials + (slot * 2 + t) * (static_cast<int64_t>(DP) + 2) * 128;
+  return a.partials + (slot * tiles_of(DP) + t) * (static_cast<int64_t>(DP) + 2) * 128;
+}
+
+template <typename V>
+__device__ __forceinline__ V load_cg(const float* p) {
+  V v;
+  if constexpr (sizeof(V) == 16) {
+    const float4 f = __ldcg(reinterpret_cast<const float4*>(p));
+    v.v[0] = f.x, v.v[1] = f.y, v.v[2] = f.z, v.v[3] = f.w;
+  } else {
+    const float2 f = __ldcg(reinterpret_cast<const float2*>(p));
+    v.v[0] = f.x, v.v[1] = f.y;
+  }
+  return v;
 }
 
 // ----------------------------------------------------------------- roles
@@ -410,9 +433,26 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
   auto scale_of = [&](const float* scales, int64_t page) {
     return L::kCoded && page >= 0 && page < a.num_pages ? __ldcg(scales + page * a.scale_stride + g.h) : 0.0f;
   };
+  auto load_q = [&](const Segment& g, const Tiles& tiles) {  // lane t: tile t
+    if (lane < 2 && tiles.end(lane) > g.j0) {
+      if (q_loads > 0) ok = wait_for(sm, sm.bar(kQEmpty0 + lane), (q_loads - 1) & 1);
+      ++q_loads;
+      if (ok) {
+        mbar_arrive_expect_tx(sm.bar(kQFull0 + lane), L::kHalves * a.tile_tokens * a.group * 128u);
+#pragma unroll
+        for (int c = 0; c < L::kHalves; ++c) {
+          tma_load_3d(sm.base + lane * L::kTile + c * L::kHalf, mq, c * 64, g.h * a.group, static_cast<int>(g.s.first) + tiles.tok0(lane),
+                      sm.bar(kQFull0 + lane), once);
+        }
+      }
+    }
+    ok = __all_sync(0xffffffffu, ok);
+  };
+  bool first_segment = true;
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
     int64_t page = page_of(g.j0), page1 = page_of(g.j0 + 1);
+    if (first_segment) load_q(g, tiles);
     float ks = scale_of(a.k_scale, page), vs = scale_of(a.v_scale, page);
     for (int j = g.j0; ok && j < g.j1; ++j, ++unit) {
       const int64_t page2 = page_of(j + 2);
@@ -466,23 +506,11 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
           slot = 0;
           phase ^= 1;
         }
-        if (kv == 0 && j == g.j0) {  // behind the segment's first keys, which need not wait for Q's room; lane t: tile t
-          if (lane < 2 && tiles.end[lane] > g.j0) {
-            if (q_loads > 0) ok = wait_for(sm, sm.bar(kQEmpty0 + lane), (q_loads - 1) & 1);
-            ++q_loads;
-            if (ok) {
-              mbar_arrive_expect_tx(sm.bar(kQFull0 + lane), L::kHalves * a.tile_tokens * a.group * 128u);
-#pragma unroll
-              for (int c = 0; c < L::kHalves; ++c) {
-                tma_load_3d(sm.base + lane * L::kTile + c * L::kHalf, mq, c * 64, g.h * a.group, static_cast<int>(g.s.first) + tiles.tok0[lane],
-                            sm.bar(kQFull0 + lane), once);
-              }
-            }
-          }
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-        }
+        // Later segments' Q behind their first keys, which need not wait for its room.
+        if (kv == 0 && j == g.j0 && !first_segment) load_q(g, tiles);
+        if (!ok) break;
       }
+      first_segment = false;
       page = page1;
       page1 = page2;
       ks = ks1;
@@ -651,7 +679,7 @@ __device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, 
   };
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
-    const int end = tiles.end[t];
+    const int end = tiles.end(t);
     ring_wait();
     if (end > g.j0) {
       wait(sm.bar(kQFull0 + t), q_phase);
@@ -790,14 +818,14 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
   while (ok && w.next(a, g)) {
     const Tiles tiles(a, g);
     const int tok = row / a.group, head = row - tok * a.group;
-    const bool valid = row < a.tile_tokens * a.group && tiles.tok0[t] + tok < g.s.n;
-    const int limit = valid ? keys_of(a, g.s, tiles.tok0[t] + tok) : 0;
+    const bool valid = row < a.tile_tokens * a.group && tiles.tok0(t) + tok < g.s.n;
+    const int limit = valid ? keys_of(a, g.s, tiles.tok0(t) + tok) : 0;
     float m = -INFINITY, l = 0.0f;
     uint32_t u = unit;
     for (int j = g.j0; j < g.j1; ++j, ++u) {
       const bool special = tiles.special(j);
       const uint32_t fix = u % kFixSlots;
-      if (j >= tiles.end[t]) {  // the other tile's units: only the count of special ones goes on
+      if (j >= tiles.end(t)) {  // the other tile's units: only the count of special ones goes on
         if (special) fix_phases ^= 1u << fix;
         continue;
       }
@@ -975,7 +1003,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
     if (!ok) break;
 
     // ---- the segment's rows: final, or a piece of a cut block
-    const bool active = tiles.end[t] > g.j0;
+    const bool active = tiles.end(t) > g.j0;
     if (active) {
       ok = wait_for(sm, sm.bar(kOFull0 + t), o_phase);
       o_phase ^= 1;
@@ -983,51 +1011,44 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       if (!ok) break;
       tcgen05_fence_after();
     }
-    if (tiles.tok0[t] >= g.s.n) continue;  // no rows in this tile, in any piece
-    T* const out = static_cast<T*>(a.out) + ((g.s.first + tiles.tok0[t] + tok) * a.hq + g.h * a.group + head) * static_cast<int64_t>(a.dim);
-    const bool wide = a.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
-    auto put = [&](int c, const float (&o)[32], float inv) {  // columns c .. c + 31
-      if (wide) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 16) {
-          if (c + i >= a.dim) break;
-          uint32_t r[8];
-#pragma unroll
-          for (int k = 0; k < 8; ++k) r[k] = Storage<T>::pack2(o[i + 2 * k] * inv, o[i + 2 * k + 1] * inv);
-          store32(out + c + i, r);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {  // head_dim is a multiple of 8, out 4-byte aligned
-          if (c + i < a.dim) *reinterpret_cast<uint32_t*>(out + c + i) = Storage<T>::pack2(o[i] * inv, o[i + 1] * inv);
-        }
-      }
-    };
+    if (t >= L::kTiles || tiles.tok0(t) >= g.s.n) continue;  // no rows in this tile, in any piece
+    // Rolled loops: each runs once a segment, and the time of straight code would be that of fetching it.
+    const int64_t out_row = ((g.s.first + tiles.tok0(t) + tok) * a.hq + g.h * a.group + head) * static_cast<int64_t>(a.dim);
     if (g.j0 == 0 && g.j1 == g.nt) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tO + c, o);
+      T* const out = static_cast<T*>(a.out) + out_row;
+      const bool wide = a.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
+#pragma unroll 1
+      for (int c = 0; c < a.dim; c += 16) {
+        uint32_t o[16], r[8];
+        tmem_ld16(tO + c, o);
         tmem_wait_ld();
-        float f[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(o[i]);
-        if (valid) put(c, f, inv);
+        for (int i = 0; i < 8; ++i) r[i] = Storage<T>::pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+        if (!valid) continue;
+        if (wide) {
+          store32(out + c, r);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // head_dim is even, out 4-byte aligned
+            if (c + 2 * i < a.dim) *reinterpret_cast<uint32_t*>(out + c + 2 * i) = r[i];
+          }
+        }
       }
       continue;
     }
     const int run0 = plan.run_of(g.first), run1 = plan.run_of(g.first + g.nt - 1), run = static_cast<int>(blockIdx.x);
     float* const mine = piece_at<DP>(a, 2 * static_cast<int64_t>(run) + (run == run0 ? 1 : 0), t);
     if (active) {
-#pragma unroll
-      for (int c = 0; c < DP; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tO + c, o);
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(tO + c, o);
         tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (valid) __stcg(mine + (c + i) * 128 + row, __uint_as_float(o[i]));
+        if (valid) {
+          const uint32_t lo[8] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]}, hi[8] = {o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]};
+          store32(mine + row * DP + c, lo);
+          store32(mine + row * DP + c + 8, hi);
         }
       }
     }
@@ -1042,38 +1063,76 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
     // Last: the pieces' sum, weighted by their maxima, in their order.
     fence_acq_rel_gpu();
     __syncwarp();
-    float top = -INFINITY;
-    for (int r = run0; r <= run1; ++r) {
-      const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + DP * 128 + row;
-      if (__ldcg(pc + 128) != 0.0f) top = fmaxf(top, __ldcg(pc));
-    }
-    float total = 0.0f;
-    for (int r = run0; r <= run1; ++r) {
-      const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + DP * 128 + row;
-      const float pl = __ldcg(pc + 128);
-      if (pl != 0.0f) total += pl * exp2_approx(__ldcg(pc) - top);
+    const int pieces = run1 - run0 + 1, row0 = warp * 32;
+    auto piece = [&](int k) { return piece_at<DP>(a, 2 * static_cast<int64_t>(run0 + k) + (k == 0 ? 1 : 0), t); };
+    float top = -INFINITY, total = 0.0f;  // a lane a row
+#pragma unroll 4
+    for (int k = 0; k < pieces; ++k) {
+      const float* const pc = piece(k) + DP * 128 + row;
+      const float pm = __ldcg(pc), pl = __ldcg(pc + 128);
+      if (pl == 0.0f) continue;  // a piece without a sum has no O
+      const float higher = max3(top, top, pm);
+      total = total * exp2_approx(top - higher) + pl * exp2_approx(pm - higher);
+      top = higher;
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    constexpr int kCols = DP / 32;  // a lane's columns of a row
+    using Vf = Vec<float, kCols < 4 ? kCols : 4>;
+    const int held = __popc(__ballot_sync(0xffffffffu, valid));  // the first rows
 #pragma unroll 1
-    for (int c = 0; c < DP; c += 32) {
-      if (c >= a.dim) break;
-      float o[32];
+    for (int r0 = 0; r0 < held; r0 += 4) {  // four rows of two pieces in flight
+      float acc[4][kCols];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int i = 0; i < kCols; ++i) acc[r][i] = 0.0f;
+      }
 #pragma unroll 1
-      for (int r = run0; r <= run1; ++r) {
-        const float* pc = piece_at<DP>(a, 2 * static_cast<int64_t>(r) + (r == run0 ? 1 : 0), t) + row;
-        const float pl = __ldcg(pc + (DP + 1) * 128);
-        if (valid && pl != 0.0f) {
-          const float f = exp2_approx(__ldcg(pc + DP * 128) - top);
-          float x[32];
+      for (int k0 = 0; k0 < pieces; k0 += 2) {
+        // Lanes 0 to 7 weigh the four rows' two pieces.
+        const int rr = min(31, r0 + (lane >> 1 & 3)), kk = k0 + (lane & 1);
+        const float row_top = __shfl_sync(0xffffffffu, top, rr);
+        float f = 0.0f;
+        if (kk < pieces && lane < 8) {
+          const float* const pc = piece(kk) + DP * 128 + row0 + rr;
+          const float pm = __ldcg(pc), pl = __ldcg(pc + 128);
+          f = pl == 0.0f ? 0.0f : exp2_approx(pm - row_top);
+        }
+        Vf x[4][2][kCols < 4 ? 1 : kCols / 4];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = __ldcg(pc + (c + i) * 128);
+        for (int r = 0; r < 4; ++r) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = fmaf(f, x[i], o[i]);
+          for (int k = 0; k < 2; ++k) {
+            const float* const from = piece(min(k0 + k, pieces - 1)) + (row0 + min(31, r0 + r)) * DP + lane * kCols;
+#pragma unroll
+            for (int i = 0; i < kCols; i += sizeof(Vf) / 4) x[r][k][i * 4 / sizeof(Vf)] = load_cg<Vf>(from + i);
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float fr = __shfl_sync(0xffffffffu, f, 2 * r + k);
+#pragma unroll
+            for (int i = 0; i < kCols; ++i) {
+              const float v = x[r][k][i * 4 / sizeof(Vf)].v[i % (sizeof(Vf) / 4)];
+              acc[r][i] = fr == 0.0f ? acc[r][i] : fmaf(fr, v, acc[r][i]);
+            }
+          }
         }
       }
-      if (valid) put(c, o, inv);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int from = min(31, r0 + r);
+        const float row_inv = __shfl_sync(0xffffffffu, inv, from);
+        const int64_t at = __shfl_sync(0xffffffffu, out_row, from) + lane * kCols;
+        if (r0 + r < held && lane * kCols < a.dim) {
+#pragma unroll
+          for (int i = 0; i < kCols; i += 2) {
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + at + i) = Storage<T>::pack2(acc[r][i] * row_inv, acc[r][i + 1] * row_inv);
+          }
+        }
+      }
     }
     if (lane == 0) __stcg(counter, 0u);
   }
@@ -1155,6 +1214,9 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
         const int64_t n = s.n > 0 ? head_units(a, s) * a.hkv : 0;
         if (off < n) {
           sm.words[kStartSeq] = b;
+          sm.words[kStartFirst] = static_cast<int>(s.first);
+          sm.words[kStartN] = s.n;
+          sm.words[kStartLen] = s.len;
           sm.words[kStartLo] = static_cast<int>(off & 0xffffffff);
           sm.words[kStartHi] = static_cast<int>(off >> 32);
           break;
@@ -1265,7 +1327,7 @@ cudaError_t launch(const Args& a, int sms, cudaStream_t st) {
 
 template <typename T, int CODE>
 cudaError_t launch_dim(const Args& a, int sms, cudaStream_t st) {
-  return a.dim <= 64 ? launch<T, 64, CODE>(a, sms, st) : launch<T, 128, CODE>(a, sms, st);
+  return a.dim <= 64 ? launch<T, 64, CODE>(a, sms, st) : a.dim <= 128 ? launch<T, 128, CODE>(a, sms, st) : launch<T, 256, CODE>(a, sms, st);
 }
 
 template <typename T>
@@ -1289,7 +1351,7 @@ static int box_rows_of(int page_size) {
 // by halves and groups of 8 tokens; else a box a half. A box takes its warp about 90 cycles to issue, and with pages of
 // 16 tokens 32 of them a unit took longer than the unit's products.
 static void place_tiles(Args& a, int code_type) {
-  const int halves = a.dim <= 64 ? 1 : 2;
+  const int halves = a.dim <= 64 ? 1 : a.dim <= 128 ? 2 : 4;
   a.group_bytes = 1024;
   a.half_bytes = 128 * 128;
   if (code_type != KL_CODE_NONE || a.dim != 64 * halves) return;
@@ -1312,7 +1374,7 @@ static void place_tiles(Args& a, int code_type) {
 bool tc_fits(const Args& a, int dtype, int code_type) {
   if (dtype == KL_FLOAT32) return false;
   const int unit = code_type == KL_CODE_NONE ? 8 : 16;  // elements of a cache in 16 bytes
-  if (a.dim % 8 != 0 || a.dim % unit != 0 || a.dim > 128 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
+  if (a.dim % 8 != 0 || a.dim % unit != 0 || a.dim > 256 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
   const auto stride_ok = [](int64_t stride, int64_t extent, int u) {
     return extent == 1 || (stride > 0 && stride % u == 0 && stride < (int64_t(1) << 38));
   };
@@ -1322,15 +1384,15 @@ bool tc_fits(const Args& a, int dtype, int code_type) {
 }
 
 size_t tc_partial_bytes(int head_dim, int sms) {
-  if (head_dim > 128) return 0;
-  const size_t dp = head_dim <= 64 ? 64 : 128;
-  return static_cast<size_t>(sms) * 2 * 2 * (dp + 2) * 128 * sizeof(float);
+  const size_t dp = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+  return static_cast<size_t>(sms) * 2 * tiles_of(static_cast<int>(dp)) * (dp + 2) * 128 * sizeof(float);
 }
 
 size_t tc_sync_bytes(int sms) { return 256 + static_cast<size_t>(sms) * kCountersPerCta * sizeof(uint32_t); }
 
 cudaError_t launch_tc(Args a, int dtype, int code_type, int sms, cudaStream_t st) {
   a.tile_tokens = 128 / a.group;
+  a.block_tokens = (a.dim > 128 ? 1 : 2) * a.tile_tokens;
   a.box_rows = box_rows_of(a.page_size);
   while ((1 << a.box_shift) < a.box_rows) ++a.box_shift;
   place_tiles(a, code_type);
