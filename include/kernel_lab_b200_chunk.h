@@ -127,15 +127,17 @@ int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const 
  *   served     [rows] bytes: 1, or 0 for a row that got none of what it needs
  * Lengths beyond width * page_size are clamped (KL_STATUS_LEN_CLAMPED), parents past the batch make empty rows
  * and entries outside [0, num_pages) are taken over but stand for no page (KL_STATUS_BAD_PAGE); negative
- * new_tokens count as 0. rows at most 2^24. Scratch: kl_paged_reserve_workspace_size bytes, no initialisation.
+ * new_tokens count as 0. rows at most 2^24. Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's
+ * rules (`sync` zero before its first use, left zero but for the status word; calls that overlap on the GPU need
+ * separate buffers).
  */
-int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes);
+int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes, size_t* sync_bytes);
 
 int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table, int32_t* out_lens, uint8_t* served,
                      const int32_t* block_table, const int32_t* seq_lens, const int32_t* new_tokens,
                      const int32_t* parents, int batch, int rows, int width, int page_size,
                      int64_t block_table_stride, int64_t num_pages, void* scratch, size_t scratch_bytes,
-                     uint32_t* status, void* stream);
+                     void* sync, size_t sync_bytes, void* stream);
 
 /*
  * Moves the pages in use (those that the first ceil(seq_lens[b] / page_size) entries of the rows name; *used
@@ -144,11 +146,12 @@ int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table, int32_t* 
  * block_table) receives the entries under the pages' new ids, 0 past a row's pages. Entries outside
  * [0, num_pages) are taken over (KL_STATUS_BAD_PAGE), lengths clamped as above. Scratch as above.
  */
-int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes);
+int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes, size_t* sync_bytes);
 
 int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table, int32_t* used, const int32_t* block_table,
                      const int32_t* seq_lens, int batch, int width, int page_size, int64_t block_table_stride,
-                     int64_t num_pages, void* scratch, size_t scratch_bytes, uint32_t* status, void* stream);
+                     int64_t num_pages, void* scratch, size_t scratch_bytes, void* sync, size_t sync_bytes,
+                     void* stream);
 
 #ifdef __cplusplus
 }

@@ -6,9 +6,10 @@
 // destination) pages that the copy kernel works off. Everything follows from the inputs alone (marks by
 // atomic maximum, ranks by scans), so two runs give the same table.
 //
-// Bookkeeping: one cluster of kClusterCtas CTAs of kPlanThreads threads, phases divided by cluster barriers: one
-// launch, the CTAs of a cluster being resident together by definition. It is bound by latency: table and marks
-// are a few hundred KB that stay in L2.
+// Bookkeeping is bound by latency: table and marks are a few hundred KB that stay in L2. Marks are scattered 4-byte
+// stores, which all SMs share (one cluster alone took 7 us for 65,000 of them); the rest is one cluster of kClusterCtas
+// CTAs of kPlanThreads threads, its phases divided by cluster barriers: the CTAs of a cluster are resident together by
+// definition. It clears the marks behind itself.
 // Copies: HBM-bound, 2 * bytes. CTAs take 16 KB slices of a page, all loads of a slice before its stores.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -150,6 +151,8 @@ constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kHeld = INT_MAX;  // the mark of a page that a row holds and is not about to write
 
+struct RowPlan;
+
 struct PlanArgs {
   const int32_t* block_table;
   const int32_t* seq_lens;
@@ -168,63 +171,74 @@ struct PlanArgs {
   int32_t* src;        // pairs to copy
   int32_t* dst;
   int32_t* count;      // their number
+  RowPlan* row_plan;   // [rows] (reserve)
   int64_t* begin;      // [rows]: the row's first page among those given out
   int32_t* copy_begin; // [rows]: its copy's place on the list
   int64_t* totals;     // [0]: pages needed
   uint32_t* status;
 };
 
-struct Shared {
-  long long warp_a[kPlanWarps], warp_b[kPlanWarps];
-  long long total_a, total_b;
-  long long cta_count;  // read by the other CTAs
+template <typename N>
+struct ScanSpace {
+  N warp[kPlanWarps];
+  N total;
 };
 
-// Exclusive block-wide prefix sums of two numbers a thread; the totals in sh.total_a and sh.total_b.
-__device__ __forceinline__ void scan_two(Shared& sh, long long& a, long long& b) {
+struct Shared {
+  ScanSpace<int> pages;
+  ScanSpace<long long> needs;
+  ScanSpace<int> copies;
+  int cta_count;  // read by the other CTAs
+};
+
+// Exclusive block-wide prefix sum of a number a thread; the total in sp.total.
+template <typename N>
+__device__ __forceinline__ N scan(ScanSpace<N>& sp, N v) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long ia = a, ib = b;
+  N inc = v;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const long long ya = __shfl_up_sync(0xffffffffu, ia, m), yb = __shfl_up_sync(0xffffffffu, ib, m);
-    if (lane >= m) {
-      ia += ya;
-      ib += yb;
-    }
+    const N y = __shfl_up_sync(0xffffffffu, inc, m);
+    if (lane >= m) inc += y;
   }
-  __syncthreads();  // the previous use of the arrays is over
-  if (lane == 31) {
-    sh.warp_a[warp] = ia;
-    sh.warp_b[warp] = ib;
-  }
+  __syncthreads();  // the previous use of the array is over
+  if (lane == 31) sp.warp[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    const long long wa = sh.warp_a[lane], wb = sh.warp_b[lane];
-    long long xa = wa, xb = wb;
+    const N w = sp.warp[lane];
+    N x = w;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-      const long long ya = __shfl_up_sync(0xffffffffu, xa, m), yb = __shfl_up_sync(0xffffffffu, xb, m);
-      if (lane >= m) {
-        xa += ya;
-        xb += yb;
-      }
+      const N y = __shfl_up_sync(0xffffffffu, x, m);
+      if (lane >= m) x += y;
     }
-    sh.warp_a[lane] = xa - wa;
-    sh.warp_b[lane] = xb - wb;
-    if (lane == 31) {
-      sh.total_a = xa;
-      sh.total_b = xb;
-    }
+    sp.warp[lane] = x - w;
+    if (lane == 31) sp.total = x;
   }
   __syncthreads();
-  a = ia - a + sh.warp_a[warp];
-  b = ib - b + sh.warp_b[warp];
+  return inc - v + sp.warp[warp];
+}
+
+// The CTAs' counts: their sum, and that of those before this one.
+template <typename Cluster>
+__device__ __forceinline__ void counts_before(Cluster& cluster, Shared& sh, int cta, int& before, int& all) {
+  const int lane = threadIdx.x & 31;
+  const int n = lane < kClusterCtas ? cluster.map_shared_rank(&sh, lane)->cta_count : 0;
+  all = __reduce_add_sync(0xffffffffu, n);
+  before = __reduce_add_sync(0xffffffffu, lane < cta ? n : 0);
 }
 
 struct Row {
   int parent;  // -1: empty
   int len, have;
 };
+
+// What the later phases need of a row: its length, how many pages it has, how many tokens are to come, its last page.
+struct alignas(16) RowPlan {
+  int len, have, add, last;
+};
+
+constexpr int kAhead = 8;  // entries of a row in flight a lane: a phase is a chain of round trips to L2
 
 __device__ __forceinline__ Row read_row(const PlanArgs& a, int r, bool report) {
   Row x{r, 0, 0};
@@ -266,8 +280,56 @@ __device__ __forceinline__ int4 marks_at(const PlanArgs& a, int64_t p) {
 __device__ __forceinline__ void clear_marks(const PlanArgs& a, int cta) {
   int64_t lo, hi;
   own_pages(a, cta, lo, hi);
+#pragma unroll 4
   for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
     __stcg(reinterpret_cast<int4*>(a.mark + p), make_int4(0, 0, 0, 0));
+  }
+}
+
+// Marks the pages that the rows name. A row that is to write its last page marks it with rows - r (of several the lowest
+// has the largest), any other holder with kHeld. RESERVE: the rows' entries are taken over, too. A warp takes 256
+// columns of a row.
+constexpr int kMarkThreads = 256;
+
+template <bool RESERVE>
+__global__ void __launch_bounds__(kMarkThreads) mark_pages(const __grid_constant__ PlanArgs a) {
+  wait_prior_grid();
+  allow_next_grid();
+  const int lane = threadIdx.x & 31;
+  const int64_t parts = (a.width + 32 * kAhead - 1) / (32 * kAhead), items = a.rows * max(parts, int64_t(1));
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * (kMarkThreads / 32) + (threadIdx.x >> 5); item < items;
+       item += static_cast<int64_t>(gridDim.x) * (kMarkThreads / 32)) {
+    const int r = static_cast<int>(item / max(parts, int64_t(1)));
+    const int part = static_cast<int>(item - r * max(parts, int64_t(1)));
+    const int asked = RESERVE ? __ldcg(a.new_tokens + r) : 0;
+    const Row x = read_row(a, r, part == 0 && lane == 0);
+    const int add = x.parent < 0 ? 0 : max(0, asked);
+    const bool writes = add > 0 && x.len % a.page_size != 0;
+    const int32_t* in = a.block_table + (x.parent < 0 ? 0 : x.parent) * a.bt_stride;
+    int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
+    const int c0 = part * 32 * kAhead + lane;
+    int e[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) e[u] = c0 + 32 * u < x.have ? __ldcg(in + c0 + 32 * u) : 0;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int c = c0 + 32 * u;
+      if (c < x.have) {
+        if (e[u] < 0 || e[u] >= a.num_pages) {
+          if (a.status) atomicOr(a.status, kStatusBadPage);
+        } else if (RESERVE && writes && c == x.have - 1) {
+          atomicMax(a.mark + e[u], a.rows - r);
+        } else {
+          store_mark(a.mark + e[u], kHeld);
+        }
+        if (RESERVE && c == x.have - 1) __stcg(reinterpret_cast<int4*>(a.row_plan + r), make_int4(x.len, x.have, add, e[u]));
+      }
+      if (RESERVE && c < a.width) out[c] = e[u];
+    }
+    if (RESERVE && part == 0 && lane == 0) {
+      a.out_lens[r] = x.len;
+      if (x.have == 0) __stcg(reinterpret_cast<int4*>(a.row_plan + r), make_int4(x.len, 0, add, -1));
+    }
   }
 }
 
@@ -278,97 +340,66 @@ reserve_plan(const __grid_constant__ PlanArgs a) {
   const int cta = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = cta * kPlanWarps + (threadIdx.x >> 5);
   constexpr int kWarps = kClusterCtas * kPlanWarps;
+  if (threadIdx.x == 0) sh.cta_count = 0;
+  __syncthreads();
   wait_prior_grid();
   allow_next_grid();
-  clear_marks(a, cta);
-  cluster.sync();
-
-  // Marks, and the rows' entries taken over. A row that is to write its last page marks it with rows - r (of
-  // several the lowest has the largest), any other holder with kHeld.
-  for (int r = warp; r < a.rows; r += kWarps) {
-    const Row x = read_row(a, r, lane == 0);
-    const int add = max(0, __ldcg(a.new_tokens + r));
-    const bool writes = x.parent >= 0 && add > 0 && x.len % a.page_size != 0;
-    const int32_t* in = a.block_table + (x.parent < 0 ? 0 : x.parent) * a.bt_stride;
-    int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
-    for (int c = lane; c < a.width; c += 32) {
-      int e = 0;
-      if (c < x.have) {
-        e = __ldcg(in + c);
-        if (e < 0 || e >= a.num_pages) {
-          if (a.status) atomicOr(a.status, kStatusBadPage);
-        } else if (writes && c == x.have - 1) {
-          atomicMax(a.mark + e, a.rows - r);
-        } else {
-          store_mark(a.mark + e, kHeld);
-        }
-      }
-      out[c] = e;
-    }
-    if (lane == 0) a.out_lens[r] = x.len;
-  }
-  cluster.sync();
 
   // What each row needs, summed in order (CTA 0); the free pages of each CTA's part.
   int64_t lo, hi;
   own_pages(a, cta, lo, hi);
-  long long mine = 0, none = 0;
+  int mine = 0;
+#pragma unroll 4
   for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
     const int4 m = marks_at(a, p);
     mine += (m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0);
   }
-  scan_two(sh, mine, none);
-  if (threadIdx.x == 0) sh.cta_count = sh.total_a;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) atomicAdd(&sh.cta_count, mine);
   if (cta == 0) {
-    long long need_before = 0, copies_before = 0;
+    long long need_before = 0;
+    int copies_before = 0;
     for (int base = 0; base < a.rows; base += kPlanThreads) {
       const int r = base + threadIdx.x;
-      long long need = 0, copy = 0;
+      long long need = 0;
+      int copy = 0;
       if (r < a.rows) {
-        const Row x = read_row(a, r, false);
-        const long long add = x.parent < 0 ? 0 : max(0, __ldcg(a.new_tokens + r));
-        if (x.len + add <= static_cast<long long>(a.width) * a.page_size) {
-          if (add > 0 && x.len % a.page_size != 0) {
-            const int last = __ldcg(a.block_table + x.parent * a.bt_stride + x.have - 1);
-            if (last >= 0 && last < a.num_pages) copy = __ldcg(a.mark + last) != a.rows - r;
-          }
-          need = copy + (x.len + add + a.page_size - 1) / a.page_size - x.have;
+        const int4 v = __ldcg(reinterpret_cast<const int4*>(a.row_plan + r));
+        const RowPlan x{v.x, v.y, v.z, v.w};
+        const long long end = static_cast<long long>(x.len) + x.add;
+        if (end <= static_cast<long long>(a.width) * a.page_size) {
+          if (x.add > 0 && x.len % a.page_size != 0 && x.last >= 0 && x.last < a.num_pages) copy = __ldcg(a.mark + x.last) != a.rows - r;
+          need = copy + (end + a.page_size - 1) / a.page_size - x.have;
         } else {
           need = -1;  // does not fit
         }
       }
       const bool fits = need >= 0;
-      long long n = fits ? need : 0, k = copy;
-      scan_two(sh, n, k);
+      const long long n = scan(sh.needs, fits ? need : 0);
+      const int k = scan(sh.copies, copy);
       if (r < a.rows) {
         a.begin[r] = fits ? need_before + n : -1;
-        a.copy_begin[r] = copy ? static_cast<int32_t>(copies_before + k) : -1;
+        a.copy_begin[r] = copy ? copies_before + k : -1;
       }
-      need_before += sh.total_a;
-      copies_before += sh.total_b;
+      need_before += sh.needs.total;
+      copies_before += sh.copies.total;
     }
     if (threadIdx.x == 0) {
       a.totals[0] = need_before;
-      *a.count = static_cast<int32_t>(copies_before);
+      *a.count = copies_before;
     }
   }
   cluster.sync();
 
   // The lowest free pages in order, as many as are needed.
-  long long before = 0, all = 0;
-  for (int c = 0; c < kClusterCtas; ++c) {
-    const long long n = cluster.map_shared_rank(&sh, c)->cta_count;
-    if (c < cta) before += n;
-    all += n;
-  }
-  const long long wanted = min(static_cast<long long>(__ldcg(a.totals)), all);
+  int before, all;
+  counts_before(cluster, sh, cta, before, all);
+  const int wanted = static_cast<int>(min(static_cast<long long>(__ldcg(a.totals)), static_cast<long long>(all)));
   for (int64_t p0 = lo; p0 < hi && before < wanted; p0 += kPlanThreads * 4) {
     const int64_t p = p0 + threadIdx.x * 4;
     int4 m = make_int4(kHeld, kHeld, kHeld, kHeld);
     if (p < hi) m = marks_at(a, p);
-    long long at = (m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0), unused = 0;
-    scan_two(sh, at, unused);
-    at += before;
+    int at = before + scan(sh.pages, (m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0));
     const int marks[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -377,16 +408,17 @@ reserve_plan(const __grid_constant__ PlanArgs a) {
         ++at;
       }
     }
-    before += sh.total_a;
+    before += sh.pages.total;
   }
   cluster.sync();  // also: no CTA has left while another reads its count
+  clear_marks(a, cta);
 
   for (int r = warp; r < a.rows; r += kWarps) {
-    const Row x = read_row(a, r, false);
-    const long long add = x.parent < 0 ? 0 : max(0, __ldcg(a.new_tokens + r));
+    const int4 v = __ldcg(reinterpret_cast<const int4*>(a.row_plan + r));
     const long long begin = __ldcg(a.begin + r);
     const int copy_at = __ldcg(a.copy_begin + r);
-    const int grown = begin < 0 ? 0 : static_cast<int>((x.len + add + a.page_size - 1) / a.page_size - x.have);
+    const RowPlan x{v.x, v.y, v.z, v.w};
+    const int grown = begin < 0 ? 0 : static_cast<int>((static_cast<long long>(x.len) + x.add + a.page_size - 1) / a.page_size - x.have);
     const int copies = copy_at >= 0;
     const bool ok = begin >= 0 && (grown + copies == 0 || begin + grown + copies <= all);
     int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
@@ -396,7 +428,7 @@ reserve_plan(const __grid_constant__ PlanArgs a) {
       if (copies) {
         int from = -1, to = -1;
         if (ok) {
-          from = __ldcg(a.block_table + x.parent * a.bt_stride + x.have - 1);
+          from = x.last;
           to = __ldcg(a.pool_list + begin);
           out[x.have - 1] = to;
         }
@@ -415,40 +447,23 @@ compact_plan(const __grid_constant__ PlanArgs a) {
   const int cta = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = cta * kPlanWarps + (threadIdx.x >> 5);
   constexpr int kWarps = kClusterCtas * kPlanWarps;
+  if (threadIdx.x == 0) sh.cta_count = 0;
+  __syncthreads();
   wait_prior_grid();
   allow_next_grid();
-  clear_marks(a, cta);
-  cluster.sync();
-  for (int r = warp; r < a.rows; r += kWarps) {
-    const Row x = read_row(a, r, lane == 0);
-    const int32_t* in = a.block_table + static_cast<int64_t>(r) * a.bt_stride;
-    for (int c = lane; c < x.have; c += 32) {
-      const int e = __ldcg(in + c);
-      if (e >= 0 && e < a.num_pages) {
-        store_mark(a.mark + e, kHeld);
-      } else if (a.status) {
-        atomicOr(a.status, kStatusBadPage);
-      }
-    }
-  }
-  cluster.sync();
-
   int64_t lo, hi;
   own_pages(a, cta, lo, hi);
-  long long mine = 0, none = 0;
+  int mine = 0;
+#pragma unroll 4
   for (int64_t p = lo + threadIdx.x * 4; p < hi; p += kPlanThreads * 4) {
     const int4 m = marks_at(a, p);
-    mine += min(a.num_pages, p + 4) - p - ((m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0));
+    mine += static_cast<int>(min(a.num_pages, p + 4) - p) - ((m.x == 0) + (m.y == 0) + (m.z == 0) + (m.w == 0));
   }
-  scan_two(sh, mine, none);
-  if (threadIdx.x == 0) sh.cta_count = sh.total_a;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) atomicAdd(&sh.cta_count, mine);
   cluster.sync();
-  long long before = 0, used = 0;
-  for (int c = 0; c < kClusterCtas; ++c) {
-    const long long n = cluster.map_shared_rank(&sh, c)->cta_count;
-    if (c < cta) before += n;
-    used += n;
-  }
+  int before, used;
+  counts_before(cluster, sh, cta, before, used);
   // Page p with L(p) pages in use below it. The free ones below `used` come in order as number p - L(p), the
   // ones in use from `used` on, counted down from the last, as number used - 1 - L(p): as many as the former.
   // In ascending order they are number L(p) - L(used), and L(used) = used - (free ones below it).
@@ -457,11 +472,10 @@ compact_plan(const __grid_constant__ PlanArgs a) {
     int4 m = make_int4(0, 0, 0, 0);
     if (p < hi) m = marks_at(a, p);
     const int marks[4] = {m.x, m.y, m.z, m.w};
-    long long at = 0, unused = 0;
+    int at = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) at += marks[u] != 0 && p + u < a.num_pages && p < hi;
-    scan_two(sh, at, unused);
-    at += before;
+    at = before + scan(sh.pages, at);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int64_t id = p + u;
@@ -469,13 +483,13 @@ compact_plan(const __grid_constant__ PlanArgs a) {
       const bool in_use = marks[u] != 0;
       if (in_use && id >= used) a.pool_list[used - 1 - at] = static_cast<int32_t>(id);  // last first
       if (!in_use && id < used) __stcg(a.dst + (id - at), static_cast<int32_t>(id));
-      if (id == used - 1) *a.count = static_cast<int32_t>(used - at - in_use);  // free ones below `used`
+      if (id == used - 1) *a.count = used - at - in_use;  // free ones below `used`
       at += in_use;
     }
-    before += sh.total_a;
+    before += sh.pages.total;
   }
   if (cta == 0 && threadIdx.x == 0) {
-    *a.used = static_cast<int32_t>(used);
+    *a.used = used;
     if (used == 0) *a.count = 0;
   }
   cluster.sync();  // also: no CTA has left while another reads its count
@@ -490,12 +504,22 @@ compact_plan(const __grid_constant__ PlanArgs a) {
     const Row x = read_row(a, r, false);
     const int32_t* in = a.block_table + static_cast<int64_t>(r) * a.bt_stride;
     int32_t* out = a.out_table + static_cast<int64_t>(r) * a.width;
-    for (int c = lane; c < a.width; c += 32) {
-      int e = c < x.have ? __ldcg(in + c) : 0;
-      if (c < x.have && e >= used && e < a.num_pages) e = __ldcg(a.mark + e) - 1;
-      out[c] = e;
+    for (int c0 = lane; c0 < a.width; c0 += 32 * kAhead) {
+      int e[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) e[u] = c0 + 32 * u < x.have ? __ldcg(in + c0 + 32 * u) : 0;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (c0 + 32 * u < x.have && e[u] >= used && e[u] < a.num_pages) e[u] = __ldcg(a.mark + e[u]) - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (c0 + 32 * u < a.width) out[c0 + 32 * u] = e[u];
+      }
     }
   }
+  cluster.sync();
+  clear_marks(a, cta);
 }
 
 size_t rounded(size_t n) { return (n + 255) & ~size_t(255); }
@@ -508,16 +532,26 @@ size_t cut(PlanArgs& a, uint8_t* p, int64_t num_pages, int64_t rows, int64_t pai
     off += rounded(bytes);
     return at;
   };
-  const size_t pages = static_cast<size_t>(num_pages + 3) / 4 * 4;
   a.totals = reinterpret_cast<int64_t*>(take(16));
   a.count = reinterpret_cast<int32_t*>(take(4));
-  a.mark = reinterpret_cast<int32_t*>(take(pages * 4));
-  a.pool_list = reinterpret_cast<int32_t*>(take(pages * 4));
+  a.pool_list = reinterpret_cast<int32_t*>(take(static_cast<size_t>(num_pages) * 4));
   a.src = reinterpret_cast<int32_t*>(take(static_cast<size_t>(pairs) * 4));
   a.dst = reinterpret_cast<int32_t*>(take(static_cast<size_t>(pairs) * 4));
+  a.row_plan = reinterpret_cast<RowPlan*>(take(static_cast<size_t>(rows) * sizeof(RowPlan)));
   a.begin = reinterpret_cast<int64_t*>(take(static_cast<size_t>(rows) * 8));
   a.copy_begin = reinterpret_cast<int32_t*>(take(static_cast<size_t>(rows) * 4));
   return off;
+}
+
+// Status word and marks, which every call leaves zero.
+constexpr size_t kMarksAt = 256;
+size_t sync_size(int64_t num_pages) { return kMarksAt + static_cast<size_t>(num_pages + 3) / 4 * 16; }
+
+cudaError_t launch_marks(void (*kernel)(PlanArgs), const PlanArgs& a, cudaStream_t st) {
+  const int64_t parts = std::max<int64_t>(1, (a.width + 32 * kAhead - 1) / (32 * kAhead));
+  const int64_t warps = kMarkThreads / 32, blocks = (a.rows * parts + warps - 1) / warps;
+  return launch_kernel(true, kernel, dim3(static_cast<unsigned>(std::min<int64_t>(std::max<int64_t>(blocks, 1), sm_count() * 8))),
+                       dim3(kMarkThreads), 0, st, a);
 }
 
 constexpr int kMaxRows = 1 << 24;
@@ -550,11 +584,12 @@ extern "C" int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* 
   return static_cast<int>(launch_copies(pools, src, dst, pairs, nullptr, num_pages, status, static_cast<cudaStream_t>(stream)));
 }
 
-extern "C" int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes) {
+extern "C" int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes, size_t* sync_bytes) {
   using namespace klb::page_pool;
-  if (num_pages < 0 || num_pages > INT32_MAX - 8 || rows < 0 || rows > kMaxRows || !scratch_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  if (num_pages < 0 || num_pages > INT32_MAX - 8 || rows < 0 || rows > kMaxRows || !scratch_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
   PlanArgs a{};
   *scratch_bytes = cut(a, nullptr, num_pages, rows, rows);
+  *sync_bytes = sync_size(num_pages);
   return 0;
 }
 
@@ -562,7 +597,7 @@ extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table
                                 const int32_t* block_table, const int32_t* seq_lens, const int32_t* new_tokens,
                                 const int32_t* parents, int batch, int rows, int width, int page_size,
                                 int64_t block_table_stride, int64_t num_pages, void* scratch, size_t scratch_bytes,
-                                uint32_t* status, void* stream) {
+                                void* sync, size_t sync_bytes, void* stream) {
   using namespace klb::page_pool;
   const int invalid = static_cast<int>(cudaErrorInvalidValue);
   if (!valid(pools) || !sizes_ok(batch, rows, width, page_size, block_table_stride, num_pages)) return invalid;
@@ -571,7 +606,10 @@ extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table
   if (!out_lens || !served || !new_tokens || (batch > 0 && !seq_lens) || (width > 0 && (!out_table || (batch > 0 && !block_table)))) return invalid;
   PlanArgs a{};
   const size_t need = cut(a, static_cast<uint8_t*>(scratch), num_pages, rows, rows);
-  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) return invalid;
+  if (!scratch || scratch_bytes < need || !sync || sync_bytes < sync_size(num_pages)) return invalid;
+  if (reinterpret_cast<uintptr_t>(scratch) % 16 || reinterpret_cast<uintptr_t>(sync) % 16) return invalid;
+  a.status = static_cast<uint32_t*>(sync);
+  a.mark = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(sync) + kMarksAt);
   a.block_table = block_table;
   a.seq_lens = seq_lens;
   a.new_tokens = new_tokens;
@@ -585,33 +623,38 @@ extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table
   a.rows = rows;
   a.width = width;
   a.page_size = page_size;
-  a.status = status;
   if (tables_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = klb::launch_kernel(true, reserve_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  cudaError_t e = launch_marks(mark_pages<true>, a, st);
   if (e != cudaSuccess) return static_cast<int>(e);
-  return static_cast<int>(launch_copies(pools, a.src, a.dst, rows, a.count, num_pages, status, st));
+  e = klb::launch_kernel(true, reserve_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return static_cast<int>(launch_copies(pools, a.src, a.dst, rows, a.count, num_pages, a.status, st));
 }
 
-extern "C" int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes) {
+extern "C" int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes, size_t* sync_bytes) {
   using namespace klb::page_pool;
-  if (num_pages < 0 || num_pages > INT32_MAX - 8 || !scratch_bytes) return static_cast<int>(cudaErrorInvalidValue);
+  if (num_pages < 0 || num_pages > INT32_MAX - 8 || !scratch_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
   PlanArgs a{};
   *scratch_bytes = cut(a, nullptr, num_pages, 0, num_pages);
+  *sync_bytes = sync_size(num_pages);
   return 0;
 }
 
 extern "C" int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table, int32_t* used,
                                 const int32_t* block_table, const int32_t* seq_lens, int batch, int width,
                                 int page_size, int64_t block_table_stride, int64_t num_pages, void* scratch,
-                                size_t scratch_bytes, uint32_t* status, void* stream) {
+                                size_t scratch_bytes, void* sync, size_t sync_bytes, void* stream) {
   using namespace klb::page_pool;
   const int invalid = static_cast<int>(cudaErrorInvalidValue);
   if (!valid(pools) || !sizes_ok(batch, batch, width, page_size, block_table_stride, num_pages) || !used) return invalid;
   if (batch > 0 && (!seq_lens || (width > 0 && (!out_table || !block_table)))) return invalid;
   PlanArgs a{};
   const size_t need = cut(a, static_cast<uint8_t*>(scratch), num_pages, 0, num_pages);
-  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 16) return invalid;
+  if (!scratch || scratch_bytes < need || !sync || sync_bytes < sync_size(num_pages)) return invalid;
+  if (reinterpret_cast<uintptr_t>(scratch) % 16 || reinterpret_cast<uintptr_t>(sync) % 16) return invalid;
+  a.status = static_cast<uint32_t*>(sync);
+  a.mark = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(sync) + kMarksAt);
   a.block_table = block_table;
   a.seq_lens = seq_lens;
   a.out_table = out_table;
@@ -622,11 +665,12 @@ extern "C" int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table
   a.rows = batch;
   a.width = width;
   a.page_size = page_size;
-  a.status = status;
   if (tables_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = klb::launch_kernel(true, compact_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  cudaError_t e = launch_marks(mark_pages<false>, a, st);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  e = klb::launch_kernel(true, compact_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
   if (e != cudaSuccess) return static_cast<int>(e);
   // Pages with ids of `used` and more that go below it: at most half of them.
-  return static_cast<int>(launch_copies(pools, a.src, a.dst, num_pages / 2, a.count, num_pages, status, st));
+  return static_cast<int>(launch_copies(pools, a.src, a.dst, num_pages / 2, a.count, num_pages, a.status, st));
 }

@@ -1019,17 +1019,17 @@ void paged_reserve(at::Tensor& out_table, at::Tensor& out_lens, at::Tensor& serv
   if (rows == 0) return;
   const c10::cuda::CUDAGuard guard(p.device);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  size_t bytes = 0;
-  check_status(kl_paged_reserve_workspace_size(p.num_pages, static_cast<int>(rows), &bytes), "paged_reserve (workspace)");
-  const Scratch s = scratch_for(p.device, stream, bytes, 4);
+  size_t bytes = 0, sync_bytes = 0;
+  check_status(kl_paged_reserve_workspace_size(p.num_pages, static_cast<int>(rows), &bytes, &sync_bytes), "paged_reserve (workspace)");
+  const Scratch s = scratch_for(p.device, stream, bytes, sync_bytes);
   const kl_page_pools_t pools = p.c();
   check_status(kl_paged_reserve(&pools, out_table.data_ptr<int32_t>(), out_lens.data_ptr<int32_t>(),
                                 reinterpret_cast<uint8_t*>(served.data_ptr<bool>()), block_table.data_ptr<int32_t>(),
                                 seq_lens.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(),
                                 parents ? parents->data_ptr<int32_t>() : nullptr, static_cast<int>(batch), static_cast<int>(rows),
                                 static_cast<int>(block_table.size(1)), static_cast<int>(page_size), block_table.stride(0), p.num_pages,
-                                s.partials.data_ptr(), static_cast<size_t>(s.partials.numel()),
-                                static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+                                s.partials.data_ptr(), static_cast<size_t>(s.partials.numel()), s.sync.data_ptr(),
+                                static_cast<size_t>(s.sync.numel()), stream),
                "paged_reserve");
 }
 
@@ -1043,14 +1043,15 @@ void paged_compact(at::Tensor& out_table, at::Tensor& used, at::TensorList cache
   TORCH_CHECK(used.scalar_type() == at::kInt && used.numel() == 1 && used.device() == p.device, "used is one int32 on the caches' device");
   const c10::cuda::CUDAGuard guard(p.device);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  size_t bytes = 0;
-  check_status(kl_paged_compact_workspace_size(p.num_pages, &bytes), "paged_compact (workspace)");
-  const Scratch s = scratch_for(p.device, stream, bytes, 4);
+  size_t bytes = 0, sync_bytes = 0;
+  check_status(kl_paged_compact_workspace_size(p.num_pages, &bytes, &sync_bytes), "paged_compact (workspace)");
+  const Scratch s = scratch_for(p.device, stream, bytes, sync_bytes);
   const kl_page_pools_t pools = p.c();
   check_status(kl_paged_compact(&pools, out_table.data_ptr<int32_t>(), used.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(),
                                 seq_lens.data_ptr<int32_t>(), static_cast<int>(batch), static_cast<int>(block_table.size(1)),
                                 static_cast<int>(page_size), block_table.stride(0), p.num_pages, s.partials.data_ptr(),
-                                static_cast<size_t>(s.partials.numel()), static_cast<uint32_t*>(s.sync.data_ptr()), stream),
+                                static_cast<size_t>(s.partials.numel()), s.sync.data_ptr(),
+                                static_cast<size_t>(s.sync.numel()), stream),
                "paged_compact");
 }
 

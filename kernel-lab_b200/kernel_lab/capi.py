@@ -110,13 +110,13 @@ CHUNK_SIGNATURES = {
         + [_c_int, _c_i64, _c_int, _c_float, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
     ),
     "kl_paged_copy_pages": (_c_int, [_c_poolsp, _c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_vp]),
-    "kl_paged_reserve_workspace_size": (_c_int, [_c_i64, _c_int, _c_szp]),
+    "kl_paged_reserve_workspace_size": (_c_int, [_c_i64, _c_int, _c_szp, _c_szp]),
     "kl_paged_reserve": (
-        _c_int, [_c_poolsp] + [_c_vp] * 7 + [_c_int] * 4 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp],
+        _c_int, [_c_poolsp] + [_c_vp] * 7 + [_c_int] * 4 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
     ),
-    "kl_paged_compact_workspace_size": (_c_int, [_c_i64, _c_szp]),
+    "kl_paged_compact_workspace_size": (_c_int, [_c_i64, _c_szp, _c_szp]),
     "kl_paged_compact": (
-        _c_int, [_c_poolsp] + [_c_vp] * 4 + [_c_int] * 3 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp],
+        _c_int, [_c_poolsp] + [_c_vp] * 4 + [_c_int] * 3 + [_c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp],
     ),
 }
 

@@ -100,26 +100,27 @@ def test_no_ops_and_refusals_without_a_device():
                 {"p": pools(stride=63)}, {"p": pools(size=-1)}):
         assert copy(**bad) == INVALID, bad
     assert lib.kl_paged_copy_pages(None, 16, 16, 3, 10, None, None) == INVALID
-    size = ctypes.c_size_t()
-    assert lib.kl_paged_reserve_workspace_size(1000, 64, ctypes.byref(size)) == 0 and size.value >= 2 * 4000 + 20 * 64
-    assert lib.kl_paged_reserve_workspace_size(-1, 64, ctypes.byref(size)) == lib.kl_paged_reserve_workspace_size(5, -1, ctypes.byref(size)) == INVALID
-    assert lib.kl_paged_compact_workspace_size(-1, ctypes.byref(size)) == lib.kl_paged_compact_workspace_size(5, None) == INVALID
+    size, sync = ctypes.c_size_t(), ctypes.c_size_t()
+    out = ctypes.byref(size), ctypes.byref(sync)
+    assert lib.kl_paged_reserve_workspace_size(1000, 64, *out) == 0 and size.value >= 4000 + 36 * 64 and sync.value >= 4256
+    assert lib.kl_paged_reserve_workspace_size(-1, 64, *out) == lib.kl_paged_reserve_workspace_size(5, -1, *out) == INVALID
+    assert lib.kl_paged_compact_workspace_size(-1, *out) == lib.kl_paged_compact_workspace_size(5, None, None) == INVALID
 
-    def reserve(p=None, out=1 << 20, table=1 << 16, parents=None, batch=4, rows=4, width=4, page=16, bt=4, pages=10, bytes_=1 << 20, ptr=256):
+    def reserve(p=None, out=1 << 20, table=1 << 16, parents=None, batch=4, rows=4, width=4, page=16, bt=4, pages=10, bytes_=1 << 20, ptr=256, sync=256):
         return lib.kl_paged_reserve(ctypes.byref(pools() if p is None else p), out, ptr, ptr, table, ptr, ptr, parents, batch, rows, width,
-                                    page, bt, pages, 256, bytes_, None, None)
+                                    page, bt, pages, 256, bytes_, sync, bytes_, None)
 
     assert reserve(batch=0, rows=0) == 0
     for bad in ({"batch": -1, "rows": -1}, {"rows": 5}, {"page": 0}, {"bt": 3}, {"pages": -1}, {"bytes_": 64}, {"ptr": None}, {"out": None},
                 {"table": None}, {"out": 1 << 16}, {"out": (1 << 16) + 60}, {"rows": (1 << 24) + 1, "parents": 16},
-                {"width": 1 << 28, "bt": 1 << 28}, {"p": pools(stride=3)}):
+                {"width": 1 << 28, "bt": 1 << 28}, {"p": pools(stride=3)}, {"sync": None}, {"sync": 264}):
         assert reserve(**bad) == INVALID, bad
 
-    def compact(p=None, out=1 << 20, used=16, table=1 << 16, batch=4, width=4, page=16, bt=4, pages=10, bytes_=1 << 20, lens=16):
+    def compact(p=None, out=1 << 20, used=16, table=1 << 16, batch=4, width=4, page=16, bt=4, pages=10, bytes_=1 << 20, lens=16, sync=256):
         return lib.kl_paged_compact(ctypes.byref(pools() if p is None else p), out, used, table, lens, batch, width, page, bt, pages, 256,
-                                    bytes_, None, None)
+                                    bytes_, sync, bytes_, None)
 
-    for bad in ({"batch": -1}, {"used": None}, {"out": 1 << 16}, {"table": None}, {"lens": None}, {"page": 0}, {"bytes_": 64}, {"bt": 1}):
+    for bad in ({"batch": -1}, {"used": None}, {"out": 1 << 16}, {"table": None}, {"lens": None}, {"page": 0}, {"bytes_": 64}, {"bt": 1}, {"sync": None}):
         assert compact(**bad) == INVALID, bad
 
 
