@@ -36,7 +36,6 @@ namespace {
 
 constexpr int kBN = 128;                 // keys of a unit
 constexpr int kLoadWarp = 8, kMmaWarp = 9, kFixWarp = 11, kWidenWarp = 12;
-constexpr int kByFma = 3;                // of 8 exponentials, those on the multiply-add pipes
 constexpr float kLazy = 8.0f;            // log2 by which a maximum may be passed before O is rescaled
 constexpr uint64_t kWaitCycles = 2000000000ull;  // about one second
 // Units whose marks are told apart. A tile passes over the special units that it has no part in: that no wait of it is a phase
@@ -53,9 +52,12 @@ struct Layout {
   static constexpr bool kCoded = CODE != KL_CODE_NONE;
   // Two softmax warpgroups; load, each tile's products, V; over an 8-bit cache four warps that widen its codes.
   static constexpr int kThreads = kCoded ? 512 : 384;
-  // Registers: 256 * 192 + 256 * 64 = 512 * 128, 256 * 208 + 128 * 88 = 384 * 168, the launch's.
-  static constexpr int kSoftmaxRegs = kCoded ? 192 : 208, kOtherRegs = kCoded ? 64 : 88;
+  // Registers: 256 * 136 + 256 * 120 = 512 * 128, 256 * 176 + 128 * 152 = 384 * 168, the launch's.
+  static constexpr int kSoftmaxRegs = kCoded ? 136 : 176, kOtherRegs = kCoded ? 120 : 152;
   static constexpr int kTiles = tiles_of(DP);
+  // Of 8 exponentials, those on the multiply-add pipes (a prompt of 8192 tokens: 581 us with none, 558 with 3, 580 with 3 and
+  // longer loops). Over codes the warps are short of issue slots (chunks over 8192 tokens: 1249 us with none, 1277 with 3).
+  static constexpr int kByFma = kCoded ? 0 : 3;
   static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a 16-bit row
   static constexpr uint32_t kHalf = 128u * 128u;            // 128 rows of one
   static constexpr uint32_t kTile = kHalves * kHalf;
@@ -908,7 +910,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           if constexpr (L::kCoded) f = plain ? scales[c / 8 + i / 4] : 1.0f;
           float x0, x1;
           const uint64_t e2 = fma2(x2, L::kCoded ? pair(f, f) : sl2, sh2);
-          if (i * kByFma % 8 < kByFma) {
+          if (i * L::kByFma % 8 < L::kByFma) {
             exp2_pair<std::is_same<TV, __half>::value ? 4 : 3>(e2, x0, x1);
           } else {
             unpair(e2, x0, x1);
@@ -1171,7 +1173,7 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
   wait_prior_grid();
   allow_next_grid();
   __syncwarp();
-  if (warp == 0) {  // not before the previous grid has ended: a CTA of it could wait for these columns
+  if (warp == kFixWarp) {  // not before the previous grid has ended: a CTA of it could wait for these columns
     tmem_alloc(sm.base + L::kWords + 4 * kTmem, 512);
     tmem_relinquish();
   }
@@ -1250,7 +1252,7 @@ __global__ void __launch_bounds__(Layout<DP, CODE>::kThreads, 1) tc_kernel(const
   }
   tcgen05_fence_before();
   __syncthreads();
-  if (warp == 0) {
+  if (warp == kFixWarp) {
     __syncwarp();
     tmem_dealloc(tmem, 512);
   }
