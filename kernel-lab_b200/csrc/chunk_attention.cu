@@ -225,7 +225,7 @@ extern "C" int kl_paged_chunk_attention_workspace_size(int dtype, int code_type,
                                                        size_t* partial_bytes, size_t* sync_bytes) {
   if (!partial_bytes || !sync_bytes) return static_cast<int>(cudaErrorInvalidValue);
   const int sms = klb::chunk_attention::sm_count();
-  *partial_bytes = klb::chunk_attention::tc_partial_bytes(head_dim, sms);
+  *partial_bytes = dtype == KL_FLOAT32 ? 0 : klb::chunk_attention::tc_partial_bytes(head_dim, sms);
   *sync_bytes = klb::chunk_attention::tc_sync_bytes(sms);
   return 0;
 }

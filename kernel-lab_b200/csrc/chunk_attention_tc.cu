@@ -1378,7 +1378,7 @@ bool tc_fits(const Args& a, int dtype, int code_type) {
   const int unit = code_type == KL_CODE_NONE ? 8 : 16;  // elements of a cache in 16 bytes
   if (a.dim % 8 != 0 || a.dim % unit != 0 || a.dim > 256 || a.group > 128 || a.page_size % 8 != 0 || !(a.scale_log2 > 0.0f)) return false;
   const auto stride_ok = [](int64_t stride, int64_t extent, int u) {
-    return extent == 1 || (stride > 0 && stride % u == 0 && stride < (int64_t(1) << 38));
+    return extent == 1 || (stride > 0 && stride % u == 0 && stride < (int64_t(1) << 35));
   };
   return aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && (reinterpret_cast<uintptr_t>(a.out) & 3) == 0 &&
          stride_ok(a.q_stride, a.tokens, 8) && stride_ok(a.head_stride, a.hkv, unit) && stride_ok(a.token_stride, a.page_size, unit) &&

@@ -144,6 +144,34 @@ def test_meta_kernels():
     assert table.shape == (3, 4) and used.shape == ()
 
 
+def test_fake_tensors_and_dispatch_modes_see_the_operators():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    from kernel_lab import cuda_ops
+
+    class Seen(TorchDispatchMode):
+        names: list[str] = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with FakeTensorMode():
+        i = lambda *s: torch.empty(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+        k = torch.empty(10, 16, 2, 64, device="cuda")
+        assert cuda_ops.paged_chunk_attention(torch.empty(9, 8, 64, device="cuda"), k, k, i(3, 4), i(3), i(4)).shape == (9, 8, 64)
+        assert cuda_ops.paged_reserve([k], i(3, 4), i(3), i(3))[2].dtype is torch.bool
+    meta = lambda *s: torch.empty(*s, dtype=torch.int32, device="meta")  # noqa: E731
+    k = torch.empty(10, 16, 2, 64, device="meta")
+    with Seen():
+        cuda_ops.paged_compact([k, k], meta(3, 4), meta(3))
+        cuda_ops.paged_copy_pages([k], meta(2), meta(2))
+        cuda_ops.paged_kv_append(k, k, k[:, 0], k[:, 0], meta(3, 4), meta(3), indptr=meta(4))
+    for name in ("paged_compact", "paged_copy_pages", "paged_kv_append_chunks"):
+        assert any(name in n for n in Seen.names), name
+
+
 def test_cpu_tensors_are_refused():
     from kernel_lab import cuda_ops
 

@@ -242,6 +242,71 @@ def test_strided_queries(stride, dim):
     p.check(p.run(flipped))
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+@pytest.mark.parametrize("page", [8, 16, 64])
+@pytest.mark.parametrize("layout", ["heads", "interleaved", "padded", "fused"])
+@pytest.mark.parametrize("hkv", [1, 2])
+def test_caches_of_any_layout(dim, page, layout, hkv):
+    """Pages head by head, keys beside values in one pool, pages and tokens with gaps, keys and values of a token side by side."""
+    from kernel_lab import cuda_ops
+
+    p = Problem(EDGES, 4 * hkv, hkv, dim, page, torch.bfloat16, seed=18)
+    k, v = p.cache["k"].cuda(), p.cache["v"].cuda()
+    if layout == "heads":
+        k, v = (x.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for x in (k, v))
+    elif layout == "interleaved":
+        both = torch.stack([k, v], dim=1)
+        k, v = both[:, 0], both[:, 1]
+    elif layout == "fused":
+        both = torch.cat([k, v], dim=2)
+        k, v = both[:, :, :hkv], both[:, :, hkv:]
+    else:
+        k, v = (torch.nn.functional.pad(x, (0, 8, 0, 1, 0, 3), value=float("nan"))[:, :page, :hkv, :dim] for x in (k, v))
+    ints = [torch.from_numpy(np.asarray(x, np.int32)).cuda() for x in (p.table, p.lens, p.indptr)]
+    p.check(cuda_ops.paged_chunk_attention(p.q.cuda(), k, v, *ints))
+
+
+def test_a_pool_of_one_page():
+    p = Problem([(5, 16)], 8, 2, 128, 16, torch.float16, seed=19, spare=0)
+    p.check(p.run())
+
+
+@pytest.mark.parametrize("kind", ["same", "block8"])
+def test_captured_calls_replay_beside_one_another(kind):
+    """Two graphs and eager calls, whose split blocks all meet in scratch, on three streams."""
+    problems = [Problem([(1, 5000), (3, 900), (40, 64)], 8, 2, 128, 16, torch.bfloat16, kind, seed=s) for s in (20, 21)]
+    from kernel_lab import cuda_ops
+
+    name = "paged_chunk_attention" + {"same": "", "block8": "_block8"}[kind]
+    calls = []
+    for p in problems:
+        args = [p.q.cuda(), p.device_cache("k"), p.device_cache("v")]
+        args += [p.scale[n].cuda() for n in "kv"] if kind == "block8" else []
+        args += [torch.from_numpy(np.asarray(x, np.int32)).cuda() for x in (p.table, p.lens, p.indptr)]
+        calls.append(lambda args=args: getattr(cuda_ops, name)(*args))
+    eager = [c() for c in calls]
+    graphs = []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = c()
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    extra = []
+    for _ in range(20):
+        for (g, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            extra.append(calls[0]())
+    torch.cuda.synchronize()
+    for (_, out), want, p in zip(graphs, eager, problems):
+        assert torch.equal(out, want)
+        p.check(out)
+    assert all(torch.equal(e, eager[0]) for e in extra)
+
+
 def test_caches_at_odd_addresses():
     """Caches whose rows start on no 16 bytes."""
     from kernel_lab import cuda_ops

@@ -298,3 +298,18 @@ def test_a_captured_step_replays_with_other_inputs():
         want = torch.einsum("hij,jhd->ihd", torch.softmax(s, -1), values)
         # bf16: probabilities and outputs rounded, 2^-8 each of values of at most 4.
         assert (out[ptr[b] : ptr[b + 1]].double() - want).abs().max() <= 2 * 4 * 2.0**-8
+
+
+def test_the_example_runs():
+    """A prompt of 602 tokens in 38 pages; four samples, three with a copy of the last page; two go on, at 605 + 1 and 608 - 2 + 1."""
+    import importlib.util
+
+    from tests.conftest import REPO
+
+    spec = importlib.util.spec_from_file_location("chunk_step", REPO / "examples" / "chunk_step.py")
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.main()
+    assert got["tokens"] == (602 + 1 + 5 + 1) + (602 + 1 + 3 + 1)
+    # 37 full pages shared, the 38th each row's own, the 39th (tokens from 608 on) the first row's.
+    assert got["pages after the fork"] == 37 + 4 and got["pages at the end"] == 37 + 2 + 1
