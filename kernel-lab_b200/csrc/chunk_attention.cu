@@ -19,8 +19,9 @@ namespace chunk_attention {
 // ----------------------------------------------------------------- CUDA-core kernel
 //
 // Any dtype, cache, group, head_dim up to 256, page size and stride. A CTA takes kRows rows of one KV head and
-// walks their keys kKeys at a time: K and V widened to fp32 in shared memory, a thread per four scores, eight
-// threads a row for the softmax and for the row's output.
+// walks their keys kKeys at a time: K and V widened to fp32 in shared memory (rows padded with zeros to whole float4s), a thread
+// per four scores, eight threads a row for the softmax and for the row's output. Bound by shared-memory loads: a float4 of
+// q and four of K for 16 multiply-adds.
 
 constexpr int kRows = 16, kKeys = 32, kThreads = 128, kMaxDim = 256;
 
@@ -37,7 +38,12 @@ struct Code<int8_t> {
   static __device__ __forceinline__ float load(int8_t v) { return static_cast<float>(v); }
 };
 
-size_t generic_smem(int dim) { return sizeof(float) * (static_cast<size_t>(kRows) * dim + kKeys * (2 * dim + 1) + kRows * kKeys); }
+// Floats between rows of K (and of q and V without the last four): whole float4s, K's rows in turn on other banks.
+__host__ __device__ __forceinline__ int padded(int dim) { return (dim + 3) / 4 * 4; }
+size_t generic_smem(int dim) {
+  const size_t d = padded(dim);
+  return sizeof(float) * (kRows * d + kKeys * (2 * d + 4) + kRows * kKeys);
+}
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant__ Args a) {
@@ -47,10 +53,11 @@ __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant
   __shared__ int64_t s_page[kKeys];  // a key's page, -1: not to be attended to
   __shared__ int s_slot[kKeys];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, dim = a.dim;
-  float* sq = smem;                  // [kRows][dim]
-  float* sk = sq + kRows * dim;      // [kKeys][dim + 1]
-  float* sv = sk + kKeys * (dim + 1);
-  float* sp = sv + kKeys * dim;      // [kRows][kKeys]; -1: masked
+  const int wide = padded(dim), k_row = wide + 4;
+  float* sq = smem;                  // [kRows][wide]
+  float* sk = sq + kRows * wide;     // [kKeys][wide + 4]
+  float* sv = sk + kKeys * k_row;    // [kKeys][wide]
+  float* sp = sv + kKeys * wide;     // [kRows][kKeys]; -1: masked
   wait_prior_grid();
   allow_next_grid();
 
@@ -90,22 +97,21 @@ __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant
   const Seq s = read_seq(a, b, tid == 0);
   const int64_t row0 = static_cast<int64_t>(s_found[1]) * kRows, rows = static_cast<int64_t>(s.n) * a.group;
 
-  for (int i = tid; i < kRows * dim; i += kThreads) {
-    const int64_t r = row0 + i / dim;
-    float x = 0.0f;
-    if (r < rows) {
-      const int64_t token = s.first + r / a.group;
-      x = Storage<T>::load(static_cast<const T*>(a.q)[token * a.q_stride + (kvh * a.group + r % a.group) * static_cast<int64_t>(dim) + i % dim]);
-    }
-    sq[i] = x;
+  for (int i = warp; i < kRows; i += kThreads / 32) {
+    const int64_t r = row0 + i;
+    const bool there = r < rows;
+    const int64_t token = s.first + (there ? r / a.group : 0);
+    const T* const from = static_cast<const T*>(a.q) + token * a.q_stride + (kvh * a.group + (there ? r % a.group : 0)) * static_cast<int64_t>(dim);
+    for (int d = lane; d < wide; d += 32) sq[i * wide + d] = there && d < dim ? Storage<T>::load(from[d]) : 0.0f;
   }
   const int r = tid >> 3, part = tid & 7;  // this thread's row, and its eighth of the row
   const int64_t my_row = row0 + r;
   const int limit = my_row < rows ? keys_of(a, s, static_cast<int>(my_row / a.group)) : 0;
   const int last_limit = keys_of(a, s, static_cast<int>((min(rows, row0 + kRows) - 1) / a.group));
-  float acc[kMaxDim / 8];
+  constexpr int kParts = kMaxDim / 32;  // float4s of the row's output a thread: columns 4 * part + 32 * i
+  float4 acc[kParts];
 #pragma unroll
-  for (int i = 0; i < kMaxDim / 8; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < kParts; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float m = -INFINITY, l = 0.0f;
 
   for (int k0 = 0; k0 < last_limit; k0 += kKeys) {
@@ -124,30 +130,57 @@ __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant
       s_slot[tid] = j % a.page_size;
     }
     __syncthreads();
-    for (int i = tid; i < kKeys * dim; i += kThreads) {
-      const int j = i / dim, d = i - j * dim;
+    // A warp's four keys, 64 columns of each in flight.
+    constexpr int kMine = kKeys / (kThreads / 32);
+    float ks[kMine], vs[kMine];
+    int64_t at[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = warp + i * (kThreads / 32);
       const int64_t page = s_page[j];
-      float x = 0.0f, y = 0.0f;
-      if (page >= 0) {
-        const int64_t at = page * a.page_stride + s_slot[j] * a.token_stride + kvh * a.head_stride + d;
-        x = Code<C>::load(static_cast<const C*>(a.k)[at]);
-        y = Code<C>::load(static_cast<const C*>(a.v)[at]);
-        if (!std::is_same<C, T>::value) {
-          x *= __ldcg(a.k_scale + page * a.scale_stride + kvh);
-          y *= __ldcg(a.v_scale + page * a.scale_stride + kvh);
+      at[i] = page < 0 ? -1 : page * a.page_stride + s_slot[j] * a.token_stride + kvh * a.head_stride;
+      ks[i] = vs[i] = 1.0f;
+      if (!std::is_same<C, T>::value && page >= 0) {
+        ks[i] = __ldcg(a.k_scale + page * a.scale_stride + kvh);
+        vs[i] = __ldcg(a.v_scale + page * a.scale_stride + kvh);
+      }
+    }
+    for (int d0 = lane; d0 < wide; d0 += 64) {
+      float x[kMine][2], y[kMine][2];
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int d = d0 + 32 * u;
+          const bool there = at[i] >= 0 && d < dim;
+          x[i][u] = there ? Code<C>::load(static_cast<const C*>(a.k)[at[i] + d]) : 0.0f;
+          y[i][u] = there ? Code<C>::load(static_cast<const C*>(a.v)[at[i] + d]) : 0.0f;
         }
       }
-      sk[j * (dim + 1) + d] = x;
-      sv[i] = y;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int j = warp + i * (kThreads / 32);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int d = d0 + 32 * u;
+          if (d >= wide) break;
+          sk[j * k_row + d] = std::is_same<C, T>::value || at[i] < 0 ? x[i][u] : x[i][u] * ks[i];
+          sv[j * wide + d] = std::is_same<C, T>::value || at[i] < 0 ? y[i][u] : y[i][u] * vs[i];
+        }
+      }
     }
     __syncthreads();
     float x[kKeys / 8];
 #pragma unroll
     for (int i = 0; i < kKeys / 8; ++i) x[i] = 0.0f;
-    for (int d = 0; d < dim; ++d) {
-      const float qd = sq[r * dim + d];
+#pragma unroll 4
+    for (int d = 0; d < wide; d += 4) {
+      const float4 qd = *reinterpret_cast<const float4*>(sq + r * wide + d);
 #pragma unroll
-      for (int i = 0; i < kKeys / 8; ++i) x[i] = fmaf(qd, sk[(part + 8 * i) * (dim + 1) + d], x[i]);
+      for (int i = 0; i < kKeys / 8; ++i) {
+        const float4 kd = *reinterpret_cast<const float4*>(sk + (part + 8 * i) * k_row + d);
+        x[i] = fmaf(qd.x, kd.x, fmaf(qd.y, kd.y, fmaf(qd.z, kd.z, fmaf(qd.w, kd.w, x[i]))));
+      }
     }
     float mc = -INFINITY;
     bool seen[kKeys / 8];
@@ -175,14 +208,19 @@ __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant
     l = l * alpha + sum;
     __syncwarp();  // a row's eight threads are in one warp
 #pragma unroll
-    for (int i = 0; i < kMaxDim / 8; ++i) acc[i] *= alpha;
+    for (int i = 0; i < kParts; ++i) acc[i] = make_float4(acc[i].x * alpha, acc[i].y * alpha, acc[i].z * alpha, acc[i].w * alpha);
+#pragma unroll 4
     for (int j = 0; j < kKeys; ++j) {
       const float p = sp[r * kKeys + j];
       if (p < 0.0f) continue;  // masked, whatever V holds
 #pragma unroll
-      for (int i = 0; i < kMaxDim / 8; ++i) {
-        const int d = part + 8 * i;
-        if (d < dim) acc[i] = fmaf(p, sv[j * dim + d], acc[i]);
+      for (int i = 0; i < kParts; ++i) {
+        if (32 * i >= wide) break;
+        const int d = 4 * part + 32 * i;
+        if (d < wide) {
+          const float4 v = *reinterpret_cast<const float4*>(sv + j * wide + d);
+          acc[i] = make_float4(fmaf(p, v.x, acc[i].x), fmaf(p, v.y, acc[i].y), fmaf(p, v.z, acc[i].z), fmaf(p, v.w, acc[i].w));
+        }
       }
     }
   }
@@ -190,9 +228,13 @@ __global__ void __launch_bounds__(kThreads) generic_kernel(const __grid_constant
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   T* out = static_cast<T*>(a.out) + ((s.first + my_row / a.group) * a.hq + kvh * a.group + my_row % a.group) * dim;
 #pragma unroll
-  for (int i = 0; i < kMaxDim / 8; ++i) {
-    const int d = part + 8 * i;
-    if (d < dim) out[d] = Storage<T>::store(acc[i] * inv);
+  for (int i = 0; i < kParts; ++i) {
+    const float o[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int d = 4 * part + 32 * i + u;
+      if (d < dim) out[d] = Storage<T>::store(o[u] * inv);
+    }
   }
 }
 

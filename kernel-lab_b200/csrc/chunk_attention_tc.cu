@@ -1091,15 +1091,6 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       }
 #pragma unroll 1
       for (int k0 = 0; k0 < pieces; k0 += 2) {
-        // Lanes 0 to 7 weigh the four rows' two pieces.
-        const int rr = min(31, r0 + (lane >> 1 & 3)), kk = k0 + (lane & 1);
-        const float row_top = __shfl_sync(0xffffffffu, top, rr);
-        float f = 0.0f;
-        if (kk < pieces && lane < 8) {
-          const float* const pc = piece(kk) + DP * 128 + row0 + rr;
-          const float pm = __ldcg(pc), pl = __ldcg(pc + 128);
-          f = pl == 0.0f ? 0.0f : exp2_approx(pm - row_top);
-        }
         Vf x[4][2][kCols < 4 ? 1 : kCols / 4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -1109,6 +1100,15 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
 #pragma unroll
             for (int i = 0; i < kCols; i += sizeof(Vf) / 4) x[r][k][i * 4 / sizeof(Vf)] = load_cg<Vf>(from + i);
           }
+        }
+        // Lanes 0 to 7 weigh the four rows' two pieces.
+        const int rr = min(31, r0 + (lane >> 1 & 3)), kk = k0 + (lane & 1);
+        const float row_top = __shfl_sync(0xffffffffu, top, rr);
+        float f = 0.0f;
+        if (kk < pieces && lane < 8) {
+          const float* const pc = piece(kk) + DP * 128 + row0 + rr;
+          const float pm = __ldcg(pc), pl = __ldcg(pc + 128);
+          f = pl == 0.0f ? 0.0f : exp2_approx(pm - row_top);
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
