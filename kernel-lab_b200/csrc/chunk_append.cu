@@ -206,7 +206,7 @@ cudaError_t launch_e4m3(const Args& a, cudaStream_t st) {
 int refused(const Args& a, int dtype) {
   if (a.batch < 0 || a.tokens < 0 || a.tokens > INT32_MAX || a.head_dim <= 0 || a.row_elems <= 0 || a.page_size <= 0 ||
       a.max_pages < 0 || a.bt_stride < a.max_pages || a.num_pages < 0 || a.new_stride < a.row_elems || !a.k_cache ||
-      !a.v_cache || !a.k_new || !a.v_new || !a.block_table || !a.positions || !a.indptr) {
+      !a.v_cache || !a.k_new || !a.v_new || (!a.block_table && a.max_pages > 0) || !a.positions || !a.indptr) {
     return static_cast<int>(cudaErrorInvalidValue);
   }
   const bool known = dtype == KL_FLOAT32 || dtype == KL_FLOAT16 || dtype == KL_BFLOAT16;

@@ -295,7 +295,7 @@ extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, con
       q_row_stride < static_cast<int64_t>(num_q_heads) * head_dim || page_stride < 0 || token_stride < 0 || head_stride < 0) {
     return invalid;
   }
-  if (!out || !q || !k_cache || !v_cache || !block_table || !seq_lens || !indptr || !sync || sync_bytes < 256) return invalid;
+  if (!out || !q || !k_cache || !v_cache || (!block_table && max_pages_per_seq > 0) || !seq_lens || !indptr || !sync || sync_bytes < 256) return invalid;
   Args a{};
   a.out = out;
   a.q = q;

@@ -17,6 +17,7 @@ LIB_PATH = Path(__file__).with_name("libkernel_lab_b200.so")
 
 KL_FLOAT32, KL_FLOAT16, KL_BFLOAT16 = 0, 1, 2
 KL_STATUS_BAD_PAGE, KL_STATUS_LEN_CLAMPED, KL_STATUS_WAIT_TIMEOUT = 1, 2, 4
+KL_STATUS_NO_PAGES = 32
 DTYPE_CODES = {torch.float32: KL_FLOAT32, torch.float16: KL_FLOAT16, torch.bfloat16: KL_BFLOAT16}
 
 _c_int, _c_i64, _c_float, _c_vp, _c_sz = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t

@@ -496,3 +496,67 @@ def test_a_prompt_in_chunks_is_the_prompt_at_once(kind):
             assert torch.equal(again.double(), outs[-1][-24:]) or (again.double() - outs[-1][-24:]).abs().max() < 2.0**-6
     # Probabilities and outputs are rounded in both: 4 roundings of bf16 of values below 4.
     assert (outs[0] - outs[1]).abs().max() <= 4 * 4 * 2.0**-8
+
+
+# ------------------------------------------------------------------ refusals
+
+
+def test_attention_refusals():
+    from kernel_lab import cuda_ops
+
+    i = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    f = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    good = {"q": f(9, 8, 64), "k_cache": f(10, 16, 2, 64), "v_cache": f(10, 16, 2, 64), "block_table": i(3, 4), "seq_lens": i(3), "indptr": i(4)}
+    cuda_ops.paged_chunk_attention(**good)
+    k = good["k_cache"]
+    for name, bad in [
+        ("q", f(9, 8, 32)), ("q", f(9, 7, 64)), ("q", f(9, 512)[:, None, :64].half()), ("q", good["q"].cpu()), ("v_cache", f(10, 16, 4, 64)[:, :, ::2]),
+        ("v_cache", f(10, 16, 1, 64)), ("k_cache", f(10, 16, 2, 128)[..., ::2]), ("block_table", i(3, 4, dtype=torch.int64)), ("block_table", i(2, 4)),
+        ("block_table", i(3, 8)[:, ::2]), ("seq_lens", i(3, dtype=torch.int64)), ("seq_lens", i(6)[::2]), ("indptr", i(3)), ("indptr", i(4).cpu()),
+        ("indptr", i(4, dtype=torch.int64)), ("indptr", i(8)[::2]),
+    ]:
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_chunk_attention(**(good | {name: bad}))
+    with pytest.raises(RuntimeError):  # head_dim above 256
+        cuda_ops.paged_chunk_attention(f(9, 8, 320), f(10, 16, 2, 320), f(10, 16, 2, 320), i(3, 4), i(3), i(4))
+    k8, s, ps = k.to(torch.float8_e4m3fn), f(2, dtype=torch.float32), f(10, 2, dtype=torch.float32)
+    tables = good["block_table"], good["seq_lens"], good["indptr"]
+    cuda_ops.paged_chunk_attention_fp8(good["q"], k8, k8, s, s, *tables)
+    cuda_ops.paged_chunk_attention_block8(good["q"], k8, k8, ps, ps, *tables)
+    for args in [(good["q"].float(), k8, k8, s, s), (good["q"], k, k, s, s), (good["q"], k8, k8, ps, ps), (good["q"], k8, k8, s, s.half())]:
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_chunk_attention_fp8(*args, *tables)
+    for args in [(good["q"], k, k, ps, ps), (good["q"], k8, k8, s, s), (good["q"].float(), k8, k8, ps, ps)]:
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_chunk_attention_block8(*args, *tables)
+
+
+def test_nothing_to_do():
+    """No tokens, no sequences, a table without columns."""
+    from kernel_lab import cuda_ops
+
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    f = lambda *s: torch.ones(*s, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+    k = f(10, 16, 2, 64)
+    assert cuda_ops.paged_chunk_attention(f(0, 8, 64), k, k, i(3, 4), i(3), i(4)).shape == (0, 8, 64)
+    assert cuda_ops.paged_chunk_attention(f(5, 8, 64), k, k, i(0, 4), i(0), i(1)).shape == (5, 8, 64)
+    ptr = torch.tensor([0, 2, 5], dtype=torch.int32, device="cuda")
+    assert (cuda_ops.paged_chunk_attention(f(5, 8, 64), k, k, i(2, 0), i(2), ptr) == 0).all()
+    cuda_ops.paged_kv_append(k, k.clone(), f(0, 2, 64), f(0, 2, 64), i(3, 4), i(3), indptr=i(4))
+
+
+def test_append_refusals():
+    from kernel_lab import cuda_ops
+
+    i = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    f = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    good = [f(10, 16, 2, 64), f(10, 16, 2, 64), f(9, 2, 64), f(9, 2, 64), i(3, 4), i(3)]
+    for at, bad in [(0, f(10, 16, 4, 64)[:, :, ::2]), (1, f(10, 16, 1, 64)), (2, f(9, 2, 32)), (3, f(9, 4, 64)[:, ::2]), (2, f(9, 2, 64, dtype=torch.half)),
+                    (4, i(2, 4)), (5, i(3, dtype=torch.int64))]:
+        args = [*good]
+        args[at] = bad
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_kv_append(*args, indptr=i(4))
+    for ptr in (i(3), i(4).cpu(), i(4, dtype=torch.int64)):
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_kv_append(*good, indptr=ptr)

@@ -313,3 +313,46 @@ def test_the_example_runs():
     assert got["tokens"] == (602 + 1 + 5 + 1) + (602 + 1 + 3 + 1)
     # 37 full pages shared, the 38th each row's own, the 39th (tokens from 608 on) the first row's.
     assert got["pages after the fork"] == 37 + 4 and got["pages at the end"] == 37 + 2 + 1
+
+
+def test_refusals():
+    from kernel_lab import cuda_ops
+
+    i = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device="cuda")  # noqa: E731
+    k = torch.zeros(10, 16, 2, 8, device="cuda")
+    for caches in ([], [k, k[:9]], [k.cpu()], [k[:, ::2]], [k[:1].expand(10, -1, -1, -1)], [k[..., :7]], [torch.zeros((), device="cuda")]):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            cuda_ops.paged_copy_pages(caches, i(2), i(2))
+    for src, dst in ((i(2), i(3)), (i(2, dtype=torch.int64), i(2, dtype=torch.int64)), (i(4)[::2], i(2)), (i(2).cpu(), i(2).cpu())):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            cuda_ops.paged_copy_pages([k], src, dst)
+    for table, lens, new, parents in ((i(3, 4), i(3), i(2), None), (i(3, 4), i(4), i(3), None), (i(3, 4), i(3), i(3), i(2)), (i(3, 8)[:, ::2], i(3), i(3), None),
+                                      (i(3, 4, dtype=torch.int64), i(3), i(3), None), (i(3, 4), i(3), i(3, dtype=torch.int64), None)):
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_reserve([k], table, lens, new, parents)
+    for size in (0, -1):
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_reserve([k], i(3, 4), i(3), i(3), page_size=size)
+        with pytest.raises(RuntimeError):
+            cuda_ops.paged_compact([k], i(3, 4), i(3), page_size=size)
+    with pytest.raises(RuntimeError):
+        cuda_ops.paged_compact([k], i(3, 4), i(4))
+    with pytest.raises(RuntimeError):  # the new table in the old one's place
+        table = i(3, 4)
+        torch.ops.kernel_lab.paged_compact(table, i(()), [k], table, i(3), 16)
+
+
+def test_nothing_to_do():
+    from kernel_lab import cuda_ops
+
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    k = torch.ones(10, 16, 2, 8, device="cuda")
+    table, lens, served = cuda_ops.paged_reserve([k], i(0, 4), i(0), i(0))
+    assert table.shape == (0, 4) and lens.numel() == served.numel() == 0
+    table, lens, served = cuda_ops.paged_reserve([k], i(2, 0), i(2), i(2))
+    assert table.shape == (2, 0) and served.all()
+    table, lens, served = cuda_ops.paged_reserve([k], i(0, 4), i(0), i(3) + 1, i(3))  # parents of no sequences
+    assert (table == 0).all() and served.all()
+    table, used = cuda_ops.paged_compact([k], i(0, 4), i(0))
+    assert table.shape == (0, 4) and int(used) == 0
+    cuda_ops.decode_status(clear=True)
