@@ -132,7 +132,8 @@ int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const 
  * and entries outside [0, num_pages) are taken over but stand for no page (KL_STATUS_BAD_PAGE); negative
  * new_tokens count as 0. rows at most 2^24. Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's
  * rules (`sync` zero before its first use, left zero but for the status word; calls that overlap on the GPU need
- * separate buffers).
+ * separate buffers). A call launches several kernels that hand data on through the scratch: nothing else that uses these
+ * buffers may be put on the stream, by another host thread for instance, until it has returned.
  */
 int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes, size_t* sync_bytes);
 

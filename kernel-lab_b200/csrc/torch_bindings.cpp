@@ -22,6 +22,9 @@
 // leaves them zero. Entries live as long as the process (a stream that is destroyed keeps its entry, so a
 // host that creates streams per request should reuse a pool of them), and so do outgrown buffers, each
 // less than 4/5 of the next: kernels in flight or another thread's launch may still use them.
+// Some calls launch kernels that hand data on through the scratch (a cascade's prefix, the marks and the plan of
+// paged_reserve and paged_compact). So a call has its stream's scratch to itself until all of them are launched, whatever
+// other threads put on that stream.
 //
 // Calls that are captured into a CUDA graph have scratch of their own, one pair per capture and
 // stream: a graph may be replayed on any stream, at the same time as other graphs and eager calls,
@@ -111,6 +114,11 @@ struct Scratch {
   at::Tensor sync;      // uint8, zero at rest
 };
 
+// Scratch for one call, and the right to launch kernels that use it.
+struct HeldScratch : Scratch {
+  std::unique_lock<std::mutex> launching;
+};
+
 size_t scratch_size(size_t bytes) { return std::max<size_t>(bytes, 256) * 5 / 4; }
 bool holds(const at::Tensor& t, size_t bytes) { return t.defined() && static_cast<size_t>(t.numel()) >= bytes; }
 
@@ -125,6 +133,7 @@ struct GraphScratch {
 
 struct ScratchPool {
   std::mutex mu;
+  std::map<std::pair<int, cudaStream_t>, std::mutex> launching;  // one of these is taken before mu, never after it
   std::map<std::pair<int, cudaStream_t>, Scratch> streams;
   std::vector<at::Tensor> outgrown;
   std::vector<std::unique_ptr<GraphScratch>> graphs;
@@ -238,20 +247,31 @@ Scratch graph_scratch(ScratchPool& pool, const at::Device& dev, cudaStream_t str
   return s;
 }
 
-// The buffers for a call on `stream`, the current one of `dev`.
-Scratch scratch_for(const at::Device& dev, cudaStream_t stream, size_t partial_bytes, size_t sync_bytes) {
+// The right to launch on `stream` with its scratch (of its own or of what it captures).
+std::unique_lock<std::mutex> launching_on(ScratchPool& pool, const at::Device& dev, cudaStream_t stream) {
+  std::mutex* mu;
+  {
+    const std::lock_guard<std::mutex> lock(pool.mu);
+    mu = &pool.launching[{dev.index(), stream}];
+  }
+  return std::unique_lock<std::mutex>(*mu);
+}
+
+// The buffers for a call on `stream`, the current one of `dev`; the result lives until the call has launched its kernels.
+HeldScratch scratch_for(const at::Device& dev, cudaStream_t stream, size_t partial_bytes, size_t sync_bytes) {
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
   unsigned long long capture = 0;
   cudaGraph_t graph = nullptr;
   C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &capturing, &capture, &graph, nullptr, nullptr));
   ScratchPool& pool = scratch_pool();
+  std::unique_lock<std::mutex> launching = launching_on(pool, dev, stream);
   const std::lock_guard<std::mutex> lock(pool.mu);
   if (capturing != cudaStreamCaptureStatusNone) {
     const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
-    return graph_scratch(pool, dev, stream, capture, graph, partial_bytes, sync_bytes);
+    return {graph_scratch(pool, dev, stream, capture, graph, partial_bytes, sync_bytes), std::move(launching)};
   }
   Scratch& s = pool.streams[{dev.index(), stream}];
-  if (holds(s.partials, partial_bytes) && holds(s.sync, sync_bytes)) return s;
+  if (holds(s.partials, partial_bytes) && holds(s.sync, sync_bytes)) return {s, std::move(launching)};
   const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
   if (!holds(s.partials, partial_bytes)) {
     const at::Tensor grown = scratch_buffer(pool, dev, partial_bytes);
@@ -269,7 +289,7 @@ Scratch scratch_for(const at::Device& dev, cudaStream_t stream, size_t partial_b
     }
     s.sync = grown;
   }
-  return s;
+  return {s, std::move(launching)};
 }
 
 void paged_decode_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
@@ -313,7 +333,7 @@ void paged_decode_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor& k
                                               max_pages, static_cast<int>(num_splits), &partial_bytes,
                                               &sync_bytes),
                "paged_decode_attention (workspace)");
-  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(kl_paged_decode(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch, num_q_heads,
                                num_kv_heads, head_dim, page_size, block_table.stride(0), max_pages,
@@ -368,7 +388,7 @@ void paged_kv_append(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor&
   if (batch == 0) return;
   const c10::cuda::CUDAGuard guard(k_new.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(k_new.device(), stream, 0, 4);
+  const HeldScratch s = scratch_for(k_new.device(), stream, 0, 4);
   check_status(kl_paged_kv_append(to_dtype(k_cache.scalar_type()), k_cache.data_ptr(), v_cache.data_ptr(),
                                   k_new.data_ptr(), v_new.data_ptr(), block_table.data_ptr<int32_t>(),
                                   positions.data_ptr<int32_t>(), static_cast<int>(batch),
@@ -426,7 +446,7 @@ void paged_decode_attention_fp8(at::Tensor& out, const at::Tensor& q, const at::
   check_status(kl_paged_decode_workspace_size(dtype, batch, num_q_heads, num_kv_heads, head_dim, page_size,
                                               max_pages, 0, &partial_bytes, &sync_bytes),
                "paged_decode_attention_fp8 (workspace)");
-  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(kl_paged_decode_fp8(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                    k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
                                    block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), batch,
@@ -468,7 +488,7 @@ void paged_kv_append_fp8(at::Tensor& k_cache, at::Tensor& v_cache, const at::Ten
   if (batch == 0) return;
   const c10::cuda::CUDAGuard guard(k_new.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(k_new.device(), stream, 0, 4);
+  const HeldScratch s = scratch_for(k_new.device(), stream, 0, 4);
   check_status(kl_paged_kv_append_fp8(to_dtype(k_new.scalar_type()), k_cache.data_ptr(), v_cache.data_ptr(),
                                       k_new.data_ptr(), v_new.data_ptr(), k_scale.data_ptr<float>(),
                                       v_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
@@ -538,7 +558,7 @@ void paged_decode_attention_cascade(at::Tensor& out, const at::Tensor& q, const 
                                                       num_kv_heads, head_dim, page_size, max_pages, max_prefix_pages,
                                                       &partial_bytes, &sync_bytes),
                "paged_decode_attention_cascade (workspace)");
-  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(
       kl_paged_decode_cascade(dtype, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                               fp8 ? k_scale->data_ptr<float>() : nullptr, fp8 ? v_scale->data_ptr<float>() : nullptr,
@@ -681,7 +701,7 @@ void paged_kv_append_block8(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor
   const int64_t row_stride = tokens == 1 ? num_kv_heads * head_dim : k_new.stride(0);
   const c10::cuda::CUDAGuard guard(k_cache.device());
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(k_cache.device(), stream, 0, 4);
+  const HeldScratch s = scratch_for(k_cache.device(), stream, 0, 4);
   check_status(
       kl_paged_kv_append_block8(to_dtype(k_new.scalar_type()), code_type, k_cache.data_ptr(), v_cache.data_ptr(),
                                 k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
@@ -733,7 +753,7 @@ void paged_decode_attention_block8(at::Tensor& out, const at::Tensor& q, const a
                                                      static_cast<int>(num_kv_heads), d, page, max_pages, num_selected,
                                                      &partial_bytes, &sync_bytes),
                "paged_decode_attention_block8 (workspace)");
-  const Scratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(q.device(), stream, partial_bytes, sync_bytes);
   check_status(
       kl_paged_decode_block8(to_dtype(q.scalar_type()), code_type, out.data_ptr(), rows.data_ptr(), k_cache.data_ptr(),
                              v_cache.data_ptr(), k_scale.data_ptr<float>(), v_scale.data_ptr<float>(),
@@ -776,7 +796,7 @@ void paged_block_select(at::Tensor& selected, const at::Tensor& q, const at::Ten
   check_status(kl_paged_block_select_workspace_size(static_cast<int>(batch), static_cast<int>(num_kv_heads), max_pages,
                                                     &scratch_bytes, &sync_bytes),
                "paged_block_select (workspace)");
-  const Scratch s = scratch_for(q.device(), stream, scratch_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(q.device(), stream, scratch_bytes, sync_bytes);
   check_status(
       kl_paged_block_select(to_dtype(q.scalar_type()), code_type, selected.data_ptr<int32_t>(), q.data_ptr(),
                             k_bounds.data_ptr(), k_scale.data_ptr<float>(), block_table.data_ptr<int32_t>(),
@@ -830,7 +850,7 @@ void append_chunks_impl(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tens
   const int64_t row_stride = tokens == 1 ? num_kv_heads * head_dim : k_new.stride(0);
   const c10::cuda::CUDAGuard guard(dev);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(dev, stream, 0, 4);
+  const HeldScratch s = scratch_for(dev, stream, 0, 4);
   uint32_t* const status = static_cast<uint32_t*>(s.sync.data_ptr());
   const int dtype = to_dtype(k_new.scalar_type()), heads = static_cast<int>(num_kv_heads), dim = static_cast<int>(head_dim);
   const int page = static_cast<int>(k_cache.size(1)), width = static_cast<int>(block_table.size(1)), b = static_cast<int>(batch);
@@ -897,7 +917,7 @@ void chunk_attention_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor
   check_status(kl_paged_chunk_attention_workspace_size(dtype, code_type, tokens, b, static_cast<int>(hq), static_cast<int>(hkv), d,
                                                        &partial_bytes, &sync_bytes),
                what);
-  const Scratch s = scratch_for(dev, stream, partial_bytes, sync_bytes);
+  const HeldScratch s = scratch_for(dev, stream, partial_bytes, sync_bytes);
   check_status(
       kl_paged_chunk_attention(dtype, code_type, out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                k_scale ? k_scale->data_ptr<float>() : nullptr, v_scale ? v_scale->data_ptr<float>() : nullptr,
@@ -987,7 +1007,7 @@ void paged_copy_pages(at::TensorList caches, const at::Tensor& src, const at::Te
   if (src.numel() == 0) return;
   const c10::cuda::CUDAGuard guard(p.device);
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-  const Scratch s = scratch_for(p.device, stream, 0, 4);
+  const HeldScratch s = scratch_for(p.device, stream, 0, 4);
   const kl_page_pools_t pools = p.c();
   check_status(kl_paged_copy_pages(&pools, src.data_ptr<int32_t>(), dst.data_ptr<int32_t>(), src.numel(), p.num_pages,
                                    static_cast<uint32_t*>(s.sync.data_ptr()), stream),
@@ -1021,7 +1041,7 @@ void paged_reserve(at::Tensor& out_table, at::Tensor& out_lens, at::Tensor& serv
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   size_t bytes = 0, sync_bytes = 0;
   check_status(kl_paged_reserve_workspace_size(p.num_pages, static_cast<int>(rows), &bytes, &sync_bytes), "paged_reserve (workspace)");
-  const Scratch s = scratch_for(p.device, stream, bytes, sync_bytes);
+  const HeldScratch s = scratch_for(p.device, stream, bytes, sync_bytes);
   const kl_page_pools_t pools = p.c();
   check_status(kl_paged_reserve(&pools, out_table.data_ptr<int32_t>(), out_lens.data_ptr<int32_t>(),
                                 reinterpret_cast<uint8_t*>(served.data_ptr<bool>()), block_table.data_ptr<int32_t>(),
@@ -1045,7 +1065,7 @@ void paged_compact(at::Tensor& out_table, at::Tensor& used, at::TensorList cache
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   size_t bytes = 0, sync_bytes = 0;
   check_status(kl_paged_compact_workspace_size(p.num_pages, &bytes, &sync_bytes), "paged_compact (workspace)");
-  const Scratch s = scratch_for(p.device, stream, bytes, sync_bytes);
+  const HeldScratch s = scratch_for(p.device, stream, bytes, sync_bytes);
   const kl_page_pools_t pools = p.c();
   check_status(kl_paged_compact(&pools, out_table.data_ptr<int32_t>(), used.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(),
                                 seq_lens.data_ptr<int32_t>(), static_cast<int>(batch), static_cast<int>(block_table.size(1)),
