@@ -554,6 +554,15 @@ cudaError_t launch_marks(void (*kernel)(PlanArgs), const PlanArgs& a, cudaStream
                        dim3(kMarkThreads), 0, st, a);
 }
 
+// The marks and the plan after them, which zeroes the marks. Where it cannot be launched, they are zeroed all the same.
+cudaError_t launch_plan(void (*marks)(PlanArgs), void (*plan)(PlanArgs), const PlanArgs& a, cudaStream_t st) {
+  cudaError_t e = launch_marks(marks, a, st);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(true, plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  if (e != cudaSuccess) (void)cudaMemsetAsync(a.mark, 0, sync_size(a.num_pages) - kMarksAt, st);
+  return e;
+}
+
 constexpr int kMaxRows = 1 << 24;
 
 bool sizes_ok(int batch, int rows, int width, int page_size, int64_t bt_stride, int64_t num_pages) {
@@ -625,9 +634,7 @@ extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table
   a.page_size = page_size;
   if (tables_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_marks(mark_pages<true>, a, st);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  e = klb::launch_kernel(true, reserve_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  const cudaError_t e = launch_plan(mark_pages<true>, reserve_plan, a, st);
   if (e != cudaSuccess) return static_cast<int>(e);
   return static_cast<int>(launch_copies(pools, a.src, a.dst, rows, a.count, num_pages, a.status, st));
 }
@@ -667,9 +674,7 @@ extern "C" int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table
   a.page_size = page_size;
   if (tables_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_marks(mark_pages<false>, a, st);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  e = klb::launch_kernel(true, compact_plan, dim3(kClusterCtas), dim3(kPlanThreads), 0, st, a);
+  const cudaError_t e = launch_plan(mark_pages<false>, compact_plan, a, st);
   if (e != cudaSuccess) return static_cast<int>(e);
   // Pages with ids of `used` and more that go below it: at most half of them.
   return static_cast<int>(launch_copies(pools, a.src, a.dst, num_pages / 2, a.count, num_pages, a.status, st));

@@ -177,6 +177,13 @@ at::Tensor scratch_buffer(ScratchPool& pool, const at::Device& dev, size_t bytes
   return at::empty({size}, opts);
 }
 
+// A call whose wait ran out leaves counters behind that later calls would go on from: zeroed once its status has been read.
+void zero_after_timeout(const at::Tensor& sync, uint32_t status, cudaStream_t stream) {
+  if (!(status & KL_STATUS_WAIT_TIMEOUT)) return;
+  C10_CUDA_CHECK(cudaMemsetAsync(sync.data_ptr(), 0, sync.numel(), stream));
+  C10_CUDA_CHECK(cudaStreamSynchronize(stream));
+}
+
 // Takes back the scratch of graphs that are gone.
 void collect_ended_graphs(ScratchPool& pool) {
   if (!pool.any_ended.load(std::memory_order_acquire)) return;
@@ -190,7 +197,9 @@ void collect_ended_graphs(ScratchPool& pool) {
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(g->device));
     for (const Scratch& s : g->grown) {
       uint32_t status = 0;
-      check_status(kl_paged_decode_read_status(s.sync.data_ptr(), &status, 1, side_stream(pool, g->device)), "scratch");
+      const cudaStream_t side = side_stream(pool, g->device);
+      check_status(kl_paged_decode_read_status(s.sync.data_ptr(), &status, 1, side), "scratch");
+      zero_after_timeout(s.sync, status, side);
       pool.spare_status[g->device] |= status;
       pool.spare[g->device].push_back(s);
     }
@@ -1075,6 +1084,18 @@ void paged_compact(at::Tensor& out_table, at::Tensor& used, at::TensorList cache
                "paged_compact");
 }
 
+// The sync buffers of the current device and stream and of the graphs captured on the device. With pool.mu held.
+std::vector<at::Tensor> sync_buffers(ScratchPool& pool, const at::Device& dev, cudaStream_t stream) {
+  std::vector<at::Tensor> buffers;
+  const auto it = pool.streams.find({dev.index(), stream});
+  if (it != pool.streams.end() && it->second.sync.defined()) buffers.push_back(it->second.sync);
+  for (const auto& p : pool.graphs) {
+    if (p->device != dev.index()) continue;
+    for (const Scratch& s : p->grown) buffers.push_back(s.sync);
+  }
+  return buffers;
+}
+
 // Status bits (KL_STATUS_*) left by decode calls on the current device and stream and by the graphs
 // captured on the device.
 int64_t decode_status(bool clear) {
@@ -1082,17 +1103,13 @@ int64_t decode_status(bool clear) {
   const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
   std::vector<at::Tensor> words;
   uint32_t status = 0;
+  ScratchPool& pool = scratch_pool();
+  const std::unique_lock<std::mutex> launching = launching_on(pool, dev, stream);
   {
-    ScratchPool& pool = scratch_pool();
     const std::lock_guard<std::mutex> lock(pool.mu);
     const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
     collect_ended_graphs(pool);
-    const auto it = pool.streams.find({dev.index(), stream});
-    if (it != pool.streams.end() && it->second.sync.defined()) words.push_back(it->second.sync);
-    for (const auto& p : pool.graphs) {
-      if (p->device != dev.index()) continue;
-      for (const Scratch& s : p->grown) words.push_back(s.sync);
-    }
+    words = sync_buffers(pool, dev, stream);
     uint32_t& gone = pool.spare_status[dev.index()];
     status = gone;
     if (clear) gone = 0;
@@ -1100,9 +1117,18 @@ int64_t decode_status(bool clear) {
   for (const at::Tensor& sync : words) {
     uint32_t bits = 0;
     check_status(kl_paged_decode_read_status(sync.data_ptr(), &bits, clear ? 1 : 0, stream), "decode_status");
+    if (clear) zero_after_timeout(sync, bits, stream);
     status |= bits;
   }
   return status;
+}
+
+// The buffers that decode_status() reads, for tests.
+std::vector<at::Tensor> current_sync_buffers() {
+  const at::Device dev(at::kCUDA, c10::cuda::current_device());
+  ScratchPool& pool = scratch_pool();
+  const std::lock_guard<std::mutex> lock(pool.mu);
+  return sync_buffers(pool, dev, at::cuda::getCurrentCUDAStream().stream());
 }
 
 // Whether a call on these tensors (or None) may go past the dispatcher without anyone's noticing: plain CUDA tensors, and no
@@ -1378,6 +1404,7 @@ TORCH_LIBRARY_IMPL(kernel_lab, Meta, m) {
 PYBIND11_MODULE(_C, m) {
   m.def("decode_status", &decode_status, pybind11::arg("clear") = false,
         "Status bits left by calls on the current device and stream and by the graphs captured on the device.");
+  m.def("current_sync_buffers", &current_sync_buffers, "The scratch that decode_status() reads and clears, for tests.");
   m.def("direct", &direct);
   m.def("rms_norm_fp8", &rms_norm_fp8_new);
   m.def("fused_add_rms_norm_fp8", &fused_add_rms_norm_fp8_new);

@@ -442,6 +442,8 @@ def paged_compact(
 
 def decode_status(clear: bool = False) -> int:
     """KL_STATUS_* bits left by decode, append and selection calls on the current device and stream, and
-    by those of CUDA graphs captured on the device (synchronises)."""
+    by those of CUDA graphs captured on the device (synchronises). After bit 4 (a wait inside a kernel ran out: the
+    results of that call, and of later ones on its scratch, are invalid) ``clear`` also zeroes the scratch's counters,
+    and calls work again; no graph that has the bit may run meanwhile."""
     _require()
     return int(_C.decode_status(clear))

@@ -2,7 +2,9 @@
 
 from __future__ import annotations
 
+import gc
 import threading
+import time
 
 import numpy as np
 import pytest
@@ -73,3 +75,70 @@ def test_threads_share_a_stream():
     assert not wrong
     with torch.cuda.stream(stream):
         assert cuda_ops.decode_status(clear=True) == 0
+
+
+def spoil(sync):
+    """What a call leaves whose wait ran out: the status bit, and counters (page marks, for the bookkeeping) that are not zero."""
+    words = sync[: sync.numel() // 4 * 4].view(torch.int32)
+    words[64:] = 1
+    words[0] = 4
+
+
+@pytest.mark.parametrize("call", [Pages, Attention])
+def test_clearing_a_timeout_makes_the_scratch_usable_again(call):
+    """No wait runs out here: its traces are written by hand. Nothing runs on them before they are cleared."""
+    from kernel_lab import _C, cuda_ops
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        cuda_ops.decode_status(clear=True)
+        run = call(5)
+        want = run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = run()
+        graph.replay()
+        stream.synchronize()
+        buffers = _C.current_sync_buffers()
+        for s in buffers:
+            spoil(s)
+        stream.synchronize()
+        assert cuda_ops.decode_status() == 4  # reading alone changes nothing
+        assert all(int(s[256]) == 1 for s in buffers)
+        assert cuda_ops.decode_status(clear=True) == 4 and cuda_ops.decode_status() == 0
+        assert not any(s.any() for s in buffers)
+        for _ in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(run(), want))
+            for t in got:
+                t.zero_()
+            graph.replay()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert cuda_ops.decode_status(clear=True) == 0
+
+
+def test_a_dead_graphs_timeout_is_cleared_before_its_scratch_is_used_again():
+    from kernel_lab import _C, cuda_ops
+
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        cuda_ops.decode_status(clear=True)
+        run = Attention(6)
+        want = run()
+        before = {s.data_ptr() for s in _C.current_sync_buffers()}
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run()
+        owned = [s for s in _C.current_sync_buffers() if s.data_ptr() not in before]
+        assert len(owned) == 1
+        spoil(owned[0])
+        stream.synchronize()
+        del graph
+        gc.collect()
+        time.sleep(0.05)
+        assert cuda_ops.decode_status(clear=True) == 4
+        assert not owned[0].any()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            got = run()
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and cuda_ops.decode_status() == 0
