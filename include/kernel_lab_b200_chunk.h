@@ -74,10 +74,11 @@ int kl_paged_kv_append_chunks_fp8(int dtype, void* k_cache, void* v_cache, const
  * times its value scale is rounded to bf16.
  *
  * Scratch from kl_paged_chunk_attention_workspace_size, under kl_paged_decode's rules (`sync` zero before its
- * first use, left zero but for the status word; calls that overlap on the GPU need separate buffers). After
- * KL_STATUS_WAIT_TIMEOUT the output is invalid and `sync` has to be zeroed again. fp16 and bf16 with head_dim a multiple
- * of 8 (of 16 over 8-bit caches), groups of up to 128 query heads, pages of a multiple of 8 tokens, a positive scale and
- * 16-byte aligned rows run on the tensor cores; everything else runs on the CUDA cores.
+ * first use, left zero but for the status word; calls that overlap on the GPU need separate buffers); partials start at a
+ * multiple of 32 bytes, sync at one of 4. After KL_STATUS_WAIT_TIMEOUT the output is invalid and `sync` has to be zeroed
+ * again. fp16 and bf16 with head_dim a multiple of 8 (of 16 over 8-bit caches), groups of up to 128 query heads, pages of a
+ * multiple of 8 tokens, a positive scale and 16-byte aligned rows run on the tensor cores; everything else runs on the
+ * CUDA cores.
  */
 int kl_paged_chunk_attention_workspace_size(int dtype, int code_type, int64_t tokens, int batch, int num_q_heads,
                                             int num_kv_heads, int head_dim, size_t* partial_bytes,

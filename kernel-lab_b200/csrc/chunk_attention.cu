@@ -296,6 +296,7 @@ extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, con
     return invalid;
   }
   if (!out || !q || !k_cache || !v_cache || (!block_table && max_pages_per_seq > 0) || !seq_lens || !indptr || !sync || sync_bytes < 256) return invalid;
+  if (reinterpret_cast<uintptr_t>(sync) % 4) return invalid;
   Args a{};
   a.out = out;
   a.q = q;
@@ -329,6 +330,7 @@ extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, con
   const int sms = sm_count();
   if (partials && partial_bytes >= tc_partial_bytes(head_dim, sms) && sync_bytes >= tc_sync_bytes(sms) &&
       tc_fits(a, dtype, code_type)) {
+    if (reinterpret_cast<uintptr_t>(partials) % 32) return invalid;  // pieces are stored 32 bytes at a time
     a.partials = static_cast<float*>(partials);
     a.counters = static_cast<uint32_t*>(sync) + 64;
     return static_cast<int>(launch_tc(a, dtype, code_type, sms, st));
