@@ -67,7 +67,7 @@ int kl_paged_kv_append_chunks_fp8(int dtype, void* k_cache, void* v_cache, const
  *         scale for each KV head, num_kv_heads one for each page and KV head; q is fp16 or bf16
  * Lengths beyond max_pages_per_seq * page_size are clamped (KL_STATUS_LEN_CLAMPED); pages whose id is outside
  * [0, num_pages) are skipped (KL_STATUS_BAD_PAGE). head_dim is at most 256, num_pages at least 1, batch at most
- * 65535, max_pages_per_seq * page_size below 2^31.
+ * 65535, tokens and max_pages_per_seq * page_size at most 2^31 - 257.
  *
  * Arithmetic: products accumulate in fp32, the softmax is in fp32. fp16 and bf16: a probability (relative to
  * its row's largest) is rounded to q's dtype. 8-bit caches: codes enter the products exactly, a probability

@@ -289,7 +289,7 @@ extern "C" int kl_paged_chunk_attention(int dtype, int code_type, void* out, con
   const bool coded = code_type != KL_CODE_NONE;
   if (coded && code_type != KL_CODE_E4M3 && code_type != KL_CODE_INT8) return invalid;
   if (coded && (dtype == KL_FLOAT32 || !k_scale || !v_scale || scale_page_stride < 0)) return invalid;
-  if (batch > 65535 || tokens > INT_MAX || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
+  if (batch > 65535 || tokens > INT_MAX - 256 || num_kv_heads <= 0 || num_kv_heads > 65535 || num_q_heads <= 0 || num_q_heads % num_kv_heads != 0 ||
       head_dim <= 0 || head_dim > kMaxDim || page_size <= 0 || max_pages_per_seq < 0 || block_table_stride < max_pages_per_seq ||
       num_pages < 1 || static_cast<int64_t>(max_pages_per_seq) * page_size > INT_MAX - 256 ||
       q_row_stride < static_cast<int64_t>(num_q_heads) * head_dim || page_stride < 0 || token_stride < 0 || head_stride < 0) {

@@ -916,7 +916,7 @@ void chunk_attention_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor
   check_tables(block_table, seq_lens, batch, dev, "seq_lens");
   check_indptr(indptr, batch, dev);
   for (int64_t d : k_cache.sizes()) TORCH_CHECK(d <= INT32_MAX, "cache dimensions must fit 32 bits");
-  TORCH_CHECK(batch <= 65535 && tokens <= INT32_MAX && hq <= INT32_MAX && block_table.size(1) <= INT32_MAX,
+  TORCH_CHECK(batch <= 65535 && tokens <= INT32_MAX - 256 && hq <= INT32_MAX && block_table.size(1) <= INT32_MAX,
               "too many sequences, tokens, heads or pages");
   if (batch == 0 || tokens == 0) return;
   const c10::cuda::CUDAGuard guard(dev);

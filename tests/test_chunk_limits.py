@@ -28,3 +28,10 @@ def test_pieces_are_stored_32_bytes_at_a_time(dim, code, scales):
     for at in (1, 2, 3):
         assert attend(dim=dim, code=code, scales=scales, sync=256 + at) == INVALID, at
         assert attend(dtype=0, sync=256 + at) == INVALID, at
+
+
+def test_chunks_that_32_bit_rows_cannot_count():
+    """A block has up to 256 tokens: one that ends past the last token is still counted in 32 bits."""
+    for tokens in (2**31 - 256, 2**31 - 2, 2**31 - 1, 2**31, 2**40):
+        assert attend(hq=1, hkv=1, dim=8, tokens=tokens) == INVALID, tokens
+        assert attend(hq=1, hkv=1, dim=8, tokens=tokens, dtype=0) == INVALID, tokens
