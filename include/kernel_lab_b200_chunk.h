@@ -126,7 +126,8 @@ int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const 
  *   then pages for the tokens len .. len + new_tokens[r] - 1 that its last page has no room for.
  * A row whose new tokens do not fit in the table's width, or for whose needs and those of the rows before it
  * the free pages do not suffice, gets none (KL_STATUS_NO_PAGES); a row that needs none is always served.
- *   out_table  [rows, width] int32, contiguous, not overlapping block_table: entries past a row's pages are 0
+ *   out_table  [rows, width] int32, contiguous, not overlapping block_table: entries past a row's pages are 0, which
+ *              is a page like any other: nothing may be appended for a row that was not served or is empty
  *   out_lens   [rows] int32: seq_lens[parents[r]] (new tokens not counted)
  *   served     [rows] bytes: 1, or 0 for a row that got none of what it needs
  * Lengths beyond width * page_size are clamped (KL_STATUS_LEN_CLAMPED), parents past the batch make empty rows

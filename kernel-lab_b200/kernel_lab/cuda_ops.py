@@ -406,8 +406,11 @@ def paged_reserve(
     it too (copied in every tensor of ``caches``; of several that only write to it the lowest row keeps it), then pages
     for the ``new_tokens[r]`` tokens that are to be appended at ``seq_lens[r]``. ``served[r]`` is False, and the row
     gets nothing, where the table is too narrow or the free pages run out (then
-    :func:`decode_status` has bit 32). The returned lengths do not count the new tokens. ``page_size`` is by default the
-    second dimension of the first cache."""
+    :func:`decode_status` has bit 32). Entries past a row's pages are 0, a page like any other: append for such a row at
+    position -1 (``torch.where(served, seq_lens, -1)``) and let its length be, or it writes to pages of others. An empty row
+    is served, whatever ``new_tokens`` says, and has no pages either; a parent past the last sequence makes one, without a
+    status bit. The returned lengths do not count the new tokens. ``page_size`` is by default the second dimension of the
+    first cache."""
     _require()
     caches = list(caches)
     page_size = caches[0].shape[1] if page_size is None else page_size
