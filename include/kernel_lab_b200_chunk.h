@@ -130,9 +130,9 @@ int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const 
  *              is a page like any other: nothing may be appended for a row that was not served or is empty
  *   out_lens   [rows] int32: seq_lens[parents[r]] (new tokens not counted)
  *   served     [rows] bytes: 1, or 0 for a row that got none of what it needs
- * Lengths beyond width * page_size are clamped (KL_STATUS_LEN_CLAMPED), parents past the batch make empty rows
- * and entries outside [0, num_pages) are taken over but stand for no page (KL_STATUS_BAD_PAGE); negative
- * new_tokens count as 0. rows at most 2^24. Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's
+ * Lengths beyond width * page_size are clamped (KL_STATUS_LEN_CLAMPED). Entries outside [0, num_pages) are taken over
+ * but stand for no page (KL_STATUS_BAD_PAGE). Parents past the batch make empty rows as negative ones do; they are not
+ * reported. An empty row has length 0, needs nothing and is served. Negative new_tokens count as 0. rows at most 2^24. Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's
  * rules (`sync` zero before its first use, left zero but for the status word; calls that overlap on the GPU need
  * separate buffers). A call launches several kernels that hand data on through the scratch: nothing else that uses these
  * buffers may be put on the stream, by another host thread for instance, until it has returned.
