@@ -346,7 +346,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of a pair on the multiply-add pipes, x <= 8 (NaN is not kept): 2^n 2^f with n the nearest whole number, f in [-1/2, 1/2],
+// 2^x of a pair on the multiply-add pipes, x <= 15 (NaN is not kept): 2^n 2^f with n the nearest whole number, f in [-1/2, 1/2],
 // and 2^f by 1 + c1 f + c2 f^2 + ..., the coefficients of least relative error (by linear programming over [-1/2, 1/2]):
 // 1.02e-4 with three of them (P in bf16, half a step 2^-8), 3.0e-6 with four (fp16, 2^-11). Zero from x = -127 down, exactly.
 template <int DEGREE>
@@ -818,6 +818,9 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
   using TV = std::conditional_t<L::kCoded, __nv_bfloat16, T>;  // of P and V
   const float sl = a.scale_log2;
   const uint64_t sl2 = pair(sl, sl);
+  // fp16 probabilities (and their sum) are held 2^7 times as large, at most 2^15 with kLazy: those below 2^-14 of a row's
+  // largest would lose bits to fp16's subnormals (16,000 keys of weight 2^-22 beside one of 1: 2 % of their share).
+  constexpr float kLift = std::is_same<TV, __half>::value ? 7.0f : 0.0f;
   uint32_t unit = 0, s_phase = 0, o_phase = 0, fix_phases = 0;
   bool ok = true;
   Segment g{};
@@ -900,7 +903,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           tmem_st8(tO + c, o);
         }
       }
-      const float shift = m == -INFINITY ? 0.0f : m;
+      const float shift = (m == -INFINITY ? 0.0f : m) - kLift;
       const uint64_t sh2 = pair(-shift, -shift);
       uint64_t sum[2] = {0, 0};
       // P, 32 columns at a time, over columns of S that have been read; the products with the first 64 keys may begin
