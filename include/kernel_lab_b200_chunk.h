@@ -69,9 +69,10 @@ int kl_paged_kv_append_chunks_fp8(int dtype, void* k_cache, void* v_cache, const
  * [0, num_pages) are skipped (KL_STATUS_BAD_PAGE). head_dim is at most 256, num_pages at least 1, batch at most
  * 65535, tokens and max_pages_per_seq * page_size at most 2^31 - 257.
  *
- * Arithmetic: products accumulate in fp32, the softmax is in fp32. fp16 and bf16: a probability is rounded to q's
- * dtype (fp16: to 2^-11 of itself where it is at least 2^-21 of its row's largest, by up to 2^-32 of that below). 8-bit caches: codes enter the products exactly, a probability
- * times its value scale is rounded to bf16.
+ * Arithmetic: products accumulate in fp32, the softmax is in fp32 (exponentials off by up to 1.1e-4 of themselves for bf16
+ * over 16-bit caches, 4e-6 otherwise). fp16 and bf16: a probability, over 8-bit caches one times its value scale (codes enter
+ * the products exactly), is rounded to q's dtype: bf16 to 2^-8 of itself, fp16 to 2^-11 where it is at least 2^-21 of
+ * its row's largest, by up to 2^-32 of that below.
  *
  * Scratch from kl_paged_chunk_attention_workspace_size, under kl_paged_decode's rules (`sync` zero before its
  * first use, left zero but for the status word; calls that overlap on the GPU need separate buffers); partials start at a

@@ -45,7 +45,7 @@ constexpr uint64_t kWaitCycles = 2000000000ull;  // about one second
 constexpr uint32_t kOddScales = 1u << 16;  // beside the bits of the unit's bad boxes
 // Units whose marks are told apart. A tile passes over the special units that it has no part in: that no wait of it is a phase
 // off takes slots for more units than the ring holds.
-constexpr int kFixSlots = 8, kBadSlots = 8;
+constexpr int kFixSlots = 8, kBadSlots = 6;
 constexpr int kCountersPerCta = 8;       // a counter for each warp's 32 rows of the two tiles
 
 // Tiles of a block: S and O of one take 128 + DP of the 512 columns of tensor memory.
@@ -72,8 +72,10 @@ struct Layout {
   static constexpr uint32_t kRaw = kRing + kStages * kTile;
   static constexpr uint32_t kBars = kRaw + kRawStages * kRawTile;
   static constexpr uint32_t kWords = kBars + 384;           // ints
-  static constexpr uint32_t kScales = kWords + 256;         // [kBadSlots][K, V][16]: a scale for every 8 keys
-  static constexpr uint32_t kBytes = kScales + (kCoded ? 1024 : 0) + 1024;  // slack to align the base to 1024 bytes
+  static constexpr uint32_t kScales = kWords + 256;         // [kBadSlots][K, V, log2 |V|][16]: a scale for every 8 keys
+  static constexpr uint32_t kBytes = kScales + (kCoded ? kBadSlots * 3 * 64 : 0) + 1024;  // slack to align the base to 1024 bytes
+  // A unit's marks and scales are written before its boxes wait for room: the unit kBadSlots before it has been used then.
+  static_assert(2 * kBadSlots >= kStages + kRawStages + 2, "slots of units");
   // Barriers of the rings.
   static constexpr int kFull = 24, kEmpty = kFull + kStages, kRawFull = kEmpty + kStages, kRawEmpty = kRawFull + kRawStages;
   static constexpr int kBarCount = kRawEmpty + kRawStages;
@@ -476,8 +478,9 @@ __device__ __forceinline__ void load_role(const Args& a, const Smem& sm, Walk w,
       if constexpr (L::kCoded) {
         const int from = (lane & 15) * 8 >> a.box_shift;
         const float x = __shfl_sync(0xffffffffu, ks, from), y = __shfl_sync(0xffffffffu, vs, from);
-        float* const to = reinterpret_cast<float*>(sm.ptr + L::kScales) + unit % kBadSlots * 32 + lane;
+        float* const to = reinterpret_cast<float*>(sm.ptr + L::kScales) + unit % kBadSlots * 48 + lane;
         *to = lane < 16 ? x * a.scale_log2 : y;
+        if (std::is_same<T, __half>::value && lane < 16) to[32] = __log2f(fabsf(y));
       }
       __syncwarp();
 #pragma unroll
@@ -589,7 +592,7 @@ __device__ __forceinline__ void widen_row(uint32_t raw, uint32_t tile, int row) 
   }
 }
 
-// Four warps, a thread a row: K into q's dtype, V into bf16.
+// Four warps, a thread a row.
 template <typename T, int DP, int CODE>
 __device__ __forceinline__ void widen_role(const Args& a, const Smem& sm, Walk w, int row) {
   using L = Layout<DP, CODE>;
@@ -601,11 +604,7 @@ __device__ __forceinline__ void widen_role(const Args& a, const Smem& sm, Walk w
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) return;
     const uint32_t raw = sm.base + L::kRaw + raw_slot * L::kRawTile, tile = sm.base + L::kRing + slot * L::kTile;
-    if (i & 1) {
-      widen_row<__nv_bfloat16, DP, CODE>(raw, tile, row);
-    } else {
-      widen_row<T, DP, CODE>(raw, tile, row);
-    }
+    widen_row<T, DP, CODE>(raw, tile, row);
     fence_proxy_async_smem();
     __syncwarp();
     if ((row & 31) == 0) {
@@ -638,8 +637,7 @@ template <typename T, int DP, int CODE>
 __device__ __forceinline__ void mma_role(const Args& a, const Smem& sm, Walk w, int t, uint32_t tmem) {
   using L = Layout<DP, CODE>;
   constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
-  // Over codes P V runs in bf16, whose range holds a probability times any scale.
-  constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16 || L::kCoded, 128, DP, true);
+  constexpr uint32_t IDESC_S = umma_idesc_f16(BF16, 128, kBN, false), IDESC_O = umma_idesc_f16(BF16, 128, DP, true);
   const int ksteps = (a.dim + 15) / 16;
   const uint32_t sq = uniform(desc_lo(sm.base + t * L::kTile, 16)), ring = uniform(desc_lo(sm.base + L::kRing, 0));
   const uint32_t hi = desc_hi(a.group_bytes);
@@ -757,7 +755,7 @@ __device__ __forceinline__ uint32_t row_at(const Args& a, int row, int half) {
 template <typename T, int DP, int CODE>
 __device__ __forceinline__ void fix_role(const Args& a, const Smem& sm, Walk w, int lane) {
   using L = Layout<DP, CODE>;
-  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value || L::kCoded;
+  constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kExp = BF16 ? 0x7f807f80u : 0x7c007c00u, kOne = BF16 ? 0x00800080u : 0x04000400u;
   uint32_t unit = 0;
   bool ok = true;
@@ -815,12 +813,15 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
   const int row = warp * 32 + lane;
   const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
   const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + 256 + t * 128;
-  using TV = std::conditional_t<L::kCoded, __nv_bfloat16, T>;  // of P and V
   const float sl = a.scale_log2;
   const uint64_t sl2 = pair(sl, sl);
   // fp16 probabilities (and their sum) are held 2^7 times as large, at most 2^15 with kLazy: those below 2^-14 of a row's
   // largest would lose bits to fp16's subnormals (16,000 keys of weight 2^-22 beside one of 1: 2 % of their share).
-  constexpr float kLift = std::is_same<TV, __half>::value ? 7.0f : 0.0f;
+  constexpr float kLift = std::is_same<T, __half>::value ? 7.0f : 0.0f;
+  // Over codes P holds probabilities times value scales. bf16 has the range for any of them. In fp16 they are relative to a row's
+  // largest such product so far, 2^w_ref, which follows it as m follows the scores; O is then in units of 2^(w_ref - kLift), l
+  // in those of 2^m.
+  constexpr bool kWeighted = L::kCoded && std::is_same<T, __half>::value;
   uint32_t unit = 0, s_phase = 0, o_phase = 0, fix_phases = 0;
   bool ok = true;
   Segment g{};
@@ -829,7 +830,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
     const int tok = row / a.group, head = row - tok * a.group;
     const bool valid = row < a.tile_tokens * a.group && tiles.tok0(t) + tok < g.s.n;
     const int limit = valid ? keys_of(a, g.s, tiles.tok0(t) + tok) : 0;
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY, l = 0.0f, w_ref = -INFINITY;
     uint32_t u = unit;
     for (int j = g.j0; j < g.j1; ++j, ++u) {
       const bool special = tiles.special(j);
@@ -845,7 +846,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       tcgen05_fence_after();
       const uint32_t marks = static_cast<uint32_t>(sm.words[kBad + u % kBadSlots]);
       const int cols = limit - j * kBN;  // columns that this row sees
-      const float* const scales = reinterpret_cast<const float*>(sm.ptr + L::kScales) + u % kBadSlots * 32;
+      const float* const scales = reinterpret_cast<const float*>(sm.ptr + L::kScales) + u % kBadSlots * 48;
       const bool plain = !special && marks == 0;
       if (!plain) {
         // S is put back as scaled, and -inf where masked: what follows need not ask.
@@ -865,7 +866,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       }
       // The row's maximum, 32 columns at a time, the next ones on their way.
       // The row's maximum. Rolled loops here and below: longer code would not stay in the instruction caches.
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, wx = -INFINITY;
 #pragma unroll 1
       for (int c = 0; c < 128; c += 64) {
         uint32_t s[2][32];
@@ -879,7 +880,12 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           for (int i = 0; i < 8; i += 2) {
             top = max3(top, __uint_as_float(s[q / 4][q % 4 * 8 + i]), __uint_as_float(s[q / 4][q % 4 * 8 + i + 1]));
           }
-          if constexpr (L::kCoded) top = max3(mx[q & 3], mx[q & 3], top * (plain ? scales[c / 8 + q] : 1.0f));  // no scale is negative here
+          if constexpr (L::kCoded) {
+            top *= plain ? scales[c / 8 + q] : 1.0f;  // no scale is negative here
+            // A masked group's value scale does not count, whatever it is.
+            if constexpr (kWeighted) wx = max3(wx, wx, top == -INFINITY ? top : top + scales[32 + c / 8 + q]);
+            top = max3(mx[q & 3], mx[q & 3], top);
+          }
           mx[q & 3] = top;
         }
       }
@@ -890,6 +896,15 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
         alpha = mc < INFINITY ? exp2_approx(m - mc) : NAN;
         m = mc < INFINITY ? mc : NAN;
         l *= alpha;
+      }
+      float p_scale = 1.0f;
+      if constexpr (kWeighted) {
+        alpha = 1.0f;
+        if (!(wx <= w_ref + kLazy)) {
+          alpha = wx < INFINITY ? exp2_approx(w_ref - wx) : NAN;
+          w_ref = wx < INFINITY ? wx : NAN;
+        }
+        p_scale = exp2_approx(fminf(m - w_ref + kLift, 127.0f));
       }
       if (j > g.j0 && __any_sync(0xffffffffu, !(alpha >= 1.0f))) {
         // S of this unit is complete, and so is O += P V of the one before.
@@ -903,7 +918,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           tmem_st8(tO + c, o);
         }
       }
-      const float shift = (m == -INFINITY ? 0.0f : m) - kLift;
+      const float shift = (m == -INFINITY ? 0.0f : m) - (kWeighted ? 0.0f : kLift);
       const uint64_t sh2 = pair(-shift, -shift);
       uint64_t sum[2] = {0, 0};
       // P, 32 columns at a time, over columns of S that have been read; the products with the first 64 keys may begin
@@ -918,7 +933,7 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           float x0, x1;
           const uint64_t e2 = fma2(x2, L::kCoded ? pair(f, f) : sl2, sh2);
           if (i * L::kByFma % 8 < L::kByFma) {
-            exp2_pair<std::is_same<TV, __half>::value ? 4 : 3>(e2, x0, x1);
+            exp2_pair<std::is_same<T, __half>::value ? 4 : 3>(e2, x0, x1);
           } else {
             unpair(e2, x0, x1);
             x0 = exp2_approx(x0);
@@ -927,10 +942,12 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
           const uint64_t p2 = pair(x0, x1);
           sum[i & 1] = add2(sum[i & 1], p2);
           if constexpr (L::kCoded) {
-            const float v = scales[16 + c / 8 + i / 4];
+            float v = scales[16 + c / 8 + i / 4];
+            // Finite beside a probability of zero, whatever the scale of the group.
+            if constexpr (kWeighted) v = fmaxf(fminf(v * p_scale, 3.0e38f), -3.0e38f);
             unpair(mul2(p2, pair(v, v)), x0, x1);
           }
-          p[i] = Storage<TV>::pack2(x0, x1);
+          p[i] = Storage<T>::pack2(x0, x1);
         }
         tmem_st8(tS + c / 2, p);
       };
@@ -983,12 +1000,12 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
                 const int c = c0 + k;
                 const uint4 v = lds128(sv + row_at(a, c, c8 / 8) + static_cast<uint32_t>(((c8 & 7) ^ (c & 7)) * 16));
                 const bool seen = c < cols && !(marks >> (c >> a.box_shift) & 1u);
-                const float2 p2 = Storage<TV>::unpack2(__float_as_uint(pp[k / 2]));
+                const float2 p2 = Storage<T>::unpack2(__float_as_uint(pp[k / 2]));
                 const float p = k & 1 ? p2.y : p2.x;
                 const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  const float2 f = Storage<TV>::unpack2(vw[i]);
+                  const float2 f = Storage<T>::unpack2(vw[i]);
                   if (seen) {
                     o[2 * i] = fmaf(p, f.x, o[2 * i]);
                     o[2 * i + 1] = fmaf(p, f.y, o[2 * i + 1]);
@@ -1021,10 +1038,11 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
       tcgen05_fence_after();
     }
     if (t >= L::kTiles || tiles.tok0(t) >= g.s.n) continue;  // no rows in this tile, in any piece
+    const float o_scale = !kWeighted ? 1.0f : w_ref == -INFINITY ? 0.0f : exp2_approx(w_ref - m - kLift);  // O to the units of l
     // Rolled loops: each runs once a segment, and the time of straight code would be that of fetching it.
     const int64_t out_row = ((g.s.first + tiles.tok0(t) + tok) * a.hq + g.h * a.group + head) * static_cast<int64_t>(a.dim);
     if (g.j0 == 0 && g.j1 == g.nt) {
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : o_scale / l;
       T* const out = static_cast<T*>(a.out) + out_row;
       const bool wide = a.dim % 16 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 31) == 0;
 #pragma unroll 1
@@ -1054,6 +1072,10 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
         uint32_t o[16];
         tmem_ld16(tO + c, o);
         tmem_wait_ld();
+        if constexpr (kWeighted) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * o_scale);
+        }
         if (valid) {
           const uint32_t lo[8] = {o[0], o[1], o[2], o[3], o[4], o[5], o[6], o[7]}, hi[8] = {o[8], o[9], o[10], o[11], o[12], o[13], o[14], o[15]};
           store32(mine + row * DP + c, lo);

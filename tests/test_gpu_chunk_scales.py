@@ -32,10 +32,11 @@ def test_negative_scales(kind, codes, dtype, dim, page, causal):
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("dim,page", [(64, 16), (128, 16), (256, 16), (128, 8), (128, 20)])
-def test_a_page_whose_scale_is_no_number_counts_for_those_who_see_it(kind, codes, which, value, dim, page):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_page_whose_scale_is_no_number_counts_for_those_who_see_it(kind, codes, which, value, dim, page, dtype):
     """The last page of two sequences, which only the last tokens of their chunks see."""
     for n, length in [(page + 24, 8 * page), (140, 160 + page), (300, 300)]:
-        p = Problem([(n, length), (n, length), (3, 5)], 8, 2, dim, page, torch.bfloat16, kind, codes, seed=51)
+        p = Problem([(n, length), (n, length), (3, 5)], 8, 2, dim, page, dtype, kind, codes, seed=51)
         want, tol = p.want()
         first = (length - 1) // page * page  # the page's first token
         for b in range(2):
