@@ -1202,7 +1202,9 @@ at::Tensor paged_block_select_new(const at::Tensor& q, const at::Tensor& k_cache
 
 // The chunked step's functional forms, under the same rule.
 at::Tensor rows_of_q(const at::Tensor& q) {
-  return q.dim() == 3 && q.stride(2) == 1 && (q.stride(1) == q.size(2) || q.size(1) == 1) ? q : q.contiguous();
+  const bool rows = q.dim() == 3 && q.stride(2) == 1 && (q.stride(1) == q.size(2) || q.size(1) == 1) &&
+                    (q.stride(0) >= q.size(1) * q.size(2) || q.size(0) <= 1);
+  return rows ? q : q.contiguous();
 }
 
 at::Tensor paged_chunk_attention_new(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,

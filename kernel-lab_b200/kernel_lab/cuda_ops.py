@@ -297,8 +297,9 @@ def paged_block_select(
 
 
 def _rows_of_q(q: torch.Tensor) -> torch.Tensor:
-    """q as rows of contiguous heads, any distance apart."""
-    return q if q.stride(-1) == 1 and (q.stride(1) == q.shape[2] or q.shape[1] == 1) else q.contiguous()
+    """q as rows of contiguous heads, any distance apart that keeps them from overlapping."""
+    heads = q.stride(-1) == 1 and (q.stride(1) == q.shape[2] or q.shape[1] == 1)
+    return q if heads and (q.stride(0) >= q.shape[1] * q.shape[2] or q.shape[0] <= 1) else q.contiguous()
 
 
 def paged_chunk_attention(
