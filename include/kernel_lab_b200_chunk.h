@@ -127,16 +127,18 @@ int kl_paged_copy_pages(const kl_page_pools_t* pools, const int32_t* src, const 
  *   then pages for the tokens len .. len + new_tokens[r] - 1 that its last page has no room for.
  * A row whose new tokens do not fit in the table's width, or for whose needs and those of the rows before it
  * the free pages do not suffice, gets none (KL_STATUS_NO_PAGES); a row that needs none is always served.
- *   out_table  [rows, width] int32, contiguous, not overlapping block_table: entries past a row's pages are 0, which
- *              is a page like any other: nothing may be appended for a row that was not served or is empty
+ *   out_table  [rows, width] int32, contiguous: entries past a row's pages are 0, which is a page like any other:
+ *              nothing may be appended for a row that was not served or is empty
  *   out_lens   [rows] int32: seq_lens[parents[r]] (new tokens not counted)
  *   served     [rows] bytes: 1, or 0 for a row that got none of what it needs
+ * No output overlaps an input or another output, but that out_lens may be seq_lens where parents is NULL.
  * Lengths beyond width * page_size are clamped (KL_STATUS_LEN_CLAMPED). Entries outside [0, num_pages) are taken over
  * but stand for no page (KL_STATUS_BAD_PAGE). Parents past the batch make empty rows as negative ones do; they are not
- * reported. An empty row has length 0, needs nothing and is served. Negative new_tokens count as 0. rows at most 2^24. Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's
- * rules (`sync` zero before its first use, left zero but for the status word; calls that overlap on the GPU need
- * separate buffers). A call launches several kernels that hand data on through the scratch: nothing else that uses these
- * buffers may be put on the stream, by another host thread for instance, until it has returned.
+ * reported. An empty row has length 0, needs nothing and is served. Negative new_tokens count as 0. rows at most 2^24.
+ * Scratch from kl_paged_reserve_workspace_size, under kl_paged_decode's rules (`sync` zero before its first use, left zero
+ * but for the status word; calls that overlap on the GPU need separate buffers); both start at a multiple of 16 bytes. A
+ * call launches several kernels that hand data on through the scratch: nothing else that uses these buffers may be put on
+ * the stream, by another host thread for instance, until it has returned.
  */
 int kl_paged_reserve_workspace_size(int64_t num_pages, int rows, size_t* scratch_bytes, size_t* sync_bytes);
 
@@ -149,9 +151,9 @@ int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table, int32_t* 
 /*
  * Moves the pages in use (those that the first ceil(seq_lens[b] / page_size) entries of the rows name; *used
  * of them) to the ids 0 .. *used - 1: the ones with ids of *used and more, in ascending order, to the free ids
- * below, in ascending order, in every tensor. out_table ([batch, width] int32, contiguous, not overlapping
- * block_table) receives the entries under the pages' new ids, 0 past a row's pages. Entries outside
- * [0, num_pages) are taken over (KL_STATUS_BAD_PAGE), lengths clamped as above. Scratch as above.
+ * below, in ascending order, in every tensor. out_table ([batch, width] int32, contiguous) receives the entries
+ * under the pages' new ids, 0 past a row's pages. Entries outside [0, num_pages) are taken over (KL_STATUS_BAD_PAGE),
+ * lengths clamped as above. Neither output overlaps an input or the other. Scratch as above.
  */
 int kl_paged_compact_workspace_size(int64_t num_pages, size_t* scratch_bytes, size_t* sync_bytes);
 

@@ -575,9 +575,30 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
   return na > 0 && nb > 0 && x < y + static_cast<uintptr_t>(nb) && y < x + static_cast<uintptr_t>(na);
 }
 
-bool tables_overlap(const PlanArgs& a) {
-  const int64_t in = a.batch > 0 ? ((a.batch - 1) * a.bt_stride + a.width) * 4 : 0;
-  return overlap(a.out_table, static_cast<int64_t>(a.rows) * a.width * 4, a.block_table, in);
+// Whether an output lies over an input or another output: some rows are written while others are read. The lengths alone may
+// be updated in place, where every row is its own parent.
+bool outputs_overlap(const PlanArgs& a) {
+  struct Region {
+    const void* at;
+    int64_t bytes;
+  };
+  const int64_t rows = a.rows;
+  const Region out[] = {{a.out_table, rows * a.width * 4}, {a.out_lens, a.out_lens ? rows * 4 : 0}, {a.served, a.served ? rows : 0}, {a.used, a.used ? 4 : 0}};
+  const Region in[] = {{a.block_table, a.batch > 0 ? ((a.batch - 1) * a.bt_stride + a.width) * 4 : 0},
+                       {a.seq_lens, int64_t(a.batch) * 4},
+                       {a.new_tokens, a.new_tokens ? rows * 4 : 0},
+                       {a.parents, a.parents ? rows * 4 : 0}};
+  const bool in_place = !a.parents && a.out_lens == a.seq_lens;
+  for (int o = 0; o < 4; ++o) {
+    for (int i = 0; i < 4; ++i) {
+      if (o == 1 && i == 1 && in_place) continue;
+      if (overlap(out[o].at, out[o].bytes, in[i].at, in[i].bytes)) return true;
+    }
+    for (int i = 0; i < o; ++i) {
+      if (overlap(out[o].at, out[o].bytes, out[i].at, out[i].bytes)) return true;
+    }
+  }
+  return false;
 }
 
 }  // namespace page_pool
@@ -632,7 +653,7 @@ extern "C" int kl_paged_reserve(const kl_page_pools_t* pools, int32_t* out_table
   a.rows = rows;
   a.width = width;
   a.page_size = page_size;
-  if (tables_overlap(a)) return invalid;
+  if (outputs_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_plan(mark_pages<true>, reserve_plan, a, st);
   if (e != cudaSuccess) return static_cast<int>(e);
@@ -672,7 +693,7 @@ extern "C" int kl_paged_compact(const kl_page_pools_t* pools, int32_t* out_table
   a.rows = batch;
   a.width = width;
   a.page_size = page_size;
-  if (tables_overlap(a)) return invalid;
+  if (outputs_overlap(a)) return invalid;
   const auto st = static_cast<cudaStream_t>(stream);
   const cudaError_t e = launch_plan(mark_pages<false>, compact_plan, a, st);
   if (e != cudaSuccess) return static_cast<int>(e);

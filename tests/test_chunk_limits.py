@@ -35,3 +35,30 @@ def test_chunks_that_32_bit_rows_cannot_count():
     for tokens in (2**31 - 256, 2**31 - 2, 2**31 - 1, 2**31, 2**40):
         assert attend(hq=1, hkv=1, dim=8, tokens=tokens) == INVALID, tokens
         assert attend(hq=1, hkv=1, dim=8, tokens=tokens, dtype=0) == INVALID, tokens
+
+
+def reserve(out=1 << 20, lens_out=2 << 20, served=3 << 20, table=4 << 20, lens=5 << 20, new=6 << 20, parents=None):
+    from kernel_lab import capi
+
+    pools = capi.PagePools(0, None, None, None)
+    return capi.load().kl_paged_reserve(ctypes.byref(pools), out, lens_out, served, table, lens, new, parents, 4, 4, 4, 16, 4, 10,
+                                        8 << 20, 1 << 20, 9 << 20, 1 << 20, None)
+
+
+def compact(out=1 << 20, used=2 << 20, table=4 << 20, lens=5 << 20):
+    from kernel_lab import capi
+
+    pools = capi.PagePools(0, None, None, None)
+    return capi.load().kl_paged_compact(ctypes.byref(pools), out, used, table, lens, 4, 4, 16, 4, 10, 8 << 20, 1 << 20, 9 << 20, 1 << 20, None)
+
+
+def test_outputs_of_the_bookkeeping_that_overlap_its_inputs():
+    """Rows are read while others are written."""
+    at, parents = 5 << 20, 7 << 20
+    for bad in ({"lens_out": at, "parents": parents}, {"lens_out": at + 4}, {"lens_out": at - 12}, {"lens_out": 6 << 20}, {"lens_out": 6 << 20, "parents": parents},
+                {"lens_out": parents, "parents": parents}, {"lens_out": (4 << 20) + 60}, {"served": at + 15}, {"served": 6 << 20}, {"served": (4 << 20) + 63},
+                {"served": parents + 3, "parents": parents}, {"out": at - 60}, {"out": 6 << 20}, {"out": parents, "parents": parents}, {"out": 4 << 20},
+                {"out": 2 << 20}, {"served": (1 << 20) + 8}, {"served": (2 << 20) + 8}):
+        assert reserve(**bad) == INVALID, bad
+    for bad in ({"out": at}, {"out": 4 << 20}, {"used": at + 12}, {"used": (4 << 20) + 8}, {"used": (1 << 20) + 60}):
+        assert compact(**bad) == INVALID, bad

@@ -142,3 +142,18 @@ def test_a_dead_graphs_timeout_is_cleared_before_its_scratch_is_used_again():
             got = run()
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, want)) and cuda_ops.decode_status() == 0
+
+
+def test_lengths_updated_in_place():
+    """Where every row is its own parent the new lengths may take the old ones' place, those past the table clamped."""
+    from kernel_lab import cuda_ops
+
+    cuda_ops.decode_status(clear=True)
+    table = int32([[4, 5] + [0] * 600, [7] * 602])
+    pool = [torch.arange(40, device="cuda", dtype=torch.int32)[:, None].contiguous()]
+    lens, out, served = int32([20, 602 * 16 + 5]), torch.zeros_like(table), torch.zeros(2, dtype=torch.bool, device="cuda")
+    torch.ops.kernel_lab.paged_reserve(out, lens, served, pool, table, lens, int32([20, 0]), None, 16)
+    assert cuda_ops.decode_status(clear=True) == 2
+    assert lens.tolist() == [20, 602 * 16] and served.all() and out[0].tolist() == [4, 5, 0] + [0] * 599 and (out[1] == 7).all()
+    with pytest.raises(RuntimeError):
+        torch.ops.kernel_lab.paged_reserve(out, lens, served, pool, table, lens, int32([20, 0]), int32([1, 0]), 16)
