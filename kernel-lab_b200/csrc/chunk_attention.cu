@@ -20,8 +20,9 @@ namespace chunk_attention {
 //
 // Any dtype, cache, group, head_dim up to 256, page size and stride. A CTA takes kRows rows of one KV head and
 // walks their keys kKeys at a time: K and V widened to fp32 in shared memory (rows padded with zeros to whole float4s), a thread
-// per four scores, eight threads a row for the softmax and for the row's output. Bound by shared-memory loads: a float4 of
-// q and four of K for 16 multiply-adds.
+// per four scores, eight threads a row for the softmax and for the row's output. Bound by shared-memory loads (a float4 of
+// q and four of K for 16 multiply-adds) and, with few rows, by one CTA's walk over a whole context, which is not split: fp32,
+// 8 x 4 draft tokens over up to 1024 of 32/8 heads of 128 320 us, 4 tokens over 32,768 9.6 ms.
 
 constexpr int kRows = 16, kKeys = 32, kThreads = 128, kMaxDim = 256;
 

@@ -22,8 +22,9 @@
 // case the softmax threads add that unit's P V themselves, key by key.
 //
 // Bound by the chain S -> softmax -> P -> products of a tile: 3,700 cycles a unit for its two tiles, of which the products
-// take 2,048. A prompt of 8192 tokens with 32/8 heads of 128, bf16: 560 us, 981 TFLOP/s, 0.58 of the measured matrix
-// product; 8 x 512 tokens over up to 8192 of 64/8 heads in e4m3 blocks: 1,201 us, 639 TFLOP/s.
+// take 2,048. A prompt of 8192 tokens with 32/8 heads of 128, bf16, called over and over on changing inputs: 629 us,
+// 874 TFLOP/s, 0.52 of the measured matrix product (under the power cap; in runs of 20 calls 571 us). 8 x 512 tokens over
+// up to 8192 of 64/8 heads in e4m3 blocks: 1,195 us, 643 TFLOP/s in bf16, 1,205 us in fp16.
 #include <cuda.h>
 
 #include <algorithm>
@@ -59,8 +60,9 @@ struct Layout {
   // Registers: 256 * 136 + 256 * 120 = 512 * 128, 256 * 176 + 128 * 152 = 384 * 168, the launch's.
   static constexpr int kSoftmaxRegs = kCoded ? 136 : 176, kOtherRegs = kCoded ? 120 : 152;
   static constexpr int kTiles = tiles_of(DP);
-  // Of 8 exponentials, those on the multiply-add pipes (a prompt of 8192 tokens: 581 us with none, 558 with 3, 580 with 3 and
-  // longer loops). Over codes the warps are short of issue slots (chunks over 8192 tokens: 1249 us with none, 1277 with 3).
+  // Of 8 exponentials, those on the multiply-add pipes (a prompt of 8192 tokens: 589 us with none, 571 with 3 in runs of 20
+  // calls; 638 and 632 under the power cap). Over codes the warps are short of issue slots (chunks over 8192 tokens: 1,195 us
+  // with none, 1,238 with 3).
   static constexpr int kByFma = kCoded ? 0 : 3;
   static constexpr int kHalves = DP / 64;                   // 128-byte column blocks of a 16-bit row
   static constexpr uint32_t kHalf = 128u * 128u;            // 128 rows of one
@@ -864,7 +866,6 @@ __device__ __forceinline__ void softmax_role(const Args& a, const Smem& sm, Walk
         }
         tmem_wait_st();
       }
-      // The row's maximum, 32 columns at a time, the next ones on their way.
       // The row's maximum. Rolled loops here and below: longer code would not stay in the instruction caches.
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, wx = -INFINITY;
 #pragma unroll 1

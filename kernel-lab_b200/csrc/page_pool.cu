@@ -10,7 +10,8 @@
 // stores, which all SMs share (one cluster alone took 7 us for 65,000 of them); the rest is one cluster of kClusterCtas
 // CTAs of kPlanThreads threads, its phases divided by cluster barriers: the CTAs of a cluster are resident together by
 // definition. It clears the marks behind itself.
-// Copies: HBM-bound, 2 * bytes. CTAs take 16 KB slices of a page, all loads of a slice before its stores.
+// Copies: HBM-bound, 2 * bytes. CTAs take 16 KB slices of a page, all loads of a slice before its stores (250 pages of 48
+// tensors: 135 us, 5,830 GB/s, 0.89 of the measured copy).
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 

@@ -93,7 +93,7 @@ def paged_kv_append(
     """Write each sequence's new token's K/V rows ([batch, num_kv_heads, head_dim], rows may be a
     strided view) into its pages at token index ``positions[b]`` (in place; negative skips).
     With ``indptr`` (int32 [batch + 1]) sequence b's new tokens are the rows ``indptr[b]`` .. ``indptr[b + 1] - 1``
-    and take the positions from ``positions[b]`` on.
+    and take the positions from ``positions[b]`` on. Caches are contiguous [num_pages, page_size, num_kv_heads, head_dim].
     Page ids outside the pool are skipped and reported by :func:`decode_status`."""
     _require()
     if indptr is not None:
@@ -318,7 +318,8 @@ def paged_chunk_attention(
     pages: append them first (:func:`paged_kv_append`). A token attends to the tokens up to itself, without
     ``causal`` to all ``seq_lens[b]`` (cross attention over an encoder's states). What is masked does not count,
     whatever it holds; a token that has none to attend to gets zeros. The rows of the result that are no sequence's are
-    undefined. Caches as in :func:`paged_decode_attention`, or views with any order of pages, tokens and heads in memory."""
+    undefined. Caches as in :func:`paged_decode_attention`, or views with any order of pages, tokens and heads in memory
+    (those the 16-bit and e4m3 appends here cannot write: they take contiguous caches)."""
     _require()
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     tensors = (k_cache, v_cache, block_table, seq_lens, indptr)
